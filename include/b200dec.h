@@ -242,6 +242,31 @@ int b200dec_gated_norm(const float* o, const void* gate, int64_t gate_stride, in
                        int32_t weight_len, float eps, float out_scale, void* out, int64_t out_stride, int32_t num_rows, int32_t len,
                        int32_t parts, void* stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection.
+ * Adapter a of `slots`: down[a] [parts * rank, width], up[a] [out, rank], scale[a]; contiguous, element size elem.  The projection's columns fall into
+ * `parts` (1 to 4) parts, the p-th ending before column ends[p] (out = the last one's end); part p has rows p * rank .. of down for itself.
+ * rank: a multiple of 8 up to 128 (adapters of fewer have zeros), slots up to 4096, any width and out. */
+typedef struct b200dec_adapters {
+  const void* down;
+  const void* up;
+  const float* scale;
+  int32_t slots, rank, width, parts, elem;
+  int32_t ends[4];
+} b200dec_adapters;
+
+/* A step's rows sorted by adapter, for every projection of the step.  ids int32 [num_rows]: the adapter of each row, -1: none (any other id
+ * outside [0, slots) counts as that and sets B200KV_S_BAD_POSITION).  order int32 [num_rows] and tiles int32 [max_tiles, 4] (16-byte aligned) are
+ * written; max_tiles >= num_rows / tile_rows + min(num_rows, slots + 1).  tile_rows: 16 or 128. */
+int b200dec_adapter_plan(const int32_t* ids, int32_t num_rows, int32_t slots, int32_t tile_rows, int32_t* order, int32_t* tiles,
+                         int32_t max_tiles, int32_t* status, void* stream);
+
+/* out[r] = y[r] + scale[a] * (x[r] . down[a]_p^T) . up[a]^T for the rows of a plan with as many slots; out[r] = y[r] for rows without an adapter.
+ * x [num_rows, width], y and out [num_rows, out] of element size elem, strides in elements.  out may be y itself, with the same stride; otherwise it
+ * overlaps neither y nor x.  32-bit sums, rounded once. */
+int b200dec_add_adapters(const b200dec_adapters* adapters, const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out,
+                         int64_t out_stride, const int32_t* order, const int32_t* tiles, int32_t max_tiles, int32_t tile_rows, int32_t num_rows,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -73,9 +73,17 @@ class Entries(C.Structure):
         ("num_entries", c_int32), ("num_rows", c_int32)]
 
 
+class Adapters(C.Structure):
+    """struct b200dec_adapters"""
+
+    _fields_ = [("down", c_void_p), ("up", c_void_p), ("scale", c_void_p)] + [
+        (n, c_int32) for n in ("slots", "rank", "width", "parts", "elem")] + [("ends", c_int32 * 4)]
+
+
 P_CACHE, P_TABLE = C.POINTER(Cache), C.POINTER(Table)
 P_DCACHE, P_ROWS, P_OPT = C.POINTER(DecCache), C.POINTER(DecRows), C.POINTER(AttnOptions)
 P_REC, P_REC_IN, P_ENT = C.POINTER(Recurrence), C.POINTER(RecurrenceIn), C.POINTER(Entries)
+P_ADAPTERS = C.POINTER(Adapters)
 
 # name -> (restype, argtypes); must list every function include/b200kv.h declares
 SIGNATURES = {
@@ -178,6 +186,9 @@ DECODER_SIGNATURES = {
                                           c_void_p, c_float, c_float, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "b200dec_grouped_linear": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
                                          c_void_p, c_int32, c_float, c_float, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
+    "b200dec_adapter_plan": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
+    "b200dec_add_adapters": (c_int32, [P_ADAPTERS, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32,
+                                       c_int32, c_void_p]),
 }
 SHARED_SIGNATURES = ("b200kv_version", "b200kv_error_string", "b200kv_set_chained_launch", "b200kv_get_chained_launch",
                      "b200kv_plain_next", "b200kv_branches_begin", "b200kv_branches_next", "b200kv_branches_end", "b200kv_sample_workspace_bytes", "b200kv_sample")

@@ -616,3 +616,145 @@ class Packed:
     def part(self, y: torch.Tensor, name: str) -> torch.Tensor:
         lo, hi = self.at[name]
         return y[:, lo:hi]
+
+
+# ----------------------------------------------------------------------------- low-rank adapters of many requests
+MAX_ADAPTER_RANK = 128
+
+
+@dataclass(frozen=True, eq=False)
+class Adapters:
+    """Low-rank adapters of one shared projection, a slot each: y + scale[a] * (x down[a]^T) up[a]^T.  `parts`: the projection's columns, one number
+    for each part that has a product of its own (query, key, value of a packed one); rows p * rank .. of down belong to part p."""
+
+    down: torch.Tensor  # [slots, parts * rank, width]
+    up: torch.Tensor  # [slots, out, rank]
+    scale: torch.Tensor  # fp32 [slots]
+    parts: tuple[int, ...]
+
+    def __post_init__(self):
+        d, u, s, parts = self.down, self.up, self.scale, tuple(self.parts)
+        if d.dim() != 3 or u.dim() != 3 or s.dim() != 1 or not d.is_contiguous() or not u.is_contiguous() or not s.is_contiguous():
+            raise ValueError("adapters: contiguous down [slots, parts * rank, width], up [slots, out, rank] and scale [slots] are wanted")
+        slots, out, rank = u.shape
+        if not 1 <= len(parts) <= 4 or min(parts) < 1 or sum(parts) != out:
+            raise ValueError(f"adapters: one to four parts that add up to the {out} columns, not {parts}")
+        if rank % 8 or not 8 <= rank <= MAX_ADAPTER_RANK:
+            raise ValueError(f"adapters: the rank is a multiple of 8 up to {MAX_ADAPTER_RANK}, not {rank}")
+        if not 1 <= slots <= 4096 or d.shape[:2] != (slots, len(parts) * rank) or s.shape[0] != slots or d.shape[2] < 1:
+            raise ValueError(f"adapters: down {tuple(d.shape)} and scale {tuple(s.shape)} do not fit up {tuple(u.shape)} of {len(parts)} parts")
+        if d.dtype != u.dtype or s.dtype != torch.float32 or not d.device == u.device == s.device:
+            raise ValueError("adapters: down and up of one type, a 32-bit scale, all on one device")
+        ends = [sum(parts[: i + 1]) for i in range(len(parts))]
+        st = _lib.Adapters(d.data_ptr(), u.data_ptr(), s.data_ptr(), slots, rank, d.shape[2], len(parts), _elem(d.dtype))
+        st.ends[: len(ends)] = ends
+        object.__setattr__(self, "parts", parts)
+        object.__setattr__(self, "struct", st)
+
+    @property
+    def slots(self) -> int:
+        return self.up.shape[0]
+
+    @property
+    def rank(self) -> int:
+        return self.up.shape[2]
+
+    def load(self, slot: int, pairs, scale: float) -> None:
+        """Put an adapter into a slot: a pair (down [r, width], up [columns of the part, r]) for each part, r up to the rank, or None for a part that
+        it leaves alone."""
+        if not 0 <= slot < self.slots or len(pairs) != len(self.parts):
+            raise ValueError(f"adapters: slot {slot} of {self.slots}, {len(pairs)} pairs for {len(self.parts)} parts")
+        for pair, n in zip(pairs, self.parts):
+            if pair is not None and (pair[0].dim() != 2 or pair[0].shape[0] > self.rank or pair[0].shape[1] != self.down.shape[2]
+                                     or tuple(pair[1].shape) != (n, pair[0].shape[0])):
+                raise ValueError(f"adapters: {tuple(pair[0].shape)} and {tuple(pair[1].shape)} for {self.down.shape[2]} inputs, {n} columns and "
+                                 f"ranks up to {self.rank}")
+        self.clear(slot)
+        at = 0
+        for i, (pair, n) in enumerate(zip(pairs, self.parts)):
+            if pair is not None:
+                r = pair[0].shape[0]
+                self.down[slot, i * self.rank : i * self.rank + r] = pair[0].to(self.down)
+                self.up[slot, at : at + n, :r] = pair[1].to(self.up)
+            at += n
+        self.scale[slot] = float(scale)
+
+    def clear(self, slot: int) -> None:
+        """An adapter that adds nothing."""
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"adapters: slot {slot} of {self.slots}")
+        self.down[slot] = 0
+        self.up[slot] = 0
+        self.scale[slot] = 0
+
+
+def make_adapters(slots: int, width: int, parts, rank: int, dtype, device) -> Adapters:
+    """Empty slots for adapters of up to `rank` (rounded up to a multiple of 8) beside a projection of `width` inputs."""
+    rank = _round8(rank)
+    return Adapters(torch.zeros(slots, len(parts) * rank, width, dtype=dtype, device=device),
+                    torch.zeros(slots, sum(parts), rank, dtype=dtype, device=device), torch.zeros(slots, device=device), tuple(parts))
+
+
+@dataclass(frozen=True, eq=False)
+class AdapterPlan:
+    """A step's rows sorted by adapter (plan_adapters), for all the projections of the step."""
+
+    order: torch.Tensor  # int32 [rows]
+    tiles: torch.Tensor  # int32 [max_tiles, 4]
+    slots: int
+    tile_rows: int
+
+
+def adapter_tile_rows(num_rows: int) -> int:
+    """Rows of a tile: 16 for decoding rows, 128 where rows of one adapter come in portions."""
+    return 16 if num_rows <= 128 else 128
+
+
+def _here(t: torch.Tensor) -> None:
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {t.device} while device {torch.cuda.current_device()} is the current one")
+
+
+@K._ranged
+def plan_adapters(ids: torch.Tensor, slots: int, tile_rows: int | None = None) -> AdapterPlan:
+    """Sort a step's rows by adapter.  ids int32 [rows]: each row's slot, -1: none; others outside [0, slots) count as that and set a status bit.  One launch per
+    step, for every add_adapters of it."""
+    K._require_cuda(ids)
+    _here(ids)
+    if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous():
+        raise ValueError("plan_adapters: contiguous int32 ids [rows] are wanted")
+    if not 1 <= slots <= 4096:
+        raise ValueError(f"plan_adapters: 1 to 4096 slots, not {slots}")
+    N = ids.shape[0]
+    rows = adapter_tile_rows(N) if tile_rows is None else tile_rows
+    most = N // rows + min(N, slots + 1)
+    buf = torch.empty(4 * most + N, dtype=torch.int32, device=ids.device)
+    tiles, order = buf[: 4 * most].view(most, 4), buf[4 * most :]
+    rc = _lib_dec().b200dec_adapter_plan(ids.data_ptr(), N, slots, rows, order.data_ptr(), tiles.data_ptr(), most,
+                                         K.status_word(ids.device).data_ptr(), K._stream())
+    _lib.check(rc, "plan_adapters")
+    return AdapterPlan(order, tiles, slots, rows)
+
+
+@K._ranged
+def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: AdapterPlan, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y + scale * (x down^T) up^T of every row's adapter, in one launch; rows without one stay y.  y [rows, out]: what the shared projection made of
+    x [rows, width].  Written over y unless `out` is given, which shares no memory with y or x."""
+    K._require_cuda(y, x, adapters.up, plan.order)
+    _here(y)
+    out = y if out is None else out
+    N = plan.order.shape[0]
+    if y.dtype != adapters.up.dtype or x.dtype != y.dtype or out.dtype != y.dtype:
+        raise ValueError(f"add_adapters: rows of {x.dtype}, {y.dtype} and {out.dtype} beside adapters of {adapters.up.dtype}")
+    if tuple(x.shape) != (N, adapters.down.shape[2]) or tuple(y.shape) != (N, adapters.up.shape[1]) or out.shape != y.shape:
+        raise ValueError(f"add_adapters: {tuple(x.shape)}, {tuple(y.shape)} and {tuple(out.shape)} for a plan of {N} rows")
+    if N and not x.stride(1) == y.stride(1) == out.stride(1) == 1:
+        raise ValueError("add_adapters: a row's elements lie side by side")
+    if plan.slots != adapters.slots:
+        raise ValueError(f"add_adapters: a plan for {plan.slots} slots and {adapters.slots} adapters")
+    # (a single row's stride may be anything)
+    xs, ys, os = (t.stride(0) if N > 1 else _round8(t.shape[1]) for t in (x, y, out))
+    rc = _lib_dec().b200dec_add_adapters(ctypes.byref(adapters.struct), x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, plan.order.data_ptr(),
+                                         plan.tiles.data_ptr(), plan.tiles.shape[0], plan.tile_rows, N, K._stream())
+    _lib.check(rc, "add_adapters")
+    return out

@@ -1,0 +1,211 @@
+"""Low-rank adapters of many requests beside a shared projection, against the formula in 64 bits.
+
+Bound per element: both sums in 32 bits over `width` and `rank` terms (each addition and product off by at most a step, 2^-23 of the
+sum of magnitudes), in bf16 the inner values as two terms (2^-16 of each), the result rounded once (half a step)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from inference_engine_b200 import ops
+
+    return ops
+
+
+def make(ops, rows, width, parts, rank, slots, dtype, seed=0, ids=None):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def rnd(*shape, std=1.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+    ad = ops.Adapters(rnd(slots, len(parts) * rank, width, std=width ** -0.5), rnd(slots, sum(parts), rank, std=0.5),
+                      torch.rand(slots, generator=g, device="cuda") + 0.5, parts)
+    if ids is None:
+        ids = torch.randint(-1, slots, (rows,), generator=g, device="cuda")
+    return ad, ids.to("cuda", torch.int32), rnd(rows, width), rnd(rows, sum(parts))
+
+
+def check(ad, ids, x, y, got):
+    want, size, at = y.double(), torch.zeros_like(y, dtype=torch.float64), 0
+    rank, width = ad.rank, x.shape[1]
+    for a in set(ids.tolist()):
+        if not 0 <= a < ad.slots:
+            continue
+        rows, at = (ids == a).nonzero()[:, 0], 0
+        for i, n in enumerate(ad.parts):
+            d, u = ad.down[a, i * rank : (i + 1) * rank].double(), ad.up[a, at : at + n].double()
+            s = float(ad.scale[a])
+            want[rows, at : at + n] += s * (x[rows].double() @ d.t()) @ u.t()
+            size[rows, at : at + n] += s * (x[rows].double().abs() @ d.abs().t()) @ u.abs().t()
+            at += n
+    eps = torch.finfo(y.dtype).eps / 2
+    inner = 2.0 ** -16 if y.dtype == torch.bfloat16 else 0.0
+    bound = eps * want.abs() + (1 + eps) * ((width + rank + 3) * 2.0 ** -23 + inner) * size + 2.0 ** -23 * want.abs()
+    off = (got.double() - want).abs()
+    assert (off <= bound).all(), (off / bound).max()
+    rest = ~((ids >= 0) & (ids < ad.slots))
+    assert torch.equal(got[rest], y[rest])
+
+
+SHAPES = [
+    # rows, width, parts, rank, slots, dtype
+    (1, 2048, (2048, 1024, 1024), 16, 1, torch.bfloat16),
+    (64, 2048, (2048,), 16, 48, torch.bfloat16),
+    (37, 1536, (1792, 896, 768), 24, 5, torch.bfloat16),
+    (129, 256, (512, 512), 8, 3, torch.bfloat16),
+    (300, 2048, (2048, 1024, 1024), 64, 2, torch.bfloat16),
+    (700, 6144, (2048,), 40, 3, torch.bfloat16),
+    (200, 512, (96, 40, 8, 200), 128, 2, torch.bfloat16),  # more inner values than the wide form takes
+    (17, 72, (33, 7), 8, 2, torch.bfloat16),  # parts that end inside a group, and off eight columns
+    (150, 40, (65,), 16, 4, torch.bfloat16),
+    (20, 61, (50, 14), 16, 3, torch.bfloat16),  # rows that cannot be read in 16 bytes
+    (3, 8, (1,), 8, 2, torch.bfloat16),
+    (40, 2048, (1792, 896, 768), 8, 2, torch.float32),
+    (161, 1100, (130, 3), 56, 7, torch.float32),
+    (1, 1, (5,), 8, 1, torch.float32),
+]
+
+
+@pytest.mark.parametrize("rows,width,parts,rank,slots,dtype", SHAPES)
+@pytest.mark.parametrize("tile_rows", [None, 16, 128])
+def test_against_the_formula(ops, rows, width, parts, rank, slots, dtype, tile_rows):
+    ad, ids, x, y = make(ops, rows, width, parts, rank, slots, dtype)
+    plan = ops.plan_adapters(ids, slots, tile_rows)
+    out = torch.full_like(y, float("nan"))
+    assert ops.add_adapters(y, x, ad, plan, out=out) is out
+    check(ad, ids, x, y, out)
+    again = ops.add_adapters(y.clone(), x, ad, plan)  # over y itself
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strided_rows_and_what_lies_beside_them(ops, dtype):
+    ad, ids, x, y = make(ops, 50, 128, (64, 32), 16, 3, dtype, seed=4)
+    for pad in (8, 3):
+        wide_x = torch.full((50, 128 + pad), float("nan"), dtype=dtype, device="cuda")
+        wide_y = torch.full((50, 96 + pad), float("nan"), dtype=dtype, device="cuda")
+        wide_x[:, :128], wide_y[:, :96] = x, y
+        plan = ops.plan_adapters(ids, 3)
+        got = ops.add_adapters(wide_y[:, :96], wide_x[:, :128], ad, plan)
+        check(ad, ids, x, y, got)
+        assert wide_y[:, 96:].isnan().all()
+
+
+def test_a_row_s_result_does_not_depend_on_the_others(ops):
+    ad, ids, x, y = make(ops, 90, 512, (256, 64), 16, 4, torch.bfloat16, seed=2)
+    whole = ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 4), out=torch.empty_like(y))
+    perm = torch.randperm(90, device="cuda")
+    mixed = ops.add_adapters(y[perm], x[perm], ad, ops.plan_adapters(ids[perm].contiguous(), 4))
+    assert torch.equal(mixed, whole[perm])
+    for r in (0, 41, 89):
+        one = ops.add_adapters(y[r : r + 1].clone(), x[r : r + 1], ad, ops.plan_adapters(ids[r : r + 1], 4))
+        assert torch.equal(one[0], whole[r])
+
+
+@pytest.mark.parametrize("rows", [1, 31, 128, 1500, 4099])
+@pytest.mark.parametrize("slots", [1, 7, 1500])
+def test_plan_covers_every_row_once(ops, rows, slots):
+    g = torch.Generator().manual_seed(rows)
+    ids = torch.randint(-1, slots, (rows,), generator=g).to("cuda", torch.int32)
+    plan = ops.plan_adapters(ids, slots)
+    order, ids = plan.order.tolist(), ids.tolist()
+    assert sorted(order) == list(range(rows))
+    covered = []
+    for slot, first, count, _ in plan.tiles.tolist():
+        assert 0 <= count <= plan.tile_rows
+        covered += range(first, first + count)
+        assert all(ids[order[i]] == slot for i in range(first, first + count))
+    assert sorted(covered) == list(range(rows))
+
+
+def test_ids_out_of_range_are_rows_without_an_adapter(ops):
+    from inference_engine_b200 import kernels as K
+
+    ids = torch.tensor([0, 3, -2, 1, -1, 2 ** 31 - 1, 2, 2])
+    ad, ids, x, y = make(ops, 8, 64, (64,), 8, 3, torch.bfloat16, ids=ids)
+    K.check_status()
+    got = ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 3), out=torch.empty_like(y))
+    check(ad, ids, x, y, got)
+    assert K.check_status() == 2  # a token position or id out of range
+    ops.plan_adapters(torch.tensor([-1, 0, 2], dtype=torch.int32, device="cuda"), 3)
+    assert K.check_status() == 0
+
+
+def test_nothing_to_do(ops):
+    ad, ids, x, y = make(ops, 0, 64, (64,), 8, 3, torch.bfloat16, ids=torch.zeros(0))
+    assert ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 3)).shape == (0, 64)
+    ad, ids, x, y = make(ops, 5, 64, (64,), 8, 3, torch.bfloat16, ids=torch.full((5,), -1))
+    assert torch.equal(ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 3), out=torch.empty_like(y)), y)
+
+
+def test_load_and_clear(ops):
+    for dtype in (torch.bfloat16, torch.float32):
+        ad = ops.make_adapters(3, 64, (32, 16), 12, dtype, "cuda")
+        assert ad.rank == 16
+        g = torch.Generator(device="cuda").manual_seed(1)
+        d, u = torch.randn(5, 64, generator=g, device="cuda"), torch.randn(16, 5, generator=g, device="cuda")
+        ad.load(1, [None, (d, u)], 0.25)
+        x = torch.randn(4, 64, generator=g, device="cuda").to(dtype)
+        y = torch.randn(4, 48, generator=g, device="cuda").to(dtype)
+        ids = torch.tensor([1, 0, 2, 1], dtype=torch.int32, device="cuda")
+        plan = ops.plan_adapters(ids, 3)
+        got = ops.add_adapters(y, x, ad, plan, out=torch.empty_like(y))
+        check(ad, ids, x, y, got)
+        assert torch.equal(got[:, :32], y[:, :32]) and torch.equal(got[1:3], y[1:3]) and not torch.equal(got[0], y[0])
+        ad.clear(1)
+        assert torch.equal(ops.add_adapters(y, x, ad, plan, out=torch.empty_like(y)), y)
+
+
+def test_infinities_and_nan_stay_in_their_rows(ops):
+    ad, ids, x, y = make(ops, 20, 128, (64,), 16, 2, torch.bfloat16, seed=5, ids=torch.arange(20) % 2)
+    clean = ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 2), out=torch.empty_like(y))
+    x[3, 7], x[6, 100] = float("nan"), float("inf")
+    got = ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 2), out=torch.empty_like(y))
+    rest = torch.ones(20, dtype=torch.bool, device="cuda")
+    rest[[3, 6]] = False
+    assert torch.equal(got[rest], clean[rest]) and got[3].isnan().all()
+    assert not got[6].isfinite().any()
+
+
+def test_recorded_and_on_another_stream(ops):
+    ad, ids, x, y = make(ops, 70, 256, (128, 64), 16, 5, torch.bfloat16, seed=7)
+    want = ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 5), out=torch.empty_like(y))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 5), out=torch.empty_like(y))
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    out = torch.empty_like(y)
+    with torch.cuda.graph(graph):
+        ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 5), out=out)
+    for k in range(3):  # other rows and other adapters of the rows through the same graph
+        ids.copy_(ids.roll(1))
+        x.copy_(x.roll(3, 0))
+        graph.replay()
+        check(ad, ids, x, y, out)
+
+
+def test_chained_launches(ops):
+    from inference_engine_b200 import kernels as K
+
+    ad, ids, x, y = make(ops, 64, 512, (512,), 16, 20, torch.bfloat16, seed=8)
+
+    def layers():
+        plan, h = ops.plan_adapters(ids, 20), x
+        for _ in range(6):
+            h = ops.add_adapters(y, h, ad, plan, out=torch.empty_like(y))
+        return h
+
+    want = layers()
+    K.set_early_start(True)
+    try:
+        got = layers()
+        torch.cuda.synchronize()
+    finally:
+        K.set_early_start(False)
+    assert torch.equal(got, want)
