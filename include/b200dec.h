@@ -267,6 +267,52 @@ int b200dec_add_adapters(const b200dec_adapters* adapters, const void* x, int64_
                          int64_t out_stride, const int32_t* order, const int32_t* tiles, int32_t max_tiles, int32_t tile_rows, int32_t num_rows,
                          void* stream);
 
+/* ---- what requests ask of their next token.  Every array has one element per entry where nothing else is said; NULL: none of that for any entry.
+ * history int32 [num_histories, capacity]: tokens of a request, its prompt and then its output.  slots: the entry's row of it (NULL: entry e has
+ * row e), -1: the entry is passed over.  lengths: tokens in the row; prompts: how many of them are the prompt (NULL: all).
+ * Adjusted logit of token v, 32-bit: l = l > 0 ? l / repetition : l * repetition if v is in the history; l -= frequency n + presence if it is n > 0
+ * times in the output; l += bias[i] for every bias_ids[e, i] = v ([entries, num_bias], -1: unused), in order; l = -inf unless bit v of mask
+ * mask_rows[e] is set (masks [num_masks, mask_words], bit v % 32 of word v / 32; -1: everything is allowed).
+ * Tokens, slots, lengths and mask rows out of range are left out (entries with such a slot passed over) and set B200KV_S_BAD_POSITION. */
+typedef struct b200dec_rules {
+  int32_t* history;
+  const int32_t* slots;
+  const int32_t* lengths;
+  const int32_t* prompts;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids;
+  const float* bias;
+  const uint32_t* masks;
+  const int32_t* mask_rows;
+  int32_t capacity, num_histories, num_bias, num_masks, mask_words;
+} b200dec_rules;
+
+/* out[e] = adjusted logits (logits of element size elem, row strides in elements).  out may be logits itself (elem 4, the same stride).  Rows of
+ * entries that are passed over are left as they are. */
+int b200dec_adjust_logits(const void* logits, int64_t stride, int32_t elem, const b200dec_rules* rules, float* out, int64_t out_stride,
+                          int32_t entries, int32_t vocab, int32_t* status, void* stream);
+
+/* How the next token is drawn from adjusted logits: z = (largest - l) / temperature, w = exp(-z), tokens ordered by l, equal ones by index.  Kept are the
+ * first top_k (0: all), of these the shortest run with top_p of their weight (1: all), of these the ones with w >= min_p (0: all, at most 1); the
+ * largest always.  The token is the first by index at which the kept weights so far exceed uniform (in [0, 1)) times their sum.  temperature 0:
+ * the largest logit, the first of equals.  NaN logits count as -inf.  Cuts count weights in steps of 2^-32 of the largest, and one among
+ * tokens with z >= 31.98 drops all of those.  NULL: temperature 1 (uniform 0 with it) and nothing cut; temperature needs uniform. */
+typedef struct b200dec_draw {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* uniform;
+} b200dec_draw;
+
+/* tokens[e], and logprobs[e], its logarithmic probability under the softmax of all adjusted logits (temperature 1).  -1 and -inf where every token is
+ * masked or the entry is passed over.  rules may be NULL.  append: the token is put behind the entry's history if there is room (and lengths are the
+ * caller's to count on); entries then have rows of their own.  vocab up to 393216. */
+int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t elem, const b200dec_rules* rules, const b200dec_draw* draw, int32_t entries,
+                          int32_t vocab, int32_t append, int64_t* tokens, float* logprobs, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

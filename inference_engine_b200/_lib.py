@@ -80,10 +80,24 @@ class Adapters(C.Structure):
         (n, c_int32) for n in ("slots", "rank", "width", "parts", "elem")] + [("ends", c_int32 * 4)]
 
 
+class Rules(C.Structure):
+    """struct b200dec_rules"""
+
+    _fields_ = [(n, c_void_p) for n in ("history", "slots", "lengths", "prompts", "repetition", "presence", "frequency", "bias_ids", "bias",
+                                        "masks", "mask_rows")] + [
+        (n, c_int32) for n in ("capacity", "num_histories", "num_bias", "num_masks", "mask_words")]
+
+
+class Draw(C.Structure):
+    """struct b200dec_draw"""
+
+    _fields_ = [(n, c_void_p) for n in ("temperature", "top_k", "top_p", "min_p", "uniform")]
+
+
 P_CACHE, P_TABLE = C.POINTER(Cache), C.POINTER(Table)
 P_DCACHE, P_ROWS, P_OPT = C.POINTER(DecCache), C.POINTER(DecRows), C.POINTER(AttnOptions)
 P_REC, P_REC_IN, P_ENT = C.POINTER(Recurrence), C.POINTER(RecurrenceIn), C.POINTER(Entries)
-P_ADAPTERS = C.POINTER(Adapters)
+P_ADAPTERS, P_RULES, P_DRAW = C.POINTER(Adapters), C.POINTER(Rules), C.POINTER(Draw)
 
 # name -> (restype, argtypes); must list every function include/b200kv.h declares
 SIGNATURES = {
@@ -189,6 +203,9 @@ DECODER_SIGNATURES = {
     "b200dec_adapter_plan": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "b200dec_add_adapters": (c_int32, [P_ADAPTERS, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32,
                                        c_int32, c_void_p]),
+    "b200dec_adjust_logits": (c_int32, [c_void_p, c_int64, c_int32, P_RULES, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p]),
+    "b200dec_choose_tokens": (c_int32, [c_void_p, c_int64, c_int32, P_RULES, P_DRAW, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+                                        c_void_p]),
 }
 SHARED_SIGNATURES = ("b200kv_version", "b200kv_error_string", "b200kv_set_chained_launch", "b200kv_get_chained_launch",
                      "b200kv_plain_next", "b200kv_branches_begin", "b200kv_branches_next", "b200kv_branches_end", "b200kv_sample_workspace_bytes", "b200kv_sample")

@@ -758,3 +758,151 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Ada
                                          plan.tiles.data_ptr(), plan.tiles.shape[0], plan.tile_rows, N, K._stream())
     _lib.check(rc, "add_adapters")
     return out
+
+
+# ----------------------------------------------------------------------------- what requests ask of their next token
+MAX_CHOICE_VOCAB = 393216
+
+
+def _entries_of(what: str, tensors: dict) -> int | None:
+    """The common length of a record's per-entry tensors (contiguous, on one device); None if it has none."""
+    n = None
+    for name, (t, dtype) in tensors.items():
+        if t is None:
+            continue
+        if t.dtype != dtype or t.dim() < 1 or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} is a contiguous tensor of {dtype} with an element or a row per entry, not {t.dtype} {tuple(t.shape)}")
+        if n is not None and t.shape[0] != n:
+            raise ValueError(f"{what}: {name} has {t.shape[0]} entries, others {n}")
+        n = t.shape[0]
+    return n
+
+
+@dataclass(frozen=True, eq=False)
+class Rules:
+    """Penalties for repeated tokens, biases and grammar masks of a step's entries (include/b200dec.h, b200dec_rules).  Per entry: slots, its row of the
+    history (-1: passed over), lengths, tokens there, and prompts, how many of them are the prompt (int32); repetition (1: none), presence,
+    frequency (fp32); bias_ids int32 and bias fp32 [entries, n] (id -1: unused); mask_rows int32, its row of masks, -1: none."""
+
+    history: torch.Tensor | None = None  # int32 [requests, capacity]
+    slots: torch.Tensor | None = None
+    lengths: torch.Tensor | None = None
+    prompts: torch.Tensor | None = None
+    repetition: torch.Tensor | None = None
+    presence: torch.Tensor | None = None
+    frequency: torch.Tensor | None = None
+    bias_ids: torch.Tensor | None = None
+    bias: torch.Tensor | None = None
+    masks: torch.Tensor | None = None  # int32 [masks, words of 32 tokens]
+    mask_rows: torch.Tensor | None = None
+
+    def __post_init__(self):
+        i, f = torch.int32, torch.float32
+        per_entry = {"slots": (self.slots, i), "lengths": (self.lengths, i), "prompts": (self.prompts, i), "repetition": (self.repetition, f),
+                     "presence": (self.presence, f), "frequency": (self.frequency, f), "bias_ids": (self.bias_ids, i), "bias": (self.bias, f),
+                     "mask_rows": (self.mask_rows, i)}
+        n = _entries_of("rules", per_entry)
+        for name, (t, _) in per_entry.items():
+            if t is not None and t.dim() != (2 if name.startswith("bias") else 1):
+                raise ValueError(f"rules: {name} {tuple(t.shape)} has the wrong number of dimensions")
+        for name in ("history", "masks"):
+            t = getattr(self, name)
+            if t is not None and (t.dtype != i or t.dim() != 2 or not t.is_contiguous()):
+                raise ValueError(f"rules: {name} is a contiguous int32 matrix")
+        if (self.history is None) != (self.lengths is None) or (self.history is None and self.prompts is not None):
+            raise ValueError("rules: a history, lengths and prompts belong together")
+        if self.history is None and any(t is not None for t in (self.repetition, self.presence, self.frequency)):
+            raise ValueError("rules: penalties need a history")
+        if (self.bias is None) != (self.bias_ids is None) or (self.bias is not None and self.bias.shape != self.bias_ids.shape):
+            raise ValueError("rules: as many biases as tokens for them")
+        if (self.masks is None) != (self.mask_rows is None):
+            raise ValueError("rules: masks and the entries' rows of them belong together")
+        tensors = [t for t in vars(self).values() if t is not None]
+        if len({t.device for t in tensors}) > 1:
+            raise ValueError("rules: tensors on several devices")
+        h, m = self.history, self.masks
+        object.__setattr__(self, "entries", n)
+        object.__setattr__(self, "device", tensors[0].device if tensors else None)
+        object.__setattr__(self, "struct", _lib.Rules(
+            _ptr(h), _ptr(self.slots), _ptr(self.lengths), _ptr(self.prompts), _ptr(self.repetition), _ptr(self.presence), _ptr(self.frequency),
+            _ptr(self.bias_ids), _ptr(self.bias), _ptr(m), _ptr(self.mask_rows), 0 if h is None else h.shape[1], 0 if h is None else h.shape[0],
+            0 if self.bias is None else self.bias.shape[1], 0 if m is None else m.shape[0], 0 if m is None else m.shape[1]))
+
+
+@dataclass(frozen=True, eq=False)
+class Draw:
+    """How a step's entries draw their tokens (include/b200dec.h, b200dec_draw), a number per entry: temperature (0: the largest logit), uniform
+    in [0, 1), top_k (int32, 0: all), top_p (1: all), min_p (0: all; a token's weight beside the most likely one's)."""
+
+    temperature: torch.Tensor
+    uniform: torch.Tensor
+    top_k: torch.Tensor | None = None
+    top_p: torch.Tensor | None = None
+    min_p: torch.Tensor | None = None
+
+    def __post_init__(self):
+        i, f = torch.int32, torch.float32
+        n = _entries_of("draw", {"temperature": (self.temperature, f), "uniform": (self.uniform, f), "top_k": (self.top_k, i),
+                                 "top_p": (self.top_p, f), "min_p": (self.min_p, f)})
+        tensors = [t for t in vars(self).values() if t is not None]
+        if any(t.dim() != 1 for t in tensors) or len({t.device for t in tensors}) > 1:
+            raise ValueError("draw: one number per entry, all on one device")
+        object.__setattr__(self, "entries", n)
+        object.__setattr__(self, "struct", _lib.Draw(*(_ptr(t) for t in (self.temperature, self.top_k, self.top_p, self.min_p, self.uniform))))
+
+
+def _check_logits(what: str, logits: torch.Tensor, rules: Rules | None) -> int:
+    """The row stride of a step's logits."""
+    K._require_cuda(logits)
+    _here(logits)
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or (logits.shape[1] > 1 and logits.stride(1) != 1) or not logits.shape[1]:
+        raise ValueError(f"{what}: bf16 or fp32 logits [entries, vocab] with a row's elements side by side are wanted")
+    E, V = logits.shape
+    if rules is not None:
+        if rules.entries is not None and rules.entries != E:
+            raise ValueError(f"{what}: rules for {rules.entries} entries and logits of {E}")
+        if rules.device is not None and rules.device != logits.device:
+            raise ValueError(f"{what}: rules on {rules.device}, logits on {logits.device}")
+        if rules.history is not None and rules.slots is None and rules.history.shape[0] < E:
+            raise ValueError(f"{what}: {rules.history.shape[0]} histories for {E} entries")
+        if rules.masks is not None and rules.masks.shape[1] < (V + 31) // 32:
+            raise ValueError(f"{what}: masks of {rules.masks.shape[1]} words for {V} tokens")
+    return logits.stride(0) if E > 1 else _round8(V)  # (a single row's stride may be anything)
+
+
+@K._ranged
+def adjust_logits(logits: torch.Tensor, rules: Rules, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Logits [entries, vocab] under each entry's rules, fp32.  `out`: where they go, fp32 logits themselves perhaps; rows of entries that are passed
+    over are left there as they are (uninitialised without it)."""
+    stride = _check_logits("adjust_logits", logits, rules)
+    E, V = logits.shape
+    if out is None:
+        out = torch.empty(E, V, dtype=torch.float32, device=logits.device)
+    elif out.dtype != torch.float32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or out.device != logits.device:
+        raise ValueError("adjust_logits: fp32 rows of the logits' shape are wanted")
+    rc = _lib_dec().b200dec_adjust_logits(logits.data_ptr(), stride, logits.element_size(), ctypes.byref(rules.struct), out.data_ptr(),
+                                          out.stride(0) if E > 1 else _round8(V), E, V, K.status_word(logits.device).data_ptr(), K._stream())
+    _lib.check(rc, "adjust_logits")
+    return out
+
+
+@K._ranged
+def choose_tokens(logits: torch.Tensor, draw: Draw, rules: Rules | None = None, append: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Every entry's next token under its rules and its way of drawing: (int64 [entries], its log-probability under the softmax of the adjusted
+    logits, fp32 [entries]); (-1, -inf) where nothing is allowed or the entry is passed over.  append: the token goes behind the entry's
+    history where there is room."""
+    stride = _check_logits("choose_tokens", logits, rules)
+    E, V = logits.shape
+    if draw.entries != E or draw.uniform.device != logits.device:
+        raise ValueError(f"choose_tokens: a draw for {draw.entries} entries on {draw.uniform.device}, logits of {E} on {logits.device}")
+    if V > MAX_CHOICE_VOCAB:
+        raise ValueError(f"choose_tokens: {V} tokens, at most {MAX_CHOICE_VOCAB}")
+    if append and (rules is None or rules.history is None):
+        raise ValueError("choose_tokens: nowhere to append to")
+    tokens = torch.empty(E, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(E, dtype=torch.float32, device=logits.device)
+    rc = _lib_dec().b200dec_choose_tokens(logits.data_ptr(), stride, logits.element_size(), None if rules is None else ctypes.byref(rules.struct),
+                                          ctypes.byref(draw.struct), E, V, int(append), tokens.data_ptr(), logprobs.data_ptr(),
+                                          K.status_word(logits.device).data_ptr(), K._stream())
+    _lib.check(rc, "choose_tokens")
+    return tokens, logprobs
