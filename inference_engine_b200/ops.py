@@ -699,15 +699,15 @@ def make_adapters(slots: int, width: int, parts, rank: int, dtype, device) -> Ad
 class AdapterPlan:
     """A step's rows sorted by adapter (plan_adapters), for all the projections of the step."""
 
-    order: torch.Tensor  # int32 [rows]
-    tiles: torch.Tensor  # int32 [max_tiles, 4]
+    order: torch.Tensor  # int32 [tiles, tile_rows]: rows of each tile, -1 behind them
+    tiles: torch.Tensor  # int32 [tiles, 4]: adapter and number of rows
     slots: int
-    tile_rows: int
+    rows: int
 
 
 def adapter_tile_rows(num_rows: int) -> int:
-    """Rows of a tile: 16 for decoding rows, 128 where rows of one adapter come in portions."""
-    return 16 if num_rows <= 128 else 128
+    """Rows of a tile: 16 for decoding rows, 64 where rows of one adapter come in portions."""
+    return 16 if num_rows <= 128 else 64
 
 
 def _here(t: torch.Tensor) -> None:
@@ -728,12 +728,12 @@ def plan_adapters(ids: torch.Tensor, slots: int, tile_rows: int | None = None) -
     N = ids.shape[0]
     rows = adapter_tile_rows(N) if tile_rows is None else tile_rows
     most = N // rows + min(N, slots + 1)
-    buf = torch.empty(4 * most + N, dtype=torch.int32, device=ids.device)
-    tiles, order = buf[: 4 * most].view(most, 4), buf[4 * most :]
+    tiles = torch.empty(most, 4, dtype=torch.int32, device=ids.device)
+    order = torch.empty(most, rows, dtype=torch.int32, device=ids.device)
     rc = _lib_dec().b200dec_adapter_plan(ids.data_ptr(), N, slots, rows, order.data_ptr(), tiles.data_ptr(), most,
                                          K.status_word(ids.device).data_ptr(), K._stream())
     _lib.check(rc, "plan_adapters")
-    return AdapterPlan(order, tiles, slots, rows)
+    return AdapterPlan(order, tiles, slots, N)
 
 
 @K._ranged
@@ -743,7 +743,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Ada
     K._require_cuda(y, x, adapters.up, plan.order)
     _here(y)
     out = y if out is None else out
-    N = plan.order.shape[0]
+    N = plan.rows
     if y.dtype != adapters.up.dtype or x.dtype != y.dtype or out.dtype != y.dtype:
         raise ValueError(f"add_adapters: rows of {x.dtype}, {y.dtype} and {out.dtype} beside adapters of {adapters.up.dtype}")
     if tuple(x.shape) != (N, adapters.down.shape[2]) or tuple(y.shape) != (N, adapters.up.shape[1]) or out.shape != y.shape:
@@ -755,7 +755,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Ada
     # (a single row's stride may be anything)
     xs, ys, os = (t.stride(0) if N > 1 else _round8(t.shape[1]) for t in (x, y, out))
     rc = _lib_dec().b200dec_add_adapters(ctypes.byref(adapters.struct), x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, plan.order.data_ptr(),
-                                         plan.tiles.data_ptr(), plan.tiles.shape[0], plan.tile_rows, N, K._stream())
+                                         plan.tiles.data_ptr(), *plan.order.shape, N, K._stream())
     _lib.check(rc, "add_adapters")
     return out
 

@@ -70,7 +70,7 @@ SHAPES = [
 
 
 @pytest.mark.parametrize("rows,width,parts,rank,slots,dtype", SHAPES)
-@pytest.mark.parametrize("tile_rows", [None, 16, 128])
+@pytest.mark.parametrize("tile_rows", [None, 16, 64])
 def test_against_the_formula(ops, rows, width, parts, rank, slots, dtype, tile_rows):
     ad, ids, x, y = make(ops, rows, width, parts, rank, slots, dtype)
     plan = ops.plan_adapters(ids, slots, tile_rows)
@@ -111,13 +111,10 @@ def test_plan_covers_every_row_once(ops, rows, slots):
     g = torch.Generator().manual_seed(rows)
     ids = torch.randint(-1, slots, (rows,), generator=g).to("cuda", torch.int32)
     plan = ops.plan_adapters(ids, slots)
-    order, ids = plan.order.tolist(), ids.tolist()
-    assert sorted(order) == list(range(rows))
-    covered = []
-    for slot, first, count, _ in plan.tiles.tolist():
-        assert 0 <= count <= plan.tile_rows
-        covered += range(first, first + count)
-        assert all(ids[order[i]] == slot for i in range(first, first + count))
+    ids, covered = ids.tolist(), []
+    for order, (slot, count, _, _) in zip(plan.order.tolist(), plan.tiles.tolist()):
+        assert all(ids[r] == slot for r in order[:count]) and all(r == -1 for r in order[count:])
+        covered += order[:count]
     assert sorted(covered) == list(range(rows))
 
 
