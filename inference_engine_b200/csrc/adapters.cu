@@ -217,7 +217,7 @@ __device__ __forceinline__ float4 ad_total(uint32_t at, float scale) {
 // `up` that are in shared memory or on their way.
 // The order of a product's channels is free, so that a lane loads whole 16 bytes: lane t of a row's four has channels 8t .. 8t + 7 of 32.
 template <int kRows, int kNT, int kKB, int kC, int kStages>
-__global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 2) adapter_kernel(const __grid_constant__ AdArgs a) {
+__global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : (kRows == 16 ? 3 : 2)) adapter_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ __align__(16) uint8_t ad_smem[];
   constexpr int kGroups = kRows == 16 ? 8 : 4;     // column groups of a chunk
   constexpr int kM = kRows == 16 ? 1 : 2;          // blocks of sixteen rows that a warp adds up in the second product
@@ -241,22 +241,30 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 2) adapter_kernel(co
   float* part = reinterpret_cast<float*>(ad_smem);
   const int g0 = ad_first_group<kC>(a, rank), g1 = ad_first_group<kC>(a, rank + 1);
 
-  // Columns of group g + i into place i of a stage.  Column 8 (n / 2) + 2 j + n % 2 of a group lies at 8 j + n: see below.
-  auto fetch_up = [&](int chunk) {
-    const int g = g0 + chunk * kGroups;
-    if (g < g1) {
-      const uint32_t stage = smem + a.off_u + (chunk % kStages) * (kGroups * 32 * a.u_row);
-      const int vecs = a.rank >> 3, n = min(kGroups, g1 - g) * 32 * vecs;
-      for (int i = tid; i < n; i += kAdThreads) {
-        const int at = i / vecs, v = i - at * vecs, c = at & 31;
-        const AdGroup gr = ad_group(a, g + (at >> 5));
-        const int col = gr.col + c;
-        const int place = (at & ~31) + 8 * ((c >> 1) & 3) + 2 * (c >> 3) + (c & 1);
-        const bool in = col < gr.end;
-        ad_copy16(stage + place * a.u_row + v * 16, up + (in ? (long long)col * a.rank + v * 8 : 0), in ? 16 : 0);
-      }
+  // This warp's group of each chunk, and where its columns of `up` go.  Column 8 (n / 2) + 2 j + n % 2 of a group lies at 8 j + n: see below.  In tiles of 64
+  // rows two warps share a group, and each brings half of it.
+  const int mine = kRows == 16 ? warp : warp & 3, rows_at = kRows == 16 ? 0 : 32 * (warp >> 2);
+  const uint32_t u_at = a.off_u + mine * 32 * a.u_row;
+  const int u_stage = kGroups * 32 * a.u_row, vecs = a.rank >> 3;
+  const unsigned by_vecs = (65536u + vecs - 1) / vecs;  // i / vecs of i < 512 by a product
+  auto fetch_up = [&](const AdGroup& gr, int stage) {
+    const uint16_t* src = up + (long long)gr.col * a.rank;
+    const uint32_t dst = smem + u_at + stage * u_stage;
+    const int n = gr.end ? 32 * vecs : 0;  // (a stage behind the last group may have no place)
+    for (int i = kRows == 16 ? lane : lane + (warp & 4) * 8; i < n; i += kRows == 16 ? 32 : 64) {
+      const int c = (int)((unsigned)i * by_vecs >> 16), v = i - c * vecs;
+      const int place = 8 * ((c >> 1) & 3) + 2 * (c >> 3) + (c & 1);
+      const bool in = gr.col + c < gr.end;
+      ad_copy16(dst + place * a.u_row + v * 16, in ? src + i * 8 : up, in ? 16 : 0);
     }
     ad_commit();
+  };
+  AdGroup ring[kStages];  // the groups in the stages
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) ring[i] = g0 + mine + i * kGroups < g1 ? ad_group(a, g0 + mine + i * kGroups) : AdGroup{0, 0, 0};
+  auto fetch_first = [&]() {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) fetch_up(ring[i], i);
   };
 
   float acc[kNT][4];
@@ -283,8 +291,7 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 2) adapter_kernel(co
       }
       const uint4 u0 = load_x(x0, row0, k), u1 = load_x(x1, row1, k);
       if (first) {
-#pragma unroll
-        for (int i = 0; i < kStages; ++i) fetch_up(i);
+        fetch_first();
         first = false;
       }
 #pragma unroll
@@ -354,8 +361,7 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 2) adapter_kernel(co
     }
     ad_wait<0>();
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) fetch_up(i);
+    fetch_first();
     // one half's values, then both
 #pragma unroll
     for (int h = 1; h >= 0; --h) {
@@ -379,22 +385,19 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 2) adapter_kernel(co
   // ---- the second product: 32 columns of a warp at a time, as four tiles of eight.  Tile j's column n is column 8 (n / 2) + 2 j + n % 2 of the 32, so that a
   // lane has eight columns side by side.  Lane t of a row's four has inner values 4t .. 4t + 3 of sixteen; where eight are left over, the two
   // terms of 2t and 2t + 1 share one step.
-  const int mine = kRows == 16 ? warp : warp & 3, rows_at = kRows == 16 ? 0 : 32 * (warp >> 2);  // this warp's group of a chunk, its rows
   int rows[2 * kM];
 #pragma unroll
   for (int i = 0; i < 2 * kM; ++i) rows[i] = order[rows_at + gid + 8 * i];
   const uint16_t* y = (const uint16_t*)a.y;
   uint16_t* out = (uint16_t*)a.out;
   uint4 yv[2 * kM];
-  AdGroup gr = {0, 0, 0};
-  auto load_y = [&](int g) {
-    gr = g < g1 ? ad_group(a, g) : AdGroup{0, 0, 0};
+  auto load_y = [&](const AdGroup& gr) {
     const int col = gr.col + 8 * t;
+    const bool whole = a.vec && gr.end - col >= 8;
 #pragma unroll
-    for (int i = 0; i < 2 * kM; ++i)
-      yv[i] = rows[i] >= 0 && a.vec && gr.end - col >= 8 ? *reinterpret_cast<const uint4*>(y + (long long)rows[i] * a.y_stride + col) : zero4;
+    for (int i = 0; i < 2 * kM; ++i) yv[i] = rows[i] >= 0 && whole ? *reinterpret_cast<const uint4*>(y + (long long)rows[i] * a.y_stride + col) : zero4;
   };
-  load_y(g0 + mine);  // (on its way while the inner values are exchanged)
+  load_y(ring[0]);  // (on its way while the inner values are exchanged)
 
   const int p0 = g0 < g1 ? ad_group(a, g0).part : 0, width_t = g0 < g1 ? (ad_group(a, g1 - 1).part - p0 + 1) * a.rank : 0;
   const float scale = a.scale[slot];
@@ -435,16 +438,24 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 2) adapter_kernel(co
 
   const int full = a.rank >> 4;
   const bool tail = a.rank & 8;
-  for (int chunk = 0, g = g0 + mine; g0 + chunk * kGroups < g1; ++chunk, g += kGroups) {
+  if (kRows == 16) __syncthreads();  // the finished inner values
+  auto pair_sync = [&]() {  // of the warps that share a group
+    if (kRows == 16) __syncwarp();
+    else asm volatile("bar.sync %0, 64;" ::"r"(mine + 1) : "memory");
+  };
+  for (int g = g0 + mine, stage = 0; g < g1; g += kGroups, stage = stage + 1 == kStages ? 0 : stage + 1) {
     ad_wait<kStages - 1>();
-    __syncthreads();
-    if (g < g1) {
-      const AdGroup now = gr;
+    pair_sync();
+    {
+      const AdGroup now = ring[0];
+#pragma unroll
+      for (int i = 0; i + 1 < kStages; ++i) ring[i] = ring[i + 1];
+      ring[kStages - 1] = g + kStages * kGroups < g1 ? ad_group(a, g + kStages * kGroups) : AdGroup{0, 0, 0};
       uint4 v[2 * kM];
 #pragma unroll
       for (int i = 0; i < 2 * kM; ++i) v[i] = yv[i];
-      load_y(g + kGroups);
-      const uint8_t* us = ad_smem + a.off_u + ((chunk % kStages) * kGroups * 32 + mine * 32 + gid) * a.u_row;
+      load_y(ring[0]);
+      const uint8_t* us = ad_smem + u_at + stage * u_stage + gid * a.u_row;
       const uint8_t* ts = ad_smem + a.off_t + (now.part - p0) * a.rank * 2;
       float d[kM][4][4];
 #pragma unroll
@@ -507,8 +518,8 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 2) adapter_kernel(co
         }
       }
     }
-    __syncthreads();
-    fetch_up(chunk + kStages);
+    pair_sync();
+    fetch_up(ring[kStages - 1], stage);
   }
   if constexpr (kRows == 16) ad_cluster_wait();
 }
@@ -728,9 +739,9 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, i
   }
   const int kb = (a.rank + 15) / 16;
   if (tile_rows == 16 || a.inner > kAdMaxInner) {
-    if (kb <= 1) return ad_run<16, 8, 1, 8, 4>(a, fine, s);
-    if (kb <= 2) return ad_run<16, 8, 2, 8, 4>(a, fine, s);
-    if (kb <= 4) return ad_run<16, 8, 4, 8, 2>(a, fine, s);
+    if (kb <= 1) return ad_run<16, 4, 1, 8, 4>(a, fine, s);
+    if (kb <= 2) return ad_run<16, 4, 2, 8, 4>(a, fine, s);
+    if (kb <= 4) return ad_run<16, 4, 4, 8, 2>(a, fine, s);
     return ad_run<16, 8, 8, 8, 2>(a, fine, s);
   }
   if (kb <= 1) return ad_run<64, 8, 1, 8, 4>(a, max_tiles, s);
