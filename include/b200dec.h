@@ -257,7 +257,7 @@ typedef struct b200dec_adapters {
 /* A step's rows sorted by adapter, for every projection of the step.  ids int32 [num_rows]: the adapter of each row, -1: none (any other id
  * outside [0, slots) counts as that and sets B200KV_S_BAD_POSITION).  order int32 [max_tiles, tile_rows] and tiles int32 [max_tiles, 4] (16-byte aligned)
  * are written: a tile's rows, -1 behind them, and its adapter (or -1) and number of rows.  max_tiles >= num_rows / tile_rows + min(num_rows,
- * slots + 1).  tile_rows: 16 or 64. */
+ * slots + 1).  tile_rows: 16 or 128. */
 int b200dec_adapter_plan(const int32_t* ids, int32_t num_rows, int32_t slots, int32_t tile_rows, int32_t* order, int32_t* tiles,
                          int32_t max_tiles, int32_t* status, void* stream);
 
@@ -266,7 +266,7 @@ int b200dec_adapter_plan(const int32_t* ids, int32_t num_rows, int32_t slots, in
  * overlaps neither y nor x.  32-bit sums, rounded once. */
 int b200dec_add_adapters(const b200dec_adapters* adapters, const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out,
                          int64_t out_stride, const int32_t* order, const int32_t* tiles, int32_t max_tiles, int32_t tile_rows, int32_t num_rows,
-                         void* stream);
+                         int32_t* status, void* stream);
 
 /* ---- what requests ask of their next token.  Every array has one element per entry where nothing else is said; NULL: none of that for any entry.
  * history int32 [num_histories, capacity]: tokens of a request, its prompt and then its output.  slots: the entry's row of it (NULL: entry e has

@@ -3,13 +3,14 @@
 // A packed projection has a `down` of its own for each part; a column of `up` meets the inner values of its part.
 //
 // The plan (one block, once per step) sorts the rows by adapter into tiles of at most `tile_rows` rows of one adapter.  A product is then
-// one launch: a cluster of blocks takes a tile.  Its blocks share the input channels, so that a tile's `down` is fetched by many
+// one launch: a cluster of blocks takes a tile and one part.  Its blocks share the input channels, so that a tile's `down` is fetched by many
 // multiprocessors at once; their partial inner values are summed through distributed shared memory, in a fixed order; then the blocks
-// share the output columns.  `up` comes into shared memory meanwhile, as far as there is room.
+// share the part's columns.  Tiles of 16 rows (decoding: weights are what is read) go through mma.sync from registers; tiles of 128 (portions: x, y
+// and the result are) through tcgen05.
 //
 // Precision: bf16 operands, 32-bit sums.  The inner values are scaled in 32 bits and enter the second product as two bf16 terms (16 bits of
 // mantissa): rounded to one they would cost the sum as much as its own rounding does.
-#include "dec_common.cuh"
+#include "dec_tma.cuh"
 
 namespace b200kv {
 
@@ -19,8 +20,13 @@ constexpr int kAdMaxParts = 4;
 constexpr int kAdMaxSlots = 4096;
 constexpr int kAdPlanThreads = 1024;
 constexpr int kAdSimtChannels = 512;  // input channels that the CUDA cores' form stages at a time
-constexpr int kAdMaxInner = 192;      // inner values of a row in tiles of 64 rows
-constexpr int kAdChannels = 64;       // input channels of a stage there
+constexpr int kAdSimtCluster = 8;
+constexpr int kAdTcCluster = 8;
+constexpr int kAdTcStages = 3;        // of 64 input channels
+constexpr int kAdTcCols = 64;         // output columns of a product of the tensor core
+constexpr int kAdTcUps = 3;           // their `up`s that are in shared memory or on their way
+constexpr uint32_t kAdTcTmem = 128;   // columns of tensor memory: the first product's sums, and then two of the second's
+static_assert(2 * kAdTcCols <= kAdTcTmem, "two accumulators");
 
 struct AdArgs {
   const void *down, *up;
@@ -33,13 +39,13 @@ struct AdArgs {
   int tile_rows;  // of the plan
   int rank, width, parts;
   int ends[kAdMaxParts];
-  int groups;           // of 32 output columns, none across parts
-  int inner;            // parts * rank
-  int inner_row;        // floats between rows of partial inner values
-  int t_row;            // bytes between rows of finished ones
-  int u_row;            // bytes between columns of `up` in shared memory
-  int vec;              // y and out rows can be read and written in 16 bytes
+  int inner_row;          // floats between rows of partial inner values
+  int t_row;              // bytes between rows of finished ones
+  int u_row;              // bytes between columns of `up` in shared memory
+  int ring;               // groups of columns on their way that a warp has room for
+  int vec;                // y and out rows can be read and written in 16 bytes
   uint32_t off_t, off_u;  // shared memory: the finished inner values, `up`
+  int32_t* status;
 };
 
 // ---------------------------------------------------------------------------------------------------------------- the plan
@@ -139,8 +145,8 @@ __device__ __forceinline__ float4 ad_ld_remote4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void ad_st_remote2(uint32_t addr, uint32_t a, uint32_t b) {
-  asm volatile("st.shared::cluster.v2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+__device__ __forceinline__ void ad_st_remote2(uint32_t addr, const uint2& v) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
 }
 __device__ __forceinline__ void ad_copy16(uint32_t dst, const void* src, int bytes) {  // zeros behind the first `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -149,36 +155,26 @@ __device__ __forceinline__ void ad_commit() { asm volatile("cp.async.commit_grou
 template <int kLeft>
 __device__ __forceinline__ void ad_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(kLeft) : "memory"); }
 
-// Column group g (of 32): its part, first column and the end of its part's columns.
-struct AdGroup { int part, col, end; };
-__device__ __forceinline__ AdGroup ad_group(const AdArgs& a, int g) {
-  int begin = 0;
-#pragma unroll
-  for (int p = 0; p < kAdMaxParts; ++p) {
-    if (p < a.parts) {
-      const int n = (a.ends[p] - begin + 31) >> 5;
-      if (g < n) return {p, begin + 32 * g, a.ends[p]};
-      g -= n;
-      begin = a.ends[p];
-    }
-  }
-  return {0, 0, 0};
+// The rows [first, first + n) of a cluster's tile and the columns of its part.
+struct AdJob {
+  int slot, count, part, begin, end;
+  const int32_t* order;
+};
+template <int kRows, int kC>
+__device__ __forceinline__ AdJob ad_job(const AdArgs& a) {
+  const int subs = a.tile_rows / kRows, cl = blockIdx.x / kC, at = cl / a.parts, part = cl - at * a.parts;
+  const int4 tile = a.tiles[at / subs];
+  return {tile.x, min(tile.y - (at % subs) * kRows, kRows), part, part ? a.ends[part - 1] : 0, a.ends[part], a.order + (long long)at * kRows};
 }
-template <int kC>
-__device__ __forceinline__ int ad_first_group(const AdArgs& a, int rank) { return (int)((unsigned)a.groups * (unsigned)rank / kC); }
 
-// Rows of the tile without an adapter: copied where the result has a place of its own.
-template <typename T, int kC>
-__device__ __forceinline__ void ad_copy_rows(const AdArgs& a, const int32_t* order, int count, int rank) {
+// Rows without an adapter: copied where the result has a place of its own.
+template <typename T>
+__device__ __forceinline__ void ad_copy_rows(const AdArgs& a, const AdJob& job, int rank, int cluster) {
   if (a.out == a.y) return;
-  const int lo = ad_first_group<kC>(a, rank), hi = ad_first_group<kC>(a, rank + 1);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int g = lo + warp; g < hi; g += kAdWarps) {
-    const AdGroup gr = ad_group(a, g);
-    if (gr.col + lane >= gr.end) continue;
-    for (int i = 0; i < count; ++i) {
-      const long long r = order[i];
-      ((T*)a.out)[r * a.out_stride + gr.col + lane] = ((const T*)a.y)[r * a.y_stride + gr.col + lane];
+  for (int col = job.begin + rank * kAdThreads + threadIdx.x; col < job.end; col += cluster * kAdThreads) {
+    for (int i = 0; i < job.count; ++i) {
+      const long long r = job.order[i];
+      ((T*)a.out)[r * a.out_stride + col] = ((const T*)a.y)[r * a.y_stride + col];
     }
   }
 }
@@ -210,61 +206,68 @@ __device__ __forceinline__ float4 ad_total(uint32_t at, float scale) {
   return s;
 }
 
-// ---------------------------------------------------------------------------------------------------------------- tensor cores
-// kRows 16: the warps share the block's channels and, where there are more than 64 inner values, those too; both operands go straight
-// from memory to registers.  kRows 64: a warp takes sixteen rows and half the channels, `down` is staged in shared memory for all of them.
-// kNT: blocks of eight inner values of a warp.  kKB: blocks of sixteen inner values of a part.  kC: blocks of a cluster.  kStages: chunks of columns of
-// `up` that are in shared memory or on their way.
-// The order of a product's channels is free, so that a lane loads whole 16 bytes: lane t of a row's four has channels 8t .. 8t + 7 of 32.
-template <int kRows, int kNT, int kKB, int kC, int kStages>
-__global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : (kRows == 16 ? 3 : 2)) adapter_kernel(const __grid_constant__ AdArgs a) {
+// What a lane adds to its eight columns of a row, f, which start `left` columns in front of the part's end; v: y where `whole`.
+__device__ __forceinline__ void ad_store(const AdArgs& a, int row, int col, int left, bool whole, const uint4& v, const float (&f)[8]) {
+  uint16_t* to = (uint16_t*)a.out + (long long)row * a.out_stride + col;
+  if (whole) {
+    float w[8];
+    unpack8(v, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] += f[e];
+    st_vec(to, w);
+  } else {
+    const uint16_t* from = (const uint16_t*)a.y + (long long)row * a.y_stride + col;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) st_elem(to + e, ld_elem(from + e) + f[e]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- few rows: mma.sync
+// The warps share the block's channels and, where there are more than 64 inner values, those too; both operands go straight from memory to
+// registers.  The order of a product's channels is free, so that a lane loads whole 16 bytes: lane t of a row's four has channels 8t ..
+// 8t + 7 of 32.  Second product: a warp takes groups of 32 columns, whose `up` and y come through a ring of its own.
+// kNT: blocks of eight inner values of a warp.  kKB: blocks of sixteen inner values.  kC: blocks of a cluster.  kStages: groups on their way.
+template <int kNT, int kKB, int kC, int kStages>
+__global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ __align__(16) uint8_t ad_smem[];
-  constexpr int kGroups = kRows == 16 ? 8 : 4;     // column groups of a chunk
-  constexpr int kM = kRows == 16 ? 1 : 2;          // blocks of sixteen rows that a warp adds up in the second product
   const uint32_t smem = (uint32_t)__cvta_generic_to_shared(ad_smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
-  const int rank = (int)ad_cluster_rank(), cl = blockIdx.x / kC;
+  const int rank = (int)ad_cluster_rank();
   pdl_enter();
   pdl_wait();
-  const int subs = a.tile_rows / kRows;
-  const int4 tile = a.tiles[cl / subs];
-  const int32_t* order = a.order + (long long)cl * kRows;
-  const int slot = tile.x, count = min(tile.y - (cl % subs) * kRows, kRows);
-  const int m0 = kRows == 16 ? 0 : 16 * (warp & 3);
-  const int row0 = order[m0 + gid], row1 = order[m0 + gid + 8];
-  if (count <= 0) return;  // (with the whole cluster)
-  if (slot < 0) return ad_copy_rows<uint16_t, kC>(a, order, count, rank);
-  const uint16_t* down = (const uint16_t*)a.down + (long long)slot * a.inner * a.width;
-  const uint16_t* up = (const uint16_t*)a.up + (long long)slot * a.ends[a.parts - 1] * a.rank;
+  const AdJob job = ad_job<16, kC>(a);
+  const int row0 = job.order[gid], row1 = job.order[gid + 8];
+  if (job.count <= 0) return;  // (with the whole cluster)
+  if (job.slot < 0) return ad_copy_rows<uint16_t>(a, job, rank, kC);
+  const uint16_t* down = (const uint16_t*)a.down + ((long long)job.slot * a.parts + job.part) * a.rank * a.width;
+  const uint16_t* up = (const uint16_t*)a.up + (long long)job.slot * a.ends[a.parts - 1] * a.rank;
+  const uint16_t* y = (const uint16_t*)a.y;
   const uint4 zero4 = make_uint4(0, 0, 0, 0);
   const int chunks = (a.width + 31) >> 5;
   float* part = reinterpret_cast<float*>(ad_smem);
-  const int g0 = ad_first_group<kC>(a, rank), g1 = ad_first_group<kC>(a, rank + 1);
+  const int groups = (job.end - job.begin + 31) >> 5, g0 = groups * rank / kC, g1 = groups * (rank + 1) / kC;
 
-  // This warp's group of each chunk, and where its columns of `up` go.  Column 8 (n / 2) + 2 j + n % 2 of a group lies at 8 j + n: see below.  In tiles of 64
-  // rows two warps share a group, and each brings half of it.
-  const int mine = kRows == 16 ? warp : warp & 3, rows_at = kRows == 16 ? 0 : 32 * (warp >> 2);
-  const uint32_t u_at = a.off_u + mine * 32 * a.u_row;
-  const int u_stage = kGroups * 32 * a.u_row, vecs = a.rank >> 3;
+  // A stage: 32 columns of `up`, column 8 (n / 2) + 2 j + n % 2 at 8 j + n (see below), and what this lane needs of y.
+  const int vecs = a.rank >> 3, stage_bytes = 32 * a.u_row + 1024;
+  const uint32_t ring = a.off_u + warp * a.ring * stage_bytes;
   const unsigned by_vecs = (65536u + vecs - 1) / vecs;  // i / vecs of i < 512 by a product
-  auto fetch_up = [&](const AdGroup& gr, int stage) {
-    const uint16_t* src = up + (long long)gr.col * a.rank;
-    const uint32_t dst = smem + u_at + stage * u_stage;
-    const int n = gr.end ? 32 * vecs : 0;  // (a stage behind the last group may have no place)
-    for (int i = kRows == 16 ? lane : lane + (warp & 4) * 8; i < n; i += kRows == 16 ? 32 : 64) {
-      const int c = (int)((unsigned)i * by_vecs >> 16), v = i - c * vecs;
-      const int place = 8 * ((c >> 1) & 3) + 2 * (c >> 3) + (c & 1);
-      const bool in = gr.col + c < gr.end;
-      ad_copy16(dst + place * a.u_row + v * 16, in ? src + i * 8 : up, in ? 16 : 0);
+  auto fetch = [&](int g, int stage) {
+    if (g < g1) {
+      const int col0 = job.begin + 32 * g, left = job.end - col0;
+      const uint16_t* src = up + (long long)col0 * a.rank;
+      const uint32_t dst = smem + ring + stage * stage_bytes;
+      for (int i = lane; i < 32 * vecs; i += 32) {
+        const int c = (int)((unsigned)i * by_vecs >> 16), v = i - c * vecs;
+        const int place = 8 * ((c >> 1) & 3) + 2 * (c >> 3) + (c & 1);
+        ad_copy16(dst + place * a.u_row + v * 16, c < left ? src + i * 8 : up, c < left ? 16 : 0);
+      }
+      const bool whole = a.vec && left - 8 * t >= 8;
+      const uint32_t ydst = dst + 32 * a.u_row + lane * 16;
+      if (whole && row0 >= 0) ad_copy16(ydst, y + (long long)row0 * a.y_stride + col0 + 8 * t, 16);
+      if (whole && row1 >= 0) ad_copy16(ydst + 512, y + (long long)row1 * a.y_stride + col0 + 8 * t, 16);
     }
     ad_commit();
-  };
-  AdGroup ring[kStages];  // the groups in the stages
-#pragma unroll
-  for (int i = 0; i < kStages; ++i) ring[i] = g0 + mine + i * kGroups < g1 ? ad_group(a, g0 + mine + i * kGroups) : AdGroup{0, 0, 0};
-  auto fetch_first = [&]() {
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) fetch_up(ring[i], i);
   };
 
   float acc[kNT][4];
@@ -274,277 +277,410 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : (kRows == 16 ? 3 : 2
     for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
   const uint16_t* x0 = (const uint16_t*)a.x + (long long)max(row0, 0) * a.x_stride;
   const uint16_t* x1 = (const uint16_t*)a.x + (long long)max(row1, 0) * a.x_stride;
-  auto load_x = [&](const uint16_t* x, int row, int k) { return row >= 0 && k < a.width ? *reinterpret_cast<const uint4*>(x + k) : zero4; };
-
-  if constexpr (kRows == 16) {
-    const int wn = (a.inner + 8 * kNT - 1) / (8 * kNT);                // warps side by side over the inner values
-    const int across = wn <= 1 ? 1 : (wn <= 2 ? 2 : (wn <= 4 ? 4 : 8)), deep = kAdWarps / across;
-    const int n0 = (warp % across) * kNT * 8, d = warp / across;
-    bool first = true;
-    for (int c = rank * deep + d; c < chunks || first; c += kC * deep) {
-      const int k = 32 * c + 8 * t;  // (the width is a multiple of 8)
-      uint4 w[kNT];
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        const int j = n0 + 8 * n + gid;
-        w[n] = k < a.width && j < a.inner ? __ldg(reinterpret_cast<const uint4*>(down + (long long)j * a.width + k)) : zero4;
-      }
-      const uint4 u0 = load_x(x0, row0, k), u1 = load_x(x1, row1, k);
-      if (first) {
-        fetch_first();
-        first = false;
-      }
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        ad_mma(acc[n], u0.x, u1.x, u0.y, u1.y, w[n].x, w[n].y);
-        ad_mma(acc[n], u0.z, u1.z, u0.w, u1.w, w[n].z, w[n].w);
-      }
-    }
-    // the warps' shares of the channels, in order: [deep][16][inner_row]
-    float* mine = part + d * 16 * a.inner_row;
+  const int across = a.rank <= 8 * kNT ? 1 : 2, deep = kAdWarps / across;  // warps side by side over the inner values
+  const int n0 = (warp % across) * kNT * 8, d = warp / across;
+  bool first = true;
+  for (int c = rank * deep + d; c < chunks || first; c += kC * deep) {
+    const int k = 32 * c + 8 * t;  // (the width is a multiple of 8)
+    const bool in = k < a.width;
+    uint4 w[kNT];
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      const int j = n0 + 8 * n + 2 * t;
-      if (j < a.inner) {
-        *reinterpret_cast<float2*>(mine + gid * a.inner_row + j) = make_float2(acc[n][0], acc[n][1]);
-        *reinterpret_cast<float2*>(mine + (gid + 8) * a.inner_row + j) = make_float2(acc[n][2], acc[n][3]);
-      }
+      const int j = n0 + 8 * n + gid;
+      w[n] = in && j < a.rank ? __ldg(reinterpret_cast<const uint4*>(down + (long long)j * a.width + k)) : zero4;
     }
-    __syncthreads();
-    const int quads = a.inner >> 2;
-    for (int i = tid; i < count * quads; i += kAdThreads) {
-      const int row = i / quads, at = row * a.inner_row + (i - row * quads) * 4;
-      float4 s = *reinterpret_cast<const float4*>(part + at);
-      for (int q = 1; q < deep; ++q) {
-        const float4 v = *reinterpret_cast<const float4*>(part + q * 16 * a.inner_row + at);
-        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-      }
-      *reinterpret_cast<float4*>(part + at) = s;
-    }
-  } else {
-    // stages of 64 channels, two in shared memory; the half that a warp takes of each lies 64 bytes apart in odd rows, so that two rows are at
-    // different banks
-    const int c0 = (int)((long long)((chunks + 1) / 2) * rank / kC), c1 = (int)((long long)((chunks + 1) / 2) * (rank + 1) / kC);
-    const int half = warp >> 2, stage_bytes = a.inner * 128;
-    auto fetch_down = [&](int c) {
-      if (c < c1) {
-        const uint32_t stage = smem + (c & 1) * stage_bytes;
-        for (int i = tid; i < a.inner * 8; i += kAdThreads) {
-          const int j = i >> 3, v = i & 7, k = kAdChannels * c + 8 * v;
-          ad_copy16(stage + j * 128 + ((v ^ ((j & 1) << 2)) << 4), down + (k < a.width ? (long long)j * a.width + k : 0), k < a.width ? 16 : 0);
-        }
-      }
-      ad_commit();
-    };
-    fetch_down(c0);
-    uint4 u0 = load_x(x0, row0, kAdChannels * c0 + 32 * half + 8 * t), u1 = load_x(x1, row1, kAdChannels * c0 + 32 * half + 8 * t);
-    for (int c = c0; c < c1; ++c) {
-      fetch_down(c + 1);
-      const int k = kAdChannels * (c + 1) + 32 * half + 8 * t;
-      const uint4 v0 = c + 1 < c1 ? load_x(x0, row0, k) : zero4, v1 = c + 1 < c1 ? load_x(x1, row1, k) : zero4;
-      ad_wait<1>();
-      __syncthreads();
-      if (m0 < count) {
-        const uint8_t* stage = ad_smem + (c & 1) * stage_bytes + gid * 128 + (((half * 4 + t) ^ ((gid & 1) << 2)) << 4);
+    const uint4 u0 = in && row0 >= 0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero4;
+    const uint4 u1 = in && row1 >= 0 ? *reinterpret_cast<const uint4*>(x1 + k) : zero4;
+    if (first) {
 #pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          if (8 * n < a.inner) {
-            const uint4 w = *reinterpret_cast<const uint4*>(stage + n * 1024);
-            ad_mma(acc[n], u0.x, u1.x, u0.y, u1.y, w.x, w.y);
-            ad_mma(acc[n], u0.z, u1.z, u0.w, u1.w, w.z, w.w);
-          }
-        }
-      }
-      u0 = v0;
-      u1 = v1;
-      __syncthreads();
+      for (int i = 0; i < kStages; ++i) fetch(g0 + warp + i * kAdWarps, i);
+      first = false;
     }
-    ad_wait<0>();
-    __syncthreads();
-    fetch_first();
-    // one half's values, then both
 #pragma unroll
-    for (int h = 1; h >= 0; --h) {
-      if (half == h && m0 < count) {
-#pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          if (8 * n < a.inner) {
-            float2* p0 = reinterpret_cast<float2*>(part + (m0 + gid) * a.inner_row + 8 * n + 2 * t);
-            float2* p1 = p0 + 4 * a.inner_row;
-            const float2 q0 = h ? make_float2(0.f, 0.f) : *p0, q1 = h ? make_float2(0.f, 0.f) : *p1;
-            *p0 = make_float2(acc[n][0] + q0.x, acc[n][1] + q0.y);
-            *p1 = make_float2(acc[n][2] + q1.x, acc[n][3] + q1.y);
-          }
-        }
-      }
-      if (h) __syncthreads();
+    for (int n = 0; n < kNT; ++n) {
+      ad_mma(acc[n], u0.x, u1.x, u0.y, u1.y, w[n].x, w[n].y);
+      ad_mma(acc[n], u0.z, u1.z, u0.w, u1.w, w[n].z, w[n].w);
     }
+  }
+  // the warps' shares of the channels, in order: [deep][16][inner_row]
+  float* mine = part + d * 16 * a.inner_row;
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    const int j = n0 + 8 * n + 2 * t;
+    if (j < a.rank) {
+      *reinterpret_cast<float2*>(mine + gid * a.inner_row + j) = make_float2(acc[n][0], acc[n][1]);
+      *reinterpret_cast<float2*>(mine + (gid + 8) * a.inner_row + j) = make_float2(acc[n][2], acc[n][3]);
+    }
+  }
+  __syncthreads();
+  const int quads = a.rank >> 2;
+  for (int i = tid; i < job.count * quads; i += kAdThreads) {
+    const int row = i / quads, at = row * a.inner_row + (i - row * quads) * 4;
+    float4 s = *reinterpret_cast<const float4*>(part + at);
+    for (int q = 1; q < deep; ++q) {
+      const float4 v = *reinterpret_cast<const float4*>(part + q * 16 * a.inner_row + at);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    *reinterpret_cast<float4*>(part + at) = s;
   }
   ad_cluster_arrive();
-
-  // ---- the second product: 32 columns of a warp at a time, as four tiles of eight.  Tile j's column n is column 8 (n / 2) + 2 j + n % 2 of the 32, so that a
-  // lane has eight columns side by side.  Lane t of a row's four has inner values 4t .. 4t + 3 of sixteen; where eight are left over, the two
-  // terms of 2t and 2t + 1 share one step.
-  int rows[2 * kM];
-#pragma unroll
-  for (int i = 0; i < 2 * kM; ++i) rows[i] = order[rows_at + gid + 8 * i];
-  const uint16_t* y = (const uint16_t*)a.y;
-  uint16_t* out = (uint16_t*)a.out;
-  uint4 yv[2 * kM];
-  auto load_y = [&](const AdGroup& gr) {
-    const int col = gr.col + 8 * t;
-    const bool whole = a.vec && gr.end - col >= 8;
-#pragma unroll
-    for (int i = 0; i < 2 * kM; ++i) yv[i] = rows[i] >= 0 && whole ? *reinterpret_cast<const uint4*>(y + (long long)rows[i] * a.y_stride + col) : zero4;
-  };
-  load_y(ring[0]);  // (on its way while the inner values are exchanged)
-
-  const int p0 = g0 < g1 ? ad_group(a, g0).part : 0, width_t = g0 < g1 ? (ad_group(a, g1 - 1).part - p0 + 1) * a.rank : 0;
-  const float scale = a.scale[slot];
+  const float scale = a.scale[job.slot];
   ad_cluster_wait();
-  if constexpr (kRows == 16) {
-    // every block takes what its columns need from all of them
-    const int quads = width_t >> 2;
-    for (int i = tid; i < count * quads; i += kAdThreads) {
+  if (g0 < g1) {
+    for (int i = tid; i < job.count * quads; i += kAdThreads) {
       const int row = i / quads, col = (i - row * quads) * 4;
       uint2 hi, lo;
-      ad_split(ad_total<kC>(smem + (row * a.inner_row + p0 * a.rank + col) * 4, scale), hi, lo);
+      ad_split(ad_total<kC>(smem + (row * a.inner_row + col) * 4, scale), hi, lo);
       uint8_t* to = ad_smem + a.off_t + row * a.t_row + col * 2;
       *reinterpret_cast<uint2*>(to) = hi;
-      *reinterpret_cast<uint2*>(to + width_t * 2) = lo;
+      *reinterpret_cast<uint2*>(to + a.rank * 2) = lo;
     }
-    ad_cluster_arrive();  // nobody reads another block's memory behind this
-  } else {
-    // every block sums a share of the rows over all blocks and hands it to the ones whose columns need it
-    const int quads = a.inner >> 2, n = count * quads;
-    for (int i = rank * kAdThreads + tid; i < n; i += kC * kAdThreads) {
-      const int row = i / quads, col = (i - row * quads) * 4, p = col / a.rank;
-      uint2 hi, lo;
-      ad_split(ad_total<kC>(smem + (row * a.inner_row + col) * 4, scale), hi, lo);
-#pragma unroll
-      for (int q = 0; q < kC; ++q) {
-        const int q0 = ad_first_group<kC>(a, q), q1 = ad_first_group<kC>(a, q + 1);
-        if (q0 >= q1) continue;
-        const int first = ad_group(a, q0).part, last = ad_group(a, q1 - 1).part;
-        if (p < first || p > last) continue;
-        const uint32_t dst = ad_at_rank(smem + a.off_t + row * a.t_row + (col - first * a.rank) * 2, q);
-        ad_st_remote2(dst, hi.x, hi.y);
-        ad_st_remote2(dst + (last - first + 1) * a.rank * 2, lo.x, lo.y);
-      }
-    }
-    ad_cluster_arrive();
-    ad_cluster_wait();
   }
+  ad_cluster_arrive();  // nobody reads another block's memory behind this
+  __syncthreads();
 
+  // ---- the second product: 32 columns at a time as four tiles of eight.  Tile j's column n is column 8 (n / 2) + 2 j + n % 2 of the 32, so that a lane has
+  // eight columns side by side.  Lane t of a row's four has inner values 4t .. 4t + 3 of sixteen; where eight are left over, the two terms of
+  // 2t and 2t + 1 share one step.
   const int full = a.rank >> 4;
   const bool tail = a.rank & 8;
-  if (kRows == 16) __syncthreads();  // the finished inner values
-  auto pair_sync = [&]() {  // of the warps that share a group
-    if (kRows == 16) __syncwarp();
-    else asm volatile("bar.sync %0, 64;" ::"r"(mine + 1) : "memory");
-  };
-  for (int g = g0 + mine, stage = 0; g < g1; g += kGroups, stage = stage + 1 == kStages ? 0 : stage + 1) {
+  for (int g = g0 + warp, stage = 0; g < g1; g += kAdWarps, stage = stage + 1 == kStages ? 0 : stage + 1) {
     ad_wait<kStages - 1>();
-    pair_sync();
-    {
-      const AdGroup now = ring[0];
+    __syncwarp();
+    const uint8_t* us = ad_smem + ring + stage * stage_bytes;
+    const uint4 v0 = *reinterpret_cast<const uint4*>(us + 32 * a.u_row + lane * 16), v1 = *reinterpret_cast<const uint4*>(us + 32 * a.u_row + lane * 16 + 512);
+    us += gid * a.u_row;
+    const uint8_t* t0 = ad_smem + a.off_t + gid * a.t_row;
+    const uint8_t* t1 = t0 + 8 * a.t_row;
+    float o[4][4];
 #pragma unroll
-      for (int i = 0; i + 1 < kStages; ++i) ring[i] = ring[i + 1];
-      ring[kStages - 1] = g + kStages * kGroups < g1 ? ad_group(a, g + kStages * kGroups) : AdGroup{0, 0, 0};
-      uint4 v[2 * kM];
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 2 * kM; ++i) v[i] = yv[i];
-      load_y(ring[0]);
-      const uint8_t* us = ad_smem + u_at + stage * u_stage + gid * a.u_row;
-      const uint8_t* ts = ad_smem + a.off_t + (now.part - p0) * a.rank * 2;
-      float d[kM][4][4];
+      for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
 #pragma unroll
-      for (int m = 0; m < kM; ++m)
+    for (int kb = 0; kb < kKB; ++kb) {
+      if (kb < full) {
+        const int at = 32 * kb + 8 * t;
+        const uint2 h0 = *reinterpret_cast<const uint2*>(t0 + at), h1 = *reinterpret_cast<const uint2*>(t1 + at);
+        const uint2 l0 = *reinterpret_cast<const uint2*>(t0 + a.rank * 2 + at), l1 = *reinterpret_cast<const uint2*>(t1 + a.rank * 2 + at);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < kKB; ++kb) {
-        if (kb < full) {
-          uint2 b[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const uint2*>(us + 8 * j * a.u_row + 32 * kb + 8 * t);
-#pragma unroll
-          for (int m = 0; m < kM; ++m) {
-            const uint8_t* t0 = ts + (rows_at + 16 * m + gid) * a.t_row + 32 * kb + 8 * t;
-            const uint8_t* t1 = t0 + 8 * a.t_row;
-            const uint2 h0 = *reinterpret_cast<const uint2*>(t0), h1 = *reinterpret_cast<const uint2*>(t1);
-            const uint2 l0 = *reinterpret_cast<const uint2*>(t0 + width_t * 2), l1 = *reinterpret_cast<const uint2*>(t1 + width_t * 2);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              ad_mma(d[m][j], h0.x, h1.x, h0.y, h1.y, b[j].x, b[j].y);
-              ad_mma(d[m][j], l0.x, l1.x, l0.y, l1.y, b[j].x, b[j].y);
-            }
-          }
-        } else if (kb == full && tail) {
-          uint32_t b[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const uint32_t*>(us + 8 * j * a.u_row + 32 * kb + 4 * t);
-#pragma unroll
-          for (int m = 0; m < kM; ++m) {
-            const uint8_t* t0 = ts + (rows_at + 16 * m + gid) * a.t_row + 32 * kb + 4 * t;
-            const uint8_t* t1 = t0 + 8 * a.t_row;
-            const uint32_t h0 = *reinterpret_cast<const uint32_t*>(t0), h1 = *reinterpret_cast<const uint32_t*>(t1);
-            const uint32_t l0 = *reinterpret_cast<const uint32_t*>(t0 + width_t * 2), l1 = *reinterpret_cast<const uint32_t*>(t1 + width_t * 2);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ad_mma(d[m][j], h0, h1, l0, l1, b[j], b[j]);
-          }
+        for (int j = 0; j < 4; ++j) {
+          const uint2 b = *reinterpret_cast<const uint2*>(us + 8 * j * a.u_row + at);
+          ad_mma(o[j], h0.x, h1.x, h0.y, h1.y, b.x, b.y);
+          ad_mma(o[j], l0.x, l1.x, l0.y, l1.y, b.x, b.y);
         }
-      }
-      const int col = now.col + 8 * t, left = now.end - col;  // this lane's columns
+      } else if (kb == full && tail) {
+        const int at = 32 * kb + 4 * t;
+        const uint32_t h0 = *reinterpret_cast<const uint32_t*>(t0 + at), h1 = *reinterpret_cast<const uint32_t*>(t1 + at);
+        const uint32_t l0 = *reinterpret_cast<const uint32_t*>(t0 + a.rank * 2 + at), l1 = *reinterpret_cast<const uint32_t*>(t1 + a.rank * 2 + at);
 #pragma unroll
-      for (int i = 0; i < 2 * kM; ++i) {
-        if (rows[i] < 0) continue;
-        const int m = i >> 1, h = 2 * (i & 1);
-        const float f[8] = {d[m][0][h], d[m][0][h + 1], d[m][1][h], d[m][1][h + 1], d[m][2][h], d[m][2][h + 1], d[m][3][h], d[m][3][h + 1]};
-        uint16_t* to = out + (long long)rows[i] * a.out_stride + col;
-        if (a.vec && left >= 8) {
-          float w[8];
-          unpack8(v[i], w);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] += f[e];
-          st_vec(to, w);
-        } else {
-          const uint16_t* from = y + (long long)rows[i] * a.y_stride + col;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < left) st_elem(to + e, ld_elem(from + e) + f[e]);
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b = *reinterpret_cast<const uint32_t*>(us + 8 * j * a.u_row + at);
+          ad_mma(o[j], h0, h1, l0, l1, b, b);
         }
       }
     }
-    pair_sync();
-    fetch_up(ring[kStages - 1], stage);
+    __syncwarp();
+    fetch(g + kStages * kAdWarps, stage);
+    const int col = job.begin + 32 * g + 8 * t, left = job.end - col;  // this lane's columns
+    const bool whole = a.vec && left >= 8;
+    const float f0[8] = {o[0][0], o[0][1], o[1][0], o[1][1], o[2][0], o[2][1], o[3][0], o[3][1]};
+    const float f1[8] = {o[0][2], o[0][3], o[1][2], o[1][3], o[2][2], o[2][3], o[3][2], o[3][3]};
+    if (row0 >= 0) ad_store(a, row0, col, left, whole, v0, f0);
+    if (row1 >= 0) ad_store(a, row1, col, left, whole, v1, f1);
   }
-  if constexpr (kRows == 16) ad_cluster_wait();
+  ad_cluster_wait();
+}
+
+// ---------------------------------------------------------------------------------------------------------------- portions: tcgen05
+// A tile of 128 rows is the M of both products.  First: N = the inner values, 64 channels at a time through a ring in shared memory.  Second: K =
+// the inner values' first terms and then their second ones, N = 64 columns, into one of two accumulators, so that a product runs while the
+// one before it is added to y.  Operands lie in the 128-byte-swizzled K-major layout; they come by 16-byte asynchronous copies, since rows lie
+// in any order and the columns of `up` are put so that the accumulator's fragments hold eight columns side by side.
+// No block may wait for tensor memory that another cluster's holds, as clusters could then wait for one another: at most two blocks share a
+// multiprocessor (ad_tc_smem sees to that) and take a quarter of it each, and the next kernel of a chain is not brought up before they have it.
+__device__ __forceinline__ uint64_t ad_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16 instruction descriptor: fp32 accumulator, bf16 operands, both K-major, M = 128, N = n
+__device__ __forceinline__ uint32_t ad_idesc(uint32_t n) { return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
+__device__ __forceinline__ void ad_tc_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void ad_tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void ad_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void ad_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void ad_proxy_fence() { asm volatile("fence.proxy.async;\n" ::: "memory"); }
+// This thread's lane, eight columns.
+__device__ __forceinline__ void ad_tc_ld8(uint32_t addr, float (&f)[8]) {
+  uint32_t u[8];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "r"(addr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(u[i]);
+}
+// Sixteen lanes, 32 columns, as the fragments of four tiles of 16 x 8: f[4 j + i], rows lane / 4 (i < 2) and lane / 4 + 8, columns 8 j + 2 (lane % 4) + i % 2.
+__device__ __forceinline__ void ad_tc_ld_tiles(uint32_t addr, float (&f)[16]) {
+  uint32_t u[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]),
+        "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(u[i]);
+}
+
+__global__ void __launch_bounds__(kAdThreads, 2) adapter_tiles_kernel(const __grid_constant__ AdArgs a) {
+  extern __shared__ uint8_t ad_raw[];
+  __shared__ int rows_of[128];
+  __shared__ __align__(8) uint64_t bars[kAdTcStages + 2];
+  __shared__ uint32_t tmem_word;
+  constexpr int kC = kAdTcCluster;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
+  const int rank = (int)ad_cluster_rank();
+  pdl_wait();
+  const AdJob job = ad_job<128, kC>(a);
+  if (job.count <= 0) return;  // (with the whole cluster)
+  if (job.slot < 0) return ad_copy_rows<uint16_t>(a, job, rank, kC);
+  const uint32_t smem = ((uint32_t)__cvta_generic_to_shared(ad_raw) + 1023u) & ~1023u;
+  uint8_t* base = ad_raw + (smem - (uint32_t)__cvta_generic_to_shared(ad_raw));
+  const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
+  const auto bar_stage = [&](int s) { return bar + 8 * s; };
+  const auto bar_acc = [&](int s) { return bar + 8 * (kAdTcStages + s); };
+  if (tid < 128) rows_of[tid] = job.order[tid];
+  if (tid == 0) {
+    for (int s = 0; s < kAdTcStages + 2; ++s) dt_mbar_init(bar + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_word)), "r"(kAdTcTmem) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  ad_before_sync();
+  __syncthreads();
+  ad_after_sync();
+  pdl_trigger();
+  const uint32_t tmem = tmem_word;
+  bool dead = false;
+
+  // ---- first product: [128 rows] x [inner values, up to a multiple of 16], this block's share of the channels
+  const uint16_t* down = (const uint16_t*)a.down + ((long long)job.slot * a.parts + job.part) * a.rank * a.width;
+  const uint16_t* up = (const uint16_t*)a.up + (long long)job.slot * a.ends[a.parts - 1] * a.rank;
+  const int inner16 = (a.rank + 15) & ~15, steps = (a.width + 63) >> 6;
+  const int s0 = steps * rank / kC, n = steps * (rank + 1) / kC - s0;
+  const uint32_t stage_bytes = 16384 + inner16 * 128;
+  auto fetch = [&](int i) {
+    if (i < n) {
+      const uint32_t xs = smem + (i % kAdTcStages) * stage_bytes, ds = xs + 16384;
+      const int k = 64 * (s0 + i) + 8 * (tid & 7);
+      const bool in = k < a.width;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = (tid >> 3) + 32 * j, row = rows_of[r];
+        const bool on = in && row >= 0;
+        ad_copy16(xs + r * 128 + (((tid & 7) ^ (r & 7)) << 4), (const uint16_t*)a.x + (on ? (long long)row * a.x_stride + k : 0), on ? 16 : 0);
+      }
+      for (int r = tid >> 3; r < inner16; r += 32) {
+        const bool on = in && r < a.rank;
+        ad_copy16(ds + r * 128 + (((tid & 7) ^ (r & 7)) << 4), down + (on ? (long long)r * a.width + k : 0), on ? 16 : 0);
+      }
+    }
+    ad_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kAdTcStages; ++i) fetch(i);
+  for (int i = 0; i < n; ++i) {
+    ad_wait<kAdTcStages - 2>();
+    ad_proxy_fence();
+    __syncthreads();
+    if (tid == 0) {
+      ad_after_sync();
+      const uint32_t xs = smem + (i % kAdTcStages) * stage_bytes;
+      const uint64_t da = ad_desc(xs), db = ad_desc(xs + 16384);
+      const uint32_t idesc = ad_idesc(inner16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ad_tc_mma(tmem, da + 2 * j, db + 2 * j, idesc, (i | j) != 0);
+      ad_tc_commit(bar_stage(i % kAdTcStages));
+    }
+    if (i >= 1) {
+      const int free = i - 1;  // its product has had a step's time
+      if (free + kAdTcStages < n && !dt_mbar_wait(bar_stage(free % kAdTcStages), (free / kAdTcStages) & 1)) dead = true;
+      fetch(free + kAdTcStages);
+    }
+  }
+  if (n > 0 && !dt_mbar_wait(bar_stage((n - 1) % kAdTcStages), ((n - 1) / kAdTcStages) & 1)) dead = true;
+  ad_wait<0>();
+  ad_after_sync();
+  __syncthreads();  // (all copies into the ring have ended: what follows lies over it)
+
+  // ---- second product's columns
+  const int cols = job.end - job.begin, tiles = (cols + kAdTcCols - 1) / kAdTcCols;
+  const int c0 = tiles * rank / kC, c1 = tiles * (rank + 1) / kC;
+  const int blocks = (inner16 + 63) >> 6;  // of 64 inner values
+  const uint32_t u_stage = blocks * kAdTcCols * 128, u_base = smem + a.off_u;
+  const int vecs = inner16 >> 3;
+  const unsigned by_vecs = (65536u + vecs - 1) / vecs;  // i / vecs of i < 2048 by a product
+  auto fetch_up = [&](int c) {
+    if (c < c1) {
+      const uint32_t dst = u_base + ((c - c0) % kAdTcUps) * u_stage;
+      const int col0 = job.begin + kAdTcCols * c;
+      for (int i = tid; i < kAdTcCols * vecs; i += kAdThreads) {
+        const int at = (int)((unsigned)i * by_vecs >> 16), v = i - at * vecs, w = at & 31;
+        const int place = (at & ~31) + 8 * ((w >> 1) & 3) + 2 * (w >> 3) + (w & 1);
+        const bool on = col0 + at < job.end && 8 * v < a.rank;
+        ad_copy16(dst + (v >> 3) * (kAdTcCols * 128) + place * 128 + (((v & 7) ^ (place & 7)) << 4), up + (on ? (long long)(col0 + at) * a.rank + 8 * v : 0), on ? 16 : 0);
+      }
+    }
+    ad_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kAdTcUps; ++i) fetch_up(c0 + i);
+
+  // ---- partial inner values, summed over the cluster, as operand of the second product
+  float* part = reinterpret_cast<float*>(base + a.off_t);
+  const int q = warp & 3, half = warp >> 2;  // this warp's lanes of tensor memory; it shares them with another one
+  if (32 * q < job.count) {
+    for (int c = 8 * half; c < a.rank; c += 16) {
+      float f[8];
+      if (n > 0) {
+        ad_tc_ld8(tmem + ((uint32_t)(32 * q) << 16) + c, f);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = 0.f;
+      }
+      float4* to = reinterpret_cast<float4*>(part + (32 * q + lane) * a.inner_row + c);
+      to[0] = make_float4(f[0], f[1], f[2], f[3]);
+      to[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  }
+  ad_before_sync();
+  ad_cluster_arrive();
+  int rows[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rows[i] = rows_of[32 * q + 8 * i + gid];
+  uint4 yv[2][4];  // of the next two products
+  auto load_y = [&](uint4 (&to)[4], int c) {
+    const int col = job.begin + kAdTcCols * c + 32 * half + 8 * t;
+    const bool whole = c < c1 && a.vec && job.end - col >= 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      to[i] = whole && rows[i] >= 0 ? *reinterpret_cast<const uint4*>((const uint16_t*)a.y + (long long)rows[i] * a.y_stride + col) : make_uint4(0, 0, 0, 0);
+  };
+  load_y(yv[0], c0);
+  load_y(yv[1], c0 + 1);
+  const float scale = a.scale[job.slot];
+  ad_cluster_wait();
+  {
+    const int quads = a.rank >> 2, total = job.count * quads;
+    for (int i = rank * kAdThreads + tid; i < total; i += kC * kAdThreads) {
+      const int row = i / quads, col = (i - row * quads) * 4;
+      uint2 hi, lo;
+      ad_split(ad_total<kC>(smem + a.off_t + (row * a.inner_row + col) * 4, scale), hi, lo);
+      const auto at = [&](int k) { return smem + (k >> 6) * 16384 + row * 128 + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2; };
+      const uint32_t at_hi = at(col), at_lo = at(inner16 + col);
+      const bool pad = col >= a.rank - 8 && (a.rank & 8);  // what lies behind a term's values is zero
+#pragma unroll
+      for (int p = 0; p < kC; ++p) {
+        if (tiles * p / kC == tiles * (p + 1) / kC) continue;  // no columns there
+        ad_st_remote2(ad_at_rank(at_hi, p), hi);
+        ad_st_remote2(ad_at_rank(at_lo, p), lo);
+        if (pad) {
+          ad_st_remote2(ad_at_rank(at(col + 8), p), make_uint2(0, 0));
+          ad_st_remote2(ad_at_rank(at(inner16 + col + 8), p), make_uint2(0, 0));
+        }
+      }
+    }
+  }
+  ad_proxy_fence();
+  ad_cluster_arrive();
+  ad_cluster_wait();
+  ad_proxy_fence();
+
+  // ---- second product
+  auto multiply = [&](int c) {  // by one thread
+    ad_after_sync();
+    const int s = (c - c0) & 1;
+    const uint32_t d = tmem + s * kAdTcCols, us = u_base + ((c - c0) % kAdTcUps) * u_stage, idesc = ad_idesc(kAdTcCols);
+    for (int term = 0; term < 2; ++term) {
+      for (int k = 0; k < inner16; k += 16) {
+        const int ka = term * inner16 + k;
+        ad_tc_mma(d, ad_desc(smem + (ka >> 6) * 16384) + ((ka & 63) >> 3), ad_desc(us + (k >> 6) * (kAdTcCols * 128)) + ((k & 63) >> 3), idesc, ka != 0);
+      }
+    }
+    ad_tc_commit(bar_acc(s));
+  };
+  if (c0 < c1) {
+    ad_wait<kAdTcUps - 1>();
+    ad_proxy_fence();
+    ad_before_sync();
+    __syncthreads();
+    if (tid == 0) multiply(c0);
+  }
+  for (int c = c0; c < c1; ++c) {
+    const int i = c - c0, s = i & 1;
+    if (c + 1 < c1) {
+      ad_wait<kAdTcUps - 2>();
+      ad_proxy_fence();
+      __syncthreads();  // the next one's columns are there, its accumulator has been read
+      if (tid == 0) multiply(c + 1);
+    }
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = yv[0][j];
+      yv[0][j] = yv[1][j];
+    }
+    load_y(yv[1], c + 2);
+    if (!dt_mbar_wait(bar_acc(s), (i >> 1) & 1)) dead = true;
+    dead = __any_sync(0xffffffffu, dead);
+    ad_after_sync();
+    fetch_up(c + kAdTcUps);
+    if (32 * q < job.count && !dead) {
+      const int col = job.begin + kAdTcCols * c + 32 * half + 8 * t, left = job.end - col;
+      const bool whole = a.vec && left >= 8;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float f[16];
+        ad_tc_ld_tiles(tmem + ((uint32_t)(32 * q + 16 * m) << 16) + s * kAdTcCols + 32 * half, f);
+        const float f0[8] = {f[0], f[1], f[4], f[5], f[8], f[9], f[12], f[13]};
+        const float f1[8] = {f[2], f[3], f[6], f[7], f[10], f[11], f[14], f[15]};
+        if (rows[2 * m] >= 0) ad_store(a, rows[2 * m], col, left, whole, v[2 * m], f0);
+        if (rows[2 * m + 1] >= 0) ad_store(a, rows[2 * m + 1], col, left, whole, v[2 * m + 1], f1);
+      }
+    }
+    ad_before_sync();
+  }
+  ad_wait<0>();
+  if (dead && a.status) atomicOr(a.status, B200KV_S_TIMEOUT);
+  __syncthreads();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kAdTcTmem) : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------------------------- CUDA cores
 // 32-bit models, and bf16 rows that cannot be read in 16 bytes: sixteen rows a cluster, 32-bit products.
-constexpr int kAdSimtCluster = 8;
-
 template <typename T>
 __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ __align__(16) uint8_t ad_smem[];
   constexpr int kC = kAdSimtCluster;
   const uint32_t smem = (uint32_t)__cvta_generic_to_shared(ad_smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = (int)ad_cluster_rank(), cl = blockIdx.x / kC;
+  const int rank = (int)ad_cluster_rank();
   pdl_enter();
   pdl_wait();
-  const int subs = a.tile_rows / 16;
-  const int4 tile = a.tiles[cl / subs];
-  const int32_t* order = a.order + (long long)cl * 16;
-  const int slot = tile.x, count = min(tile.y - (cl % subs) * 16, 16);
-  if (count <= 0) return;
-  if (slot < 0) return ad_copy_rows<T, kC>(a, order, count, rank);
-  const T* down = (const T*)a.down + (long long)slot * a.inner * a.width;
-  const T* up = (const T*)a.up + (long long)slot * a.ends[a.parts - 1] * a.rank;
+  const AdJob job = ad_job<16, kC>(a);
+  if (job.count <= 0) return;
+  if (job.slot < 0) return ad_copy_rows<T>(a, job, rank, kC);
+  const T* down = (const T*)a.down + ((long long)job.slot * a.parts + job.part) * a.rank * a.width;
+  const T* up = (const T*)a.up + (long long)job.slot * a.ends[a.parts - 1] * a.rank;
   float* part = reinterpret_cast<float*>(ad_smem);
   float* xs = part + 16 * a.inner_row;
   const int k0 = (int)((long long)a.width * rank / kC), k1 = (int)((long long)a.width * (rank + 1) / kC);
@@ -554,10 +690,10 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
     __syncthreads();
     for (int i = tid; i < 16 * kAdSimtChannels; i += kAdThreads) {
       const int row = i / kAdSimtChannels, k = i % kAdSimtChannels;
-      xs[i] = row < count && k < n ? ld_elem((const T*)a.x + (long long)order[row] * a.x_stride + s0 + k) : 0.f;
+      xs[i] = row < job.count && k < n ? ld_elem((const T*)a.x + (long long)job.order[row] * a.x_stride + s0 + k) : 0.f;
     }
     __syncthreads();
-    for (int j = warp; j < a.inner; j += kAdWarps) {
+    for (int j = warp; j < a.rank; j += kAdWarps) {
       float s[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = 0.f;
@@ -575,23 +711,21 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
   }
   ad_cluster_arrive();
   ad_cluster_wait();
-  const int g0 = ad_first_group<kC>(a, rank), g1 = ad_first_group<kC>(a, rank + 1);
-  const int p0 = g0 < g1 ? ad_group(a, g0).part : 0, quads = g0 < g1 ? ((ad_group(a, g1 - 1).part - p0 + 1) * a.rank) >> 2 : 0;
-  const float scale = a.scale[slot];
+  const int quads = a.rank >> 2;
+  const float scale = a.scale[job.slot];
   for (int i = tid; i < 16 * quads; i += kAdThreads) {
     const int row = i / quads, col = (i - row * quads) * 4;
-    *reinterpret_cast<float4*>(ad_smem + a.off_t + row * a.t_row + col * 4) = ad_total<kC>(smem + (row * a.inner_row + p0 * a.rank + col) * 4, scale);
+    *reinterpret_cast<float4*>(ad_smem + a.off_t + row * a.t_row + col * 4) = ad_total<kC>(smem + (row * a.inner_row + col) * 4, scale);
   }
   ad_cluster_arrive();
   __syncthreads();
-  for (int g = g0 + warp; g < g1; g += kAdWarps) {
-    const AdGroup gr = ad_group(a, g);
-    const int col = gr.col + lane;
-    if (col >= gr.end) continue;
+  const int cols = job.end - job.begin;
+  const int c1 = job.begin + (int)((long long)cols * (rank + 1) / kC);
+  for (int col = job.begin + (int)((long long)cols * rank / kC) + tid; col < c1; col += kAdThreads) {
     float d[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) d[r] = 0.f;
-    const uint8_t* ts = ad_smem + a.off_t + (gr.part - p0) * a.rank * 4;
+    const uint8_t* ts = ad_smem + a.off_t;
     for (int j = 0; j < a.rank; j += 4) {
       float u[4];
       ld_elem4(up + (long long)col * a.rank + j, u);
@@ -603,8 +737,8 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      if (r < count) {
-        const long long row = order[r];
+      if (r < job.count) {
+        const long long row = job.order[r];
         st_elem((T*)a.out + row * a.out_stride + col, ld_elem((const T*)a.y + row * a.y_stride + col) + d[r]);
       }
     }
@@ -619,7 +753,6 @@ template <typename... KArgs>
 static int ad_launch(void (*kernel)(KArgs...), const AdArgs& a, int clusters, int cluster, size_t smem, cudaStream_t stream) {
   if (smem > kAdMostSmem) return B200KV_E_SHAPE;
   if (!allow_smem(kernel, kAdMostSmem)) return launch_result(cudaErrorInvalidValue);
-  if (cluster > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return launch_result(cudaErrorInvalidValue);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * cluster));
   cfg.blockDim = dim3(kAdThreads);
@@ -636,47 +769,30 @@ static int ad_launch(void (*kernel)(KArgs...), const AdArgs& a, int clusters, in
   return launch_result(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
-// Most parts that the columns of one block touch.
-static int ad_parts_spanned(const AdArgs& a, int cluster) {
-  int most = 1;
-  for (int q = 0; q < cluster; ++q) {
-    const int g0 = (int)((unsigned)a.groups * (unsigned)q / cluster), g1 = (int)((unsigned)a.groups * (unsigned)(q + 1) / cluster);
-    if (g0 >= g1) continue;
-    int begin = 0, at = 0, lo = 0, hi = 0;
-    for (int p = 0; p < a.parts; ++p) {
-      const int n = (a.ends[p] - begin + 31) / 32;
-      if (g0 >= at && g0 < at + n) lo = p;
-      if (g1 - 1 >= at && g1 - 1 < at + n) hi = p;
-      at += n;
-      begin = a.ends[p];
-    }
-    if (hi - lo + 1 > most) most = hi - lo + 1;
-  }
-  return most;
+template <int kNT, int kKB, int kC, int kStages>
+static int ad_rows(AdArgs a, int clusters, int most_cols, cudaStream_t stream) {
+  a.inner_row = a.rank + 4;                    // (rows apart by other banks)
+  a.t_row = (a.rank * 4 + 63) / 64 * 64 + 32;  // both terms; four rows at different banks
+  a.u_row = a.rank * 2;
+  while (a.u_row % 64 != 32) a.u_row += 16;    // four columns at different banks
+  const int deep = a.rank <= 8 * kNT ? kAdWarps : kAdWarps / 2;
+  a.off_t = (uint32_t)(deep * 16 * a.inner_row * 4);
+  a.off_u = a.off_t + 16 * a.t_row;
+  a.ring = ((most_cols + 31) / 32 + kC * kAdWarps - 1) / (kC * kAdWarps);  // (a warp has no more groups than that)
+  if (a.ring > kStages) a.ring = kStages;
+  return ad_launch(adapter_rows_kernel<kNT, kKB, kC, kStages>, a, clusters, kC, a.off_u + (size_t)kAdWarps * a.ring * (32 * a.u_row + 1024), stream);
 }
 
-template <int kRows, int kNT, int kKB, int kC, int kStages>
-static int ad_run(AdArgs a, int clusters, cudaStream_t stream) {
-  constexpr int kGroups = kRows == 16 ? 8 : 4;
-  const int spanned = ad_parts_spanned(a, kC) * a.rank;
-  a.inner_row = a.inner + 4;                    // (rows apart by other banks)
-  a.t_row = (spanned * 4 + 63) / 64 * 64 + 32;  // both terms; four rows at different banks
-  a.u_row = a.rank * 2;
-  while (a.u_row % 64 != 32) a.u_row += 16;     // four columns at different banks
-  size_t first;
-  if (kRows == 16) {
-    const int wn = (a.inner + 8 * kNT - 1) / (8 * kNT), deep = kAdWarps / (wn <= 1 ? 1 : (wn <= 2 ? 2 : (wn <= 4 ? 4 : 8)));
-    first = (size_t)deep * 16 * a.inner_row * 4;
-  } else {
-    const size_t staged = (size_t)2 * a.inner * 128, partial = (size_t)kRows * a.inner_row * 4;
-    first = staged > partial ? staged : partial;
-  }
-  a.off_t = (uint32_t)((first + 15) / 16 * 16);
-  a.off_u = a.off_t + kRows * a.t_row;
-  int stages = kStages;
-  const int chunks = ((a.groups + kC - 1) / kC + kGroups - 1) / kGroups;  // of a block, at most
-  if (stages > chunks) stages = chunks;
-  return ad_launch(adapter_kernel<kRows, kNT, kKB, kC, kStages>, a, clusters, kC, a.off_u + (size_t)stages * kGroups * 32 * a.u_row, stream);
+// Shared memory of a tile of 128 rows: the ring, and over it the second product's operand and the partial inner values; the columns of `up`.
+static size_t ad_tc_smem(AdArgs* a) {
+  const int inner16 = (a->rank + 15) / 16 * 16;
+  const size_t ring = (size_t)kAdTcStages * (16384 + inner16 * 128), terms = (size_t)(2 * inner16 + 63) / 64 * 16384;
+  a->inner_row = a->rank + 4;
+  a->off_t = (uint32_t)terms;
+  const size_t over = terms + (size_t)128 * a->inner_row * 4;
+  a->off_u = (uint32_t)(((ring > over ? ring : over) + 1023) / 1024 * 1024);
+  const size_t all = 1024 + a->off_u + (size_t)kAdTcUps * ((inner16 + 63) / 64) * kAdTcCols * 128;
+  return all > 80 * 1024 ? all : 80 * 1024;
 }
 
 }  // namespace b200kv
@@ -687,8 +803,8 @@ extern "C" int b200dec_adapter_plan(const int32_t* ids, int32_t num_rows, int32_
                                     int32_t max_tiles, int32_t* status, void* stream) {
   if (num_rows == 0) return B200KV_OK;
   if (!ids || !order || !tiles) return B200KV_E_NULL;
-  if (num_rows < 0 || num_rows > (1 << 26) || slots < 1 || slots > kAdMaxSlots) return B200KV_E_RANGE;
-  if (tile_rows != 16 && tile_rows != 64) return B200KV_E_SHAPE;
+  if (num_rows < 0 || num_rows > (1 << 24) || slots < 1 || slots > kAdMaxSlots) return B200KV_E_RANGE;
+  if (tile_rows != 16 && tile_rows != 128) return B200KV_E_SHAPE;
   if (max_tiles < num_rows / tile_rows + (num_rows < slots + 1 ? num_rows : slots + 1)) return B200KV_E_WORKSPACE;
   if ((long long)max_tiles * tile_rows > 0x7fffffffLL) return B200KV_E_RANGE;
   if (!aligned(tiles, 16) || !aligned(ids, 4) || !aligned(order, 4)) return B200KV_E_ALIGN;
@@ -699,53 +815,52 @@ extern "C" int b200dec_adapter_plan(const int32_t* ids, int32_t num_rows, int32_
 
 extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out,
                                     int64_t out_stride, const int32_t* order, const int32_t* tiles, int32_t max_tiles, int32_t tile_rows,
-                                    int32_t num_rows, void* stream) {
+                                    int32_t num_rows, int32_t* status, void* stream) {
   if (num_rows == 0) return B200KV_OK;
   if (!ad || !ad->down || !ad->up || !ad->scale || !x || !y || !out || !order || !tiles) return B200KV_E_NULL;
   if (num_rows < 0 || max_tiles < 1 || ad->slots < 1 || ad->slots > kAdMaxSlots) return B200KV_E_RANGE;
   if (ad->elem != 2 && ad->elem != 4) return B200KV_E_SHAPE;
   if (ad->parts < 1 || ad->parts > kAdMaxParts || ad->rank < 8 || ad->rank > 128 || ad->rank % 8 || ad->width < 1) return B200KV_E_SHAPE;
-  if (tile_rows != 16 && tile_rows != 64) return B200KV_E_SHAPE;
+  if (ad->width > (1 << 24)) return B200KV_E_RANGE;
+  if (tile_rows != 16 && tile_rows != 128) return B200KV_E_SHAPE;
   AdArgs a = {};
   a.down = ad->down; a.up = ad->up; a.scale = ad->scale; a.x = x; a.y = y; a.out = out;
   a.x_stride = x_stride; a.y_stride = y_stride; a.out_stride = out_stride;
   a.order = order; a.tiles = (const int4*)tiles; a.tile_rows = tile_rows;
-  a.rank = ad->rank; a.width = ad->width; a.parts = ad->parts;
+  a.rank = ad->rank; a.width = ad->width; a.parts = ad->parts; a.status = status;
   bool even = true;
+  int most = 0;
   for (int p = 0, begin = 0; p < ad->parts; ++p) {
-    if (ad->ends[p] <= begin || ad->ends[p] > (1 << 28)) return B200KV_E_SHAPE;
+    if (ad->ends[p] <= begin || ad->ends[p] > (1 << 24)) return B200KV_E_SHAPE;
     even = even && begin % 8 == 0;
     a.ends[p] = ad->ends[p];
-    a.groups += (ad->ends[p] - begin + 31) / 32;
+    if (ad->ends[p] - begin > most) most = ad->ends[p] - begin;
     begin = ad->ends[p];
   }
   const int cols = a.ends[a.parts - 1];
   if (x_stride < a.width || y_stride < cols || out_stride < cols || out == x) return B200KV_E_SHAPE;
-  if ((out == y && out_stride != y_stride) || (long long)max_tiles * tile_rows > 0x7fffffffLL) return B200KV_E_RANGE;
+  if ((out == y && out_stride != y_stride) || (long long)max_tiles * tile_rows * a.parts > 0x0fffffffLL) return B200KV_E_RANGE;
   if (!aligned(ad->down, 16) || !aligned(ad->up, 16) || !aligned(ad->scale, 4) || !aligned(tiles, 16) || !aligned(order, 4) || !aligned(x, ad->elem) ||
       !aligned(y, ad->elem) || !aligned(out, ad->elem))
     return B200KV_E_ALIGN;
-  a.inner = a.parts * a.rank;
   a.vec = even && aligned(y, 16) && aligned(out, 16) && y_stride % 8 == 0 && out_stride % 8 == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  const int fine = max_tiles * (tile_rows / 16);  // clusters with sixteen rows each
+  const int clusters = max_tiles * a.parts, fine = clusters * (tile_rows / 16);  // the latter with sixteen rows each
   if (ad->elem == 4 || a.width % 8 || x_stride % 8 || !aligned(x, 16)) {
-    a.inner_row = a.inner;
-    a.t_row = ad_parts_spanned(a, kAdSimtCluster) * a.rank * 4;
+    a.inner_row = a.rank;
+    a.t_row = a.rank * 4;
     a.off_t = 16u * a.inner_row * 4 + 16u * kAdSimtChannels * 4;
     const size_t smem = a.off_t + (size_t)16 * a.t_row;
     return ad->elem == 4 ? ad_launch(adapter_simt_kernel<float>, a, fine, kAdSimtCluster, smem, s)
                          : ad_launch(adapter_simt_kernel<uint16_t>, a, fine, kAdSimtCluster, smem, s);
   }
-  const int kb = (a.rank + 15) / 16;
-  if (tile_rows == 16 || a.inner > kAdMaxInner) {
-    if (kb <= 1) return ad_run<16, 4, 1, 8, 4>(a, fine, s);
-    if (kb <= 2) return ad_run<16, 4, 2, 8, 4>(a, fine, s);
-    if (kb <= 4) return ad_run<16, 4, 4, 8, 2>(a, fine, s);
-    return ad_run<16, 8, 8, 8, 2>(a, fine, s);
+  if (tile_rows == 128) {
+    const size_t smem = ad_tc_smem(&a);
+    return ad_launch(adapter_tiles_kernel, a, clusters, kAdTcCluster, smem, s);
   }
-  if (kb <= 1) return ad_run<64, 8, 1, 8, 4>(a, max_tiles, s);
-  if (kb <= 2) return ad_run<64, 16, 2, 8, 2>(a, max_tiles, s);
-  if (kb <= 4) return ad_run<64, 24, 4, 8, 2>(a, max_tiles, s);
-  return ad_run<64, 24, 8, 8, 2>(a, max_tiles, s);
+  const int kb = (a.rank + 15) / 16;
+  if (kb <= 1) return ad_rows<2, 1, 8, 3>(a, fine, most, s);
+  if (kb <= 2) return ad_rows<4, 2, 8, 3>(a, fine, most, s);
+  if (kb <= 4) return ad_rows<8, 4, 8, 2>(a, fine, most, s);
+  return ad_rows<8, 8, 8, 2>(a, fine, most, s);
 }

@@ -706,8 +706,8 @@ class AdapterPlan:
 
 
 def adapter_tile_rows(num_rows: int) -> int:
-    """Rows of a tile: 16 for decoding rows, 64 where rows of one adapter come in portions."""
-    return 16 if num_rows <= 128 else 64
+    """Rows of a tile: 16 for decoding rows, 128 where rows of one adapter come in portions."""
+    return 16 if num_rows <= 128 else 128
 
 
 def _here(t: torch.Tensor) -> None:
@@ -755,7 +755,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Ada
     # (a single row's stride may be anything)
     xs, ys, os = (t.stride(0) if N > 1 else _round8(t.shape[1]) for t in (x, y, out))
     rc = _lib_dec().b200dec_add_adapters(ctypes.byref(adapters.struct), x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, plan.order.data_ptr(),
-                                         plan.tiles.data_ptr(), *plan.order.shape, N, K._stream())
+                                         plan.tiles.data_ptr(), *plan.order.shape, N, K.status_word(y.device).data_ptr(), K._stream())
     _lib.check(rc, "add_adapters")
     return out
 

@@ -70,7 +70,7 @@ SHAPES = [
 
 
 @pytest.mark.parametrize("rows,width,parts,rank,slots,dtype", SHAPES)
-@pytest.mark.parametrize("tile_rows", [None, 16, 64])
+@pytest.mark.parametrize("tile_rows", [None, 16, 128])
 def test_against_the_formula(ops, rows, width, parts, rank, slots, dtype, tile_rows):
     ad, ids, x, y = make(ops, rows, width, parts, rank, slots, dtype)
     plan = ops.plan_adapters(ids, slots, tile_rows)
