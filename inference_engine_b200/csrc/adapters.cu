@@ -11,6 +11,7 @@
 // Precision: bf16 operands, 32-bit sums.  The inner values are scaled in 32 bits and enter the second product as two bf16 terms (16 bits of
 // mantissa): rounded to one they would cost the sum as much as its own rounding does.
 #include "dec_tma.cuh"
+#include <cstdlib>
 
 namespace b200kv {
 
@@ -21,7 +22,6 @@ constexpr int kAdMaxSlots = 4096;
 constexpr int kAdPlanThreads = 1024;
 constexpr int kAdSimtChannels = 512;  // input channels that the CUDA cores' form stages at a time
 constexpr int kAdSimtCluster = 8;
-constexpr int kAdTcCluster = 8;
 constexpr int kAdTcStages = 3;        // of 64 input channels
 constexpr int kAdTcCols = 64;         // output columns of a product of the tensor core
 constexpr int kAdTcUps = 3;           // their `up`s that are in shared memory or on their way
@@ -206,17 +206,23 @@ __device__ __forceinline__ float4 ad_total(uint32_t at, float scale) {
   return s;
 }
 
-// What a lane adds to its eight columns of a row, f, which start `left` columns in front of the part's end; v: y where `whole`.
-__device__ __forceinline__ void ad_store(const AdArgs& a, int row, int col, int left, bool whole, const uint4& v, const float (&f)[8]) {
-  uint16_t* to = (uint16_t*)a.out + (long long)row * a.out_stride + col;
+__device__ __forceinline__ uint32_t ad_pack(float lo, float hi) {
+  uint32_t v;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
+}
+// What a lane adds to its eight columns of a row, f, which start `left` columns in front of the part's end; v: y's where `whole`.
+__device__ __forceinline__ void ad_store(const uint16_t* from, uint16_t* to, int left, bool whole, const uint4& v, const float (&f)[8]) {
   if (whole) {
     float w[8];
     unpack8(v, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] += f[e];
-    st_vec(to, w);
+    uint4 o;
+    o.x = ad_pack(w[0] + f[0], w[1] + f[1]);
+    o.y = ad_pack(w[2] + f[2], w[3] + f[3]);
+    o.z = ad_pack(w[4] + f[4], w[5] + f[5]);
+    o.w = ad_pack(w[6] + f[6], w[7] + f[7]);
+    *reinterpret_cast<uint4*>(to) = o;
   } else {
-    const uint16_t* from = (const uint16_t*)a.y + (long long)row * a.y_stride + col;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e < left) st_elem(to + e, ld_elem(from + e) + f[e]);
@@ -386,8 +392,9 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kern
     const bool whole = a.vec && left >= 8;
     const float f0[8] = {o[0][0], o[0][1], o[1][0], o[1][1], o[2][0], o[2][1], o[3][0], o[3][1]};
     const float f1[8] = {o[0][2], o[0][3], o[1][2], o[1][3], o[2][2], o[2][3], o[3][2], o[3][3]};
-    if (row0 >= 0) ad_store(a, row0, col, left, whole, v0, f0);
-    if (row1 >= 0) ad_store(a, row1, col, left, whole, v1, f1);
+    uint16_t* out = (uint16_t*)a.out + col;
+    if (row0 >= 0) ad_store(y + (long long)row0 * a.y_stride + col, out + (long long)row0 * a.out_stride, left, whole, v0, f0);
+    if (row1 >= 0) ad_store(y + (long long)row1 * a.y_stride + col, out + (long long)row1 * a.out_stride, left, whole, v1, f1);
   }
   ad_cluster_wait();
 }
@@ -397,7 +404,7 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kern
 // the inner values' first terms and then their second ones, N = 64 columns, into one of two accumulators, so that a product runs while the
 // one before it is added to y.  Operands lie in the 128-byte-swizzled K-major layout; they come by 16-byte asynchronous copies, since rows lie
 // in any order and the columns of `up` are put so that the accumulator's fragments hold eight columns side by side.
-// No block may wait for tensor memory that another cluster's holds, as clusters could then wait for one another: at most two blocks share a
+// No block may wait for tensor memory that another cluster's holds, as clusters could then wait for one another: at most three blocks share a
 // multiprocessor (ad_tc_smem sees to that) and take a quarter of it each, and the next kernel of a chain is not brought up before they have it.
 __device__ __forceinline__ uint64_t ad_desc(uint32_t saddr) {
   return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -415,7 +422,8 @@ __device__ __forceinline__ void ad_tc_commit(uint32_t bar) {
 }
 __device__ __forceinline__ void ad_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void ad_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
-__device__ __forceinline__ void ad_proxy_fence() { asm volatile("fence.proxy.async;\n" ::: "memory"); }
+// (of shared memory alone: one of all memory would wait for the stores to the result as well)
+__device__ __forceinline__ void ad_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 // This thread's lane, eight columns.
 __device__ __forceinline__ void ad_tc_ld8(uint32_t addr, float (&f)[8]) {
   uint32_t u[8];
@@ -439,12 +447,12 @@ __device__ __forceinline__ void ad_tc_ld_tiles(uint32_t addr, float (&f)[16]) {
   for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(u[i]);
 }
 
-__global__ void __launch_bounds__(kAdThreads, 2) adapter_tiles_kernel(const __grid_constant__ AdArgs a) {
+template <int kC>
+__global__ void __launch_bounds__(kAdThreads, 3) adapter_tiles_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ uint8_t ad_raw[];
   __shared__ int rows_of[128];
   __shared__ __align__(8) uint64_t bars[kAdTcStages + 2];
   __shared__ uint32_t tmem_word;
-  constexpr int kC = kAdTcCluster;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
   const int rank = (int)ad_cluster_rank();
   pdl_wait();
@@ -542,8 +550,6 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_tiles_kernel(const __gr
     }
     ad_commit();
   };
-#pragma unroll
-  for (int i = 0; i < kAdTcUps; ++i) fetch_up(c0 + i);
 
   // ---- partial inner values, summed over the cluster, as operand of the second product
   float* part = reinterpret_cast<float*>(base + a.off_t);
@@ -564,19 +570,25 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_tiles_kernel(const __gr
   }
   ad_before_sync();
   ad_cluster_arrive();
+  // this lane's first column of its four rows
   int rows[4];
+  const uint16_t* from[4];
+  uint16_t* to[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) rows[i] = rows_of[32 * q + 8 * i + gid];
-  uint4 yv[2][4];  // of the next two products
-  auto load_y = [&](uint4 (&to)[4], int c) {
-    const int col = job.begin + kAdTcCols * c + 32 * half + 8 * t;
-    const bool whole = c < c1 && a.vec && job.end - col >= 8;
+  for (int i = 0; i < 4; ++i) {
+    rows[i] = rows_of[32 * q + 8 * i + gid];
+    const int col = job.begin + 32 * half + 8 * t;
+    from[i] = (const uint16_t*)a.y + (long long)max(rows[i], 0) * a.y_stride + col;
+    to[i] = (uint16_t*)a.out + (long long)max(rows[i], 0) * a.out_stride + col;
+  }
+  uint4 yv[4] = {};  // of the next product
+  auto load_y = [&](uint4 (&v)[4], int c) {
+    const bool whole = c < c1 && a.vec && cols - (kAdTcCols * c + 32 * half + 8 * t) >= 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      to[i] = whole && rows[i] >= 0 ? *reinterpret_cast<const uint4*>((const uint16_t*)a.y + (long long)rows[i] * a.y_stride + col) : make_uint4(0, 0, 0, 0);
+      if (whole && rows[i] >= 0) v[i] = *reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c);
   };
-  load_y(yv[0], c0);
-  load_y(yv[1], c0 + 1);
+  load_y(yv, c0);
   const float scale = a.scale[job.slot];
   ad_cluster_wait();
   {
@@ -600,10 +612,12 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_tiles_kernel(const __gr
       }
     }
   }
-  ad_proxy_fence();
+  asm volatile("fence.proxy.async.shared::cluster;\n" ::: "memory");
   ad_cluster_arrive();
   ad_cluster_wait();
-  ad_proxy_fence();
+  asm volatile("fence.proxy.async.shared::cluster;\n" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < kAdTcUps; ++i) fetch_up(c0 + i);  // where the partial values were
 
   // ---- second product
   auto multiply = [&](int c) {  // by one thread
@@ -635,17 +649,14 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_tiles_kernel(const __gr
     }
     uint4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = yv[0][j];
-      yv[0][j] = yv[1][j];
-    }
-    load_y(yv[1], c + 2);
+    for (int j = 0; j < 4; ++j) v[j] = yv[j];
+    load_y(yv, c + 1);
     if (!dt_mbar_wait(bar_acc(s), (i >> 1) & 1)) dead = true;
     dead = __any_sync(0xffffffffu, dead);
     ad_after_sync();
     fetch_up(c + kAdTcUps);
     if (32 * q < job.count && !dead) {
-      const int col = job.begin + kAdTcCols * c + 32 * half + 8 * t, left = job.end - col;
+      const int left = cols - (kAdTcCols * c + 32 * half + 8 * t);
       const bool whole = a.vec && left >= 8;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -653,8 +664,8 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_tiles_kernel(const __gr
         ad_tc_ld_tiles(tmem + ((uint32_t)(32 * q + 16 * m) << 16) + s * kAdTcCols + 32 * half, f);
         const float f0[8] = {f[0], f[1], f[4], f[5], f[8], f[9], f[12], f[13]};
         const float f1[8] = {f[2], f[3], f[6], f[7], f[10], f[11], f[14], f[15]};
-        if (rows[2 * m] >= 0) ad_store(a, rows[2 * m], col, left, whole, v[2 * m], f0);
-        if (rows[2 * m + 1] >= 0) ad_store(a, rows[2 * m + 1], col, left, whole, v[2 * m + 1], f1);
+        if (rows[2 * m] >= 0) ad_store(from[2 * m] + kAdTcCols * c, to[2 * m] + kAdTcCols * c, left, whole, v[2 * m], f0);
+        if (rows[2 * m + 1] >= 0) ad_store(from[2 * m + 1] + kAdTcCols * c, to[2 * m + 1] + kAdTcCols * c, left, whole, v[2 * m + 1], f1);
       }
     }
     ad_before_sync();
@@ -783,16 +794,17 @@ static int ad_rows(AdArgs a, int clusters, int most_cols, cudaStream_t stream) {
   return ad_launch(adapter_rows_kernel<kNT, kKB, kC, kStages>, a, clusters, kC, a.off_u + (size_t)kAdWarps * a.ring * (32 * a.u_row + 1024), stream);
 }
 
-// Shared memory of a tile of 128 rows: the ring, and over it the second product's operand and the partial inner values; the columns of `up`.
+// Shared memory of a tile of 128 rows: the ring; over it the second product's operand, and the partial inner values and then the columns of `up`.
+// Not less than lets three blocks share a multiprocessor.
 static size_t ad_tc_smem(AdArgs* a) {
   const int inner16 = (a->rank + 15) / 16 * 16;
   const size_t ring = (size_t)kAdTcStages * (16384 + inner16 * 128), terms = (size_t)(2 * inner16 + 63) / 64 * 16384;
   a->inner_row = a->rank + 4;
   a->off_t = (uint32_t)terms;
-  const size_t over = terms + (size_t)128 * a->inner_row * 4;
-  a->off_u = (uint32_t)(((ring > over ? ring : over) + 1023) / 1024 * 1024);
-  const size_t all = 1024 + a->off_u + (size_t)kAdTcUps * ((inner16 + 63) / 64) * kAdTcCols * 128;
-  return all > 80 * 1024 ? all : 80 * 1024;
+  a->off_u = (uint32_t)terms;
+  const size_t ups = (size_t)kAdTcUps * ((inner16 + 63) / 64) * kAdTcCols * 128, partial = (size_t)128 * a->inner_row * 4;
+  const size_t over = terms + (ups > partial ? ups : partial), all = 1024 + (ring > over ? ring : over);
+  return all > 60 * 1024 ? all : 60 * 1024;
 }
 
 }  // namespace b200kv
@@ -856,9 +868,13 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, i
   }
   if (tile_rows == 128) {
     const size_t smem = ad_tc_smem(&a);
-    return ad_launch(adapter_tiles_kernel, a, clusters, kAdTcCluster, smem, s);
+    const char* ce = getenv("AD_C");
+    return ce && ce[0] == '4' ? ad_launch(adapter_tiles_kernel<4>, a, clusters, 4, smem, s) : ad_launch(adapter_tiles_kernel<8>, a, clusters, 8, smem, s);
   }
   const int kb = (a.rank + 15) / 16;
+  const char* ce = getenv("AD_C");
+  if (ce && ce[0] == '4' && kb <= 1) return ad_rows<2, 1, 4, 3>(a, fine, most, s);
+  if (ce && ce[0] == '2' && kb <= 1) return ad_rows<2, 1, 2, 3>(a, fine, most, s);
   if (kb <= 1) return ad_rows<2, 1, 8, 3>(a, fine, most, s);
   if (kb <= 2) return ad_rows<4, 2, 8, 3>(a, fine, most, s);
   if (kb <= 4) return ad_rows<8, 4, 8, 2>(a, fine, most, s);
