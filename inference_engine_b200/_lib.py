@@ -202,7 +202,8 @@ DECODER_SIGNATURES = {
                                          c_void_p, c_int32, c_float, c_float, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "b200dec_adapter_plan": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "b200dec_add_adapters": (c_int32, [P_ADAPTERS, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32,
-                                       c_int32, c_void_p, c_void_p]),
+                                       c_int32, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "b200dec_add_adapters_workspace": (c_size_t, [P_ADAPTERS, c_int32, c_int32]),
     "b200dec_adjust_logits": (c_int32, [c_void_p, c_int64, c_int32, P_RULES, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p]),
     "b200dec_choose_tokens": (c_int32, [c_void_p, c_int64, c_int32, P_RULES, P_DRAW, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                         c_void_p]),

@@ -24,8 +24,7 @@ constexpr int kAdSimtChannels = 512;  // input channels that the CUDA cores' for
 constexpr int kAdSimtCluster = 8;
 constexpr int kAdTcStages = 3;        // of 64 input channels
 constexpr int kAdTcCols = 64;         // output columns of a product of the tensor core
-constexpr int kAdTcUps = 3;           // their `up`s that are in shared memory or on their way
-constexpr uint32_t kAdTcTmem = 128;   // columns of tensor memory: the first product's sums, and then two of the second's
+constexpr uint32_t kAdTcTmem = 128;   // columns of tensor memory that it is added up in: two of them
 static_assert(2 * kAdTcCols <= kAdTcTmem, "two accumulators");
 
 struct AdArgs {
@@ -46,6 +45,12 @@ struct AdArgs {
   int vec;                // y and out rows can be read and written in 16 bytes
   uint32_t off_t, off_u;  // shared memory: the finished inner values, `up`
   int32_t* status;
+  // tiles of 128 rows
+  void* terms;            // [tile][part][blocks of 64 inner values, both terms][128 rows of 128 bytes]: the second product's operand
+  int blocks;
+  int group_parts, part_groups;  // parts of a cluster of the first product
+  uint32_t tmem_cols;
+  int block_cols;         // columns of a block of the second product
 };
 
 // ---------------------------------------------------------------------------------------------------------------- the plan
@@ -400,12 +405,15 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kern
 }
 
 // ---------------------------------------------------------------------------------------------------------------- portions: tcgen05
-// A tile of 128 rows is the M of both products.  First: N = the inner values, 64 channels at a time through a ring in shared memory.  Second: K =
-// the inner values' first terms and then their second ones, N = 64 columns, into one of two accumulators, so that a product runs while the
-// one before it is added to y.  Operands lie in the 128-byte-swizzled K-major layout; they come by 16-byte asynchronous copies, since rows lie
-// in any order and the columns of `up` are put so that the accumulator's fragments hold eight columns side by side.
-// No block may wait for tensor memory that another cluster's holds, as clusters could then wait for one another: at most three blocks share a
-// multiprocessor (ad_tc_smem sees to that) and take a quarter of it each, and the next kernel of a chain is not brought up before they have it.
+// Two launches.  First product: a cluster takes a tile of 128 rows (the M of tcgen05.mma) and all parts side by side (N), its blocks share the channels, 64
+// at a time through a ring in shared memory; the sums go to a workspace as the second product's operand lies in shared memory.  Second product: a
+// block takes a tile and up to 256 columns of a part, 64 at a time into one of two accumulators, so that a product runs while the one before
+// it is added to y; K = the inner values' first terms and then their second ones.  With both in one launch, clusters of whole tiles were the unit that
+// multiprocessors are filled by: 2000 rows of rank 64 beside [2048 -> 12288] took 55 us, of which the columns were 23.
+// Operands lie in the 128-byte-swizzled K-major layout; they come by 16-byte asynchronous copies, since rows lie in any order and the columns of
+// `up` are put so that the accumulator's fragments hold eight columns side by side.
+// No block of a cluster may wait for tensor memory that another cluster's holds, as clusters could then wait for one another: ad_first_smem sees to it that the
+// blocks that fit a multiprocessor fit three quarters of its tensor memory, and the next kernel is not brought up before they have theirs.
 __device__ __forceinline__ uint64_t ad_desc(uint32_t saddr) {
   return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
@@ -447,30 +455,32 @@ __device__ __forceinline__ void ad_tc_ld_tiles(uint32_t addr, float (&f)[16]) {
   for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(u[i]);
 }
 
-template <int kC>
-__global__ void __launch_bounds__(kAdThreads, 3) adapter_tiles_kernel(const __grid_constant__ AdArgs a) {
+constexpr int kAdFirstCluster = 8;
+
+__global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ uint8_t ad_raw[];
   __shared__ int rows_of[128];
-  __shared__ __align__(8) uint64_t bars[kAdTcStages + 2];
+  __shared__ __align__(8) uint64_t bars[kAdTcStages];
   __shared__ uint32_t tmem_word;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
+  constexpr int kC = kAdFirstCluster;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)ad_cluster_rank();
   pdl_wait();
-  const AdJob job = ad_job<128, kC>(a);
-  if (job.count <= 0) return;  // (with the whole cluster)
-  if (job.slot < 0) return ad_copy_rows<uint16_t>(a, job, rank, kC);
+  // the parts that this cluster takes
+  const int cl = blockIdx.x / kC, at = cl / a.part_groups, p0 = (cl - at * a.part_groups) * a.group_parts, np = min(a.group_parts, a.parts - p0);
+  const int4 tile = a.tiles[at];
+  const int count = tile.y;
+  if (count <= 0 || tile.x < 0) return;  // (with the whole cluster)
   const uint32_t smem = ((uint32_t)__cvta_generic_to_shared(ad_raw) + 1023u) & ~1023u;
   uint8_t* base = ad_raw + (smem - (uint32_t)__cvta_generic_to_shared(ad_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
-  const auto bar_stage = [&](int s) { return bar + 8 * s; };
-  const auto bar_acc = [&](int s) { return bar + 8 * (kAdTcStages + s); };
-  if (tid < 128) rows_of[tid] = job.order[tid];
+  if (tid < 128) rows_of[tid] = a.order[(long long)at * 128 + tid];
   if (tid == 0) {
-    for (int s = 0; s < kAdTcStages + 2; ++s) dt_mbar_init(bar + 8 * s, 1);
+    for (int s = 0; s < kAdTcStages; ++s) dt_mbar_init(bar + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_word)), "r"(kAdTcTmem) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_word)), "r"(a.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   ad_before_sync();
@@ -480,10 +490,8 @@ __global__ void __launch_bounds__(kAdThreads, 3) adapter_tiles_kernel(const __gr
   const uint32_t tmem = tmem_word;
   bool dead = false;
 
-  // ---- first product: [128 rows] x [inner values, up to a multiple of 16], this block's share of the channels
-  const uint16_t* down = (const uint16_t*)a.down + ((long long)job.slot * a.parts + job.part) * a.rank * a.width;
-  const uint16_t* up = (const uint16_t*)a.up + (long long)job.slot * a.ends[a.parts - 1] * a.rank;
-  const int inner16 = (a.rank + 15) & ~15, steps = (a.width + 63) >> 6;
+  const int inner = np * a.rank, inner16 = (inner + 15) & ~15, steps = (a.width + 63) >> 6;
+  const uint16_t* down = (const uint16_t*)a.down + ((long long)tile.x * a.parts + p0) * a.rank * a.width;
   const int s0 = steps * rank / kC, n = steps * (rank + 1) / kC - s0;
   const uint32_t stage_bytes = 16384 + inner16 * 128;
   auto fetch = [&](int i) {
@@ -498,7 +506,7 @@ __global__ void __launch_bounds__(kAdThreads, 3) adapter_tiles_kernel(const __gr
         ad_copy16(xs + r * 128 + (((tid & 7) ^ (r & 7)) << 4), (const uint16_t*)a.x + (on ? (long long)row * a.x_stride + k : 0), on ? 16 : 0);
       }
       for (int r = tid >> 3; r < inner16; r += 32) {
-        const bool on = in && r < a.rank;
+        const bool on = in && r < inner;
         ad_copy16(ds + r * 128 + (((tid & 7) ^ (r & 7)) << 4), down + (on ? (long long)r * a.width + k : 0), on ? 16 : 0);
       }
     }
@@ -517,45 +525,24 @@ __global__ void __launch_bounds__(kAdThreads, 3) adapter_tiles_kernel(const __gr
       const uint32_t idesc = ad_idesc(inner16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) ad_tc_mma(tmem, da + 2 * j, db + 2 * j, idesc, (i | j) != 0);
-      ad_tc_commit(bar_stage(i % kAdTcStages));
+      ad_tc_commit(bar + 8 * (i % kAdTcStages));
     }
     if (i >= 1) {
       const int free = i - 1;  // its product has had a step's time
-      if (free + kAdTcStages < n && !dt_mbar_wait(bar_stage(free % kAdTcStages), (free / kAdTcStages) & 1)) dead = true;
+      if (free + kAdTcStages < n && !dt_mbar_wait(bar + 8 * (free % kAdTcStages), (free / kAdTcStages) & 1)) dead = true;
       fetch(free + kAdTcStages);
     }
   }
-  if (n > 0 && !dt_mbar_wait(bar_stage((n - 1) % kAdTcStages), ((n - 1) / kAdTcStages) & 1)) dead = true;
+  if (n > 0 && !dt_mbar_wait(bar + 8 * ((n - 1) % kAdTcStages), ((n - 1) / kAdTcStages) & 1)) dead = true;
   ad_wait<0>();
+  dead = __any_sync(0xffffffffu, dead);
   ad_after_sync();
-  __syncthreads();  // (all copies into the ring have ended: what follows lies over it)
+  __syncthreads();  // (all copies into the ring have ended: the partial values lie over it)
 
-  // ---- second product's columns
-  const int cols = job.end - job.begin, tiles = (cols + kAdTcCols - 1) / kAdTcCols;
-  const int c0 = tiles * rank / kC, c1 = tiles * (rank + 1) / kC;
-  const int blocks = (inner16 + 63) >> 6;  // of 64 inner values
-  const uint32_t u_stage = blocks * kAdTcCols * 128, u_base = smem + a.off_u;
-  const int vecs = inner16 >> 3;
-  const unsigned by_vecs = (65536u + vecs - 1) / vecs;  // i / vecs of i < 2048 by a product
-  auto fetch_up = [&](int c) {
-    if (c < c1) {
-      const uint32_t dst = u_base + ((c - c0) % kAdTcUps) * u_stage;
-      const int col0 = job.begin + kAdTcCols * c;
-      for (int i = tid; i < kAdTcCols * vecs; i += kAdThreads) {
-        const int at = (int)((unsigned)i * by_vecs >> 16), v = i - at * vecs, w = at & 31;
-        const int place = (at & ~31) + 8 * ((w >> 1) & 3) + 2 * (w >> 3) + (w & 1);
-        const bool on = col0 + at < job.end && 8 * v < a.rank;
-        ad_copy16(dst + (v >> 3) * (kAdTcCols * 128) + place * 128 + (((v & 7) ^ (place & 7)) << 4), up + (on ? (long long)(col0 + at) * a.rank + 8 * v : 0), on ? 16 : 0);
-      }
-    }
-    ad_commit();
-  };
-
-  // ---- partial inner values, summed over the cluster, as operand of the second product
-  float* part = reinterpret_cast<float*>(base + a.off_t);
+  float* part = reinterpret_cast<float*>(base);
   const int q = warp & 3, half = warp >> 2;  // this warp's lanes of tensor memory; it shares them with another one
-  if (32 * q < job.count) {
-    for (int c = 8 * half; c < a.rank; c += 16) {
+  if (32 * q < count) {
+    for (int c = 8 * half; c < inner; c += 16) {
       float f[8];
       if (n > 0) {
         ad_tc_ld8(tmem + ((uint32_t)(32 * q) << 16) + c, f);
@@ -570,98 +557,156 @@ __global__ void __launch_bounds__(kAdThreads, 3) adapter_tiles_kernel(const __gr
   }
   ad_before_sync();
   ad_cluster_arrive();
+  const float scale = a.scale[tile.x];
+  ad_cluster_wait();
+  // every block sums a share of the rows over all blocks
+  const int quads = inner >> 2, rank16 = (a.rank + 15) & ~15, row0 = 128 / kC * rank;
+  const int items = max(0, min(128 / kC, count - row0)) * quads;
+  uint8_t* out = (uint8_t*)a.terms + ((long long)at * a.parts + p0) * a.blocks * 16384;
+  for (int i = tid; i < items; i += kAdThreads) {
+    const int r = i / quads, row = row0 + r, col = (i - r * quads) * 4, p = col / a.rank, j = col - p * a.rank;
+    uint2 hi, lo;
+    ad_split(ad_total<kC>(smem + (row * a.inner_row + col) * 4, scale), hi, lo);
+    uint8_t* to = out + (long long)p * a.blocks * 16384 + row * 128;
+    const auto place = [&](int k) { return reinterpret_cast<uint2*>(to + (k >> 6) * 16384 + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2); };
+    *place(j) = hi;
+    *place(rank16 + j) = lo;
+    if (j >= a.rank - 8 && (a.rank & 8)) {  // what lies behind a term's values is zero
+      *place(j + 8) = make_uint2(0, 0);
+      *place(rank16 + j + 8) = make_uint2(0, 0);
+    }
+  }
+  asm volatile("fence.proxy.async.global;\n" ::: "memory");  // (the next kernel reads them by bulk copies)
+  if (dead && a.status) atomicOr(a.status, B200KV_S_TIMEOUT);
+  ad_cluster_arrive();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+  ad_cluster_wait();  // nobody reads another block's memory behind this
+}
+
+// grid (column blocks over all parts, tiles)
+__global__ void __launch_bounds__(kAdThreads, 3) adapter_second_kernel(const __grid_constant__ AdArgs a) {
+  extern __shared__ uint8_t ad_raw[];
+  __shared__ __align__(8) uint64_t bars[3];
+  __shared__ uint32_t tmem_word;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
+  if ((blockIdx.x | blockIdx.y) == 0) pdl_wait();
+  // What the first product's kernel waited for is there as soon as this one is brought up; the inner values are not.
+  const int4 tile = a.tiles[blockIdx.y];
+  const int count = tile.y;
+  int part = 0, block = blockIdx.x, begin = 0;
+  for (; part < a.parts - 1; ++part) {
+    const int n = (a.ends[part] - begin + a.block_cols - 1) / a.block_cols;
+    if (block < n) break;
+    block -= n;
+    begin = a.ends[part];
+  }
+  begin += block * a.block_cols;
+  const int end = min(a.ends[part], begin + a.block_cols), cols = end - begin;
+  const int32_t* order = a.order + (long long)blockIdx.y * 128;
+  if (count <= 0) return pdl_wait();
+  if (tile.x < 0) {
+    pdl_wait();
+    if (a.out == a.y) return;
+    for (int i = warp; i < count; i += kAdWarps) {
+      const long long r = order[i];
+      for (int c = begin + lane; c < end; c += 32) ((uint16_t*)a.out)[r * a.out_stride + c] = ((const uint16_t*)a.y)[r * a.y_stride + c];
+    }
+    return;
+  }
+  const uint32_t smem = ((uint32_t)__cvta_generic_to_shared(ad_raw) + 1023u) & ~1023u;
+  const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars), bar_terms = bar + 16;  // accumulators; the inner values
+  const int q = warp & 3, half = warp >> 2;  // this warp's lanes of tensor memory, its half of 64 columns
   // this lane's first column of its four rows
   int rows[4];
   const uint16_t* from[4];
   uint16_t* to[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    rows[i] = rows_of[32 * q + 8 * i + gid];
-    const int col = job.begin + 32 * half + 8 * t;
+    rows[i] = order[32 * q + 8 * i + gid];
+    const int col = begin + 32 * half + 8 * t;
     from[i] = (const uint16_t*)a.y + (long long)max(rows[i], 0) * a.y_stride + col;
     to[i] = (uint16_t*)a.out + (long long)max(rows[i], 0) * a.out_stride + col;
   }
   uint4 yv[4] = {};  // of the next product
-  auto load_y = [&](uint4 (&v)[4], int c) {
-    const bool whole = c < c1 && a.vec && cols - (kAdTcCols * c + 32 * half + 8 * t) >= 8;
+  auto load_y = [&](int c) {
+    const bool whole = a.vec && cols - (kAdTcCols * c + 32 * half + 8 * t) >= 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (whole && rows[i] >= 0) v[i] = *reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c);
+      if (whole && rows[i] >= 0) yv[i] = *reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c);
   };
-  load_y(yv, c0);
-  const float scale = a.scale[job.slot];
-  ad_cluster_wait();
+  load_y(0);
+  // the block's columns of `up`, behind the inner values
+  const int rank16 = (a.rank + 15) & ~15, blocks = (rank16 + 63) >> 6, vecs = rank16 >> 3, products = (cols + kAdTcCols - 1) / kAdTcCols;
+  const uint32_t us = smem + a.blocks * 16384, u_product = blocks * kAdTcCols * 128;
   {
-    const int quads = a.rank >> 2, total = job.count * quads;
-    for (int i = rank * kAdThreads + tid; i < total; i += kC * kAdThreads) {
-      const int row = i / quads, col = (i - row * quads) * 4;
-      uint2 hi, lo;
-      ad_split(ad_total<kC>(smem + a.off_t + (row * a.inner_row + col) * 4, scale), hi, lo);
-      const auto at = [&](int k) { return smem + (k >> 6) * 16384 + row * 128 + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2; };
-      const uint32_t at_hi = at(col), at_lo = at(inner16 + col);
-      const bool pad = col >= a.rank - 8 && (a.rank & 8);  // what lies behind a term's values is zero
-#pragma unroll
-      for (int p = 0; p < kC; ++p) {
-        if (tiles * p / kC == tiles * (p + 1) / kC) continue;  // no columns there
-        ad_st_remote2(ad_at_rank(at_hi, p), hi);
-        ad_st_remote2(ad_at_rank(at_lo, p), lo);
-        if (pad) {
-          ad_st_remote2(ad_at_rank(at(col + 8), p), make_uint2(0, 0));
-          ad_st_remote2(ad_at_rank(at(inner16 + col + 8), p), make_uint2(0, 0));
-        }
-      }
+    const uint16_t* up = (const uint16_t*)a.up + ((long long)tile.x * a.ends[a.parts - 1] + begin) * a.rank;
+    const unsigned by_vecs = (65536u + vecs - 1) / vecs;  // i / vecs of i < 4096 by a product
+    for (int i = tid; i < products * kAdTcCols * vecs; i += kAdThreads) {
+      const int at = (int)((unsigned)i * by_vecs >> 16), v = i - at * vecs, w = at & 31;
+      const int place = (at & 32) + 8 * ((w >> 1) & 3) + 2 * (w >> 3) + (w & 1);
+      const bool on = at < cols && 8 * v < a.rank;
+      ad_copy16(us + (at >> 6) * u_product + (v >> 3) * (kAdTcCols * 128) + place * 128 + (((v & 7) ^ (place & 7)) << 4),
+                up + (on ? (long long)at * a.rank + 8 * v : 0), on ? 16 : 0);
     }
+    ad_commit();
   }
-  asm volatile("fence.proxy.async.shared::cluster;\n" ::: "memory");
-  ad_cluster_arrive();
-  ad_cluster_wait();
-  asm volatile("fence.proxy.async.shared::cluster;\n" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < kAdTcUps; ++i) fetch_up(c0 + i);  // where the partial values were
-
-  // ---- second product
+  if (tid == 0) {
+    for (int s = 0; s < 3; ++s) dt_mbar_init(bar + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_word)), "r"(kAdTcTmem) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  ad_wait<0>();
+  ad_proxy_fence();
+  ad_before_sync();
+  __syncthreads();
+  ad_after_sync();
+  const uint32_t tmem = tmem_word;
+  bool dead = false;
+  pdl_trigger();
+  pdl_wait();
   auto multiply = [&](int c) {  // by one thread
-    ad_after_sync();
-    const int s = (c - c0) & 1;
-    const uint32_t d = tmem + s * kAdTcCols, us = u_base + ((c - c0) % kAdTcUps) * u_stage, idesc = ad_idesc(kAdTcCols);
-    for (int term = 0; term < 2; ++term) {
-      for (int k = 0; k < inner16; k += 16) {
-        const int ka = term * inner16 + k;
-        ad_tc_mma(d, ad_desc(smem + (ka >> 6) * 16384) + ((ka & 63) >> 3), ad_desc(us + (k >> 6) * (kAdTcCols * 128)) + ((k & 63) >> 3), idesc, ka != 0);
-      }
+    const uint32_t d = tmem + (c & 1) * kAdTcCols, idesc = ad_idesc(kAdTcCols);
+    for (int k = 0; k < 2 * rank16; k += 16) {
+      const int ku = k < rank16 ? k : k - rank16;
+      ad_tc_mma(d, ad_desc(smem + (k >> 6) * 16384) + ((k & 63) >> 3),
+                ad_desc(us + c * u_product + (ku >> 6) * (kAdTcCols * 128)) + ((ku & 63) >> 3), idesc, k != 0);
     }
-    ad_tc_commit(bar_acc(s));
+    ad_tc_commit(bar + 8 * (c & 1));
   };
-  if (c0 < c1) {
-    ad_wait<kAdTcUps - 1>();
-    ad_proxy_fence();
-    ad_before_sync();
-    __syncthreads();
-    if (tid == 0) multiply(c0);
+  if (tid == 0) {
+    const uint32_t bytes = a.blocks * 16384;
+    asm volatile("fence.proxy.async.global;\n" ::: "memory");
+    dt_expect_tx(bar_terms, bytes);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(smem), "l"((const uint8_t*)a.terms + ((long long)blockIdx.y * a.parts + part) * bytes), "r"(bytes), "r"(bar_terms) : "memory");
+    if (!dt_mbar_wait(bar_terms, 0)) dead = true;
+    multiply(0);
   }
-  for (int c = c0; c < c1; ++c) {
-    const int i = c - c0, s = i & 1;
-    if (c + 1 < c1) {
-      ad_wait<kAdTcUps - 2>();
-      ad_proxy_fence();
-      __syncthreads();  // the next one's columns are there, its accumulator has been read
-      if (tid == 0) multiply(c + 1);
+  for (int c = 0; c < products; ++c) {
+    if (c + 1 < products) {
+      __syncthreads();  // the next one's accumulator has been read
+      if (tid == 0) {
+        ad_after_sync();
+        multiply(c + 1);
+      }
     }
     uint4 v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = yv[j];
-    load_y(yv, c + 1);
-    if (!dt_mbar_wait(bar_acc(s), (i >> 1) & 1)) dead = true;
+    if (c + 1 < products) load_y(c + 1);
+    if (!dt_mbar_wait(bar + 8 * (c & 1), (c >> 1) & 1)) dead = true;
     dead = __any_sync(0xffffffffu, dead);
     ad_after_sync();
-    fetch_up(c + kAdTcUps);
-    if (32 * q < job.count && !dead) {
+    if (32 * q < count && !dead) {
       const int left = cols - (kAdTcCols * c + 32 * half + 8 * t);
       const bool whole = a.vec && left >= 8;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         float f[16];
-        ad_tc_ld_tiles(tmem + ((uint32_t)(32 * q + 16 * m) << 16) + s * kAdTcCols + 32 * half, f);
+        ad_tc_ld_tiles(tmem + ((uint32_t)(32 * q + 16 * m) << 16) + (c & 1) * kAdTcCols + 32 * half, f);
         const float f0[8] = {f[0], f[1], f[4], f[5], f[8], f[9], f[12], f[13]};
         const float f1[8] = {f[2], f[3], f[6], f[7], f[10], f[11], f[14], f[15]};
         if (rows[2 * m] >= 0) ad_store(from[2 * m] + kAdTcCols * c, to[2 * m] + kAdTcCols * c, left, whole, v[2 * m], f0);
@@ -670,7 +715,6 @@ __global__ void __launch_bounds__(kAdThreads, 3) adapter_tiles_kernel(const __gr
     }
     ad_before_sync();
   }
-  ad_wait<0>();
   if (dead && a.status) atomicOr(a.status, B200KV_S_TIMEOUT);
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kAdTcTmem) : "memory");
@@ -794,18 +838,19 @@ static int ad_rows(AdArgs a, int clusters, int most_cols, cudaStream_t stream) {
   return ad_launch(adapter_rows_kernel<kNT, kKB, kC, kStages>, a, clusters, kC, a.off_u + (size_t)kAdWarps * a.ring * (32 * a.u_row + 1024), stream);
 }
 
-// Shared memory of a tile of 128 rows: the ring; over it the second product's operand, and the partial inner values and then the columns of `up`.
-// Not less than lets three blocks share a multiprocessor.
-static size_t ad_tc_smem(AdArgs* a) {
-  const int inner16 = (a->rank + 15) / 16 * 16;
-  const size_t ring = (size_t)kAdTcStages * (16384 + inner16 * 128), terms = (size_t)(2 * inner16 + 63) / 64 * 16384;
-  a->inner_row = a->rank + 4;
-  a->off_t = (uint32_t)terms;
-  a->off_u = (uint32_t)terms;
-  const size_t ups = (size_t)kAdTcUps * ((inner16 + 63) / 64) * kAdTcCols * 128, partial = (size_t)128 * a->inner_row * 4;
-  const size_t over = terms + (ups > partial ? ups : partial), all = 1024 + (ring > over ? ring : over);
-  return all > 60 * 1024 ? all : 60 * 1024;
+// Tiles of 128 rows: the parts of a cluster, tensor memory and shared memory of the first product.
+static size_t ad_first(AdArgs* a) {
+  a->group_parts = a->parts * a->rank <= 256 ? a->parts : 256 / a->rank;
+  a->part_groups = (a->parts + a->group_parts - 1) / a->group_parts;
+  const int inner = a->group_parts * a->rank, inner16 = (inner + 15) / 16 * 16;
+  a->tmem_cols = 32;
+  while ((int)a->tmem_cols < inner16) a->tmem_cols *= 2;
+  a->inner_row = inner + 4;  // (rows apart by other banks)
+  const size_t ring = (size_t)kAdTcStages * (16384 + inner16 * 128), partial = (size_t)128 * a->inner_row * 4;
+  const size_t all = 1024 + (ring > partial ? ring : partial), least = (a->tmem_cols > 128 ? 116 : 60) * 1024;  // one block a multiprocessor, three
+  return all > least ? all : least;
 }
+static int ad_terms_blocks(int rank) { return (2 * ((rank + 15) / 16 * 16) + 63) / 64; }
 
 }  // namespace b200kv
 
@@ -825,9 +870,14 @@ extern "C" int b200dec_adapter_plan(const int32_t* ids, int32_t num_rows, int32_
                                       (int)num_rows, (int)slots, (int)tile_rows, order, (int4*)tiles, (int)max_tiles, status));
 }
 
+extern "C" size_t b200dec_add_adapters_workspace(const b200dec_adapters* ad, int32_t max_tiles, int32_t tile_rows) {
+  if (!ad || tile_rows != 128 || ad->elem != 2 || max_tiles < 1 || ad->parts < 1 || ad->rank < 8) return 0;
+  return (size_t)max_tiles * ad->parts * ad_terms_blocks(ad->rank) * 16384;
+}
+
 extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out,
                                     int64_t out_stride, const int32_t* order, const int32_t* tiles, int32_t max_tiles, int32_t tile_rows,
-                                    int32_t num_rows, int32_t* status, void* stream) {
+                                    int32_t num_rows, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   if (num_rows == 0) return B200KV_OK;
   if (!ad || !ad->down || !ad->up || !ad->scale || !x || !y || !out || !order || !tiles) return B200KV_E_NULL;
   if (num_rows < 0 || max_tiles < 1 || ad->slots < 1 || ad->slots > kAdMaxSlots) return B200KV_E_RANGE;
@@ -851,7 +901,7 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, i
   }
   const int cols = a.ends[a.parts - 1];
   if (x_stride < a.width || y_stride < cols || out_stride < cols || out == x) return B200KV_E_SHAPE;
-  if ((out == y && out_stride != y_stride) || (long long)max_tiles * tile_rows * a.parts > 0x0fffffffLL) return B200KV_E_RANGE;
+  if ((out == y && out_stride != y_stride) || (long long)max_tiles * tile_rows * a.parts > 0x0fffffffLL || (tile_rows == 128 && max_tiles > 65535)) return B200KV_E_RANGE;
   if (!aligned(ad->down, 16) || !aligned(ad->up, 16) || !aligned(ad->scale, 4) || !aligned(tiles, 16) || !aligned(order, 4) || !aligned(x, ad->elem) ||
       !aligned(y, ad->elem) || !aligned(out, ad->elem))
     return B200KV_E_ALIGN;
@@ -867,9 +917,22 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, i
                          : ad_launch(adapter_simt_kernel<uint16_t>, a, fine, kAdSimtCluster, smem, s);
   }
   if (tile_rows == 128) {
-    const size_t smem = ad_tc_smem(&a);
-    const char* ce = getenv("AD_C");
-    return ce && ce[0] == '4' ? ad_launch(adapter_tiles_kernel<4>, a, clusters, 4, smem, s) : ad_launch(adapter_tiles_kernel<8>, a, clusters, 8, smem, s);
+    a.blocks = ad_terms_blocks(a.rank);
+    a.terms = workspace;
+    if (!workspace || workspace_bytes < b200dec_add_adapters_workspace(ad, max_tiles, tile_rows)) return B200KV_E_WORKSPACE;
+    if (!aligned(workspace, 16)) return B200KV_E_ALIGN;
+    const size_t smem = ad_first(&a);
+    if (int rc = ad_launch(adapter_first_kernel, a, max_tiles * a.part_groups, kAdFirstCluster, smem, s)) return rc;
+    const int ublocks = ((a.rank + 15) / 16 * 16 + 63) / 64;
+    a.block_cols = ublocks > 1 ? 128 : 256;
+    const char* bc = getenv("AD_B");
+    if (bc) a.block_cols = atoi(bc);
+    int col_blocks = 0;
+    for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) col_blocks += (a.ends[p] - begin + a.block_cols - 1) / a.block_cols;
+    const size_t second = 1024 + (size_t)a.blocks * 16384 + (size_t)a.block_cols * ublocks * 128;
+    if (!allow_smem(adapter_second_kernel, kAdMostSmem)) return launch_result(cudaErrorInvalidValue);
+    // brought up while the first one runs, whatever launches of the library are: it waits for it, and nothing else stands between them
+    return launch_result(launch_kernel(true, adapter_second_kernel, dim3((unsigned)col_blocks, (unsigned)max_tiles), dim3(kAdThreads), second, s, a));
   }
   const int kb = (a.rank + 15) / 16;
   const char* ce = getenv("AD_C");

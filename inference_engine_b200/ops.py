@@ -754,8 +754,13 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Ada
         raise ValueError(f"add_adapters: a plan for {plan.slots} slots and {adapters.slots} adapters")
     # (a single row's stride may be anything)
     xs, ys, os = (t.stride(0) if N > 1 else _round8(t.shape[1]) for t in (x, y, out))
-    rc = _lib_dec().b200dec_add_adapters(ctypes.byref(adapters.struct), x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, plan.order.data_ptr(),
-                                         plan.tiles.data_ptr(), *plan.order.shape, N, K.status_word(y.device).data_ptr(), K._stream())
+    lib, ad, (tiles, tile_rows) = _lib_dec(), ctypes.byref(adapters.struct), plan.order.shape
+    ws, nbytes = None, 0
+    if tile_rows > 16:
+        nbytes = lib.b200dec_add_adapters_workspace(ad, tiles, tile_rows)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=y.device)
+    rc = lib.b200dec_add_adapters(ad, x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, plan.order.data_ptr(), plan.tiles.data_ptr(), tiles,
+                                  tile_rows, N, _ptr(ws), nbytes, K.status_word(y.device).data_ptr(), K._stream())
     _lib.check(rc, "add_adapters")
     return out
 
