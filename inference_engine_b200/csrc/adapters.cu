@@ -11,7 +11,6 @@
 // Precision: bf16 operands, 32-bit sums.  The inner values are scaled in 32 bits and enter the second product as two bf16 terms (16 bits of
 // mantissa): rounded to one they would cost the sum as much as its own rounding does.
 #include "dec_tma.cuh"
-#include <cstdlib>
 
 namespace b200kv {
 
@@ -22,10 +21,8 @@ constexpr int kAdMaxSlots = 4096;
 constexpr int kAdPlanThreads = 1024;
 constexpr int kAdSimtChannels = 512;  // input channels that the CUDA cores' form stages at a time
 constexpr int kAdSimtCluster = 8;
-constexpr int kAdTcStages = 3;        // of 64 input channels
-constexpr int kAdTcCols = 64;         // output columns of a product of the tensor core
-constexpr uint32_t kAdTcTmem = 128;   // columns of tensor memory that it is added up in: two of them
-static_assert(2 * kAdTcCols <= kAdTcTmem, "two accumulators");
+constexpr int kAdTcCols = 128;        // output columns of a product of the tensor core
+constexpr int kAdSecondThreads = 320;
 
 struct AdArgs {
   const void *down, *up;
@@ -50,7 +47,7 @@ struct AdArgs {
   int blocks;
   int group_parts, part_groups;  // parts of a cluster of the first product
   uint32_t tmem_cols;
-  int block_cols;         // columns of a block of the second product
+  int run;                // column blocks of a block of the second product
 };
 
 // ---------------------------------------------------------------------------------------------------------------- the plan
@@ -407,8 +404,7 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kern
 // ---------------------------------------------------------------------------------------------------------------- portions: tcgen05
 // Two launches.  First product: a cluster takes a tile of 128 rows (the M of tcgen05.mma) and all parts side by side (N), its blocks share the channels, 64
 // at a time through a ring in shared memory; the sums go to a workspace as the second product's operand lies in shared memory.  Second product: a
-// block takes a tile and up to 256 columns of a part, 64 at a time into one of two accumulators, so that a product runs while the one before
-// it is added to y; K = the inner values' first terms and then their second ones.  With both in one launch, clusters of whole tiles were the unit that
+// block takes a tile and a run of columns of a part, 128 at a time; K = the inner values' first terms and then their second ones.  With both in one launch, clusters of whole tiles were the unit that
 // multiprocessors are filled by: 2000 rows of rank 64 beside [2048 -> 12288] took 55 us, of which the columns were 23.
 // Operands lie in the 128-byte-swizzled K-major layout; they come by 16-byte asynchronous copies, since rows lie in any order and the columns of
 // `up` are put so that the accumulator's fragments hold eight columns side by side.
@@ -455,14 +451,12 @@ __device__ __forceinline__ void ad_tc_ld_tiles(uint32_t addr, float (&f)[16]) {
   for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(u[i]);
 }
 
-constexpr int kAdFirstCluster = 8;
-
+template <int kC, int kStages>
 __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ uint8_t ad_raw[];
   __shared__ int rows_of[128];
-  __shared__ __align__(8) uint64_t bars[kAdTcStages];
+  __shared__ __align__(8) uint64_t bars[kStages];
   __shared__ uint32_t tmem_word;
-  constexpr int kC = kAdFirstCluster;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)ad_cluster_rank();
   pdl_wait();
@@ -476,7 +470,7 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
   if (tid < 128) rows_of[tid] = a.order[(long long)at * 128 + tid];
   if (tid == 0) {
-    for (int s = 0; s < kAdTcStages; ++s) dt_mbar_init(bar + 8 * s, 1);
+    for (int s = 0; s < kStages; ++s) dt_mbar_init(bar + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
@@ -496,7 +490,7 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
   const uint32_t stage_bytes = 16384 + inner16 * 128;
   auto fetch = [&](int i) {
     if (i < n) {
-      const uint32_t xs = smem + (i % kAdTcStages) * stage_bytes, ds = xs + 16384;
+      const uint32_t xs = smem + (i % kStages) * stage_bytes, ds = xs + 16384;
       const int k = 64 * (s0 + i) + 8 * (tid & 7);
       const bool in = k < a.width;
 #pragma unroll
@@ -513,27 +507,27 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
     ad_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kAdTcStages; ++i) fetch(i);
+  for (int i = 0; i < kStages; ++i) fetch(i);
   for (int i = 0; i < n; ++i) {
-    ad_wait<kAdTcStages - 2>();
+    ad_wait<kStages - 2>();
     ad_proxy_fence();
     __syncthreads();
     if (tid == 0) {
       ad_after_sync();
-      const uint32_t xs = smem + (i % kAdTcStages) * stage_bytes;
+      const uint32_t xs = smem + (i % kStages) * stage_bytes;
       const uint64_t da = ad_desc(xs), db = ad_desc(xs + 16384);
       const uint32_t idesc = ad_idesc(inner16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) ad_tc_mma(tmem, da + 2 * j, db + 2 * j, idesc, (i | j) != 0);
-      ad_tc_commit(bar + 8 * (i % kAdTcStages));
+      ad_tc_commit(bar + 8 * (i % kStages));
     }
     if (i >= 1) {
       const int free = i - 1;  // its product has had a step's time
-      if (free + kAdTcStages < n && !dt_mbar_wait(bar + 8 * (free % kAdTcStages), (free / kAdTcStages) & 1)) dead = true;
-      fetch(free + kAdTcStages);
+      if (free + kStages < n && !dt_mbar_wait(bar + 8 * (free % kStages), (free / kStages) & 1)) dead = true;
+      fetch(free + kStages);
     }
   }
-  if (n > 0 && !dt_mbar_wait(bar + 8 * ((n - 1) % kAdTcStages), ((n - 1) / kAdTcStages) & 1)) dead = true;
+  if (n > 0 && !dt_mbar_wait(bar + 8 * ((n - 1) % kStages), ((n - 1) / kStages) & 1)) dead = true;
   ad_wait<0>();
   dead = __any_sync(0xffffffffu, dead);
   ad_after_sync();
@@ -583,141 +577,188 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
   ad_cluster_wait();  // nobody reads another block's memory behind this
 }
 
-// grid (column blocks over all parts, tiles)
-__global__ void __launch_bounds__(kAdThreads, 3) adapter_second_kernel(const __grid_constant__ AdArgs a) {
+// grid (runs of a.run column blocks over all parts, tiles).  Warps 0 to 7 add to y, a product's two halves of columns in four quarters of rows; one lane of warp 8
+// issues the products, into two accumulators in turn; warp 9 brings the columns of `up`, two blocks in shared memory or on their way.  Two blocks
+// share a multiprocessor and hold half of its tensor memory each; neither waits for another one, so that a third could only wait for their end.
+__global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ uint8_t ad_raw[];
-  __shared__ __align__(8) uint64_t bars[3];
+  __shared__ __align__(8) uint64_t bars[9];
   __shared__ uint32_t tmem_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
   if ((blockIdx.x | blockIdx.y) == 0) pdl_wait();
   // What the first product's kernel waited for is there as soon as this one is brought up; the inner values are not.
   const int4 tile = a.tiles[blockIdx.y];
   const int count = tile.y;
-  int part = 0, block = blockIdx.x, begin = 0;
+  int part = 0, run = blockIdx.x, begin = 0;
   for (; part < a.parts - 1; ++part) {
-    const int n = (a.ends[part] - begin + a.block_cols - 1) / a.block_cols;
-    if (block < n) break;
-    block -= n;
+    const int n = ((a.ends[part] - begin + kAdTcCols - 1) / kAdTcCols + a.run - 1) / a.run;
+    if (run < n) break;
+    run -= n;
     begin = a.ends[part];
   }
-  begin += block * a.block_cols;
-  const int end = min(a.ends[part], begin + a.block_cols), cols = end - begin;
+  begin += run * a.run * kAdTcCols;
+  const int cols = min(a.ends[part] - begin, a.run * kAdTcCols), products = (cols + kAdTcCols - 1) / kAdTcCols;
   const int32_t* order = a.order + (long long)blockIdx.y * 128;
   if (count <= 0) return pdl_wait();
   if (tile.x < 0) {
     pdl_wait();
     if (a.out == a.y) return;
-    for (int i = warp; i < count; i += kAdWarps) {
+    for (int i = warp; i < count; i += kAdSecondThreads / 32) {
       const long long r = order[i];
-      for (int c = begin + lane; c < end; c += 32) ((uint16_t*)a.out)[r * a.out_stride + c] = ((const uint16_t*)a.y)[r * a.y_stride + c];
+      for (int c = begin + lane; c < begin + cols; c += 32) ((uint16_t*)a.out)[r * a.out_stride + c] = ((const uint16_t*)a.y)[r * a.y_stride + c];
     }
     return;
   }
   const uint32_t smem = ((uint32_t)__cvta_generic_to_shared(ad_raw) + 1023u) & ~1023u;
-  const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars), bar_terms = bar + 16;  // accumulators; the inner values
-  const int q = warp & 3, half = warp >> 2;  // this warp's lanes of tensor memory, its half of 64 columns
+  const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
+  const auto acc_full = [&](int i) { return bar + 8 * (i & 1); };
+  const auto acc_free = [&](int i) { return bar + 16 + 8 * (i & 1); };
+  const auto up_full = [&](int i) { return bar + 32 + 8 * (i & 1); };
+  const auto up_free = [&](int i) { return bar + 48 + 8 * (i & 1); };
+  const uint32_t bar_terms = bar + 64;
+  const int q = warp & 3, half = (warp >> 2) & 1;  // this warp's lanes of tensor memory, its half of 128 columns
   // this lane's first column of its four rows
   int rows[4];
   const uint16_t* from[4];
-  uint16_t* to[4];
+  uint4 v[2][4] = {};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    rows[i] = order[32 * q + 8 * i + gid];
-    const int col = begin + 32 * half + 8 * t;
-    from[i] = (const uint16_t*)a.y + (long long)max(rows[i], 0) * a.y_stride + col;
-    to[i] = (uint16_t*)a.out + (long long)max(rows[i], 0) * a.out_stride + col;
+    rows[i] = warp < 8 ? order[32 * q + 8 * i + gid] : -1;
+    from[i] = (const uint16_t*)a.y + (long long)max(rows[i], 0) * a.y_stride + begin + 64 * half + 8 * t;
   }
-  uint4 yv[4] = {};  // of the next product
-  auto load_y = [&](int c) {
-    const bool whole = a.vec && cols - (kAdTcCols * c + 32 * half + 8 * t) >= 8;
+  auto load_y = [&](int c, int g) {  // 32 columns
+    const bool whole = a.vec && cols - (kAdTcCols * c + 64 * half + 32 * g + 8 * t) >= 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (whole && rows[i] >= 0) yv[i] = *reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c);
+      if (whole && rows[i] >= 0) v[g][i] = *reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c + 32 * g);
   };
-  load_y(0);
-  // the block's columns of `up`, behind the inner values
-  const int rank16 = (a.rank + 15) & ~15, blocks = (rank16 + 63) >> 6, vecs = rank16 >> 3, products = (cols + kAdTcCols - 1) / kAdTcCols;
-  const uint32_t us = smem + a.blocks * 16384, u_product = blocks * kAdTcCols * 128;
-  {
-    const uint16_t* up = (const uint16_t*)a.up + ((long long)tile.x * a.ends[a.parts - 1] + begin) * a.rank;
-    const unsigned by_vecs = (65536u + vecs - 1) / vecs;  // i / vecs of i < 4096 by a product
-    for (int i = tid; i < products * kAdTcCols * vecs; i += kAdThreads) {
-      const int at = (int)((unsigned)i * by_vecs >> 16), v = i - at * vecs, w = at & 31;
-      const int place = (at & 32) + 8 * ((w >> 1) & 3) + 2 * (w >> 3) + (w & 1);
-      const bool on = at < cols && 8 * v < a.rank;
-      ad_copy16(us + (at >> 6) * u_product + (v >> 3) * (kAdTcCols * 128) + place * 128 + (((v & 7) ^ (place & 7)) << 4),
-                up + (on ? (long long)at * a.rank + 8 * v : 0), on ? 16 : 0);
+  load_y(0, 0);
+  load_y(0, 1);
+  // the rest of y on its way to L2, so that no load waits for memory
+  if (tid < 128 && a.vec && cols > kAdTcCols + 8) {
+    const int row = order[tid];
+    if (row >= 0)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"((const uint16_t*)a.y + (long long)row * a.y_stride + begin + kAdTcCols),
+                   "r"((cols - kAdTcCols) / 8 * 16) : "memory");
+  }
+  const int rank16 = (a.rank + 15) & ~15, vecs = rank16 >> 3;
+  const uint32_t us = smem + a.blocks * 16384, u_stage = ((rank16 + 63) >> 6) * kAdTcCols * 128;  // `up` lies behind the inner values
+  auto fetch_up = [&](int c) {
+    const uint16_t* up = (const uint16_t*)a.up + ((long long)tile.x * a.ends[a.parts - 1] + begin + kAdTcCols * c) * a.rank;
+    const uint32_t dst = us + (c & 1) * u_stage;
+    const unsigned by_vecs = (65536u + vecs - 1) / vecs;  // i / vecs of i < 512 by a product
+    const long long next = 32ll * a.rank;
+    const int left = cols - kAdTcCols * c;
+#pragma unroll 2
+    for (int i = lane; i < 32 * vecs; i += 32) {  // of each 32 columns
+      const int at = (int)((unsigned)i * by_vecs >> 16), k = i - at * vecs;
+      const int place = 8 * ((at >> 1) & 3) + 2 * (at >> 3) + (at & 1);
+      const uint32_t to = dst + (k >> 3) * (kAdTcCols * 128) + place * 128 + (((k & 7) ^ (place & 7)) << 4);
+      const int bytes = 8 * k < a.rank ? 16 : 0;
+      const uint16_t* src = bytes ? up + at * a.rank + 8 * k : up;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const bool on = at + 32 * g < left;
+        ad_copy16(to + g * 4096, on ? src : (const uint16_t*)a.up, on ? bytes : 0);
+        src += next;
+      }
     }
     ad_commit();
-  }
+  };
+  if (warp == 9) fetch_up(0);
   if (tid == 0) {
-    for (int s = 0; s < 3; ++s) dt_mbar_init(bar + 8 * s, 1);
+    for (int i = 0; i < 2; ++i) {
+      dt_mbar_init(acc_full(i), 1);
+      dt_mbar_init(acc_free(i), 8);
+      dt_mbar_init(up_full(i), 1);
+      dt_mbar_init(up_free(i), 1);
+    }
+    dt_mbar_init(bar_terms, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_word)), "r"(kAdTcTmem) : "memory");
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_word)), "r"(2 * kAdTcCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
-  ad_wait<0>();
-  ad_proxy_fence();
   ad_before_sync();
   __syncthreads();
   ad_after_sync();
   const uint32_t tmem = tmem_word;
-  bool dead = false;
   pdl_trigger();
   pdl_wait();
-  auto multiply = [&](int c) {  // by one thread
-    const uint32_t d = tmem + (c & 1) * kAdTcCols, idesc = ad_idesc(kAdTcCols);
-    for (int k = 0; k < 2 * rank16; k += 16) {
-      const int ku = k < rank16 ? k : k - rank16;
-      ad_tc_mma(d, ad_desc(smem + (k >> 6) * 16384) + ((k & 63) >> 3),
-                ad_desc(us + c * u_product + (ku >> 6) * (kAdTcCols * 128)) + ((ku & 63) >> 3), idesc, k != 0);
+  bool dead = false;
+  if (warp == 9) {
+    for (int c = 1; c <= products; ++c) {
+      if (c < products) {
+        if (c >= 2 && !dt_mbar_wait(up_free(c), ((c >> 1) - 1) & 1)) dead = true;
+        fetch_up(c);
+        ad_wait<1>();
+      } else {
+        ad_wait<0>();
+      }
+      ad_proxy_fence();
+      __syncwarp();
+      if (lane == 0) dt_mbar_arrive(up_full(c - 1));
     }
-    ad_tc_commit(bar + 8 * (c & 1));
-  };
-  if (tid == 0) {
-    const uint32_t bytes = a.blocks * 16384;
-    asm volatile("fence.proxy.async.global;\n" ::: "memory");
-    dt_expect_tx(bar_terms, bytes);
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                 ::"r"(smem), "l"((const uint8_t*)a.terms + ((long long)blockIdx.y * a.parts + part) * bytes), "r"(bytes), "r"(bar_terms) : "memory");
-    if (!dt_mbar_wait(bar_terms, 0)) dead = true;
-    multiply(0);
-  }
-  for (int c = 0; c < products; ++c) {
-    if (c + 1 < products) {
-      __syncthreads();  // the next one's accumulator has been read
-      if (tid == 0) {
+  } else if (warp == 8) {
+    if (lane == 0) {
+      const uint32_t bytes = a.blocks * 16384;
+      asm volatile("fence.proxy.async.global;\n" ::: "memory");
+      dt_expect_tx(bar_terms, bytes);
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                   ::"r"(smem), "l"((const uint8_t*)a.terms + ((long long)blockIdx.y * a.parts + part) * bytes), "r"(bytes), "r"(bar_terms) : "memory");
+      if (!dt_mbar_wait(bar_terms, 0)) dead = true;
+      const uint32_t idesc = ad_idesc(kAdTcCols);
+      const uint64_t da = ad_desc(smem), db = ad_desc(us);  // (in steps of 16 bytes)
+      for (int c = 0; c < products; ++c) {
+        if (!dt_mbar_wait(up_full(c), (c >> 1) & 1)) dead = true;
+        if (c >= 2 && !dt_mbar_wait(acc_free(c), ((c >> 1) - 1) & 1)) dead = true;
         ad_after_sync();
-        multiply(c + 1);
+        for (int k = 0; k < 2 * rank16; k += 16) {
+          const int ku = k < rank16 ? k : k - rank16;
+          ad_tc_mma(tmem + (c & 1) * kAdTcCols, da + (k >> 6) * 1024 + ((k & 63) >> 3),
+                    db + (c & 1) * (u_stage >> 4) + (ku >> 6) * (kAdTcCols * 8) + ((ku & 63) >> 3), idesc, k != 0);
+        }
+        ad_tc_commit(acc_full(c));
+        ad_tc_commit(up_free(c));
       }
     }
-    uint4 v[4];
+    __syncwarp();
+  } else {
+    for (int c = 0; c < products; ++c) {
+      if (!dt_mbar_wait(acc_full(c), (c >> 1) & 1)) dead = true;
+      dead = __any_sync(0xffffffffu, dead);
+      ad_after_sync();
+      if (32 * q < count && !dead) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = yv[j];
-    if (c + 1 < products) load_y(c + 1);
-    if (!dt_mbar_wait(bar + 8 * (c & 1), (c >> 1) & 1)) dead = true;
-    dead = __any_sync(0xffffffffu, dead);
-    ad_after_sync();
-    if (32 * q < count && !dead) {
-      const int left = cols - (kAdTcCols * c + 32 * half + 8 * t);
-      const bool whole = a.vec && left >= 8;
+        for (int g = 0; g < 2; ++g) {
+          const int at = kAdTcCols * c + 32 * g, left = cols - (at + 64 * half + 8 * t);
+          const bool whole = a.vec && left >= 8;
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        float f[16];
-        ad_tc_ld_tiles(tmem + ((uint32_t)(32 * q + 16 * m) << 16) + (c & 1) * kAdTcCols + 32 * half, f);
-        const float f0[8] = {f[0], f[1], f[4], f[5], f[8], f[9], f[12], f[13]};
-        const float f1[8] = {f[2], f[3], f[6], f[7], f[10], f[11], f[14], f[15]};
-        if (rows[2 * m] >= 0) ad_store(from[2 * m] + kAdTcCols * c, to[2 * m] + kAdTcCols * c, left, whole, v[2 * m], f0);
-        if (rows[2 * m + 1] >= 0) ad_store(from[2 * m + 1] + kAdTcCols * c, to[2 * m + 1] + kAdTcCols * c, left, whole, v[2 * m + 1], f1);
+          for (int m = 0; m < 2; ++m) {
+            float f[16];
+            ad_tc_ld_tiles(tmem + ((uint32_t)(32 * q + 16 * m) << 16) + (c & 1) * kAdTcCols + 32 * g + 64 * half, f);
+            const float f0[8] = {f[0], f[1], f[4], f[5], f[8], f[9], f[12], f[13]};
+            const float f1[8] = {f[2], f[3], f[6], f[7], f[10], f[11], f[14], f[15]};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int i = 2 * m + h;
+              uint16_t* to = (uint16_t*)a.out + (long long)rows[i] * a.out_stride + begin + 64 * half + 8 * t + at;
+              if (rows[i] >= 0) ad_store(from[i] + at, to, left, whole, v[g][i], h ? f1 : f0);
+            }
+          }
+          if (c + 1 < products) load_y(c + 1, g);
+        }
       }
+      ad_before_sync();
+      __syncwarp();
+      if (lane == 0) dt_mbar_arrive(acc_free(c));
     }
-    ad_before_sync();
   }
   if (dead && a.status) atomicOr(a.status, B200KV_S_TIMEOUT);
+  ad_before_sync();
   __syncthreads();
-  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kAdTcTmem) : "memory");
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(2 * kAdTcCols) : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------------------------- CUDA cores
@@ -825,7 +866,7 @@ static int ad_launch(void (*kernel)(KArgs...), const AdArgs& a, int clusters, in
 }
 
 template <int kNT, int kKB, int kC, int kStages>
-static int ad_rows(AdArgs a, int clusters, int most_cols, cudaStream_t stream) {
+static int ad_rows_of(AdArgs a, int clusters, int most_cols, cudaStream_t stream) {
   a.inner_row = a.rank + 4;                    // (rows apart by other banks)
   a.t_row = (a.rank * 4 + 63) / 64 * 64 + 32;  // both terms; four rows at different banks
   a.u_row = a.rank * 2;
@@ -838,15 +879,26 @@ static int ad_rows(AdArgs a, int clusters, int most_cols, cudaStream_t stream) {
   return ad_launch(adapter_rows_kernel<kNT, kKB, kC, kStages>, a, clusters, kC, a.off_u + (size_t)kAdWarps * a.ring * (32 * a.u_row + 1024), stream);
 }
 
+// A cluster has as many blocks as leave all of them resident at once, three a multiprocessor: fewer fetch a tile's weights one after the other, more wait for
+// a place.  us with 8, 4 and 2 blocks, rank 16, rows of 48 adapters: three parts of [2048 -> 4096] 14.9, 11.8 and 8.4, one of [2048 -> 2048] 6.7, 6.3 and
+// 7.3, two of [2048 -> 12288] 16.7, 12.3 and 16.4, [6144 -> 2048] 7.7, 8.2 and 10.2; one row beside [2048 -> 12288] 5.6, 7.7 and 12.0.
+template <int kNT, int kKB, int kStages>
+static int ad_rows(const AdArgs& a, int clusters, int most_cols, cudaStream_t stream) {
+  const int room = 3 * device_sms();
+  if ((long long)clusters * 8 <= room) return ad_rows_of<kNT, kKB, 8, kStages>(a, clusters, most_cols, stream);
+  if ((long long)clusters * 4 <= room) return ad_rows_of<kNT, kKB, 4, kStages>(a, clusters, most_cols, stream);
+  return ad_rows_of<kNT, kKB, 2, kStages>(a, clusters, most_cols, stream);
+}
+
 // Tiles of 128 rows: the parts of a cluster, tensor memory and shared memory of the first product.
-static size_t ad_first(AdArgs* a) {
+static size_t ad_first(AdArgs* a, int stages) {
   a->group_parts = a->parts * a->rank <= 256 ? a->parts : 256 / a->rank;
   a->part_groups = (a->parts + a->group_parts - 1) / a->group_parts;
   const int inner = a->group_parts * a->rank, inner16 = (inner + 15) / 16 * 16;
   a->tmem_cols = 32;
   while ((int)a->tmem_cols < inner16) a->tmem_cols *= 2;
   a->inner_row = inner + 4;  // (rows apart by other banks)
-  const size_t ring = (size_t)kAdTcStages * (16384 + inner16 * 128), partial = (size_t)128 * a->inner_row * 4;
+  const size_t ring = (size_t)stages * (16384 + inner16 * 128), partial = (size_t)128 * a->inner_row * 4;
   const size_t all = 1024 + (ring > partial ? ring : partial), least = (a->tmem_cols > 128 ? 116 : 60) * 1024;  // one block a multiprocessor, three
   return all > least ? all : least;
 }
@@ -921,25 +973,34 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, i
     a.terms = workspace;
     if (!workspace || workspace_bytes < b200dec_add_adapters_workspace(ad, max_tiles, tile_rows)) return B200KV_E_WORKSPACE;
     if (!aligned(workspace, 16)) return B200KV_E_ALIGN;
-    const size_t smem = ad_first(&a);
-    if (int rc = ad_launch(adapter_first_kernel, a, max_tiles * a.part_groups, kAdFirstCluster, smem, s)) return rc;
+    // Clusters are of eight blocks where that many fit at once (a graphics cluster's multiprocessors are rarely a multiple of eight: about a seventh is left
+    // over), else of four, and copies run further ahead where a multiprocessor has one block anyway.
+    const size_t smem = ad_first(&a, 3), deep = ad_first(&a, 5);
+    const int first = max_tiles * a.part_groups, sms = device_sms();
+    const int fit = (int)(227 * 1024 / (smem + 2048)), room = sms * 6 / 7;
+    int rc;
+    if (first * 8 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<8, 5>, a, first, 8, deep, s);
+    else if (first * 8 <= room * fit) rc = ad_launch(adapter_first_kernel<8, 3>, a, first, 8, smem, s);
+    else if (first * 4 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<4, 5>, a, first, 4, deep, s);
+    else rc = ad_launch(adapter_first_kernel<4, 3>, a, first, 4, smem, s);
+    if (rc) return rc;
     const int ublocks = ((a.rank + 15) / 16 * 16 + 63) / 64;
-    a.block_cols = ublocks > 1 ? 128 : 256;
-    const char* bc = getenv("AD_B");
-    if (bc) a.block_cols = atoi(bc);
-    int col_blocks = 0;
-    for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) col_blocks += (a.ends[p] - begin + a.block_cols - 1) / a.block_cols;
-    const size_t second = 1024 + (size_t)a.blocks * 16384 + (size_t)a.block_cols * ublocks * 128;
-    if (!allow_smem(adapter_second_kernel, kAdMostSmem)) return launch_result(cudaErrorInvalidValue);
+    int col_blocks = 0, runs = 0;
+    for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) col_blocks += (a.ends[p] - begin + kAdTcCols - 1) / kAdTcCols;
+    // runs for which all blocks are resident at once, two a multiprocessor
+    a.run = (int)(((long long)col_blocks * max_tiles + 2 * sms - 1) / (2 * sms));
+    if (a.run < 1) a.run = 1;
+    for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) runs += ((a.ends[p] - begin + kAdTcCols - 1) / kAdTcCols + a.run - 1) / a.run;
+    const dim3 grid((unsigned)runs, (unsigned)max_tiles);
+    const size_t second = 1024 + (size_t)a.blocks * 16384 + (size_t)2 * ublocks * kAdTcCols * 128;
+    auto kernel = adapter_second_kernel;
+    if (!allow_smem(kernel, kAdMostSmem)) return launch_result(cudaErrorInvalidValue);
     // brought up while the first one runs, whatever launches of the library are: it waits for it, and nothing else stands between them
-    return launch_result(launch_kernel(true, adapter_second_kernel, dim3((unsigned)col_blocks, (unsigned)max_tiles), dim3(kAdThreads), second, s, a));
+    return launch_result(launch_kernel(true, kernel, grid, dim3(kAdSecondThreads), second, s, a));
   }
   const int kb = (a.rank + 15) / 16;
-  const char* ce = getenv("AD_C");
-  if (ce && ce[0] == '4' && kb <= 1) return ad_rows<2, 1, 4, 3>(a, fine, most, s);
-  if (ce && ce[0] == '2' && kb <= 1) return ad_rows<2, 1, 2, 3>(a, fine, most, s);
-  if (kb <= 1) return ad_rows<2, 1, 8, 3>(a, fine, most, s);
-  if (kb <= 2) return ad_rows<4, 2, 8, 3>(a, fine, most, s);
-  if (kb <= 4) return ad_rows<8, 4, 8, 2>(a, fine, most, s);
-  return ad_rows<8, 8, 8, 2>(a, fine, most, s);
+  if (kb <= 1) return ad_rows<2, 1, 3>(a, fine, most, s);
+  if (kb <= 2) return ad_rows<4, 2, 3>(a, fine, most, s);
+  if (kb <= 4) return ad_rows<8, 4, 2>(a, fine, most, s);
+  return ad_rows<8, 8, 2>(a, fine, most, s);
 }
