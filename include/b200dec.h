@@ -254,21 +254,27 @@ typedef struct b200dec_adapters {
   int32_t ends[4];
 } b200dec_adapters;
 
-/* A step's rows sorted by adapter, for every projection of the step.  ids int32 [num_rows]: the adapter of each row, -1: none (any other id
- * outside [0, slots) counts as that and sets B200KV_S_BAD_POSITION).  order int32 [max_tiles, tile_rows] and tiles int32 [max_tiles, 4] (16-byte aligned)
- * are written: a tile's rows, -1 behind them, and its adapter (or -1) and number of rows.  max_tiles >= num_rows / tile_rows + min(num_rows,
- * slots + 1).  tile_rows: 16 or 128. */
-int b200dec_adapter_plan(const int32_t* ids, int32_t num_rows, int32_t slots, int32_t tile_rows, int32_t* order, int32_t* tiles,
-                         int32_t max_tiles, int32_t* status, void* stream);
+/* A step's rows sorted by adapter, for every projection of the step: the caller's buffers and the numbers that they are for.  order int32
+ * [max_tiles, tile_rows]: a tile's rows, -1 behind them; tiles int32 [max_tiles, 4] (16-byte aligned): its adapter (or -1) and number of rows.
+ * tile_rows: 16 or 128; max_tiles >= num_rows / tile_rows + min(num_rows, slots + 1). */
+typedef struct b200dec_adapter_plan {
+  int32_t* order;
+  int32_t* tiles;
+  int32_t max_tiles, tile_rows, num_rows, slots;
+} b200dec_adapter_plan_t;
+
+/* Fills a plan.  ids int32 [num_rows]: the adapter of each row, -1: none (any other id outside [0, slots) counts as that and sets
+ * B200KV_S_BAD_POSITION). */
+int b200dec_adapter_plan(const int32_t* ids, const b200dec_adapter_plan_t* plan, int32_t* status, void* stream);
 
 /* out[r] = y[r] + scale[a] * (x[r] . down[a]_p^T) . up[a]^T for the rows of a plan with as many slots; out[r] = y[r] for rows without an adapter.
  * x [num_rows, width], y and out [num_rows, out] of element size elem, strides in elements.  out may be y itself, with the same stride; otherwise it
  * overlaps neither y nor x.  32-bit sums, rounded once.  workspace: 16-byte aligned, of the size that b200dec_add_adapters_workspace says (0 for tiles
  * of 16 rows); nothing in it outlasts the call. */
-size_t b200dec_add_adapters_workspace(const b200dec_adapters* adapters, int32_t max_tiles, int32_t tile_rows);
-int b200dec_add_adapters(const b200dec_adapters* adapters, const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out,
-                         int64_t out_stride, const int32_t* order, const int32_t* tiles, int32_t max_tiles, int32_t tile_rows, int32_t num_rows,
-                         void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+size_t b200dec_add_adapters_workspace(const b200dec_adapters* adapters, const b200dec_adapter_plan_t* plan);
+int b200dec_add_adapters(const b200dec_adapters* adapters, const b200dec_adapter_plan_t* plan, const void* x, int64_t x_stride, const void* y,
+                         int64_t y_stride, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, int32_t* status,
+                         void* stream);
 
 /* ---- what requests ask of their next token.  Every array has one element per entry where nothing else is said; NULL: none of that for any entry.
  * history int32 [num_histories, capacity]: tokens of a request, its prompt and then its output.  slots: the entry's row of it (NULL: entry e has

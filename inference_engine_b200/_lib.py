@@ -80,6 +80,12 @@ class Adapters(C.Structure):
         (n, c_int32) for n in ("slots", "rank", "width", "parts", "elem")] + [("ends", c_int32 * 4)]
 
 
+class AdapterPlan(C.Structure):
+    """struct b200dec_adapter_plan"""
+
+    _fields_ = [("order", c_void_p), ("tiles", c_void_p), ("max_tiles", c_int32), ("tile_rows", c_int32), ("num_rows", c_int32), ("slots", c_int32)]
+
+
 class Rules(C.Structure):
     """struct b200dec_rules"""
 
@@ -97,7 +103,7 @@ class Draw(C.Structure):
 P_CACHE, P_TABLE = C.POINTER(Cache), C.POINTER(Table)
 P_DCACHE, P_ROWS, P_OPT = C.POINTER(DecCache), C.POINTER(DecRows), C.POINTER(AttnOptions)
 P_REC, P_REC_IN, P_ENT = C.POINTER(Recurrence), C.POINTER(RecurrenceIn), C.POINTER(Entries)
-P_ADAPTERS, P_RULES, P_DRAW = C.POINTER(Adapters), C.POINTER(Rules), C.POINTER(Draw)
+P_ADAPTERS, P_PLAN, P_RULES, P_DRAW = C.POINTER(Adapters), C.POINTER(AdapterPlan), C.POINTER(Rules), C.POINTER(Draw)
 
 # name -> (restype, argtypes); must list every function include/b200kv.h declares
 SIGNATURES = {
@@ -200,10 +206,10 @@ DECODER_SIGNATURES = {
                                           c_void_p, c_float, c_float, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "b200dec_grouped_linear": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
                                          c_void_p, c_int32, c_float, c_float, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
-    "b200dec_adapter_plan": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
-    "b200dec_add_adapters": (c_int32, [P_ADAPTERS, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32,
-                                       c_int32, c_void_p, c_size_t, c_void_p, c_void_p]),
-    "b200dec_add_adapters_workspace": (c_size_t, [P_ADAPTERS, c_int32, c_int32]),
+    "b200dec_adapter_plan": (c_int32, [c_void_p, P_PLAN, c_void_p, c_void_p]),
+    "b200dec_add_adapters_workspace": (c_size_t, [P_ADAPTERS, P_PLAN]),
+    "b200dec_add_adapters": (c_int32, [P_ADAPTERS, P_PLAN, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p,
+                                       c_void_p]),
     "b200dec_adjust_logits": (c_int32, [c_void_p, c_int64, c_int32, P_RULES, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p]),
     "b200dec_choose_tokens": (c_int32, [c_void_p, c_int64, c_int32, P_RULES, P_DRAW, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                         c_void_p]),

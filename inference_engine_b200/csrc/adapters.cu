@@ -908,35 +908,44 @@ static int ad_terms_blocks(int rank) { return (2 * ((rank + 15) / 16 * 16) + 63)
 
 using namespace b200kv;
 
-extern "C" int b200dec_adapter_plan(const int32_t* ids, int32_t num_rows, int32_t slots, int32_t tile_rows, int32_t* order, int32_t* tiles,
-                                    int32_t max_tiles, int32_t* status, void* stream) {
-  if (num_rows == 0) return B200KV_OK;
-  if (!ids || !order || !tiles) return B200KV_E_NULL;
-  if (num_rows < 0 || num_rows > (1 << 24) || slots < 1 || slots > kAdMaxSlots) return B200KV_E_RANGE;
-  if (tile_rows != 16 && tile_rows != 128) return B200KV_E_SHAPE;
-  if (max_tiles < num_rows / tile_rows + (num_rows < slots + 1 ? num_rows : slots + 1)) return B200KV_E_WORKSPACE;
-  if ((long long)max_tiles * tile_rows > 0x7fffffffLL) return B200KV_E_RANGE;
-  if (!aligned(tiles, 16) || !aligned(ids, 4) || !aligned(order, 4)) return B200KV_E_ALIGN;
-  const int threads = num_rows <= 256 && slots < 256 ? 256 : kAdPlanThreads;
-  return launch_result(launch_chained(adapter_plan_kernel, dim3(1), dim3(threads), (size_t)(slots + 1) * 4, (cudaStream_t)stream, ids,
-                                      (int)num_rows, (int)slots, (int)tile_rows, order, (int4*)tiles, (int)max_tiles, status));
+static int ad_check_plan(const b200dec_adapter_plan_t* plan) {
+  if (!plan->order || !plan->tiles) return B200KV_E_NULL;
+  if (plan->num_rows < 0 || plan->num_rows > (1 << 24) || plan->slots < 1 || plan->slots > kAdMaxSlots) return B200KV_E_RANGE;
+  if (plan->tile_rows != 16 && plan->tile_rows != 128) return B200KV_E_SHAPE;
+  if (plan->max_tiles < plan->num_rows / plan->tile_rows + (plan->num_rows < plan->slots + 1 ? plan->num_rows : plan->slots + 1)) return B200KV_E_WORKSPACE;
+  if ((long long)plan->max_tiles * plan->tile_rows * kAdMaxParts > 0x0fffffffLL || (plan->tile_rows == 128 && plan->max_tiles > 65535)) return B200KV_E_RANGE;
+  return aligned(plan->tiles, 16) && aligned(plan->order, 4) ? B200KV_OK : B200KV_E_ALIGN;
 }
 
-extern "C" size_t b200dec_add_adapters_workspace(const b200dec_adapters* ad, int32_t max_tiles, int32_t tile_rows) {
-  if (!ad || tile_rows != 128 || ad->elem != 2 || max_tiles < 1 || ad->parts < 1 || ad->rank < 8) return 0;
-  return (size_t)max_tiles * ad->parts * ad_terms_blocks(ad->rank) * 16384;
+extern "C" int b200dec_adapter_plan(const int32_t* ids, const b200dec_adapter_plan_t* plan, int32_t* status, void* stream) {
+  if (!plan) return B200KV_E_NULL;
+  if (plan->num_rows == 0) return B200KV_OK;
+  if (!ids) return B200KV_E_NULL;
+  if (int rc = ad_check_plan(plan)) return rc;
+  if (!aligned(ids, 4)) return B200KV_E_ALIGN;
+  const int threads = plan->num_rows <= 256 && plan->slots < 256 ? 256 : kAdPlanThreads;
+  return launch_result(launch_chained(adapter_plan_kernel, dim3(1), dim3(threads), (size_t)(plan->slots + 1) * 4, (cudaStream_t)stream, ids,
+                                      (int)plan->num_rows, (int)plan->slots, (int)plan->tile_rows, plan->order, (int4*)plan->tiles, (int)plan->max_tiles, status));
 }
 
-extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out,
-                                    int64_t out_stride, const int32_t* order, const int32_t* tiles, int32_t max_tiles, int32_t tile_rows,
-                                    int32_t num_rows, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-  if (num_rows == 0) return B200KV_OK;
-  if (!ad || !ad->down || !ad->up || !ad->scale || !x || !y || !out || !order || !tiles) return B200KV_E_NULL;
-  if (num_rows < 0 || max_tiles < 1 || ad->slots < 1 || ad->slots > kAdMaxSlots) return B200KV_E_RANGE;
+extern "C" size_t b200dec_add_adapters_workspace(const b200dec_adapters* ad, const b200dec_adapter_plan_t* plan) {
+  if (!ad || !plan || plan->tile_rows != 128 || ad->elem != 2 || plan->max_tiles < 1 || ad->parts < 1 || ad->rank < 8) return 0;
+  return (size_t)plan->max_tiles * ad->parts * ad_terms_blocks(ad->rank) * 16384;
+}
+
+extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_adapter_plan_t* plan, const void* x, int64_t x_stride, const void* y,
+                                    int64_t y_stride, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, int32_t* status,
+                                    void* stream) {
+  if (!ad || !plan) return B200KV_E_NULL;
+  if (plan->num_rows == 0) return B200KV_OK;
+  if (!ad->down || !ad->up || !ad->scale || !x || !y || !out) return B200KV_E_NULL;
+  if (int rc = ad_check_plan(plan)) return rc;
+  if (ad->slots != plan->slots) return B200KV_E_SHAPE;
   if (ad->elem != 2 && ad->elem != 4) return B200KV_E_SHAPE;
   if (ad->parts < 1 || ad->parts > kAdMaxParts || ad->rank < 8 || ad->rank > 128 || ad->rank % 8 || ad->width < 1) return B200KV_E_SHAPE;
   if (ad->width > (1 << 24)) return B200KV_E_RANGE;
-  if (tile_rows != 16 && tile_rows != 128) return B200KV_E_SHAPE;
+  const int max_tiles = plan->max_tiles, tile_rows = plan->tile_rows;
+  const int32_t *order = plan->order, *tiles = plan->tiles;
   AdArgs a = {};
   a.down = ad->down; a.up = ad->up; a.scale = ad->scale; a.x = x; a.y = y; a.out = out;
   a.x_stride = x_stride; a.y_stride = y_stride; a.out_stride = out_stride;
@@ -953,9 +962,8 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, i
   }
   const int cols = a.ends[a.parts - 1];
   if (x_stride < a.width || y_stride < cols || out_stride < cols || out == x) return B200KV_E_SHAPE;
-  if ((out == y && out_stride != y_stride) || (long long)max_tiles * tile_rows * a.parts > 0x0fffffffLL || (tile_rows == 128 && max_tiles > 65535)) return B200KV_E_RANGE;
-  if (!aligned(ad->down, 16) || !aligned(ad->up, 16) || !aligned(ad->scale, 4) || !aligned(tiles, 16) || !aligned(order, 4) || !aligned(x, ad->elem) ||
-      !aligned(y, ad->elem) || !aligned(out, ad->elem))
+  if (out == y && out_stride != y_stride) return B200KV_E_SHAPE;
+  if (!aligned(ad->down, 16) || !aligned(ad->up, 16) || !aligned(ad->scale, 4) || !aligned(x, ad->elem) || !aligned(y, ad->elem) || !aligned(out, ad->elem))
     return B200KV_E_ALIGN;
   a.vec = even && aligned(y, 16) && aligned(out, 16) && y_stride % 8 == 0 && out_stride % 8 == 0;
   cudaStream_t s = (cudaStream_t)stream;
@@ -971,7 +979,7 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const void* x, i
   if (tile_rows == 128) {
     a.blocks = ad_terms_blocks(a.rank);
     a.terms = workspace;
-    if (!workspace || workspace_bytes < b200dec_add_adapters_workspace(ad, max_tiles, tile_rows)) return B200KV_E_WORKSPACE;
+    if (!workspace || workspace_bytes < b200dec_add_adapters_workspace(ad, plan)) return B200KV_E_WORKSPACE;
     if (!aligned(workspace, 16)) return B200KV_E_ALIGN;
     // Clusters are of eight blocks where that many fit at once (a graphics cluster's multiprocessors are rarely a multiple of eight: about a seventh is left
     // over), else of four, and copies run further ahead where a multiprocessor has one block anyway.

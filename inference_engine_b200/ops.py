@@ -648,16 +648,9 @@ class Adapters:
         ends = [sum(parts[: i + 1]) for i in range(len(parts))]
         st = _lib.Adapters(d.data_ptr(), u.data_ptr(), s.data_ptr(), slots, rank, d.shape[2], len(parts), _elem(d.dtype))
         st.ends[: len(ends)] = ends
-        object.__setattr__(self, "parts", parts)
-        object.__setattr__(self, "struct", st)
-
-    @property
-    def slots(self) -> int:
-        return self.up.shape[0]
-
-    @property
-    def rank(self) -> int:
-        return self.up.shape[2]
+        for name, value in dict(parts=parts, struct=st, ref=ctypes.byref(st), slots=slots, out=out, rank=rank, width=d.shape[2],
+                                device_index=u.get_device()).items():
+            object.__setattr__(self, name, value)
 
     def load(self, slot: int, pairs, scale: float) -> None:
         """Put an adapter into a slot: a pair (down [r, width], up [columns of the part, r]) for each part, r up to the rank, or None for a part that
@@ -665,9 +658,9 @@ class Adapters:
         if not 0 <= slot < self.slots or len(pairs) != len(self.parts):
             raise ValueError(f"adapters: slot {slot} of {self.slots}, {len(pairs)} pairs for {len(self.parts)} parts")
         for pair, n in zip(pairs, self.parts):
-            if pair is not None and (pair[0].dim() != 2 or pair[0].shape[0] > self.rank or pair[0].shape[1] != self.down.shape[2]
+            if pair is not None and (pair[0].dim() != 2 or pair[0].shape[0] > self.rank or pair[0].shape[1] != self.width
                                      or tuple(pair[1].shape) != (n, pair[0].shape[0])):
-                raise ValueError(f"adapters: {tuple(pair[0].shape)} and {tuple(pair[1].shape)} for {self.down.shape[2]} inputs, {n} columns and "
+                raise ValueError(f"adapters: {tuple(pair[0].shape)} and {tuple(pair[1].shape)} for {self.width} inputs, {n} columns and "
                                  f"ranks up to {self.rank}")
         self.clear(slot)
         at = 0
@@ -695,14 +688,25 @@ def make_adapters(slots: int, width: int, parts, rank: int, dtype, device) -> Ad
                     torch.zeros(slots, sum(parts), rank, dtype=dtype, device=device), torch.zeros(slots, device=device), tuple(parts))
 
 
-@dataclass(frozen=True, eq=False)
 class AdapterPlan:
     """A step's rows sorted by adapter (plan_adapters), for all the projections of the step."""
 
-    order: torch.Tensor  # int32 [tiles, tile_rows]: rows of each tile, -1 behind them
-    tiles: torch.Tensor  # int32 [tiles, 4]: adapter and number of rows
-    slots: int
-    rows: int
+    def __init__(self, buf: torch.Tensor, rows: int, slots: int, tiles: int, tile_rows: int):
+        self.buf, self.rows, self.slots, self.num_tiles, self.tile_rows = buf, rows, slots, tiles, tile_rows
+        self.device_index = buf.get_device()
+        at = buf.data_ptr()
+        self.struct = _lib.AdapterPlan(at + 16 * tiles, at, tiles, tile_rows, rows, slots)
+        self.ref = ctypes.byref(self.struct)
+
+    @property
+    def tiles(self) -> torch.Tensor:
+        """int32 [tiles, 4]: adapter (-1: none) and number of rows."""
+        return self.buf[: 4 * self.num_tiles].view(self.num_tiles, 4)
+
+    @property
+    def order(self) -> torch.Tensor:
+        """int32 [tiles, tile_rows]: the rows of each tile, -1 behind them."""
+        return self.buf[4 * self.num_tiles :].view(self.num_tiles, self.tile_rows)
 
 
 def adapter_tile_rows(num_rows: int) -> int:
@@ -711,7 +715,7 @@ def adapter_tile_rows(num_rows: int) -> int:
 
 
 def _here(t: torch.Tensor) -> None:
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"tensors on {t.device} while device {torch.cuda.current_device()} is the current one")
 
 
@@ -727,41 +731,49 @@ def plan_adapters(ids: torch.Tensor, slots: int, tile_rows: int | None = None) -
         raise ValueError(f"plan_adapters: 1 to 4096 slots, not {slots}")
     N = ids.shape[0]
     rows = adapter_tile_rows(N) if tile_rows is None else tile_rows
+    if rows not in (16, 128):
+        raise ValueError(f"plan_adapters: tiles of 16 or 128 rows, not {rows}")
     most = N // rows + min(N, slots + 1)
-    tiles = torch.empty(most, 4, dtype=torch.int32, device=ids.device)
-    order = torch.empty(most, rows, dtype=torch.int32, device=ids.device)
-    rc = _lib_dec().b200dec_adapter_plan(ids.data_ptr(), N, slots, rows, order.data_ptr(), tiles.data_ptr(), most,
-                                         K.status_word(ids.device).data_ptr(), K._stream())
+    plan = AdapterPlan(torch.empty((4 + rows) * most, dtype=torch.int32, device=ids.device), N, slots, most, rows)
+    rc = _lib_dec().b200dec_adapter_plan(ids.data_ptr(), plan.ref, K.status_word(ids.device).data_ptr(), K._stream())
     _lib.check(rc, "plan_adapters")
-    return AdapterPlan(order, tiles, slots, N)
+    return plan
 
 
 @K._ranged
 def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: AdapterPlan, out: torch.Tensor | None = None) -> torch.Tensor:
-    """y + scale * (x down^T) up^T of every row's adapter, in one launch; rows without one stay y.  y [rows, out]: what the shared projection made of
-    x [rows, width].  Written over y unless `out` is given, which shares no memory with y or x."""
-    K._require_cuda(y, x, adapters.up, plan.order)
-    _here(y)
-    out = y if out is None else out
-    N = plan.rows
-    if y.dtype != adapters.up.dtype or x.dtype != y.dtype or out.dtype != y.dtype:
-        raise ValueError(f"add_adapters: rows of {x.dtype}, {y.dtype} and {out.dtype} beside adapters of {adapters.up.dtype}")
-    if tuple(x.shape) != (N, adapters.down.shape[2]) or tuple(y.shape) != (N, adapters.up.shape[1]) or out.shape != y.shape:
+    """y + scale * (x down^T) up^T of every row's adapter; rows without one stay y.  y [rows, out]: what the shared projection made of x [rows, width].
+    Written over y unless `out` is given, which shares no memory with y or x."""
+    if out is None:
+        out = y
+    N, dtype, dev = plan.rows, adapters.up.dtype, plan.device_index
+    if not y.get_device() == x.get_device() == out.get_device() == adapters.device_index == dev:
+        K._require_cuda(y, x, out, adapters.up)
+        raise ValueError("add_adapters: rows, adapters and plan on one device are wanted")
+    if dev != torch._C._cuda_getDevice():
+        _here(y)
+    if y.dtype != dtype or x.dtype != dtype or out.dtype != dtype:
+        raise ValueError(f"add_adapters: rows of {x.dtype}, {y.dtype} and {out.dtype} beside adapters of {dtype}")
+    if x.shape != (N, adapters.width) or y.shape != (N, adapters.out) or out.shape != y.shape:
         raise ValueError(f"add_adapters: {tuple(x.shape)}, {tuple(y.shape)} and {tuple(out.shape)} for a plan of {N} rows")
-    if N and not x.stride(1) == y.stride(1) == out.stride(1) == 1:
-        raise ValueError("add_adapters: a row's elements lie side by side")
     if plan.slots != adapters.slots:
         raise ValueError(f"add_adapters: a plan for {plan.slots} slots and {adapters.slots} adapters")
-    # (a single row's stride may be anything)
-    xs, ys, os = (t.stride(0) if N > 1 else _round8(t.shape[1]) for t in (x, y, out))
-    lib, ad, (tiles, tile_rows) = _lib_dec(), ctypes.byref(adapters.struct), plan.order.shape
-    ws, nbytes = None, 0
-    if tile_rows > 16:
-        nbytes = lib.b200dec_add_adapters_workspace(ad, tiles, tile_rows)
+    if N > 1:
+        (xs, x1), (ys, y1), (os, o1) = x.stride(), y.stride(), out.stride()
+        if not x1 == y1 == o1 == 1:
+            raise ValueError("add_adapters: a row's elements lie side by side")
+    else:  # a single row's stride may be anything
+        if N and not x.stride(1) == y.stride(1) == out.stride(1) == 1:
+            raise ValueError("add_adapters: a row's elements lie side by side")
+        xs, ys, os = _round8(adapters.width), _round8(adapters.out), _round8(adapters.out)
+    lib, ws, nbytes = _lib_dec(), None, 0
+    if plan.tile_rows > 16:
+        nbytes = lib.b200dec_add_adapters_workspace(adapters.ref, plan.ref)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=y.device)
-    rc = lib.b200dec_add_adapters(ad, x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, plan.order.data_ptr(), plan.tiles.data_ptr(), tiles,
-                                  tile_rows, N, _ptr(ws), nbytes, K.status_word(y.device).data_ptr(), K._stream())
-    _lib.check(rc, "add_adapters")
+    rc = lib.b200dec_add_adapters(adapters.ref, plan.ref, x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, None if ws is None else ws.data_ptr(), nbytes,
+                                  K.status_word(y.device).data_ptr(), K._stream())
+    if rc:
+        _lib.check(rc, "add_adapters")
     return out
 
 
