@@ -13,8 +13,10 @@
 // happens on the multiprocessors.  With m the largest, z = (m - l) / temperature and w = exp(-z), tokens are ordered by l (equal ones by
 // index).  Kept are the first top_k; of these the shortest run whose weight is at least top_p of theirs; of these the ones with w >= min_p.
 // The token is the first, by index, at which the kept weights so far exceed uniform * their sum.
-// A cut is found by histograms of z (counts, and weights as integers, so that no order of additions matters), down to the few tokens of
-// one bin, which are put in order by comparison.
+// A cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the likelier tokens, or over the others if
+// it does not lie there, down to the few tokens of one bin, which are put in order by comparison.  Blocks tell one another sums of bins, and read
+// from one another only the bins among which the cut lies: a barrier of the cluster each for the largest logit, the histogram, the bin's
+// tokens and the kept weights.
 #include "dec_common.cuh"
 
 namespace b200kv {
@@ -180,14 +182,11 @@ adjust_logits_kernel(const T* logits, long long stride, const TcRules r, float* 
 // ---------------------------------------------------------------------------------------------------------------- the choice
 constexpr int kTcThreads = 512;
 constexpr int kTcWarps = kTcThreads / 32;
-constexpr int kTcCluster = 8;
-constexpr int kTcBins = 2048;
-constexpr int kTcPerRank = kTcBins / kTcCluster;
-constexpr float kTcBinsPerUnit = 64.f;  // of z: 32 units in all, behind which a token's weight is below 1.3e-14
-constexpr int kTcMembers = 2048;        // tokens of one bin that are put in order
-constexpr int kTcMaxLocal = 48 * 1024;  // columns of a block
-constexpr uint32_t kTcHistBytes = kTcBins * 12;
-static_assert(kTcMembers * 12 <= kTcHistBytes, "a bin's tokens take the place of the histogram");
+constexpr int kTcMaxCluster = 8;
+constexpr int kTcBins = 1024, kTcCoarse = 32;  // and sums of 32 bins
+constexpr int kTcMembers = 1024;               // tokens of one bin that are put in order
+constexpr int kTcMaxLocal = 48 * 1024;         // columns of a block
+constexpr uint32_t kTcRowAt = kTcBins * 12 + kTcMembers * 12;  // the histogram, a bin's tokens, the row
 
 struct TcDraw {
   const float* temperature;
@@ -197,27 +196,36 @@ struct TcDraw {
 
 // What the blocks of a cluster tell one another; every block has a copy of its own.
 struct TcMail {
-  float best[kTcCluster];
-  int best_at[kTcCluster];
-  double rest[kTcCluster], mass[kTcCluster];
-  unsigned long long bin_mass[kTcCluster];
-  uint32_t bin_count[kTcCluster];
-  uint32_t found;  // 1: this bin, 2: the cut lies behind all tokens, 3: among tokens of no weight
+  float best[kTcMaxCluster];
+  float rest[kTcMaxCluster];
+  int first[kTcMaxCluster], equal[kTcMaxCluster];  // of the largest ones
+  double mass[kTcMaxCluster];    // the weights that are drawn from
+  float weight[kTcMaxCluster];   // of the tokens among which a share is kept
+  unsigned long long coarse_mass[kTcMaxCluster][kTcCoarse];
+  uint32_t coarse_count[kTcMaxCluster][kTcCoarse];
+  uint32_t listed_by[kTcMaxCluster];
+  uint32_t ties[kTcMaxCluster];
+  // within the block
+  uint32_t listed;
   int bin;
   uint32_t count_before, members;
-  unsigned long long mass_before, mass_all;
+  unsigned long long mass_before, mass_in;
   float cut_behind;
   int cut_at;
-  uint32_t listed;
-  uint32_t ties[kTcCluster];
 };
 
-__device__ __forceinline__ uint32_t tc_rank() {
+__device__ __forceinline__ int tc_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
+  return (int)r;
+}
+__device__ __forceinline__ int tc_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return (int)r;
 }
 __device__ __forceinline__ void tc_cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 // The address of a variable of this block in block `rank`'s shared memory.
@@ -236,12 +244,17 @@ __device__ __forceinline__ uint32_t tc_get(uint32_t at) {
   asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
 }
+// By one warp: lane q to block q.
 template <typename V>
-__device__ __forceinline__ void tc_tell(V* mine, V v) {  // by one thread, to every block
-#pragma unroll
-  for (int q = 0; q < kTcCluster; ++q) tc_put(tc_there(mine, q), v);
+__device__ __forceinline__ void tc_tell(V* mine, V v, int blocks) {
+  if ((int)(threadIdx.x & 31) < blocks) tc_put(tc_there(mine, threadIdx.x & 31), v);
 }
-
+template <typename V>
+__device__ __forceinline__ V tc_warp_sum(V v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 template <typename V>
 __device__ __forceinline__ V tc_warp_scan(V v) {  // inclusive
   const int lane = threadIdx.x & 31;
@@ -252,225 +265,314 @@ __device__ __forceinline__ V tc_warp_scan(V v) {  // inclusive
   }
   return v;
 }
-// Sums over the threads in front of this one (what the thread in front of it has for `upto`) and up to it; `all`: over the block.  tmp: one value
-// per warp.
-template <typename V>
-__device__ __forceinline__ V tc_block_before(V v, V* tmp, V& upto, V& all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const V s = tc_warp_scan(v);
-  const V prev = __shfl_up_sync(0xffffffffu, s, 1);
-  if (lane == 31) tmp[warp] = s;
-  __syncthreads();
-  V before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kTcWarps; ++w) {
-    if (w == warp) before = total;
-    total += tmp[w];
-  }
-  __syncthreads();
-  all = total;
-  upto = before + s;
-  return before + (lane ? prev : (V)0);
+__device__ __forceinline__ float tc_exp2(float x) {  // two steps of the last place
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+constexpr float kTcLog2e = 1.4426950408889634f;
 
+// A row in shared memory and who looks at what: warp w has the columns [w * span, (w + 1) * span) of its block, four to a lane at a time.
 struct TcRow {
-  float* row;   // this block's adjusted logits
-  int v0, n;    // its columns
-  int lo, hi;   // this thread's, of the block
-  int rank;
-  float m, inv_tau;
+  float* row;       // this block's adjusted logits; -inf behind its columns
+  int v0, lo, hi;   // the block's first column; this warp's columns of the block, multiples of 128
+  int rank, blocks;
+  float m;
+  float unit;       // log2(e) / temperature: z below is in units of ln 2
   TcMail* mail;
-  uint32_t* hist;  // counts, upper and lower halves of weights
-  double* tmp;     // kTcWarps
-  // how far behind the largest logit, in units of the temperature
+  uint32_t* hist;   // counts, upper and lower halves of weights
+  float* list_far;  // a bin's tokens: how far behind the largest, column, weight
+  int* list_at;
+  uint32_t* list_w;
+  // how far behind the largest logit
   __device__ __forceinline__ float behind(float l) const { return l == m ? 0.f : m - l; }
-  __device__ __forceinline__ float z(float l) const { return __fmul_rn(behind(l), inv_tau); }
+  __device__ __forceinline__ float z(float l) const { return __fmul_rn(behind(l), unit); }
   // a weight in steps of 2^-32 of the largest (which is one step short)
-  __device__ __forceinline__ uint32_t steps(float z) const { return __float2uint_rn(expf(-z) * 4294967296.f); }
+  __device__ __forceinline__ uint32_t steps(float z) const { return __float2uint_rn(tc_exp2(-z) * 4294967296.f); }
+  // no token with a smaller logit has a z up to this
+  __device__ __forceinline__ float floor(float z) const { return __fsub_rd(m, __fmul_ru(__fdiv_ru(z, unit), 1.00001f)); }
+  // f(column of the block, logit) of all, and of those that are not below a floor: few, where it cuts the bulk of a vocabulary off
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = lo + 4 * (threadIdx.x & 31); i < hi; i += 128) {
+      const float4 l = *reinterpret_cast<const float4*>(row + i);
+      f(i, l.x);
+      f(i + 1, l.y);
+      f(i + 2, l.z);
+      f(i + 3, l.w);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each_above(float floor, F f) const {
+    for (int i = lo + 4 * (threadIdx.x & 31); i < hi; i += 128) {
+      const float4 l = *reinterpret_cast<const float4*>(row + i);
+      if (fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w)) < floor) continue;
+      const float v[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j)
+        if (!(v[j] < floor)) f(i + j, v[j]);
+    }
+  }
 };
 
 // A bin of z, and the last token that is kept: of all (exact: how far it is behind the largest, and its column), or of the bin's (its column).
 struct TcCut {
-  bool exact;
-  float behind;
-  int at;
-  float base, scale;
-  int bin, level;
+  bool on = false, exact = false;
+  float behind = 0.f;
+  int at = 0;
+  float base = 0.f, scale = 1.f;
+  int bin = 0;
+  float floor = -INFINITY;  // no token below it is kept
   // -1: in front of the bin, 0: in it, 1: behind it.  Differences of nearby values and products with powers of two are exact.
   __device__ __forceinline__ int side(float z) const {
     const float x = (z - base) * scale;
-    if (level && !(x >= 0.f && x < (float)kTcBins)) return x < 0.f ? -1 : 1;
-    const int b = x < (float)(kTcBins - 1) ? (int)x : kTcBins - 1;
+    if (!(x >= 0.f && x < (float)kTcBins)) return x < 0.f ? -1 : 1;
+    const int b = (int)x;
     return b < bin ? -1 : b > bin;
+  }
+  __device__ __forceinline__ bool keeps(const TcRow& c, int i, float l) const {
+    if (!on) return true;
+    const float far = c.behind(l);
+    const int s = exact ? (far < behind ? -1 : far > behind) : side(__fmul_rn(far, c.unit));
+    return s < 0 || (s == 0 && c.v0 + i <= at);
   }
 };
 
-// Where the cut lies that keeps the first `k` tokens (kMass false), or the shortest run with `p` of the weight (kMass true); false: nothing is cut.
-// By all threads of the cluster.
+// Where the cut lies that keeps the first `k` tokens (kMass false), or the shortest run with `p` of the weight (kMass true), of those that `had` keeps;
+// off where nothing is cut.  By all threads of the cluster.  weighed: every block has told its tokens' weight.
 template <bool kMass>
-__device__ bool tc_select(const TcRow& c, uint32_t k, float p, TcCut& cut) {
+__device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, const TcCut& had, bool weighed) {
   TcMail& mail = *c.mail;
-  const int tid = threadIdx.x;
-  float base = 0.f, scale = kTcBinsPerUnit;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // z < 16, weights above 2^-16; then up to 80; then down into a bin
+  float base = 0.f, scale = kTcBins / 16.f, top = 16.f;
+  int level = 0;
   uint32_t count_before = 0;
   unsigned long long mass_before = 0;
   double target = 0.;
-  for (int level = 0;; ++level) {
-    __syncthreads();  // (what was told before has been read)
-    for (int i = tid; i < 3 * kTcBins; i += kTcThreads) c.hist[i] = 0;
-    if (tid == 0) {
-      mail.found = 0;
-      mail.listed = 0;
-    }
+  for (bool first = true;; first = false) {
+    const bool weigh = kMass && first && !weighed;
+    __syncthreads();  // (what was found before has been read)
+    for (int i = tid; i < (kMass ? 3 : 1) * kTcBins; i += kTcThreads) c.hist[i] = 0;
+    if (tid == 0) mail.listed = 0;
     __syncthreads();
-    for (int i = c.lo; i < c.hi; ++i) {
-      const float l = c.row[i];
-      if (l == -INFINITY) continue;
-      const float z = c.z(l), at = (z - base) * scale;
-      if (level && !(at >= 0.f && at < (float)kTcBins)) continue;
-      const int b = at < (float)(kTcBins - 1) ? (int)at : kTcBins - 1;
+    float weight = 0.f;
+    c.each_above(weigh ? had.floor : fmaxf(had.floor, c.floor(top)), [&](int i, float l) {
+      const float z = c.z(l), x = (z - base) * scale;
+      if (!had.keeps(c, i, l)) return;
+      if (weigh) weight += tc_exp2(-z);
+      if (!(x >= 0.f && x < (float)kTcBins)) return;
+      const int b = (int)x;
       atomicAdd(&c.hist[b], 1u);
       if (kMass) {
         const uint32_t q = c.steps(z);
         atomicAdd(&c.hist[kTcBins + b], q >> 16);
         atomicAdd(&c.hist[2 * kTcBins + b], q & 0xffffu);
       }
+    });
+    if (weigh) {
+      weight = tc_warp_sum(weight);
+      if (lane == 0) c.list_far[warp] = weight;  // (nothing is listed yet)
+    }
+    __syncthreads();
+    if (weigh && warp == 0) tc_tell(&mail.weight[c.rank], tc_warp_sum(lane < kTcWarps ? c.list_far[lane] : 0.f), c.blocks);
+    for (int i = warp; i < kTcCoarse; i += kTcWarps) {
+      const int b = 32 * i + lane;
+      const uint32_t count = tc_warp_sum(c.hist[b]);
+      tc_tell(&mail.coarse_count[c.rank][i], count, c.blocks);
+      if (kMass) tc_tell(&mail.coarse_mass[c.rank][i], tc_warp_sum(((unsigned long long)c.hist[kTcBins + b] << 16) + c.hist[2 * kTcBins + b]), c.blocks);
     }
     tc_cluster_sync();
-    // this block's share of the bins, over all blocks
-    uint32_t count = 0;
-    unsigned long long mass = 0;
-    if (tid < kTcPerRank) {
-      const uint32_t* mine = c.hist + c.rank * kTcPerRank + tid;
+    if (kMass && first) {
+      float all = 0.f;
+      for (int q = 0; q < c.blocks; ++q) all += mail.weight[q];
+      target = fmax((double)p * (double)all * 4294967296., 0.5);
+    }
+    // the sum of bins, then the bin, that the cut lies in: every block for itself
+    if (warp == 0) {
+      uint32_t count = 0;
+      unsigned long long mass = 0;
+      for (int q = 0; q < c.blocks; ++q) {
+        count += mail.coarse_count[q][lane];
+        if (kMass) mass += mail.coarse_mass[q][lane];
+      }
+      uint32_t c_upto = tc_warp_scan(count);
+      unsigned long long m_upto = kMass ? tc_warp_scan(mass) : 0;
+      const uint32_t c_all = __shfl_sync(0xffffffffu, c_upto, 31);
+      const unsigned long long m_all = __shfl_sync(0xffffffffu, m_upto, 31);
+      const auto reached = [&]() { return kMass ? (double)(mass_before + m_upto) >= target : count_before + c_upto >= k; };
+      const unsigned hit = __ballot_sync(0xffffffffu, reached());
+      if (hit) {
+        const int group = __ffs(hit) - 1;
+        uint32_t cb = count_before + __shfl_sync(0xffffffffu, c_upto - count, group);
+        unsigned long long mb = mass_before + __shfl_sync(0xffffffffu, m_upto - mass, group);
+        const uint32_t* bin = c.hist + 32 * group + lane;
+        // (all on their way before the first is waited for)
+        uint32_t n[kTcMaxCluster], hi[kTcMaxCluster], lo[kTcMaxCluster];
 #pragma unroll
-      for (int q = 0; q < kTcCluster; ++q) {
-        count += tc_get(tc_there(mine, q));
-        if (kMass) mass += ((unsigned long long)tc_get(tc_there(mine + kTcBins, q)) << 16) + tc_get(tc_there(mine + 2 * kTcBins, q));
-      }
-    }
-    uint32_t block_count, unused_count;
-    unsigned long long block_mass = 0, m_before = 0, unused_mass;
-    uint32_t c_before = tc_block_before(count, reinterpret_cast<uint32_t*>(c.tmp), unused_count, block_count);
-    if (kMass) m_before = tc_block_before(mass, reinterpret_cast<unsigned long long*>(c.tmp), unused_mass, block_mass);
-    if (tid == 0) {
-      tc_tell(&mail.bin_count[c.rank], block_count);
-      if (kMass) tc_tell(&mail.bin_mass[c.rank], block_mass);
-    }
-    tc_cluster_sync();
-    uint32_t all_count = 0;
-    unsigned long long all_mass = 0;
-    c_before += count_before;
-    m_before += mass_before;
-    for (int q = 0; q < kTcCluster; ++q) {
-      if (q < c.rank) {
-        c_before += mail.bin_count[q];
-        if (kMass) m_before += mail.bin_mass[q];
-      }
-      all_count += mail.bin_count[q];
-      if (kMass) all_mass += mail.bin_mass[q];
-    }
-    if (level == 0) {
-      if (!kMass && all_count <= k) return false;
-      if (kMass) target = fmax((double)p * (double)all_mass, 0.5);
-    }
-    // the bin that the cut lies in
-    const bool here = kMass ? (double)m_before < target && (double)(m_before + mass) >= target : c_before < k && c_before + count >= k;
-    if (tid < kTcPerRank && here && count) {
-      const int b = c.rank * kTcPerRank + tid;
-      tc_tell(&mail.bin, b);
-      tc_tell(&mail.count_before, c_before);
-      tc_tell(&mail.mass_before, m_before);
-      tc_tell(&mail.mass_all, mass);
-      tc_tell(&mail.members, count);
-      tc_tell(&mail.found, level == 0 && b == kTcBins - 1 ? 3u : 1u);
-    }
-    tc_cluster_sync();
-    if (!mail.found) return false;
-    cut = TcCut{false, 0.f, -1, base, scale, mail.bin, level};
-    if (mail.found == 3) return true;  // every token in front of the last bin is kept, those in it have no weight
-    const uint32_t members = mail.members;
-    count_before = mail.count_before;
-    mass_before = mail.mass_before;
-    auto member = [&](float l) { return l != -INFINITY && cut.side(c.z(l)) == 0; };
-    if (members <= kTcMembers) {
-      // to block 0, whose histogram is read by nobody any more: how far behind, column and weight
-      for (int i = c.lo; i < c.hi; ++i) {
-        const float l = c.row[i];
-        if (!member(l)) continue;
-        uint32_t at;
-        asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(tc_there(&mail.listed, 0)) : "memory");
-        if (at >= (uint32_t)kTcMembers) continue;
-        tc_put(tc_there(c.hist + at, 0), c.behind(l));
-        tc_put(tc_there(c.hist + kTcMembers + at, 0), c.v0 + i);
-        if (kMass) tc_put(tc_there(c.hist + 2 * kTcMembers + at, 0), c.steps(c.z(l)));
-      }
-      tc_cluster_sync();
-      if (c.rank == 0) {
-        const uint32_t num = min(mail.listed, (uint32_t)kTcMembers);
-        const float* far = reinterpret_cast<const float*>(c.hist);
-        const int* at = reinterpret_cast<const int*>(c.hist + kTcMembers);
-        const uint32_t* w = c.hist + 2 * kTcMembers;
-        for (uint32_t i = tid; i < num; i += kTcThreads) {
-          uint32_t before = 0;
-          unsigned long long weight = 0;
-          for (uint32_t j = 0; j < num; ++j) {
-            if (far[j] < far[i] || (far[j] == far[i] && at[j] < at[i])) {
-              ++before;
-              if (kMass) weight += w[j];
+        for (int q = 0; q < kTcMaxCluster; ++q) {
+          n[q] = hi[q] = lo[q] = 0;
+          if (q < c.blocks) {
+            n[q] = tc_get(tc_there(bin, q));
+            if (kMass) {
+              hi[q] = tc_get(tc_there(bin + kTcBins, q));
+              lo[q] = tc_get(tc_there(bin + 2 * kTcBins, q));
             }
           }
-          const bool last = kMass ? (double)(mass_before + weight) < target && (double)(mass_before + weight + w[i]) >= target : count_before + before + 1 == k;
-          if (last) {
-            tc_tell(&mail.cut_behind, far[i]);
-            tc_tell(&mail.cut_at, at[i]);
+        }
+        count = 0;
+        mass = 0;
+#pragma unroll
+        for (int q = 0; q < kTcMaxCluster; ++q) {
+          count += n[q];
+          mass += ((unsigned long long)hi[q] << 16) + lo[q];
+        }
+        c_upto = tc_warp_scan(count);
+        m_upto = kMass ? tc_warp_scan(mass) : 0;
+        const unsigned at = __ballot_sync(0xffffffffu, kMass ? (double)(mb + m_upto) >= target : cb + c_upto >= k);
+        if (lane == __ffs(at) - 1) {
+          mail.bin = 32 * group + lane;
+          mail.count_before = cb + c_upto - count;
+          mail.mass_before = mb + m_upto - mass;
+          mail.members = count;
+          mail.mass_in = mass;
+        }
+      } else if (lane == 0) {
+        mail.bin = -1;
+        mail.count_before = count_before + c_all;
+        mail.mass_before = mass_before + m_all;
+      }
+    }
+    __syncthreads();
+    count_before = mail.count_before;
+    mass_before = mail.mass_before;
+    if (mail.bin < 0) {
+      if (base > 0.f) return TcCut();  // fewer tokens, or less weight, than would be kept; weights below 2^-80 do not count.  (A bin's parts have the bin's sums.)
+      tc_cluster_sync();  // (the blocks read this one's bins)
+      base = 16.f;
+      scale = kTcBins / 64.f;
+      top = 80.f;
+      continue;
+    }
+    TcCut cut;
+    cut.on = true;
+    cut.base = base;
+    cut.scale = scale;
+    cut.bin = mail.bin;
+    cut.floor = c.floor(base + (float)(mail.bin + 1) / scale);
+    const uint32_t members = mail.members;
+    const unsigned long long mass_in = mail.mass_in;
+    if (members <= kTcMembers) {
+      // the bin's tokens: every block's own, then all of them where the histogram was
+      c.each_above(cut.floor, [&](int i, float l) {
+        const float z = c.z(l);
+        if (cut.side(z) != 0 || !had.keeps(c, i, l)) return;
+        const uint32_t at = atomicAdd(&mail.listed, 1u);  // (no more than the cluster has)
+        c.list_far[at] = c.behind(l);
+        c.list_at[at] = c.v0 + i;
+        if (kMass) c.list_w[at] = c.steps(z);
+      });
+      __syncthreads();
+      if (warp == 0) tc_tell(&mail.listed_by[c.rank], mail.listed, c.blocks);
+      tc_cluster_sync();
+      float* all_far = reinterpret_cast<float*>(c.hist);
+      int* all_at = reinterpret_cast<int*>(c.hist + kTcMembers);
+      uint32_t* all_w = c.hist + 2 * kTcMembers;
+      uint32_t num = 0;
+      for (int q = 0; q < c.blocks; ++q) {
+        const uint32_t theirs = mail.listed_by[q];
+        for (uint32_t i = tid; i < theirs; i += kTcThreads) {
+          const uint32_t far = tc_get(tc_there(c.list_far + i, q)), at = tc_get(tc_there(c.list_at + i, q)), w = kMass ? tc_get(tc_there(c.list_w + i, q)) : 0;
+          all_far[num + i] = __uint_as_float(far);
+          all_at[num + i] = (int)at;
+          if (kMass) all_w[num + i] = w;
+        }
+        num += theirs;
+      }
+      tc_cluster_sync();  // (and nobody reads another block's list behind this)
+      for (uint32_t i = tid; i < num; i += kTcThreads) {
+        const float far = all_far[i];
+        const int at = all_at[i];
+        uint32_t before = 0;
+        unsigned long long weight_before = mass_before;
+        for (uint32_t j = 0; j < num; ++j) {
+          const float other = all_far[j];
+          if (other < far || (other == far && all_at[j] < at)) {
+            ++before;
+            if (kMass) weight_before += all_w[j];
           }
         }
+        if (kMass ? (double)weight_before < target && (double)(weight_before + all_w[i]) >= target : count_before + before + 1 == k) {
+          mail.cut_behind = far;
+          mail.cut_at = at;
+        }
       }
-      tc_cluster_sync();
+      __syncthreads();
       cut.exact = true;
       cut.behind = mail.cut_behind;
       cut.at = mail.cut_at;
-      return true;
+      return cut;
     }
     if (level < 2) {
+      tc_cluster_sync();  // (the blocks read this one's bins)
+      top = base + (float)(mail.bin + 1) / scale;
       base += (float)mail.bin / scale;
       scale *= (float)kTcBins;
+      ++level;
       continue;
     }
-    // more tokens than that within 2^-28 of one another: equal ones, by index
-    uint32_t want = kMass ? (uint32_t)fmin(fmax(ceil((target - (double)mass_before) * members / fmax((double)mail.mass_all, 1.)), 1.), (double)members) : k - count_before;
-    uint32_t mine = 0, upto, block;
-    for (int i = c.lo; i < c.hi; ++i) mine += member(c.row[i]);
-    uint32_t before = tc_block_before(mine, reinterpret_cast<uint32_t*>(c.tmp), upto, block);
-    if (tid == 0) tc_tell(&mail.ties[c.rank], block);
+    // more tokens than that within 2^-24 of one another: equal ones, by index
+    const uint32_t want = kMass ? (uint32_t)fmin(fmax(ceil((target - (double)mass_before) * members / fmax((double)mass_in, 1.)), 1.), (double)members) : k - count_before;
+    const auto member = [&](int i, float l) { return cut.side(c.z(l)) == 0 && had.keeps(c, i, l); };
+    uint32_t mine = 0;
+    c.each([&](int i, float l) { mine += member(i, l); });
+    mine = tc_warp_sum(mine);
+    uint32_t* tmp = reinterpret_cast<uint32_t*>(c.list_far);
+    if (lane == 0) tmp[warp] = mine;
+    __syncthreads();
+    if (warp == 0) tc_tell(&mail.ties[c.rank], tc_warp_sum(lane < kTcWarps ? tmp[lane] : 0u), c.blocks);
     tc_cluster_sync();
+    uint32_t before = 0;
     for (int q = 0; q < c.rank; ++q) before += mail.ties[q];
-    if (before < want && before + mine >= want) {
-      for (int i = c.lo; i < c.hi; ++i) {
-        if (member(c.row[i]) && ++before == want) tc_tell(&mail.cut_at, c.v0 + i);
+    for (int w = 0; w < warp; ++w) before += tmp[w];
+    if (before < want && before + mine >= want) {  // this warp has it
+      for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
+        const int i = i0 + 4 * lane;
+        const float4 l = *reinterpret_cast<const float4*>(c.row + i);
+        const bool in[4] = {member(i, l.x), member(i + 1, l.y), member(i + 2, l.z), member(i + 3, l.w)};
+        const uint32_t here = in[0] + in[1] + in[2] + in[3], upto = tc_warp_scan(here), all = __shfl_sync(0xffffffffu, upto, 31);
+        if (before < want && before + all >= want) {
+          uint32_t at = before + upto - here;
+          for (int j = 0; j < 4; ++j)
+            if (in[j] && ++at == want)
+              for (int q = 0; q < c.blocks; ++q) tc_put(tc_there(&mail.cut_at, q), c.v0 + i + j);
+        }
+        before += all;
       }
     }
     tc_cluster_sync();
     cut.at = mail.cut_at;
-    return true;
+    return cut;
   }
 }
 
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kTcThreads)
-choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const TcDraw d, int V, int cols, int seg, bool append, long long* tokens,
+// vec: rows aligned to 16 bytes
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, 2)
+choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const TcDraw d, int V, int cols, bool vec, bool append, long long* tokens,
                      float* logprobs, int32_t* status) {
   extern __shared__ __align__(16) uint8_t tc_smem[];
   __shared__ TcMail mail;
-  __shared__ double tmp[kTcWarps];
-  __shared__ float tmp_v[kTcWarps];
-  __shared__ int tmp_i[kTcWarps];
+  __shared__ float tmp_f[kTcWarps];
+  __shared__ int tmp_i[kTcWarps], tmp_n[kTcWarps];
+  __shared__ double tmp_d[kTcWarps];
   pdl_enter();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   TcRow c;
-  c.rank = (int)tc_rank();
-  const int e = blockIdx.x / kTcCluster;
+  c.rank = tc_rank();
+  c.blocks = tc_size();
+  const int e = blockIdx.x / c.blocks;
   const bool report = c.rank == 0;
   const TcEntry t = tc_entry(r, e, report && tid == 0, status);
   if (t.idle) {
@@ -483,83 +585,96 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   // no block writes to another one before that has begun
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
   c.hist = reinterpret_cast<uint32_t*>(tc_smem);
-  c.row = reinterpret_cast<float*>(tc_smem + kTcHistBytes);
+  c.list_far = reinterpret_cast<float*>(c.hist + 3 * kTcBins);
+  c.list_at = reinterpret_cast<int*>(c.list_far + kTcMembers);
+  c.list_w = reinterpret_cast<uint32_t*>(c.list_at + kTcMembers);
+  c.row = reinterpret_cast<float*>(tc_smem + kTcRowAt);
   c.mail = &mail;
-  c.tmp = tmp;
   c.v0 = c.rank * cols;
-  c.n = max(0, min(cols, V - c.v0));
-  c.lo = min(c.n, tid * seg);
-  c.hi = min(c.n, c.lo + seg);
+  const int n = max(0, min(cols, V - c.v0)), padded = (n + 127) & ~127;
+  const int span = ((padded >> 7) + kTcWarps - 1) / kTcWarps * 128;
+  c.lo = min(padded, warp * span);
+  c.hi = min(padded, c.lo + span);
 
-  // ---- the row
-  uint32_t* table = reinterpret_cast<uint32_t*>(c.row);  // each place holds a count until its logit comes
-  if (t.penalties) {
-    for (int i = tid; i < c.n; i += kTcThreads) table[i] = 0;
-    __syncthreads();
-    tc_count(t, V, c.v0, c.n, table, report, status);
-    __syncthreads();
-  }
+  // ---- the row; its first columns on their way while the history is counted
   const T* src = logits + (long long)e * stride + c.v0;
-  constexpr int kN = kVec ? 8 : 1;
-  for (int i = tid * kN; i < c.n; i += kTcThreads * kN) {
-    float f[kN];
-    const bool whole = i + kN <= c.n;
-    if (whole) {
-      tc_load<T, kN>(src + i, f);
+  constexpr int kAhead = 2;
+  float ahead[kAhead][8];
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s) {
+    const int i = 8 * (tid + s * kTcThreads);
+    if (vec && i + 8 <= n) {
+      ld_vec(src + i, ahead[s]);
     } else {
 #pragma unroll
-      for (int j = 0; j < kN; ++j) f[j] = i + j < c.n ? ld_elem(src + i + j) : 0.f;
+      for (int j = 0; j < 8; ++j) ahead[s][j] = i + j < n ? ld_elem(src + i + j) : -INFINITY;
     }
-    const uint32_t bits = t.mask ? t.mask[(c.v0 + i) >> 5] >> ((c.v0 + i) & 31) : ~0u;
-    float seen[kN];
-    if (t.penalties) {
-      if (whole) tc_load<float, kN>(c.row + i, seen);
-      else
-#pragma unroll
-        for (int j = 0; j < kN; ++j) seen[j] = i + j < c.n ? c.row[i + j] : 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      if (t.penalties) f[j] = tc_penalised(t, f[j], __float_as_uint(seen[j]));
-      if (!(bits >> j & 1u) || f[j] != f[j]) f[j] = -INFINITY;
-    }
-    if (whole) st_vec(c.row + i, f);
-    else
-#pragma unroll
-      for (int j = 0; j < kN; ++j)
-        if (i + j < c.n) c.row[i + j] = f[j];
   }
-  __syncthreads();
+  uint32_t* table = reinterpret_cast<uint32_t*>(c.row);  // each place holds a count until its logit comes
+  if (t.penalties) {
+    for (int i = 4 * tid; i < padded; i += 4 * kTcThreads) *reinterpret_cast<uint4*>(table + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    tc_count(t, V, c.v0, n, table, report, status);
+    __syncthreads();
+  }
+  float best = -INFINITY;
+  const auto settle = [&](int i, float (&f)[8]) {
+    if (t.penalties) {
+      float seen[8];
+      ld_vec(c.row + i, seen);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = tc_penalised(t, f[j], __float_as_uint(seen[j]));
+    }
+    const uint32_t bits = t.mask && i < n ? t.mask[(c.v0 + i) >> 5] >> ((c.v0 + i) & 31) : ~0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (!(bits >> j & 1u) || f[j] != f[j]) f[j] = -INFINITY;
+      best = fmaxf(best, f[j]);
+    }
+    st_vec(c.row + i, f);
+  };
+  const auto load = [&](int i, float (&f)[8]) {
+    if (vec && i + 8 <= n) {
+      ld_vec(src + i, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = i + j < n ? ld_elem(src + i + j) : -INFINITY;
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s) {
+    const int i = 8 * (tid + s * kTcThreads);
+    if (i < padded) settle(i, ahead[s]);
+  }
+  for (int i = 8 * (tid + kAhead * kTcThreads); i < padded; i += 8 * kTcThreads) {
+    float f[8];
+    load(i, f);
+    settle(i, f);
+  }
   if (r.num_bias) {
-    tc_bias(r, t, e, V, c.v0, c.n, report, status, [&](int id, float s) {
+    __syncthreads();
+    tc_bias(r, t, e, V, c.v0, n, report, status, [&](int id, float s) {
       const float l = __fadd_rn(c.row[id - c.v0], s);
       c.row[id - c.v0] = l == l ? l : -INFINITY;
     });
     __syncthreads();
+    best = -INFINITY;
+    c.each([&](int, float l) { best = fmaxf(best, l); });
   }
-
-  // ---- the largest, the first one of equals
-  float best = -INFINITY;
-  int at = 0x7fffffff;
-  for (int i = c.lo; i < c.hi; ++i)
-    if (c.row[i] > best) { best = c.row[i]; at = c.v0 + i; }
-  auto better = [&](float v, int i) {
-    if (v > best || (v == best && i < at)) { best = v; at = i; }
-  };
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
-  if (lane == 0) { tmp_v[warp] = best; tmp_i[warp] = at; }
+  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (lane == 0) tmp_f[warp] = best;
   __syncthreads();
   asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
-  if (tid == 0) {
-    for (int w = 1; w < kTcWarps; ++w) better(tmp_v[w], tmp_i[w]);
-    tc_tell(&mail.best[c.rank], best);
-    tc_tell(&mail.best_at[c.rank], at);
+  if (warp == 0) {
+    best = lane < kTcWarps ? tmp_f[lane] : -INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    tc_tell(&mail.best[c.rank], best, c.blocks);
   }
   tc_cluster_sync();
   best = mail.best[0];
-  at = mail.best_at[0];
-  for (int q = 1; q < kTcCluster; ++q) better(mail.best[q], mail.best_at[q]);
+  for (int q = 1; q < c.blocks; ++q) best = fmaxf(best, mail.best[q]);
   c.m = best;
   if (best == -INFINITY) {  // nothing is allowed
     if (report && tid == 0) {
@@ -572,71 +687,136 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   const int k = d.top_k ? d.top_k[e] : 0;
   const float p = d.top_p ? d.top_p[e] : 1.f, min_p = d.min_p ? d.min_p[e] : 0.f;
   const bool greedy = !(tau > 0.f) || k == 1;
-  c.inv_tau = greedy ? 1.f : fminf(__fdiv_rn(1.f, tau), 3e38f);  // (finite: the largest is 0 units behind itself)
+  c.unit = greedy ? kTcLog2e : fminf(__fdiv_rn(kTcLog2e, tau), 3e38f);  // (finite: the largest is 0 units behind itself)
 
-  // ---- weights beside the largest's, at temperature 1: the token's probability is exp(-behind) / (1 + rest)
-  float rest = 0.f;
-  for (int i = c.lo; i < c.hi; ++i)
-    if (c.v0 + i != at) rest += expf(-c.behind(c.row[i]));
-  double block_rest, unused;
-  tc_block_before((double)rest, tmp, unused, block_rest);
-  if (tid == 0) tc_tell(&mail.rest[c.rank], block_rest);
-
-  if (!greedy) {
-    TcCut cut;
-    auto apply = [&]() {
-      for (int i = c.lo; i < c.hi; ++i) {
-        const float l = c.row[i], far = c.behind(l);
-        const int side = cut.exact ? (far < cut.behind ? -1 : far > cut.behind) : cut.side(c.z(l));
-        if (side > 0 || (side == 0 && c.v0 + i > cut.at)) c.row[i] = -INFINITY;
-      }
-    };
-    if (k > 0 && k < V && tc_select<false>(c, (uint32_t)k, 0.f, cut)) apply();
-    if (p < 1.f && tc_select<true>(c, 0, p > 0.f ? p : 0.f, cut)) apply();
+  // ---- weights beside the largest ones', at temperature 1: a token's probability is exp(-behind) / (number of the largest + rest); and at the entry's
+  float rest = 0.f, part = 0.f;
+  int first = 0x7fffffff, equal = 0;
+  c.each([&](int i, float l) {
+    if (l == c.m) {
+      first = min(first, c.v0 + i);
+      ++equal;
+    } else {
+      rest += tc_exp2((l - c.m) * kTcLog2e);
+      part += tc_exp2((l - c.m) * c.unit);
+    }
+  });
+  part += (float)equal;
+  double mine = tc_warp_sum((double)part);
+  rest = tc_warp_sum(rest);
+  equal = tc_warp_sum(equal);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+  if (lane == 0) {
+    tmp_f[warp] = rest;
+    tmp_i[warp] = first;
+    tmp_n[warp] = equal;
+    tmp_d[warp] = mine;
   }
-  int token = at;
+  __syncthreads();
+  if (warp == 0) {
+    rest = tc_warp_sum(lane < kTcWarps ? tmp_f[lane] : 0.f);
+    equal = tc_warp_sum(lane < kTcWarps ? tmp_n[lane] : 0);
+    first = lane < kTcWarps ? tmp_i[lane] : 0x7fffffff;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+    double block = 0.;
+    for (int w = 0; w < kTcWarps; ++w) block += tmp_d[w];
+    tc_tell(&mail.rest[c.rank], rest, c.blocks);
+    tc_tell(&mail.equal[c.rank], equal, c.blocks);
+    tc_tell(&mail.first[c.rank], first, c.blocks);
+    tc_tell(&mail.mass[c.rank], block, c.blocks);
+    tc_tell(&mail.weight[c.rank], (float)block, c.blocks);
+  }
+
+  TcCut by_count, by_mass;
+  const bool some = k > 0 && k < V, share = p < 1.f;
+  if (!greedy) {
+    if (some) by_count = tc_select<false>(c, (uint32_t)k, 0.f, by_mass, false);
+    if (share) by_mass = tc_select<true>(c, 0, p > 0.f ? p : 0.f, by_count, !by_count.on);
+  }
+  int token = -1;
   float taken = 0.f;  // how far behind the largest it is
   if (greedy) {
-    tc_cluster_sync();  // the other blocks' rests
+    tc_cluster_sync();  // the other blocks' sums
     if (!report || tid != 0) return;
   } else {
-    // ---- the kept weights, thread after thread in order of the columns
-    auto weight = [&](int i) {
-      const float l = c.row[i];
-      if (l == -INFINITY) return 0.f;
-      const float w = expf(-c.z(l));
-      return w >= min_p || l == c.m ? w : 0.f;
+    // ---- the kept weights, warp after warp in order of the columns
+    const bool cuts = by_count.on || by_mass.on || min_p > 0.f;
+    const float floor = fmaxf(fmaxf(by_count.floor, by_mass.floor), min_p > 0.f ? c.floor(fmaxf(-log2f(min_p), 0.f) + 0.001f) : -INFINITY);
+    const auto weight = [&](int i, float l) {
+      if (l < floor) return 0.f;
+      const float w = tc_exp2(-c.z(l));
+      return !cuts || ((w >= min_p || l == c.m) && by_mass.keeps(c, i, l) && by_count.keeps(c, i, l)) ? w : 0.f;
     };
-    float mine = 0.f;
-    for (int i = c.lo; i < c.hi; ++i) mine += weight(i);
-    double block, upto;
-    const double before = tc_block_before((double)mine, tmp, upto, block);
-    if (tid == 0) tc_tell(&mail.mass[c.rank], block);
+    if (cuts) {
+      part = 0.f;
+      c.each_above(floor, [&](int i, float l) { part += weight(i, l); });
+      mine = tc_warp_sum((double)part);
+      __syncthreads();  // (the sums so far have been read)
+      if (lane == 0) tmp_d[warp] = mine;
+      __syncthreads();
+      if (warp == 0) {
+        double block = 0.;
+        for (int w = 0; w < kTcWarps; ++w) block += tmp_d[w];
+        tc_tell(&mail.mass[c.rank], block, c.blocks);
+      }
+    }
     tc_cluster_sync();
-    double all = 0., start = 0.;
-    for (int q = 0; q < kTcCluster; ++q) {
-      if (q == c.rank) start = all;
+    double all = 0., from = 0., before = 0.;
+    for (int q = 0; q < c.blocks; ++q) {
+      if (q == c.rank) from = all;
       all += mail.mass[q];
     }
-    // the thread that the goal falls to (each begins where the one in front ends); its own sums, as above, say which column
+    // the warp that the goal falls to: each begins where the one in front ends
+    for (int w = 0; w < warp; ++w) before += tmp_d[w];
+    const double to = from + (before + mine);
+    from += before;
     const float u = d.uniform ? d.uniform[e] : 0.f;
-    const double goal = all * (double)fminf(fmaxf(u, 0.f), 1.f - 5.9604645e-8f), from = start + before;
-    if (goal < from || goal >= start + upto) return;
-    float sum = 0.f;
-    for (int i = c.lo; i < c.hi; ++i) {
-      const float w = weight(i);
-      sum += w;
-      if (w > 0.f) {
-        token = c.v0 + i;
-        taken = c.behind(c.row[i]);
+    const double goal = all * (double)fminf(fmaxf(u, 0.f), 1.f - 5.9604645e-8f);
+    if (goal < from || goal >= to) return;
+    for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
+      const int i = i0 + 4 * lane;
+      const float4 l = *reinterpret_cast<const float4*>(c.row + i);
+      const float f[4] = {l.x, l.y, l.z, l.w};
+      float w[4], here = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = weight(i + j, f[j]);
+        here += w[j];
       }
-      if (from + (double)sum > goal) break;
+      const double upto = tc_warp_scan((double)here);
+      double run = from + (upto - (double)here);
+      int at = -1;
+      float far = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        run += (double)w[j];
+        if (w[j] > 0.f && at < 0 && run > goal) {
+          at = c.v0 + i + j;
+          far = c.behind(f[j]);
+        }
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, at >= 0);
+      if (hit) {
+        token = __shfl_sync(0xffffffffu, at, __ffs(hit) - 1);
+        taken = __shfl_sync(0xffffffffu, far, __ffs(hit) - 1);
+        break;
+      }
+      from += __shfl_sync(0xffffffffu, upto, 31);
     }
+    if (lane != 0) return;
   }
+  int largest = 0x7fffffff, same = 0;
   double others = 0.;
-  for (int q = 0; q < kTcCluster; ++q) others += mail.rest[q];
+  for (int q = 0; q < c.blocks; ++q) {
+    others += mail.rest[q];
+    same += mail.equal[q];
+    largest = min(largest, mail.first[q]);
+  }
+  if (token < 0) token = largest;  // (greedy, or the last bit of a sum)
   tokens[e] = token;
-  logprobs[e] = -(float)((double)taken + log1p(others));
+  logprobs[e] = -(float)((double)taken + log1p(others + (same - 1)));
   if (append && t.history && t.length < r.capacity) r.history[(long long)t.slot * r.capacity + t.length] = token;
 }
 
@@ -684,7 +864,7 @@ extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t
   if (entries == 0) return B200KV_OK;
   if (!logits || !draw || !tokens || !logprobs) return B200KV_E_NULL;
   if (draw->temperature && !draw->uniform) return B200KV_E_NULL;
-  if (entries < 0 || entries > (1 << 24) || vocab < 1 || vocab > kTcCluster * kTcMaxLocal) return B200KV_E_RANGE;
+  if (entries < 0 || entries > (1 << 24) || vocab < 1 || vocab > kTcMaxCluster * kTcMaxLocal) return B200KV_E_RANGE;
   if ((elem != 2 && elem != 4) || stride < vocab) return B200KV_E_SHAPE;
   if (!aligned(logits, elem) || !aligned(tokens, 8) || !aligned(logprobs, 4)) return B200KV_E_ALIGN;
   for (const void* p : {(const void*)draw->temperature, (const void*)draw->top_k, (const void*)draw->top_p, (const void*)draw->min_p, (const void*)draw->uniform})
@@ -692,26 +872,29 @@ extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t
   TcRules r;
   if (int rc = tc_rules(rules, vocab, &r)) return rc;
   const TcDraw d{draw->temperature, draw->top_k, draw->top_p, draw->min_p, draw->uniform};
-  const int cols = ((vocab + kTcCluster - 1) / kTcCluster + 31) / 32 * 32;
-  const int seg = (cols + kTcThreads - 1) / kTcThreads | 1;  // odd: a warp's threads are at different banks
+  // Halved while that leaves a block few columns, or as many blocks as are not resident at once (two a multiprocessor, but for the rest of a graphics
+  // cluster), and two blocks still share a multiprocessor.
+  int blocks = kTcMaxCluster;
+  const auto share = [&](int n) { return ((vocab + n - 1) / n + 127) / 128 * 128; };
+  while (blocks > 1 && share(blocks / 2) <= 20 * 1024 && (share(blocks) < 2048 || (long long)entries * blocks > device_sms() * 12 / 7)) blocks /= 2;
+  const int cols = share(blocks);
   const bool vec = aligned(logits, 16) && stride * elem % 16 == 0;
   auto go = [&](auto kernel, auto* src) {
-    if (!allow_smem(kernel, kTcHistBytes + kTcMaxLocal * 4)) return launch_result(cudaErrorInvalidValue);
+    if (!allow_smem(kernel, kTcRowAt + kTcMaxLocal * 4)) return launch_result(cudaErrorInvalidValue);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)entries * kTcCluster);
+    cfg.gridDim = dim3((unsigned)(entries * blocks));
     cfg.blockDim = dim3(kTcThreads);
-    cfg.dynamicSmemBytes = kTcHistBytes + (size_t)cols * 4;
+    cfg.dynamicSmemBytes = kTcRowAt + (size_t)cols * 4;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kTcCluster;
+    attr[0].val.clusterDim.x = blocks;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = take_chained_launch((cudaStream_t)stream) ? 2 : 1;
-    return launch_result(cudaLaunchKernelEx(&cfg, kernel, src, (long long)stride, r, d, (int)vocab, cols, seg, append != 0, (long long*)tokens, logprobs, status));
+    return launch_result(cudaLaunchKernelEx(&cfg, kernel, src, (long long)stride, r, d, (int)vocab, cols, vec, append != 0, (long long*)tokens, logprobs, status));
   };
-  if (elem == 4) return vec ? go(choose_tokens_kernel<float, true>, (const float*)logits) : go(choose_tokens_kernel<float, false>, (const float*)logits);
-  return vec ? go(choose_tokens_kernel<uint16_t, true>, (const uint16_t*)logits) : go(choose_tokens_kernel<uint16_t, false>, (const uint16_t*)logits);
+  return elem == 4 ? go(choose_tokens_kernel<float>, (const float*)logits) : go(choose_tokens_kernel<uint16_t>, (const uint16_t*)logits);
 }
