@@ -13,7 +13,8 @@
 // happens on the multiprocessors.  With m the largest, z = (m - l) / temperature and w = exp(-z), tokens are ordered by l (equal ones by
 // index).  Kept are the first top_k; of these the shortest run whose weight is at least top_p of theirs; of these the ones with w >= min_p.
 // The token is the first, by index, at which the kept weights so far exceed uniform * their sum.
-// A cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the likelier tokens, or over the others if
+// Where no more than 512 tokens are within a weight of 2^-12 of the largest and the cuts lie among those, one block takes them all, puts them in order and draws.
+// Otherwise a cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the likelier tokens, or over the others if
 // it does not lie there, down to the few tokens of one bin, which are put in order by comparison.  Blocks tell one another sums of bins, and read
 // from one another only the bins among which the cut lies: a barrier of the cluster each for the largest logit, the histogram, the bin's
 // tokens and the kept weights.
@@ -186,6 +187,10 @@ constexpr int kTcMaxCluster = 8;
 constexpr int kTcBins = 1024, kTcCoarse = 32;  // and sums of 32 bins
 constexpr int kTcMembers = 1024;               // tokens of one bin that are put in order
 constexpr int kTcMaxLocal = 48 * 1024;         // columns of a block
+constexpr int kTcShort = 512;                  // likely tokens that are drawn from without histograms: one a thread
+constexpr float kTcShortZ = 12.f;              // weights from 2^-12 on
+constexpr int kTcShortWarp = 64;               // of a warp's columns
+static_assert(kTcShort == kTcThreads && kTcShortWarp * kTcWarps <= kTcMembers && 5 * kTcShort <= 3 * kTcBins, "places of the likely tokens");
 constexpr uint32_t kTcRowAt = kTcBins * 12 + kTcMembers * 12;  // the histogram, a bin's tokens, the row
 
 struct TcDraw {
@@ -204,6 +209,8 @@ struct TcMail {
   unsigned long long coarse_mass[kTcMaxCluster][kTcCoarse];
   uint32_t coarse_count[kTcMaxCluster][kTcCoarse];
   uint32_t listed_by[kTcMaxCluster];
+  uint32_t likely[kTcMaxCluster];  // number of likely tokens; more than kTcShort: some warp had no place for its own
+  uint32_t settled;
   uint32_t ties[kTcMaxCluster];
   // within the block
   uint32_t listed;
@@ -377,10 +384,12 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     __syncthreads();
     if (weigh && warp == 0) tc_tell(&mail.weight[c.rank], tc_warp_sum(lane < kTcWarps ? c.list_far[lane] : 0.f), c.blocks);
     for (int i = warp; i < kTcCoarse; i += kTcWarps) {
-      const int b = 32 * i + lane;
-      const uint32_t count = tc_warp_sum(c.hist[b]);
-      tc_tell(&mail.coarse_count[c.rank][i], count, c.blocks);
-      if (kMass) tc_tell(&mail.coarse_mass[c.rank][i], tc_warp_sum(((unsigned long long)c.hist[kTcBins + b] << 16) + c.hist[2 * kTcBins + b]), c.blocks);
+      const int b = 32 * i + lane;  // (no sum of halves reaches 2^32: a block has fewer than 2^16 columns)
+      tc_tell(&mail.coarse_count[c.rank][i], __reduce_add_sync(0xffffffffu, c.hist[b]), c.blocks);
+      if (kMass) {
+        const uint32_t hi = __reduce_add_sync(0xffffffffu, c.hist[kTcBins + b]), lo = __reduce_add_sync(0xffffffffu, c.hist[2 * kTcBins + b]);
+        tc_tell(&mail.coarse_mass[c.rank][i], ((unsigned long long)hi << 16) + lo, c.blocks);
+      }
     }
     tc_cluster_sync();
     if (kMass && first) {
@@ -566,6 +575,8 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   __shared__ float tmp_f[kTcWarps];
   __shared__ int tmp_i[kTcWarps], tmp_n[kTcWarps];
   __shared__ double tmp_d[kTcWarps];
+  __shared__ int tmp_s[kTcWarps];
+  __shared__ unsigned long long tmp_u[kTcWarps];
   pdl_enter();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -692,15 +703,40 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   // ---- weights beside the largest ones', at temperature 1: a token's probability is exp(-behind) / (number of the largest + rest); and at the entry's
   float rest = 0.f, part = 0.f;
   int first = 0x7fffffff, equal = 0;
-  c.each([&](int i, float l) {
-    if (l == c.m) {
-      first = min(first, c.v0 + i);
-      ++equal;
-    } else {
-      rest += tc_exp2((l - c.m) * kTcLog2e);
-      part += tc_exp2((l - c.m) * c.unit);
+  const bool some = k > 0 && k < V, share = p < 1.f, cuts = some || share || min_p > 0.f;
+  const bool in_reach = !greedy && cuts && k <= kTcShort && (some || share || min_p >= 0.00025f);  // (2^-12 is 0.000244)
+  const float likely = in_reach ? c.floor(kTcShortZ) : INFINITY;
+  int found = 0;  // by this warp, in order of the columns
+  for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
+    const int i = i0 + 4 * lane;
+    const float4 l4 = *reinterpret_cast<const float4*>(c.row + i);
+    const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (l[j] == c.m) {
+        first = min(first, c.v0 + i + j);
+        ++equal;
+      } else {
+        rest += tc_exp2((l[j] - c.m) * kTcLog2e);
+        part += tc_exp2((l[j] - c.m) * c.unit);
+      }
     }
-  });
+    if (__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= likely)) {
+      const int here = (l[0] >= likely) + (l[1] >= likely) + (l[2] >= likely) + (l[3] >= likely), upto = tc_warp_scan(here);
+      int at = found + upto - here;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (l[j] >= likely) {
+          if (at < kTcShortWarp) {
+            c.list_far[warp * kTcShortWarp + at] = l[j];
+            c.list_at[warp * kTcShortWarp + at] = c.v0 + i + j;
+          }
+          ++at;
+        }
+      }
+      found += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
   part += (float)equal;
   double mine = tc_warp_sum((double)part);
   rest = tc_warp_sum(rest);
@@ -712,6 +748,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     tmp_i[warp] = first;
     tmp_n[warp] = equal;
     tmp_d[warp] = mine;
+    tmp_s[warp] = found;
   }
   __syncthreads();
   if (warp == 0) {
@@ -727,10 +764,134 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     tc_tell(&mail.first[c.rank], first, c.blocks);
     tc_tell(&mail.mass[c.rank], block, c.blocks);
     tc_tell(&mail.weight[c.rank], (float)block, c.blocks);
+    const int mine_of = lane < kTcWarps ? tmp_s[lane] : 0;
+    const bool full = __any_sync(0xffffffffu, mine_of > kTcShortWarp);
+    tc_tell(&mail.likely[c.rank], full ? (uint32_t)kTcShort + 1 : __reduce_add_sync(0xffffffffu, (uint32_t)mine_of), c.blocks);
+  }
+
+  // ---- few likely tokens
+  if (in_reach) {
+    // this block's side by side, behind the warps' own
+    float* own_l = reinterpret_cast<float*>(c.hist);
+    int* own_at = reinterpret_cast<int*>(c.hist + kTcShort);
+    int at = 0;
+    for (int w = 0; w < warp; ++w) at += tmp_s[w];
+    for (int i = lane; i < min(found, kTcShortWarp); i += 32) {
+      if (at + i < kTcShort) {
+        own_l[at + i] = c.list_far[warp * kTcShortWarp + i];
+        own_at[at + i] = c.list_at[warp * kTcShortWarp + i];
+      }
+    }
+    tc_cluster_sync();
+    uint32_t num = 0;
+    for (int q = 0; q < c.blocks; ++q) num += mail.likely[q];
+    if (num <= (uint32_t)kTcShort) {
+      if (report) {
+        // one a thread, in order of the columns
+        float l = -INFINITY;
+        int col = 0x7fffffff;
+        uint32_t before = 0;
+        for (int q = 0; q < c.blocks; ++q) {
+          const uint32_t theirs = mail.likely[q];
+          if (tid >= before && tid < before + theirs) {
+            l = __uint_as_float(tc_get(tc_there(own_l + (tid - before), q)));
+            col = (int)tc_get(tc_there(own_at + (tid - before), q));
+          }
+          before += theirs;
+        }
+        const float far = c.behind(l), w = tid < num ? tc_exp2(-__fmul_rn(far, c.unit)) : 0.f;
+        const uint32_t q = tid < num ? __float2uint_rn(w * 4294967296.f) : 0u;
+        // how many of them are in front of each, shared out over the threads
+        float* all_l = c.list_far;
+        uint32_t* rank_of = c.hist + 2 * kTcShort;
+        unsigned long long* sorted = reinterpret_cast<unsigned long long*>(c.hist + 3 * kTcShort);
+        all_l[tid] = l;
+        rank_of[tid] = 0;
+        sorted[tid] = 0;
+        __syncthreads();
+        const uint32_t each = num ? (uint32_t)kTcThreads / num : 1, group = each ? tid / num : 0;
+        if (group < each) {
+          const uint32_t i = tid - group * num;
+          const float mine_l = all_l[i];
+          uint32_t front = 0;
+          for (uint32_t j = group; j < num; j += each) front += all_l[j] > mine_l || (all_l[j] == mine_l && j < i);
+          atomicAdd(&rank_of[i], front);
+        }
+        __syncthreads();
+        const uint32_t mine_rank = rank_of[tid];
+        if (tid < num) sorted[mine_rank] = q;
+        __syncthreads();
+        // weights in front of each place
+        const unsigned long long here = sorted[tid], upto_w = tc_warp_scan(here);
+        if (lane == 31) tmp_u[warp] = upto_w;
+        __syncthreads();
+        unsigned long long front_w = upto_w - here;
+        for (int w2 = 0; w2 < warp; ++w2) front_w += tmp_u[w2];
+        sorted[tid] = front_w;
+        if (tid == kTcThreads - 1) mail.mass_before = front_w + here;  // of all
+        __syncthreads();
+        const unsigned long long all_w = mail.mass_before;
+        double target = INFINITY;
+        bool ok = num > 0 && (!some || num >= (uint32_t)k);
+        if (share) {
+          double of;
+          if (some) {
+            of = (double)((uint32_t)k < num ? sorted[k] : all_w);
+          } else {
+            of = 0.;
+            for (int b = 0; b < c.blocks; ++b) of += mail.mass[b];
+            of *= 4294967296.;
+          }
+          target = fmax((double)(p > 0.f ? p : 0.f) * of, 0.5);
+          ok = ok && (double)all_w >= target;
+        }
+        if (ok) {
+          const bool keep = tid < num && (!some || mine_rank < (uint32_t)k) && (double)sorted[mine_rank] < target && (w >= min_p || l == c.m);
+          const double kept = keep ? (double)w : 0., upto_k = tc_warp_scan(kept);
+          __syncthreads();
+          if (lane == 31) tmp_d[warp] = upto_k;
+          __syncthreads();
+          double from = 0., all = 0.;
+          for (int w2 = 0; w2 < kTcWarps; ++w2) {
+            if (w2 == warp) from = all;
+            all += tmp_d[w2];
+          }
+          const float u = d.uniform ? d.uniform[e] : 0.f;
+          const double goal = all * (double)fminf(fmaxf(u, 0.f), 1.f - 5.9604645e-8f);
+          // the first kept one that reaches beyond the goal; by a sum's last bit perhaps none, then the last one
+          const unsigned hit = __ballot_sync(0xffffffffu, keep && from + upto_k > goal), any = __ballot_sync(0xffffffffu, keep);
+          if (lane == 0) {
+            tmp_i[warp] = hit ? warp * 32 + __ffs(hit) - 1 : 0x7fffffff;
+            tmp_n[warp] = any ? warp * 32 + 31 - __clz(any) : -1;
+          }
+          __syncthreads();
+          int pick = 0x7fffffff, last = -1;
+          for (int w2 = 0; w2 < kTcWarps; ++w2) {
+            pick = min(pick, tmp_i[w2]);
+            last = max(last, tmp_n[w2]);
+          }
+          if (pick == 0x7fffffff) pick = last;
+          if (tid == pick) {
+            double others = 0.;
+            int same = 0;
+            for (int b = 0; b < c.blocks; ++b) {
+              others += mail.rest[b];
+              same += mail.equal[b];
+            }
+            tokens[e] = col;
+            logprobs[e] = -(float)((double)far + log1p(others + (same - 1)));
+            if (append && t.history && t.length < r.capacity) r.history[(long long)t.slot * r.capacity + t.length] = col;
+          }
+        }
+        __syncthreads();
+        if (warp == 0) tc_tell(&mail.settled, (uint32_t)ok, c.blocks);
+      }
+      tc_cluster_sync();
+      if (mail.settled) return;
+    }
   }
 
   TcCut by_count, by_mass;
-  const bool some = k > 0 && k < V, share = p < 1.f;
   if (!greedy) {
     if (some) by_count = tc_select<false>(c, (uint32_t)k, 0.f, by_mass, false);
     if (share) by_mass = tc_select<true>(c, 0, p > 0.f ? p : 0.f, by_count, !by_count.on);
@@ -742,7 +903,6 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     if (!report || tid != 0) return;
   } else {
     // ---- the kept weights, warp after warp in order of the columns
-    const bool cuts = by_count.on || by_mass.on || min_p > 0.f;
     const float floor = fmaxf(fmaxf(by_count.floor, by_mass.floor), min_p > 0.f ? c.floor(fmaxf(-log2f(min_p), 0.f) + 0.001f) : -INFINITY);
     const auto weight = [&](int i, float l) {
       if (l < floor) return 0.f;
