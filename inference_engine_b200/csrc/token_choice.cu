@@ -13,7 +13,7 @@
 // happens on the multiprocessors.  With m the largest, z = (m - l) / temperature and w = exp(-z), tokens are ordered by l (equal ones by
 // index).  Kept are the first top_k; of these the shortest run whose weight is at least top_p of theirs; of these the ones with w >= min_p.
 // The token is the first, by index, at which the kept weights so far exceed uniform * their sum.
-// Where no more than 512 tokens are within a weight of 2^-12 of the largest and the cuts lie among those, one block takes them all, puts them in order and draws.
+// Where no more than 512 tokens are within a weight of 2^-16, or else of 2^-12, of the largest and the cuts lie among those, one block takes them all, puts them in order and draws.
 // Otherwise a cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the likelier tokens, or over the others if
 // it does not lie there, down to the few tokens of one bin, which are put in order by comparison.  Blocks tell one another sums of bins, and read
 // from one another only the bins among which the cut lies: a barrier of the cluster each for the largest logit, the histogram, the bin's
@@ -188,7 +188,8 @@ constexpr int kTcBins = 1024, kTcCoarse = 32;  // and sums of 32 bins
 constexpr int kTcMembers = 1024;               // tokens of one bin that are put in order
 constexpr int kTcMaxLocal = 48 * 1024;         // columns of a block
 constexpr int kTcShort = 512;                  // likely tokens that are drawn from without histograms: one a thread
-constexpr float kTcShortZ = 12.f;              // weights from 2^-12 on
+constexpr float kTcShortZ[2] = {16.f, 12.f};   // weights from 2^-16 on, or from 2^-12 on if those are too many
+constexpr uint32_t kTcNoPlace = 1u << 20;
 constexpr int kTcShortWarp = 64;               // of a warp's columns
 static_assert(kTcShort == kTcThreads && kTcShortWarp * kTcWarps <= kTcMembers && 5 * kTcShort <= 3 * kTcBins, "places of the likely tokens");
 constexpr uint32_t kTcRowAt = kTcBins * 12 + kTcMembers * 12;  // the histogram, a bin's tokens, the row
@@ -206,17 +207,15 @@ struct TcMail {
   int first[kTcMaxCluster], equal[kTcMaxCluster];  // of the largest ones
   double mass[kTcMaxCluster];    // the weights that are drawn from
   float weight[kTcMaxCluster];   // of the tokens among which a share is kept
-  unsigned long long coarse_mass[kTcMaxCluster][kTcCoarse];
-  uint32_t coarse_count[kTcMaxCluster][kTcCoarse];
+  uint32_t coarse[3][kTcCoarse];   // of this block: counts, upper and lower halves of weights
   uint32_t listed_by[kTcMaxCluster];
-  uint32_t likely[kTcMaxCluster];  // number of likely tokens; more than kTcShort: some warp had no place for its own
+  uint32_t likely[2][kTcMaxCluster];  // number of likely tokens, and of the likelier ones; kTcNoPlace: some warp had no place for its own
   uint32_t settled;
   uint32_t ties[kTcMaxCluster];
   // within the block
+  uint32_t fetched[3][kTcMaxCluster][kTcCoarse];
   uint32_t listed;
-  int bin;
-  uint32_t count_before, members;
-  unsigned long long mass_before, mass_in;
+  unsigned long long all_mass;
   float cut_behind;
   int cut_at;
 };
@@ -385,10 +384,10 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     if (weigh && warp == 0) tc_tell(&mail.weight[c.rank], tc_warp_sum(lane < kTcWarps ? c.list_far[lane] : 0.f), c.blocks);
     for (int i = warp; i < kTcCoarse; i += kTcWarps) {
       const int b = 32 * i + lane;  // (no sum of halves reaches 2^32: a block has fewer than 2^16 columns)
-      tc_tell(&mail.coarse_count[c.rank][i], __reduce_add_sync(0xffffffffu, c.hist[b]), c.blocks);
-      if (kMass) {
-        const uint32_t hi = __reduce_add_sync(0xffffffffu, c.hist[kTcBins + b]), lo = __reduce_add_sync(0xffffffffu, c.hist[2 * kTcBins + b]);
-        tc_tell(&mail.coarse_mass[c.rank][i], ((unsigned long long)hi << 16) + lo, c.blocks);
+#pragma unroll
+      for (int w = 0; w < (kMass ? 3 : 1); ++w) {
+        const uint32_t sum = __reduce_add_sync(0xffffffffu, c.hist[w * kTcBins + b]);
+        if (lane == 0) mail.coarse[w][i] = sum;
       }
     }
     tc_cluster_sync();
@@ -397,80 +396,59 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       for (int q = 0; q < c.blocks; ++q) all += mail.weight[q];
       target = fmax((double)p * (double)all * 4294967296., 0.5);
     }
-    // the sum of bins, then the bin, that the cut lies in: every block for itself
-    if (warp == 0) {
-      uint32_t count = 0;
-      unsigned long long mass = 0;
+    // the sum of bins, then the bin, that the cut lies in: every block for itself, a warp fetching from each
+    const auto fetch = [&](const uint32_t* at, int apart) {  // at: this lane's place in a block
+      if (warp < c.blocks) {
+        uint32_t v[3];
+#pragma unroll
+        for (int w = 0; w < (kMass ? 3 : 1); ++w) v[w] = tc_get(tc_there(at + w * apart, warp));
+#pragma unroll
+        for (int w = 0; w < (kMass ? 3 : 1); ++w) mail.fetched[w][warp][lane] = v[w];
+      }
+      __syncthreads();
+    };
+    uint32_t count, c_upto;
+    unsigned long long mass, m_upto;
+    const auto add_up = [&]() {
+      count = 0;
+      mass = 0;
       for (int q = 0; q < c.blocks; ++q) {
-        count += mail.coarse_count[q][lane];
-        if (kMass) mass += mail.coarse_mass[q][lane];
+        count += mail.fetched[0][q][lane];
+        if (kMass) mass += ((unsigned long long)mail.fetched[1][q][lane] << 16) + mail.fetched[2][q][lane];
       }
-      uint32_t c_upto = tc_warp_scan(count);
-      unsigned long long m_upto = kMass ? tc_warp_scan(mass) : 0;
-      const uint32_t c_all = __shfl_sync(0xffffffffu, c_upto, 31);
-      const unsigned long long m_all = __shfl_sync(0xffffffffu, m_upto, 31);
-      const auto reached = [&]() { return kMass ? (double)(mass_before + m_upto) >= target : count_before + c_upto >= k; };
-      const unsigned hit = __ballot_sync(0xffffffffu, reached());
-      if (hit) {
-        const int group = __ffs(hit) - 1;
-        uint32_t cb = count_before + __shfl_sync(0xffffffffu, c_upto - count, group);
-        unsigned long long mb = mass_before + __shfl_sync(0xffffffffu, m_upto - mass, group);
-        const uint32_t* bin = c.hist + 32 * group + lane;
-        // (all on their way before the first is waited for)
-        uint32_t n[kTcMaxCluster], hi[kTcMaxCluster], lo[kTcMaxCluster];
-#pragma unroll
-        for (int q = 0; q < kTcMaxCluster; ++q) {
-          n[q] = hi[q] = lo[q] = 0;
-          if (q < c.blocks) {
-            n[q] = tc_get(tc_there(bin, q));
-            if (kMass) {
-              hi[q] = tc_get(tc_there(bin + kTcBins, q));
-              lo[q] = tc_get(tc_there(bin + 2 * kTcBins, q));
-            }
-          }
-        }
-        count = 0;
-        mass = 0;
-#pragma unroll
-        for (int q = 0; q < kTcMaxCluster; ++q) {
-          count += n[q];
-          mass += ((unsigned long long)hi[q] << 16) + lo[q];
-        }
-        c_upto = tc_warp_scan(count);
-        m_upto = kMass ? tc_warp_scan(mass) : 0;
-        const unsigned at = __ballot_sync(0xffffffffu, kMass ? (double)(mb + m_upto) >= target : cb + c_upto >= k);
-        if (lane == __ffs(at) - 1) {
-          mail.bin = 32 * group + lane;
-          mail.count_before = cb + c_upto - count;
-          mail.mass_before = mb + m_upto - mass;
-          mail.members = count;
-          mail.mass_in = mass;
-        }
-      } else if (lane == 0) {
-        mail.bin = -1;
-        mail.count_before = count_before + c_all;
-        mail.mass_before = mass_before + m_all;
-      }
-    }
-    __syncthreads();
-    count_before = mail.count_before;
-    mass_before = mail.mass_before;
-    if (mail.bin < 0) {
+      c_upto = count_before + tc_warp_scan(count);
+      m_upto = mass_before + (kMass ? tc_warp_scan(mass) : 0);
+      return __ballot_sync(0xffffffffu, kMass ? (double)m_upto >= target : c_upto >= k);
+    };
+    fetch(&mail.coarse[0][lane], kTcCoarse);
+    unsigned hit = add_up();  // (by every warp alike)
+    if (!hit) {
+      count_before = __shfl_sync(0xffffffffu, c_upto, 31);
+      mass_before = __shfl_sync(0xffffffffu, m_upto, 31);
+      tc_cluster_sync();  // (the blocks read this one's sums)
       if (base > 0.f) return TcCut();  // fewer tokens, or less weight, than would be kept; weights below 2^-80 do not count.  (A bin's parts have the bin's sums.)
-      tc_cluster_sync();  // (the blocks read this one's bins)
       base = 16.f;
       scale = kTcBins / 64.f;
       top = 80.f;
       continue;
     }
+    const int group = __ffs(hit) - 1;
+    count_before = __shfl_sync(0xffffffffu, c_upto - count, group);
+    mass_before = __shfl_sync(0xffffffffu, m_upto - mass, group);
+    __syncthreads();  // (every warp has added up)
+    fetch(c.hist + 32 * group + lane, kTcBins);
+    hit = add_up();
+    const int in_group = __ffs(hit) - 1, bin = 32 * group + in_group;
+    const uint32_t members = __shfl_sync(0xffffffffu, count, in_group);
+    const unsigned long long mass_in = __shfl_sync(0xffffffffu, mass, in_group);
+    count_before = __shfl_sync(0xffffffffu, c_upto - count, in_group);
+    mass_before = __shfl_sync(0xffffffffu, m_upto - mass, in_group);
     TcCut cut;
     cut.on = true;
     cut.base = base;
     cut.scale = scale;
-    cut.bin = mail.bin;
-    cut.floor = c.floor(base + (float)(mail.bin + 1) / scale);
-    const uint32_t members = mail.members;
-    const unsigned long long mass_in = mail.mass_in;
+    cut.bin = bin;
+    cut.floor = c.floor(base + (float)(bin + 1) / scale);
     if (members <= kTcMembers) {
       // the bin's tokens: every block's own, then all of them where the histogram was
       c.each_above(cut.floor, [&](int i, float l) {
@@ -488,15 +466,15 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       int* all_at = reinterpret_cast<int*>(c.hist + kTcMembers);
       uint32_t* all_w = c.hist + 2 * kTcMembers;
       uint32_t num = 0;
-      for (int q = 0; q < c.blocks; ++q) {
-        const uint32_t theirs = mail.listed_by[q];
-        for (uint32_t i = tid; i < theirs; i += kTcThreads) {
-          const uint32_t far = tc_get(tc_there(c.list_far + i, q)), at = tc_get(tc_there(c.list_at + i, q)), w = kMass ? tc_get(tc_there(c.list_w + i, q)) : 0;
-          all_far[num + i] = __uint_as_float(far);
-          all_at[num + i] = (int)at;
-          if (kMass) all_w[num + i] = w;
-        }
-        num += theirs;
+      for (int q = 0; q < c.blocks; ++q) num += mail.listed_by[q];
+      for (uint32_t i = tid; i < num; i += kTcThreads) {
+        int q = 0;
+        uint32_t at = i;
+        while (at >= mail.listed_by[q]) at -= mail.listed_by[q++];
+        const uint32_t far = tc_get(tc_there(c.list_far + at, q)), column = tc_get(tc_there(c.list_at + at, q)), w = kMass ? tc_get(tc_there(c.list_w + at, q)) : 0;
+        all_far[i] = __uint_as_float(far);
+        all_at[i] = (int)column;
+        if (kMass) all_w[i] = w;
       }
       tc_cluster_sync();  // (and nobody reads another block's list behind this)
       for (uint32_t i = tid; i < num; i += kTcThreads) {
@@ -524,8 +502,8 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     }
     if (level < 2) {
       tc_cluster_sync();  // (the blocks read this one's bins)
-      top = base + (float)(mail.bin + 1) / scale;
-      base += (float)mail.bin / scale;
+      top = base + (float)(bin + 1) / scale;
+      base += (float)bin / scale;
       scale *= (float)kTcBins;
       ++level;
       continue;
@@ -575,7 +553,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   __shared__ float tmp_f[kTcWarps];
   __shared__ int tmp_i[kTcWarps], tmp_n[kTcWarps];
   __shared__ double tmp_d[kTcWarps];
-  __shared__ int tmp_s[kTcWarps];
+  __shared__ int tmp_s[kTcWarps], tmp_l[kTcWarps];
   __shared__ unsigned long long tmp_u[kTcWarps];
   pdl_enter();
   pdl_wait();
@@ -705,8 +683,8 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   int first = 0x7fffffff, equal = 0;
   const bool some = k > 0 && k < V, share = p < 1.f, cuts = some || share || min_p > 0.f;
   const bool in_reach = !greedy && cuts && k <= kTcShort && (some || share || min_p >= 0.00025f);  // (2^-12 is 0.000244)
-  const float likely = in_reach ? c.floor(kTcShortZ) : INFINITY;
-  int found = 0;  // by this warp, in order of the columns
+  const float likely = in_reach ? c.floor(kTcShortZ[0]) : INFINITY, likelier = in_reach ? c.floor(kTcShortZ[1]) : INFINITY;
+  int found = 0, found_likelier = 0;  // by this warp, in order of the columns
   for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
     const int i = i0 + 4 * lane;
     const float4 l4 = *reinterpret_cast<const float4*>(c.row + i);
@@ -723,6 +701,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     }
     if (__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= likely)) {
       const int here = (l[0] >= likely) + (l[1] >= likely) + (l[2] >= likely) + (l[3] >= likely), upto = tc_warp_scan(here);
+      found_likelier += (l[0] >= likelier) + (l[1] >= likelier) + (l[2] >= likelier) + (l[3] >= likelier);
       int at = found + upto - here;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -750,6 +729,8 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     tmp_d[warp] = mine;
     tmp_s[warp] = found;
   }
+  found_likelier = __reduce_add_sync(0xffffffffu, found_likelier);
+  if (lane == 0) tmp_l[warp] = found_likelier;
   __syncthreads();
   if (warp == 0) {
     rest = tc_warp_sum(lane < kTcWarps ? tmp_f[lane] : 0.f);
@@ -764,40 +745,52 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     tc_tell(&mail.first[c.rank], first, c.blocks);
     tc_tell(&mail.mass[c.rank], block, c.blocks);
     tc_tell(&mail.weight[c.rank], (float)block, c.blocks);
-    const int mine_of = lane < kTcWarps ? tmp_s[lane] : 0;
-    const bool full = __any_sync(0xffffffffu, mine_of > kTcShortWarp);
-    tc_tell(&mail.likely[c.rank], full ? (uint32_t)kTcShort + 1 : __reduce_add_sync(0xffffffffu, (uint32_t)mine_of), c.blocks);
+    const uint32_t many = lane < kTcWarps ? tmp_s[lane] : 0, fewer = lane < kTcWarps ? tmp_l[lane] : 0;
+    const bool full = __any_sync(0xffffffffu, many > (uint32_t)kTcShortWarp);
+    tc_tell(&mail.likely[0][c.rank], full ? kTcNoPlace : __reduce_add_sync(0xffffffffu, many), c.blocks);
+    tc_tell(&mail.likely[1][c.rank], full ? kTcNoPlace : __reduce_add_sync(0xffffffffu, fewer), c.blocks);
   }
 
   // ---- few likely tokens
   if (in_reach) {
-    // this block's side by side, behind the warps' own
-    float* own_l = reinterpret_cast<float*>(c.hist);
-    int* own_at = reinterpret_cast<int*>(c.hist + kTcShort);
-    int at = 0;
-    for (int w = 0; w < warp; ++w) at += tmp_s[w];
-    for (int i = lane; i < min(found, kTcShortWarp); i += 32) {
-      if (at + i < kTcShort) {
-        own_l[at + i] = c.list_far[warp * kTcShortWarp + i];
-        own_at[at + i] = c.list_at[warp * kTcShortWarp + i];
-      }
-    }
     tc_cluster_sync();
-    uint32_t num = 0;
-    for (int q = 0; q < c.blocks; ++q) num += mail.likely[q];
-    if (num <= (uint32_t)kTcShort) {
+    uint32_t num = 0, fewer = 0;
+    for (int q = 0; q < c.blocks; ++q) {
+      num += mail.likely[0][q];
+      fewer += mail.likely[1][q];
+    }
+    if (min(num, fewer) <= (uint32_t)kTcShort) {
+      // this block's side by side, of the likelier ones if there are too many of the others
+      const bool all_of_them = num <= (uint32_t)kTcShort;
+      const float least = all_of_them ? likely : likelier;
+      num = all_of_them ? num : fewer;
+      float* own_l = reinterpret_cast<float*>(c.hist);
+      int* own_at = reinterpret_cast<int*>(c.hist + kTcShort);
+      int at = 0;
+      for (int w = 0; w < warp; ++w) at += all_of_them ? tmp_s[w] : tmp_l[w];
+      for (int i0 = 0; i0 < found; i0 += 32) {
+        const int i = warp * kTcShortWarp + i0 + lane;
+        const bool in = i0 + lane < found && c.list_far[i] >= least;
+        const unsigned those = __ballot_sync(0xffffffffu, in);
+        if (in) {
+          own_l[at + __popc(those & ((1u << lane) - 1))] = c.list_far[i];
+          own_at[at + __popc(those & ((1u << lane) - 1))] = c.list_at[i];
+        }
+        at += __popc(those);
+      }
+      tc_cluster_sync();
       if (report) {
         // one a thread, in order of the columns
         float l = -INFINITY;
         int col = 0x7fffffff;
-        uint32_t before = 0;
-        for (int q = 0; q < c.blocks; ++q) {
-          const uint32_t theirs = mail.likely[q];
-          if (tid >= before && tid < before + theirs) {
-            l = __uint_as_float(tc_get(tc_there(own_l + (tid - before), q)));
-            col = (int)tc_get(tc_there(own_at + (tid - before), q));
-          }
-          before += theirs;
+        if (tid < num) {
+          int q = 0;
+          uint32_t i = tid;
+          const uint32_t* by = mail.likely[all_of_them ? 0 : 1];
+          while (i >= by[q]) i -= by[q++];
+          const uint32_t raw = tc_get(tc_there(own_l + i, q));
+          col = (int)tc_get(tc_there(own_at + i, q));
+          l = __uint_as_float(raw);
         }
         const float far = c.behind(l), w = tid < num ? tc_exp2(-__fmul_rn(far, c.unit)) : 0.f;
         const uint32_t q = tid < num ? __float2uint_rn(w * 4294967296.f) : 0u;
@@ -828,9 +821,9 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
         unsigned long long front_w = upto_w - here;
         for (int w2 = 0; w2 < warp; ++w2) front_w += tmp_u[w2];
         sorted[tid] = front_w;
-        if (tid == kTcThreads - 1) mail.mass_before = front_w + here;  // of all
+        if (tid == kTcThreads - 1) mail.all_mass = front_w + here;  // of all
         __syncthreads();
-        const unsigned long long all_w = mail.mass_before;
+        const unsigned long long all_w = mail.all_mass;
         double target = INFINITY;
         bool ok = num > 0 && (!some || num >= (uint32_t)k);
         if (share) {
