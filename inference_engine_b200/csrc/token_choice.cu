@@ -207,13 +207,13 @@ struct TcMail {
   int first[kTcMaxCluster], equal[kTcMaxCluster];  // of the largest ones
   double mass[kTcMaxCluster];    // the weights that are drawn from
   float weight[kTcMaxCluster];   // of the tokens among which a share is kept
-  uint32_t coarse[3][kTcCoarse];   // of this block: counts, upper and lower halves of weights
+  uint32_t coarse[2][kTcCoarse];   // of this block: sums of 32 bins
   uint32_t listed_by[kTcMaxCluster];
   uint32_t likely[2][kTcMaxCluster];  // number of likely tokens, and of the likelier ones; kTcNoPlace: some warp had no place for its own
   uint32_t settled;
   uint32_t ties[kTcMaxCluster];
   // within the block
-  uint32_t fetched[3][kTcMaxCluster][kTcCoarse];
+  uint32_t fetched[2][kTcMaxCluster][kTcCoarse];
   uint32_t listed;
   unsigned long long all_mass;
   float cut_behind;
@@ -286,7 +286,7 @@ struct TcRow {
   float m;
   float unit;       // log2(e) / temperature: z below is in units of ln 2
   TcMail* mail;
-  uint32_t* hist;   // counts, upper and lower halves of weights
+  uint32_t* hist;   // counts, or upper and lower halves of weights
   float* list_far;  // a bin's tokens: how far behind the largest, column, weight
   int* list_at;
   uint32_t* list_w;
@@ -313,10 +313,10 @@ struct TcRow {
     for (int i = lo + 4 * (threadIdx.x & 31); i < hi; i += 128) {
       const float4 l = *reinterpret_cast<const float4*>(row + i);
       if (fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w)) < floor) continue;
-      const float v[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll 1
-      for (int j = 0; j < 4; ++j)
-        if (!(v[j] < floor)) f(i + j, v[j]);
+      if (!(l.x < floor)) f(i, l.x);
+      if (!(l.y < floor)) f(i + 1, l.y);
+      if (!(l.z < floor)) f(i + 2, l.z);
+      if (!(l.w < floor)) f(i + 3, l.w);
     }
   }
 };
@@ -348,18 +348,18 @@ struct TcCut {
 // off where nothing is cut.  By all threads of the cluster.  weighed: every block has told its tokens' weight.
 template <bool kMass>
 __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, const TcCut& had, bool weighed) {
+  constexpr int kWords = kMass ? 2 : 1;  // of a bin: its count, or its weight's halves
   TcMail& mail = *c.mail;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // z < 16, weights above 2^-16; then up to 80; then down into a bin
   float base = 0.f, scale = kTcBins / 16.f, top = 16.f;
   int level = 0;
-  uint32_t count_before = 0;
-  unsigned long long mass_before = 0;
-  double target = 0.;
+  unsigned long long before = 0;  // counts, or weights, in front of the bins
+  double target = (double)k;
   for (bool first = true;; first = false) {
     const bool weigh = kMass && first && !weighed;
     __syncthreads();  // (what was found before has been read)
-    for (int i = tid; i < (kMass ? 3 : 1) * kTcBins; i += kTcThreads) c.hist[i] = 0;
+    for (int i = tid; i < kWords * kTcBins; i += kTcThreads) c.hist[i] = 0;
     if (tid == 0) mail.listed = 0;
     __syncthreads();
     float weight = 0.f;
@@ -369,11 +369,12 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       if (weigh) weight += tc_exp2(-z);
       if (!(x >= 0.f && x < (float)kTcBins)) return;
       const int b = (int)x;
-      atomicAdd(&c.hist[b], 1u);
       if (kMass) {
         const uint32_t q = c.steps(z);
-        atomicAdd(&c.hist[kTcBins + b], q >> 16);
-        atomicAdd(&c.hist[2 * kTcBins + b], q & 0xffffu);
+        atomicAdd(&c.hist[b], q >> 16);
+        atomicAdd(&c.hist[kTcBins + b], q & 0xffffu);
+      } else {
+        atomicAdd(&c.hist[b], 1u);
       }
     });
     if (weigh) {
@@ -385,7 +386,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     for (int i = warp; i < kTcCoarse; i += kTcWarps) {
       const int b = 32 * i + lane;  // (no sum of halves reaches 2^32: a block has fewer than 2^16 columns)
 #pragma unroll
-      for (int w = 0; w < (kMass ? 3 : 1); ++w) {
+      for (int w = 0; w < kWords; ++w) {
         const uint32_t sum = __reduce_add_sync(0xffffffffu, c.hist[w * kTcBins + b]);
         if (lane == 0) mail.coarse[w][i] = sum;
       }
@@ -399,32 +400,25 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     // the sum of bins, then the bin, that the cut lies in: every block for itself, a warp fetching from each
     const auto fetch = [&](const uint32_t* at, int apart) {  // at: this lane's place in a block
       if (warp < c.blocks) {
-        uint32_t v[3];
+        uint32_t v[kWords];
 #pragma unroll
-        for (int w = 0; w < (kMass ? 3 : 1); ++w) v[w] = tc_get(tc_there(at + w * apart, warp));
+        for (int w = 0; w < kWords; ++w) v[w] = tc_get(tc_there(at + w * apart, warp));
 #pragma unroll
-        for (int w = 0; w < (kMass ? 3 : 1); ++w) mail.fetched[w][warp][lane] = v[w];
+        for (int w = 0; w < kWords; ++w) mail.fetched[w][warp][lane] = v[w];
       }
       __syncthreads();
     };
-    uint32_t count, c_upto;
-    unsigned long long mass, m_upto;
+    unsigned long long sum, upto;  // of counts or of weights
     const auto add_up = [&]() {
-      count = 0;
-      mass = 0;
-      for (int q = 0; q < c.blocks; ++q) {
-        count += mail.fetched[0][q][lane];
-        if (kMass) mass += ((unsigned long long)mail.fetched[1][q][lane] << 16) + mail.fetched[2][q][lane];
-      }
-      c_upto = count_before + tc_warp_scan(count);
-      m_upto = mass_before + (kMass ? tc_warp_scan(mass) : 0);
-      return __ballot_sync(0xffffffffu, kMass ? (double)m_upto >= target : c_upto >= k);
+      sum = 0;
+      for (int q = 0; q < c.blocks; ++q) sum += kMass ? ((unsigned long long)mail.fetched[0][q][lane] << 16) + mail.fetched[kWords - 1][q][lane] : mail.fetched[0][q][lane];
+      upto = before + tc_warp_scan(sum);
+      return __ballot_sync(0xffffffffu, (double)upto >= target);
     };
     fetch(&mail.coarse[0][lane], kTcCoarse);
     unsigned hit = add_up();  // (by every warp alike)
     if (!hit) {
-      count_before = __shfl_sync(0xffffffffu, c_upto, 31);
-      mass_before = __shfl_sync(0xffffffffu, m_upto, 31);
+      before = __shfl_sync(0xffffffffu, upto, 31);
       tc_cluster_sync();  // (the blocks read this one's sums)
       if (base > 0.f) return TcCut();  // fewer tokens, or less weight, than would be kept; weights below 2^-80 do not count.  (A bin's parts have the bin's sums.)
       base = 16.f;
@@ -433,40 +427,39 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       continue;
     }
     const int group = __ffs(hit) - 1;
-    count_before = __shfl_sync(0xffffffffu, c_upto - count, group);
-    mass_before = __shfl_sync(0xffffffffu, m_upto - mass, group);
+    before = __shfl_sync(0xffffffffu, upto - sum, group);
     __syncthreads();  // (every warp has added up)
     fetch(c.hist + 32 * group + lane, kTcBins);
     hit = add_up();
     const int in_group = __ffs(hit) - 1, bin = 32 * group + in_group;
-    const uint32_t members = __shfl_sync(0xffffffffu, count, in_group);
-    const unsigned long long mass_in = __shfl_sync(0xffffffffu, mass, in_group);
-    count_before = __shfl_sync(0xffffffffu, c_upto - count, in_group);
-    mass_before = __shfl_sync(0xffffffffu, m_upto - mass, in_group);
+    const unsigned long long in_bin = __shfl_sync(0xffffffffu, sum, in_group);
+    before = __shfl_sync(0xffffffffu, upto - sum, in_group);
     TcCut cut;
     cut.on = true;
     cut.base = base;
     cut.scale = scale;
     cut.bin = bin;
     cut.floor = c.floor(base + (float)(bin + 1) / scale);
-    if (members <= kTcMembers) {
-      // the bin's tokens: every block's own, then all of them where the histogram was
-      c.each_above(cut.floor, [&](int i, float l) {
-        const float z = c.z(l);
-        if (cut.side(z) != 0 || !had.keeps(c, i, l)) return;
-        const uint32_t at = atomicAdd(&mail.listed, 1u);  // (no more than the cluster has)
-        c.list_far[at] = c.behind(l);
-        c.list_at[at] = c.v0 + i;
-        if (kMass) c.list_w[at] = c.steps(z);
-      });
-      __syncthreads();
-      if (warp == 0) tc_tell(&mail.listed_by[c.rank], mail.listed, c.blocks);
-      tc_cluster_sync();
+    // the bin's tokens: every block's own, then all of them where the histogram was
+    c.each_above(cut.floor, [&](int i, float l) {
+      const float z = c.z(l);
+      if (cut.side(z) != 0 || !had.keeps(c, i, l)) return;
+      const uint32_t at = atomicAdd(&mail.listed, 1u);
+      if (at >= (uint32_t)kTcMembers) return;
+      c.list_far[at] = c.behind(l);
+      c.list_at[at] = c.v0 + i;
+      if (kMass) c.list_w[at] = c.steps(z);
+    });
+    __syncthreads();
+    if (warp == 0) tc_tell(&mail.listed_by[c.rank], mail.listed, c.blocks);
+    tc_cluster_sync();
+    uint32_t members = 0;
+    for (int q = 0; q < c.blocks; ++q) members += mail.listed_by[q];
+    if (members <= (uint32_t)kTcMembers) {
+      const uint32_t num = members;
       float* all_far = reinterpret_cast<float*>(c.hist);
       int* all_at = reinterpret_cast<int*>(c.hist + kTcMembers);
       uint32_t* all_w = c.hist + 2 * kTcMembers;
-      uint32_t num = 0;
-      for (int q = 0; q < c.blocks; ++q) num += mail.listed_by[q];
       for (uint32_t i = tid; i < num; i += kTcThreads) {
         int q = 0;
         uint32_t at = i;
@@ -480,16 +473,12 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       for (uint32_t i = tid; i < num; i += kTcThreads) {
         const float far = all_far[i];
         const int at = all_at[i];
-        uint32_t before = 0;
-        unsigned long long weight_before = mass_before;
+        unsigned long long front = before;
         for (uint32_t j = 0; j < num; ++j) {
           const float other = all_far[j];
-          if (other < far || (other == far && all_at[j] < at)) {
-            ++before;
-            if (kMass) weight_before += all_w[j];
-          }
+          if (other < far || (other == far && all_at[j] < at)) front += kMass ? all_w[j] : 1u;
         }
-        if (kMass ? (double)weight_before < target && (double)(weight_before + all_w[i]) >= target : count_before + before + 1 == k) {
+        if ((double)front < target && (double)(front + (kMass ? all_w[i] : 1u)) >= target) {
           mail.cut_behind = far;
           mail.cut_at = at;
         }
@@ -509,7 +498,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       continue;
     }
     // more tokens than that within 2^-24 of one another: equal ones, by index
-    const uint32_t want = kMass ? (uint32_t)fmin(fmax(ceil((target - (double)mass_before) * members / fmax((double)mass_in, 1.)), 1.), (double)members) : k - count_before;
+    const uint32_t want = kMass ? (uint32_t)fmin(fmax(ceil((target - (double)before) * members / fmax((double)in_bin, 1.)), 1.), (double)members) : k - (uint32_t)before;
     const auto member = [&](int i, float l) { return cut.side(c.z(l)) == 0 && had.keeps(c, i, l); };
     uint32_t mine = 0;
     c.each([&](int i, float l) { mine += member(i, l); });
@@ -519,22 +508,22 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     __syncthreads();
     if (warp == 0) tc_tell(&mail.ties[c.rank], tc_warp_sum(lane < kTcWarps ? tmp[lane] : 0u), c.blocks);
     tc_cluster_sync();
-    uint32_t before = 0;
-    for (int q = 0; q < c.rank; ++q) before += mail.ties[q];
-    for (int w = 0; w < warp; ++w) before += tmp[w];
-    if (before < want && before + mine >= want) {  // this warp has it
+    uint32_t passed = 0;
+    for (int q = 0; q < c.rank; ++q) passed += mail.ties[q];
+    for (int w = 0; w < warp; ++w) passed += tmp[w];
+    if (passed < want && passed + mine >= want) {  // this warp has it
       for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
         const int i = i0 + 4 * lane;
         const float4 l = *reinterpret_cast<const float4*>(c.row + i);
         const bool in[4] = {member(i, l.x), member(i + 1, l.y), member(i + 2, l.z), member(i + 3, l.w)};
-        const uint32_t here = in[0] + in[1] + in[2] + in[3], upto = tc_warp_scan(here), all = __shfl_sync(0xffffffffu, upto, 31);
-        if (before < want && before + all >= want) {
-          uint32_t at = before + upto - here;
+        const uint32_t here = in[0] + in[1] + in[2] + in[3], there = tc_warp_scan(here), all = __shfl_sync(0xffffffffu, there, 31);
+        if (passed < want && passed + all >= want) {
+          uint32_t at = passed + there - here;
           for (int j = 0; j < 4; ++j)
             if (in[j] && ++at == want)
               for (int q = 0; q < c.blocks; ++q) tc_put(tc_there(&mail.cut_at, q), c.v0 + i + j);
         }
-        before += all;
+        passed += all;
       }
     }
     tc_cluster_sync();
@@ -683,6 +672,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   int first = 0x7fffffff, equal = 0;
   const bool some = k > 0 && k < V, share = p < 1.f, cuts = some || share || min_p > 0.f;
   const bool in_reach = !greedy && cuts && k <= kTcShort && (some || share || min_p >= 0.00025f);  // (2^-12 is 0.000244)
+  const bool weighed = !greedy && !some && (share || !cuts), same_unit = c.unit == kTcLog2e;
   const float likely = in_reach ? c.floor(kTcShortZ[0]) : INFINITY, likelier = in_reach ? c.floor(kTcShortZ[1]) : INFINITY;
   int found = 0, found_likelier = 0;  // by this warp, in order of the columns
   for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
@@ -696,7 +686,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
         ++equal;
       } else {
         rest += tc_exp2((l[j] - c.m) * kTcLog2e);
-        part += tc_exp2((l[j] - c.m) * c.unit);
+        if (weighed && !same_unit) part += tc_exp2((l[j] - c.m) * c.unit);
       }
     }
     if (__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= likely)) {
@@ -716,7 +706,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
       found += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  part += (float)equal;
+  part = (same_unit ? rest : part) + (float)equal;
   double mine = tc_warp_sum((double)part);
   rest = tc_warp_sum(rest);
   equal = tc_warp_sum(equal);
@@ -887,7 +877,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   TcCut by_count, by_mass;
   if (!greedy) {
     if (some) by_count = tc_select<false>(c, (uint32_t)k, 0.f, by_mass, false);
-    if (share) by_mass = tc_select<true>(c, 0, p > 0.f ? p : 0.f, by_count, !by_count.on);
+    if (share) by_mass = tc_select<true>(c, 0, p > 0.f ? p : 0.f, by_count, weighed);
   }
   int token = -1;
   float taken = 0.f;  // how far behind the largest it is
