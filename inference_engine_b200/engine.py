@@ -29,13 +29,43 @@ device side.  It drives any model of the registry (models/__init__.py): the mode
 step; sampling is the library's Gumbel-max sampler (greedy at tau = 0).  Besides generating (`submit_request`, `step`),
 the engine replays given tokens (`open_replay`, `replay`, `close_replay`) through the same step, cache and graphs and
 hands out the logits of any of them.
+
+Requests may bring things of their own, if the engine is made for that: a way of sampling with penalties, biases and a grammar
+(`own_sampling`; `Sampling`), and a low-rank adapter out of the model's slots (`adapters`).  Both travel in the step's input buffer, so
+the same graphs serve whatever the requests ask for; without them steps are what they were.
 """
 from __future__ import annotations
 
 import math
 import time
 from collections import deque
+from collections.abc import Callable
 from dataclasses import dataclass, field
+
+
+@dataclass(frozen=True)
+class Sampling:
+    """How one request's tokens are chosen (ops.Draw, ops.Rules): by default the most likely one.  bias: token -> what is added to its logit.
+    grammar: called with the output so far, returns the row of the engine's masks for the next token, -1: none.  seed: of the request's random
+    numbers (default: the engine's and the request's number)."""
+
+    temperature: float = 0.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    repetition: float = 1.0
+    presence: float = 0.0
+    frequency: float = 0.0
+    bias: dict[int, float] = field(default_factory=dict)
+    grammar: Callable[[list[int]], int] | None = None
+    seed: int | None = None
+
+    def __post_init__(self):
+        numbers = (self.temperature, self.top_p, self.min_p, self.repetition, self.presence, self.frequency, *self.bias.values())
+        if not all(math.isfinite(x) for x in numbers):
+            raise ValueError("sampling: a number is infinite or none")
+        if self.temperature < 0 or self.top_k < 0 or not 0 < self.top_p <= 1 or not 0 <= self.min_p <= 1 or self.repetition <= 0:
+            raise ValueError(f"sampling: {self} is out of range")
 
 
 @dataclass
@@ -48,6 +78,10 @@ class Request:
     committed: int = 0  # pages promised to this request at admission and not yet handed out
     cached_len: int = 0  # tokens currently in the cache
     output: list[int] = field(default_factory=list)
+    sampling: Sampling | None = None
+    adapter: int = -1
+    history: int = -1  # row of the engine's token histories, for requests with a way of sampling
+    rng: object = None
     admitted: bool = False
     t_submit: float = 0.0
     t_first_token: float | None = None
@@ -121,12 +155,12 @@ class Step:
 
 class Scheduler:
     def __init__(self, max_batch_size: int, max_len: int, page_size: int, pool: PagePool, max_tokens_per_step: int,
-                 min_first_chunk: int, stop_token_id: int, slots: SlotPool | None = None):
+                 min_first_chunk: int, stop_token_id: int, slots: SlotPool | None = None, histories: SlotPool | None = None):
         assert max_tokens_per_step >= max_batch_size + min_first_chunk, \
             "the budget must fit every decoding request plus one first chunk, or prefill can stall forever"
         self.max_batch_size, self.max_len, self.page_size = max_batch_size, max_len, page_size
         self.pool, self.max_tokens_per_step, self.min_first_chunk = pool, max_tokens_per_step, min_first_chunk
-        self.stop_token_id, self.slots = stop_token_id, slots
+        self.stop_token_id, self.slots, self.histories = stop_token_id, slots, histories
         self.running: list[Request] = []
         self.waiting: deque[Request] = deque()
         self.next_id = 0
@@ -175,6 +209,8 @@ class Scheduler:
             r.committed, r.admitted = self.lifetime_pages(r), True
             if self.slots is not None:
                 r.slot = self.slots.take()
+            if self.histories is not None:
+                r.history = self.histories.take()
             self.running.append(r)
             entries.append((r, r.prompt_ids[:n]))
             budget -= n
@@ -193,12 +229,17 @@ class Scheduler:
         for (r, toks), tok in zip(step.entries, sampled):
             r.cached_len += len(toks)
             if r.decoding:
-                r.output.append(int(tok))
-                if len(r.output) == 1:
-                    r.t_first_token = now
-                if tok == self.stop_token_id or len(r.output) >= r.max_new_tokens or r.cached_len + 1 >= self.max_len:
+                none = tok < 0 and self.histories is not None  # its rules allow no token: the request ends
+                if not none:
+                    r.output.append(int(tok))
+                    if len(r.output) == 1:
+                        r.t_first_token = now
+                if none or tok == self.stop_token_id or len(r.output) >= r.max_new_tokens or r.cached_len + 1 >= self.max_len:
                     self.pool.release(r.pages, r.committed)
                     r.pages, r.committed = [], 0
+                    if self.histories is not None:
+                        self.histories.release(r.history)
+                        r.history = -1
                     if self.slots is not None:
                         self.slots.release(r.slot)
                         r.slot = -1
@@ -210,14 +251,19 @@ class Scheduler:
 
 class Engine:
     """Scheduler + device execution.  `model`: an instance of a registered model class on a CUDA device.  `num_slots`: state
-    slots of a stateful model, one per live request (default: one per request of the largest batch)."""
+    slots of a stateful model, one per live request (default: one per request of the largest batch).  `own_sampling`: requests may have a
+    Sampling of their own (the others take the most likely token; tau is for engines without), of up to `max_bias` biased tokens, under grammars of
+    up to `num_masks` masks (set_mask).  `adapters`: requests may name a slot of the model's adapters (model.make_adapters before)."""
 
     slots: SlotPool | None = None
+    # what an entry's sampling comes to on the device, an array each, int32 and then fp32
+    SAMPLING_INTS = ("slots", "lengths", "prompts", "mask_rows", "top_k")
+    SAMPLING_FLOATS = ("repetition", "presence", "frequency", "temperature", "top_p", "min_p", "uniform")
 
     def __init__(self, model, max_batch_size: int, max_len: int, stop_token_id: int, page_size: int | None = None,
                  num_pages: int | None = None, max_tokens_per_step: int = 1024, min_first_chunk: int = 64,
                  max_graph_tokens: int = 512, use_graphs: bool = True, block_m: int = 128, tau: float = 0.0, seed: int = 0,
-                 num_slots: int | None = None):
+                 num_slots: int | None = None, own_sampling: bool = False, max_bias: int = 16, num_masks: int = 64, adapters: bool = False):
         import numpy as np
         import torch
 
@@ -245,8 +291,19 @@ class Engine:
         self.pool = PagePool(num_pages, first=self.scratch_pages)
         if getattr(model, "stateful", False):
             self.slots = SlotPool(max_batch_size if num_slots is None else num_slots)
+        self.own_sampling, self.max_bias, self.seed = own_sampling, max_bias, seed
+        self.adapter_slots = 0
+        if adapters:
+            if getattr(model, "adapters", None) is None:
+                raise ValueError("the model has no slots for adapters: make_adapters comes first")
+            self.adapter_slots = next(iter(model.adapters[0].values())).slots
+        if own_sampling:
+            if max_bias < 0 or num_masks < 1:
+                raise ValueError("own_sampling needs room for a mask, and not less than none for biases")
+            self.history = torch.zeros(max_batch_size, max_len, dtype=torch.int32, device=self.device)
+            self.masks = torch.full((num_masks, (model.vocab + 31) // 32), -1, dtype=torch.int32, device=self.device)
         self.sched = Scheduler(max_batch_size, max_len, page_size, self.pool, max_tokens_per_step, min_first_chunk,
-                               stop_token_id, self.slots)
+                               stop_token_id, self.slots, SlotPool(max_batch_size) if own_sampling else None)
         per_slot = {} if self.slots is None else {"slots": self.slots.capacity}
         self.caches = model.make_caches(num_pages, page_size, self.max_pages * page_size, **per_slot)
         # one int32 buffer per kind of step, filled on the host and copied in one piece
@@ -271,11 +328,38 @@ class Engine:
             self.capture()
 
     # ------------------------------------------------------------------ public surface (engine.py:120-142)
-    def submit_request(self, prompt_ids: list[int], max_new_tokens: int) -> Request:
-        return self.sched.submit(prompt_ids, max_new_tokens)
+    def submit_request(self, prompt_ids: list[int], max_new_tokens: int, sampling: Sampling | None = None, adapter: int = -1) -> Request:
+        if sampling is not None:
+            if not self.own_sampling:
+                raise ValueError("the engine was made without own_sampling")
+            if len(sampling.bias) > self.max_bias or any(not 0 <= t < self.model.vocab for t in sampling.bias):
+                raise ValueError(f"up to {self.max_bias} biased tokens of 0 .. {self.model.vocab - 1} are wanted")
+        if adapter != -1 and not 0 <= adapter < self.adapter_slots:
+            raise ValueError(f"adapter {adapter}: the engine has {self.adapter_slots} slots")
+        r = self.sched.submit(prompt_ids, max_new_tokens)
+        r.sampling, r.adapter = sampling, adapter
+        if self.own_sampling:
+            if any(not 0 <= t < self.model.vocab for t in r.prompt_ids):
+                self.sched.waiting.pop()
+                raise ValueError(f"a prompt has ids outside 0 .. {self.model.vocab - 1}")
+            s = sampling.seed if sampling is not None else None
+            r.rng = self.np.random.default_rng([self.seed, r.id] if s is None else s)
+        return r
 
-    def generate(self, prompts: list[list[int]], max_new_tokens: int) -> list[Request]:
-        reqs = [self.submit_request(p, max_new_tokens) for p in prompts]
+    def set_mask(self, row: int, allowed) -> None:
+        """Mask `row` allows these token ids and no others (in stream order: steps that run already keep the one before)."""
+        if not self.own_sampling or not 0 <= row < self.masks.shape[0]:
+            raise ValueError(f"mask {row}: the engine has {self.masks.shape[0] if self.own_sampling else 0}")
+        bits = self.np.zeros(self.masks.shape[1] * 32, self.np.uint8)
+        ids = self.np.asarray(list(allowed), self.np.int64)
+        if ids.size and (ids.min() < 0 or ids.max() >= self.model.vocab):
+            raise ValueError(f"a token id outside 0 .. {self.model.vocab - 1}")
+        bits[ids] = 1
+        words = self.np.packbits(bits, bitorder="little").view(self.np.int32)
+        self.masks[row].copy_(self.torch.from_numpy(words))
+
+    def generate(self, prompts: list[list[int]], max_new_tokens: int, sampling: Sampling | None = None, adapter: int = -1) -> list[Request]:
+        reqs = [self.submit_request(p, max_new_tokens, sampling, adapter) for p in prompts]
         while not self.sched.idle():
             self.step()
         return reqs
@@ -354,16 +438,86 @@ class Engine:
 
     def mixed_layout(self, n_tokens: int, live: int | None = None) -> list[int]:
         """Field lengths of a step with prefill padded to n_tokens: ids, positions, seq_ids, cu_seqlens,
-        cached_lens, cu_cached, tile_start, num_decoding, block table, state slots.  The same n_tokens always gives a bucket the
-        same layout, so its fields always sit at the same addresses."""
+        cached_lens, cu_cached, tile_start, num_decoding, block table, state slots, and what the requests ask.  The same n_tokens always
+        gives a bucket the same layout, so its fields always sit at the same addresses."""
         E = self.step_entries(n_tokens, live)
-        return [n_tokens, n_tokens, n_tokens, E + 1, E, E + 1, math.ceil(n_tokens / self.block_m) + E, 1, E * self.max_pages, E]
+        return [n_tokens, n_tokens, n_tokens, E + 1, E, E + 1, math.ceil(n_tokens / self.block_m) + E, 1, E * self.max_pages, E,
+                self.asks_size(E, n_tokens)]
+
+    def asks_size(self, entries: int, rows: int) -> int:
+        """Adapters of the rows; then, per entry, the sampling fields and the biases (tokens, values)."""
+        n = rows if self.adapter_slots else 0
+        if self.own_sampling:
+            n += (len(self.SAMPLING_INTS) + len(self.SAMPLING_FLOATS) + 2 * self.max_bias) * entries
+        return n
+
+    def fill_asks(self, buf, step: Step, entries: int, rows: int) -> None:
+        """What the step's requests ask, into its part of the host buffer."""
+        np, at = self.np, 0
+        if self.adapter_slots:
+            buf[:rows] = -1
+            for r, toks in step.entries:
+                buf[at : at + len(toks)] = r.adapter
+                at += len(toks)
+            at = rows
+        if not self.own_sampling:
+            return
+        # a field each; entries that need no token, and places without an entry, are passed over
+        ints = buf[at : at + len(self.SAMPLING_INTS) * entries].reshape(-1, entries)
+        at += ints.size
+        floats = buf[at : at + len(self.SAMPLING_FLOATS) * entries].view(np.float32).reshape(-1, entries)
+        at += floats.size
+        ids = buf[at : at + self.max_bias * entries].reshape(entries, self.max_bias)
+        bias = buf[at + ids.size : at + 2 * ids.size].view(np.float32).reshape(entries, self.max_bias)
+        ints[:], floats[:], ids[:] = np.array([[-1], [0], [0], [-1], [0]]), np.array([[1], [0], [0], [0], [1], [0], [0]], np.float32), -1
+        plain = Sampling()
+        for e, (r, toks) in enumerate(step.entries):
+            if r.history < 0 or r.cached_len + len(toks) < len(r.prompt_ids):
+                continue
+            if not r.output:  # the first token comes next: its history is the prompt
+                host = self.torch.tensor(r.prompt_ids, dtype=self.torch.int32).pin_memory()
+                self.history[r.history, : len(host)].copy_(host, non_blocking=True)
+            s = r.sampling or plain
+            mask = -1 if s.grammar is None else int(s.grammar(r.output))
+            if not -1 <= mask < self.masks.shape[0]:
+                raise ValueError(f"request {r.id}: its grammar asks for mask {mask} of {self.masks.shape[0]}")
+            ints[:, e] = r.history, len(r.prompt_ids) + len(r.output), len(r.prompt_ids), mask, s.top_k
+            floats[:, e] = s.repetition, s.presence, s.frequency, s.temperature, s.top_p, s.min_p, r.rng.random()
+            if s.bias:
+                ids[e, : len(s.bias)] = list(s.bias)
+                bias[e, : len(s.bias)] = list(s.bias.values())
+
+    def asks_views(self, dev, entries: int, rows: int, first: int | None = None, first_rows: int | None = None):
+        """The model's view of what was filled in, of the first entries and rows."""
+        if not len(dev):
+            return {}
+        from .models import Asks
+        from .ops import Draw, Rules
+
+        asks, at, E = Asks(), 0, entries if first is None else first
+        if self.adapter_slots:
+            asks.adapters = dev[: rows if first_rows is None else first_rows]
+            at = rows
+        if self.own_sampling:
+            f = {}
+            for name in self.SAMPLING_INTS + self.SAMPLING_FLOATS:
+                f[name] = dev[at : at + E]
+                if name in self.SAMPLING_FLOATS:
+                    f[name] = f[name].view(self.torch.float32)
+                at += entries
+            biases = {}
+            if self.max_bias:
+                n = self.max_bias
+                biases = {"bias_ids": dev[at : at + E * n].view(E, n), "bias": dev[at + entries * n :][: E * n].view(self.torch.float32).view(E, n)}
+            asks.draw = Draw(*(f.pop(name) for name in ("temperature", "uniform", "top_k", "top_p", "min_p")))
+            asks.rules = Rules(history=self.history, masks=self.masks, **f, **biases)
+        return {"asks": asks}
 
     def decode_layout(self) -> list[int]:
-        """ids, cached_lens, num_decoding, block table, state slots of a pure-decode step, sized for the largest batch; a
-        bucket of b rows uses the first b of each (same start addresses for every bucket)."""
+        """ids, cached_lens, num_decoding, block table, state slots of a pure-decode step, and what the requests ask, sized for the largest
+        batch; a bucket of b rows uses the first b of each (same start addresses for every bucket)."""
         B = self.max_batch_size
-        return [B, B, 1, B * self.max_pages, B]
+        return [B, B, 1, B * self.max_pages, B, self.asks_size(B, B)]
 
     def table_row(self, r: Request):
         """The request's block-table row as an int32 array, extended in place as pages are appended."""
@@ -399,6 +553,7 @@ class Engine:
         slots = buf[offs[9] : offs[10]]
         slots[:] = -1
         slots[: len(step.entries)] = [r.slot for r, _ in step.entries]
+        self.fill_asks(buf[offs[10] : offs[11]], step, num_entries, n_pad)
         self.dev_mixed[: len(buf)].copy_(self.host_mixed[: len(buf)], non_blocking=True)
         return plan["cu_cached"][-1]
 
@@ -416,18 +571,20 @@ class Engine:
 
     def decode_views(self, b: int):
         B = self.max_batch_size
-        ids, cached, nd, table, slots = self.dev_decode.split(self.decode_layout())
-        return ids[:b], cached[:b], nd, table.view(B, self.max_pages)[:b], slots[:b]
+        ids, cached, nd, table, slots, asks = self.dev_decode.split(self.decode_layout())
+        return ids[:b], cached[:b], nd, table.view(B, self.max_pages)[:b], slots[:b], self.asks_views(asks, B, B, b, b)
 
     # ------------------------------------------------------------------ execution
     def forward_mixed(self, n_pad: int, prefix_tokens: int = 0, live: int | None = None):
         inp, prefix = self.mixed_views(n_pad, prefix_tokens, live)
         state = {} if self.slots is None else {"slots": inp.slots}
+        sizes = self.mixed_layout(n_pad, live)
+        state |= self.asks_views(self.dev_mixed[sum(sizes[:-1]) : sum(sizes)], self.step_entries(n_pad, live), n_pad)
         return self.model.step(self.caches, inp, inp.ids, inp.cached_lens, inp.block_table, inp.num_decoding, prefix, **state)
 
     def forward_decode(self, b: int):
-        ids, cached, nd, table, slots = self.decode_views(b)
-        state = {} if self.slots is None else {"slots": slots}
+        ids, cached, nd, table, slots, asks = self.decode_views(b)
+        state = ({} if self.slots is None else {"slots": slots}) | asks
         return self.model.step(self.caches, None, ids, cached, table, nd, **state)
 
     def capture_graph(self, run):
@@ -450,6 +607,9 @@ class Engine:
         inputs during capture are a single padding entry on the scratch run, so what the warm-up writes is
         harmless."""
         self.dev_decode.zero_()  # nothing decodes
+        if n := self.decode_layout()[-1]:
+            self.fill_asks(self.np_decode[-n:], Step([], 0), self.max_batch_size, self.max_batch_size)
+            self.dev_decode[-n:].copy_(self.host_decode[-n:])
         for b in reversed(self.graph_buckets):
             self.decode_graphs[b] = self.capture_graph(lambda b=b: self.forward_decode(b))
         for n in reversed(self.token_buckets):
@@ -476,12 +636,14 @@ class Engine:
         buf[B:Bm] = 0
         buf[Bm + B : 2 * Bm] = 0
         buf[2 * Bm] = B
-        table = buf[2 * Bm + 1 : -Bm].reshape(Bm, self.max_pages)
+        slots_at = 2 * Bm + 1 + Bm * self.max_pages
+        table = buf[2 * Bm + 1 : slots_at].reshape(Bm, self.max_pages)
         for i, (r, _) in enumerate(step.entries):
             table[i] = self.table_row(r)
         table[B:] = 0
-        buf[-Bm:] = -1
-        buf[len(buf) - Bm : len(buf) - Bm + B] = [r.slot for r, _ in step.entries]
+        buf[slots_at : slots_at + Bm] = -1
+        buf[slots_at : slots_at + B] = [r.slot for r, _ in step.entries]
+        self.fill_asks(buf[slots_at + Bm :], step, Bm, Bm)
         self.dev_decode.copy_(self.host_decode, non_blocking=True)
         self.seconds["inputs"] += time.perf_counter() - t_in
         if b in self.decode_graphs:

@@ -6,9 +6,10 @@ and its instances what the engine drives:
     device, vocab, num_layers, page_size (preferred), tau, seed
     make_caches(num_pages, page_size, max_len)     the step's cache, whatever the model keeps per token
     make_prefix(max_len) / None                    scratch for the prefilling entries' cached tokens, if it wants one
-    step(caches, inp, ids, cached_lens, block_table, num_decoding, prefix) -> StepOutput
+    step(caches, inp, ids, cached_lens, block_table, num_decoding, prefix, asks=) -> StepOutput
     logits(hidden)                                 fp32 or bf16 logits of normed rows
-A class with `stateful = True` keeps a state per request beside the pages: its make_caches takes slots=, the number of state
+A class whose projections take low-rank adapters has make_adapters(slots, rank), which gives it empty slots, and `adapters`, a dict of
+ops.Adapters per layer (None before).  A class with `stateful = True` keeps a state per request beside the pages: its make_caches takes slots=, the number of state
 slots, and its step slots=, int32 [entries], the slot of every entry (-1: padding).
 """
 from __future__ import annotations
@@ -17,6 +18,9 @@ from dataclasses import dataclass
 
 import torch
 
+from .. import kernels as K
+from .. import ops
+
 MODELS: dict[str, type] = {}
 
 
@@ -24,6 +28,38 @@ MODELS: dict[str, type] = {}
 class StepOutput:
     tokens: torch.Tensor  # int64 [entries]: the sampled next token of every entry
     hidden: torch.Tensor  # [rows, width]: the final normed state of every packed row of the step
+
+
+@dataclass
+class Asks:
+    """What a step's requests bring with them."""
+
+    adapters: torch.Tensor | None = None  # int32 [rows]: every row's adapter slot, -1: none
+    draw: ops.Draw | None = None  # how the entries' tokens are drawn; None: the model's tau and seed for all
+    rules: ops.Rules | None = None
+
+
+def plan_of(model, asks: Asks | None) -> ops.AdapterPlan | None:
+    """The step's rows by adapter, for all its projections."""
+    if asks is None or asks.adapters is None:
+        return None
+    if model.adapters is None:
+        raise ValueError("rows with adapters, but the model has no slots for them (make_adapters)")
+    return ops.plan_adapters(asks.adapters, next(iter(model.adapters[0].values())).slots)
+
+
+def adapted(x: torch.Tensor, weight: torch.Tensor, adapters: ops.Adapters | None, plan: ops.AdapterPlan | None) -> torch.Tensor:
+    """The shared projection of x, and every row's adapter beside it."""
+    y = K.linear(x, weight)
+    return y if plan is None or adapters is None else ops.add_adapters(y, x, adapters, plan)
+
+
+def next_tokens(model, hidden: torch.Tensor, asks: Asks | None) -> torch.Tensor:
+    """The next token of every entry from its last normed row: int64 [entries]."""
+    logits = model.logits(hidden)
+    if asks is None or asks.draw is None:
+        return K.sample(logits, model.tau, model.seed).view(-1)
+    return ops.choose_tokens(logits, asks.draw, asks.rules, append=asks.rules is not None and asks.rules.history is not None)[0]
 
 
 def register(architecture: str):

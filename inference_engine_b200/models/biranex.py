@@ -21,7 +21,7 @@ import torch
 from .. import kernels as K
 from .. import ops
 from ..checkpoint import RandomWeights
-from . import StepOutput, register
+from . import Asks, StepOutput, next_tokens, register
 
 UNIT_EPS = 1e-6  # in the unit norm of the delta rule's queries and keys
 
@@ -278,7 +278,8 @@ class Biranex:
         return None  # attention reads the cache by page
 
     @torch.inference_mode()
-    def step(self, caches, inp, ids, cached_lens, block_table, num_decoding, prefix=None, slots=None, trace: list | None = None) -> StepOutput:
+    def step(self, caches, inp, ids, cached_lens, block_table, num_decoding, prefix=None, slots=None, trace: list | None = None,
+             asks: Asks | None = None) -> StepOutput:
         """One step; `inp is None` = pure decode.  `trace`: receives a copy of the residual after every layer."""
         rows = ops.Rows(ids.shape[0], cached_lens, num_decoding, block_table, slots=slots)
         if inp is not None:
@@ -295,7 +296,7 @@ class Biranex:
                 trace.append(x.clone())
         _, hidden = ops.scaled_add_norm(x, None, self.norm, 1.0, c.eps, dt, keep=False)
         last = hidden if inp is None else hidden[(inp.cu_seqlens[1:] - 1).clamp(min=0).long()]
-        return StepOutput(K.sample(self.logits(last), self.tau, self.seed).view(-1), hidden)
+        return StepOutput(next_tokens(self, last, asks), hidden)
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         return K.linear(hidden, self.embed, out_dtype=torch.float32)

@@ -17,7 +17,7 @@ import torch
 from .. import kernels as K
 from .. import ops
 from ..checkpoint import RandomWeights
-from . import StepOutput, register
+from . import Asks, StepOutput, adapted, next_tokens, plan_of, register
 
 GATE_SLOPE = 1.702  # y = g * sigmoid(slope * g) * (u + 1)
 
@@ -149,6 +149,7 @@ class Radivik:
         self.norm = norm("final.norm")
         self.head = take("head", cfg.vocab, W).to(device, dtype)
         self.tables: dict[ops.Rotary, torch.Tensor] = {}
+        self.adapters: list[dict[str, ops.Adapters]] | None = None
 
     @classmethod
     def from_config(cls, config: dict, weights, device, dtype: torch.dtype = torch.bfloat16) -> "Radivik":
@@ -169,8 +170,19 @@ class Radivik:
     def make_prefix(self, max_len: int) -> None:
         return None  # attention reads the cache by page
 
+    def make_adapters(self, slots: int, rank: int) -> list[dict[str, ops.Adapters]]:
+        """Empty slots for low-rank adapters beside every layer's attention projections (load fills them)."""
+        def of(m: MixerConfig) -> dict[str, ops.Adapters]:
+            parts = (m.heads * m.dim,) if m.kv_from is not None else (m.heads * m.dim, m.kv_heads * m.dim, m.kv_heads * m.vdim)
+            sizes = {"qkv": (self.width, parts), "o": (m.heads * m.vdim, (self.width,))}
+            return {n: ops.make_adapters(slots, width, parts, rank, self.dtype, self.device) for n, (width, parts) in sizes.items()}
+
+        self.adapters = [of(L.cfg.mixer) for L in self.layers]
+        return self.adapters
+
     @torch.inference_mode()
-    def step(self, caches, inp, ids, cached_lens, block_table, num_decoding, prefix=None, trace: list | None = None) -> StepOutput:
+    def step(self, caches, inp, ids, cached_lens, block_table, num_decoding, prefix=None, trace: list | None = None,
+             asks: Asks | None = None) -> StepOutput:
         """One step; `inp is None` = pure decode.  `trace`: receives a copy of the residual after every layer."""
         if inp is None:
             rows = ops.Rows(ids.shape[0], cached_lens, num_decoding, block_table)
@@ -178,13 +190,14 @@ class Radivik:
             rows = ops.Rows(ids.shape[0], cached_lens, num_decoding, block_table, inp.seq_ids, inp.positions, inp.cu_seqlens,
                             inp.tile_start, inp.block_m)
         c, dt = self.cfg, self.dtype
+        by_adapter = plan_of(self, asks)
         x, xb = ops.embed(self.embed, ids)
-        for L in self.layers:
-            m, cache = L.cfg.mixer, caches[L.cache]
-            q = ops.rope_write(K.linear(xb, L.qkv), rows, cache, self.tables[m.rotary] if m.rotary else None, m.heads,
+        for i, L in enumerate(self.layers):
+            m, cache, own = L.cfg.mixer, caches[L.cache], self.adapters[i] if by_adapter is not None else {}
+            q = ops.rope_write(adapted(xb, L.qkv, own.get("qkv"), by_adapter), rows, cache, self.tables[m.rotary] if m.rotary else None, m.heads,
                                m.kv_from is None, True, c.eps)
             a = ops.paged_attention(q, cache, rows, m.scale)
-            y = K.linear(a.view(rows.num_rows, m.heads * m.vdim), L.o)
+            y = adapted(a.view(rows.num_rows, m.heads * m.vdim), L.o, own.get("o"), by_adapter)
             x, xb = ops.scaled_add_norm(x, y, L.norm1, c.alpha, c.eps, dt, zero=L.experts.counts if L.experts else None)
             if L.experts:
                 y, places = ops.mixture(x, xb, L.experts)
@@ -193,7 +206,7 @@ class Radivik:
                 trace.append(x.clone())
         _, hidden = ops.scaled_add_norm(x, None, self.norm, 1.0, c.eps, dt, keep=False)
         last = hidden if inp is None else hidden[(inp.cu_seqlens[1:] - 1).clamp(min=0).long()]
-        return StepOutput(K.sample(self.logits(last), self.tau, self.seed).view(-1), hidden)
+        return StepOutput(next_tokens(self, last, asks), hidden)
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         return K.linear(hidden, self.head, out_dtype=torch.float32)

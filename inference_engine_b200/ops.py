@@ -839,11 +839,12 @@ class Rules:
             raise ValueError("rules: tensors on several devices")
         h, m = self.history, self.masks
         object.__setattr__(self, "entries", n)
-        object.__setattr__(self, "device", tensors[0].device if tensors else None)
+        object.__setattr__(self, "device_index", tensors[0].get_device() if tensors else None)
         object.__setattr__(self, "struct", _lib.Rules(
             _ptr(h), _ptr(self.slots), _ptr(self.lengths), _ptr(self.prompts), _ptr(self.repetition), _ptr(self.presence), _ptr(self.frequency),
             _ptr(self.bias_ids), _ptr(self.bias), _ptr(m), _ptr(self.mask_rows), 0 if h is None else h.shape[1], 0 if h is None else h.shape[0],
             0 if self.bias is None else self.bias.shape[1], 0 if m is None else m.shape[0], 0 if m is None else m.shape[1]))
+        object.__setattr__(self, "ref", ctypes.byref(self.struct))
 
 
 @dataclass(frozen=True, eq=False)
@@ -865,39 +866,46 @@ class Draw:
         if any(t.dim() != 1 for t in tensors) or len({t.device for t in tensors}) > 1:
             raise ValueError("draw: one number per entry, all on one device")
         object.__setattr__(self, "entries", n)
+        object.__setattr__(self, "device_index", self.uniform.get_device())
         object.__setattr__(self, "struct", _lib.Draw(*(_ptr(t) for t in (self.temperature, self.top_k, self.top_p, self.min_p, self.uniform))))
+        object.__setattr__(self, "ref", ctypes.byref(self.struct))
 
 
-def _check_logits(what: str, logits: torch.Tensor, rules: Rules | None) -> int:
-    """The row stride of a step's logits."""
-    K._require_cuda(logits)
-    _here(logits)
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or (logits.shape[1] > 1 and logits.stride(1) != 1) or not logits.shape[1]:
-        raise ValueError(f"{what}: bf16 or fp32 logits [entries, vocab] with a row's elements side by side are wanted")
-    E, V = logits.shape
+def _check_logits(what: str, logits: torch.Tensor, rules: Rules | None) -> tuple[int, int, int, int]:
+    """Entries, vocabulary, row stride and element size of a step's logits."""
+    dev = logits.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        K._require_cuda(logits)
+        _here(logits)
+    elem = 2 if logits.dtype == torch.bfloat16 else 4 if logits.dtype == torch.float32 else 0
+    if logits.dim() != 2 or not elem or not logits.shape[1]:
+        raise ValueError(f"{what}: bf16 or fp32 logits [entries, vocab] are wanted")
+    (E, V), (stride, one) = logits.shape, logits.stride()
+    if V > 1 and one != 1:
+        raise ValueError(f"{what}: a row's logits lie side by side")
     if rules is not None:
         if rules.entries is not None and rules.entries != E:
             raise ValueError(f"{what}: rules for {rules.entries} entries and logits of {E}")
-        if rules.device is not None and rules.device != logits.device:
-            raise ValueError(f"{what}: rules on {rules.device}, logits on {logits.device}")
-        if rules.history is not None and rules.slots is None and rules.history.shape[0] < E:
-            raise ValueError(f"{what}: {rules.history.shape[0]} histories for {E} entries")
-        if rules.masks is not None and rules.masks.shape[1] < (V + 31) // 32:
-            raise ValueError(f"{what}: masks of {rules.masks.shape[1]} words for {V} tokens")
-    return logits.stride(0) if E > 1 else _round8(V)  # (a single row's stride may be anything)
+        if rules.device_index is not None and rules.device_index != dev:
+            raise ValueError(f"{what}: rules on another device than the logits")
+        st = rules.struct
+        if st.history and not st.slots and st.num_histories < E:
+            raise ValueError(f"{what}: {st.num_histories} histories for {E} entries")
+        if st.masks and st.mask_words < (V + 31) // 32:
+            raise ValueError(f"{what}: masks of {st.mask_words} words for {V} tokens")
+    return E, V, stride if E > 1 else _round8(V), elem  # (a single row's stride may be anything)
 
 
 @K._ranged
 def adjust_logits(logits: torch.Tensor, rules: Rules, out: torch.Tensor | None = None) -> torch.Tensor:
     """Logits [entries, vocab] under each entry's rules, fp32.  `out`: where they go, fp32 logits themselves perhaps; rows of entries that are passed
     over are left there as they are (uninitialised without it)."""
-    stride = _check_logits("adjust_logits", logits, rules)
-    E, V = logits.shape
+    E, V, stride, elem = _check_logits("adjust_logits", logits, rules)
     if out is None:
         out = torch.empty(E, V, dtype=torch.float32, device=logits.device)
     elif out.dtype != torch.float32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or out.device != logits.device:
         raise ValueError("adjust_logits: fp32 rows of the logits' shape are wanted")
-    rc = _lib_dec().b200dec_adjust_logits(logits.data_ptr(), stride, logits.element_size(), ctypes.byref(rules.struct), out.data_ptr(),
+    rc = _lib_dec().b200dec_adjust_logits(logits.data_ptr(), stride, elem, rules.ref, out.data_ptr(),
                                           out.stride(0) if E > 1 else _round8(V), E, V, K.status_word(logits.device).data_ptr(), K._stream())
     _lib.check(rc, "adjust_logits")
     return out
@@ -908,9 +916,8 @@ def choose_tokens(logits: torch.Tensor, draw: Draw, rules: Rules | None = None, 
     """Every entry's next token under its rules and its way of drawing: (int64 [entries], its log-probability under the softmax of the adjusted
     logits, fp32 [entries]); (-1, -inf) where nothing is allowed or the entry is passed over.  append: the token goes behind the entry's
     history where there is room."""
-    stride = _check_logits("choose_tokens", logits, rules)
-    E, V = logits.shape
-    if draw.entries != E or draw.uniform.device != logits.device:
+    E, V, stride, elem = _check_logits("choose_tokens", logits, rules)
+    if draw.entries != E or draw.device_index != logits.get_device():
         raise ValueError(f"choose_tokens: a draw for {draw.entries} entries on {draw.uniform.device}, logits of {E} on {logits.device}")
     if V > MAX_CHOICE_VOCAB:
         raise ValueError(f"choose_tokens: {V} tokens, at most {MAX_CHOICE_VOCAB}")
@@ -918,8 +925,7 @@ def choose_tokens(logits: torch.Tensor, draw: Draw, rules: Rules | None = None, 
         raise ValueError("choose_tokens: nowhere to append to")
     tokens = torch.empty(E, dtype=torch.int64, device=logits.device)
     logprobs = torch.empty(E, dtype=torch.float32, device=logits.device)
-    rc = _lib_dec().b200dec_choose_tokens(logits.data_ptr(), stride, logits.element_size(), None if rules is None else ctypes.byref(rules.struct),
-                                          ctypes.byref(draw.struct), E, V, int(append), tokens.data_ptr(), logprobs.data_ptr(),
+    rc = _lib_dec().b200dec_choose_tokens(logits.data_ptr(), stride, elem, None if rules is None else rules.ref, draw.ref, E, V, int(append), tokens.data_ptr(), logprobs.data_ptr(),
                                           K.status_word(logits.device).data_ptr(), K._stream())
     _lib.check(rc, "choose_tokens")
     return tokens, logprobs

@@ -29,7 +29,8 @@ import torch
 
 from . import _lib
 from . import kernels as K
-from .models import StepOutput, register
+from . import ops
+from .models import Asks, StepOutput, adapted, next_tokens, plan_of, register
 
 HIDDEN, FFN, VOCAB, LAYERS = 2048, 6144, 151936, 28
 HQ, HKV, D = 16, 8, 128
@@ -225,6 +226,8 @@ class DecoderScaffold:
         self.plan_steps = True  # one kernels.plan_decode_step per forward, shared by the layers
         self.tau = 0.0  # sampling temperature (0 = greedy) and the sampler's seed, advanced by every step
         self.seed = torch.zeros(1, dtype=torch.int64, device=device)
+        self.ffn = ffn
+        self.adapters: list[dict[str, ops.Adapters]] | None = None
         self.inv_freq = ROPE_BASE ** (-torch.arange(0, D, 2, dtype=torch.float32, device=device) / D)
 
     page_size = 16  # the engine's default for this model
@@ -246,6 +249,14 @@ class DecoderScaffold:
         k = torch.empty(HKV, capacity, D, device=self.device, dtype=torch.bfloat16)
         return k, torch.empty_like(k)
 
+    def make_adapters(self, slots: int, rank: int) -> list[dict[str, ops.Adapters]]:
+        """Empty slots for low-rank adapters beside every layer's projections (load fills them)."""
+        sizes = {"qkv": (self.hidden, (HQ * D, HKV * D, HKV * D)), "o": (HQ * D, (self.hidden,)), "gate_up": (self.hidden, (self.ffn, self.ffn)),
+                 "down": (self.ffn, (self.hidden,))}
+        self.adapters = [{n: ops.make_adapters(slots, width, parts, rank, torch.bfloat16, self.device) for n, (width, parts) in sizes.items()}
+                         for _ in range(self.num_layers)]
+        return self.adapters
+
     def rope(self, positions: torch.Tensor):
         ang = positions[:, None, None] * self.inv_freq[None, None, :]  # architecture.py:387-390
         return ang.cos().to(torch.bfloat16), ang.sin().to(torch.bfloat16)
@@ -259,30 +270,32 @@ class DecoderScaffold:
 
     @torch.inference_mode()
     def step(self, caches, inp: StepInputs | None, ids, cached_lens, slot_ids, num_decoding,
-             prefix: PrefixScratch | None = None) -> StepOutput:
+             prefix: PrefixScratch | None = None, asks: Asks | None = None) -> StepOutput:
         # the decode-attention work split of this step, once for all layers (it depends on the step's metadata only)
         plan = K.plan_decode_step(cached_lens, slot_ids, num_decoding, caches[0]) if self.plan_steps else None
+        by_adapter = plan_of(self, asks)
         x = self.embed[ids.long()]
         cos, sin = self.rope(cached_lens if inp is None else inp.positions)
         N = x.shape[0]
         residual = None
-        for L, cache in zip(self.layers, caches):
+        for i, (L, cache) in enumerate(zip(self.layers, caches)):
+            own = self.adapters[i] if by_adapter is not None else {}
             if residual is None:
                 residual = x
                 normed = torch.nn.functional.rms_norm(x, (self.hidden,), L["ln1"], EPS)
             else:
                 residual, normed = K.add_rms_norm(residual, x, L["ln1"], EPS)
-            q, k, v = K.linear(normed, L["qkv"]).split([HQ * D, HKV * D, HKV * D], dim=-1)
+            q, k, v = adapted(normed, L["qkv"], own.get("qkv"), by_adapter).split([HQ * D, HKV * D, HKV * D], dim=-1)
             out = attention_ops(q.view(N, HQ, D), k.view(N, HKV, D), v.view(N, HKV, D), L["qn"], L["kn"], cos, sin,
                                 cache, inp, cached_lens, slot_ids, num_decoding, prefix, plan)
-            attn = K.linear(out.view(N, HQ * D), L["o"])
+            attn = adapted(out.view(N, HQ * D), L["o"], own.get("o"), by_adapter)
             residual, normed = K.add_rms_norm(residual, attn, L["ln2"], EPS)
-            x = K.linear(K.silu_mul(K.linear(normed, L["gate_up"])), L["down"])
+            x = adapted(K.silu_mul(adapted(normed, L["gate_up"], own.get("gate_up"), by_adapter)), L["down"], own.get("down"), by_adapter)
         _, hidden = K.add_rms_norm(residual, x, self.norm, EPS)
         x = hidden
         if inp is not None:
             x = x[(inp.cu_seqlens[1:] - 1).long()]  # each entry's last row; junk for entries without tokens
-        return StepOutput(K.sample(self.logits(x), self.tau, self.seed).view(-1), hidden)
+        return StepOutput(next_tokens(self, x, asks), hidden)
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         return K.linear(hidden, self.embed)
