@@ -45,58 +45,70 @@ struct TcEntry {
 
 __device__ __forceinline__ TcEntry tc_entry(const TcRules& r, int e, bool report, int32_t* status) {
   TcEntry t;
-  bool bad = false;
+  // (all on their way before the first is looked at)
   t.slot = r.slots ? r.slots[e] : e;
-  t.idle = t.slot < 0;
-  if (t.slot < -1 || (r.history && t.slot >= r.num_histories)) { bad = true; t.idle = true; }
-  t.length = t.prompt = 0;
-  t.history = nullptr;
-  if (r.history && !t.idle) {
-    t.length = r.lengths[e];
-    t.prompt = r.prompts ? r.prompts[e] : t.length;
-    if (t.length < 0 || t.length > r.capacity || t.prompt < 0) bad = true;
-    t.length = max(0, min(t.length, r.capacity));
-    t.prompt = max(0, t.prompt);
-    t.history = r.history + (long long)t.slot * r.capacity;
-  }
+  t.length = r.history ? r.lengths[e] : 0;
+  t.prompt = r.history && r.prompts ? r.prompts[e] : 0x7fffffff;
   t.repetition = r.repetition ? r.repetition[e] : 1.f;
   t.presence = r.presence ? r.presence[e] : 0.f;
   t.frequency = r.frequency ? r.frequency[e] : 0.f;
+  const int m = r.masks ? r.mask_rows[e] : -1;
+  bool bad = false;
+  t.idle = t.slot < 0;
+  if (t.slot < -1 || (r.history && t.slot >= r.num_histories)) { bad = true; t.idle = true; }
+  t.history = nullptr;
+  if (t.idle || !r.history) {
+    t.length = 0;
+  } else {
+    if (t.length < 0 || t.length > r.capacity || t.prompt < 0) bad = true;
+    t.length = max(0, min(t.length, r.capacity));
+    t.history = r.history + (long long)t.slot * r.capacity;
+  }
   t.penalties = t.length > 0 && (t.repetition != 1.f || t.presence != 0.f || t.frequency != 0.f);
   t.mask = nullptr;
-  if (r.masks && r.mask_rows) {
-    const int m = r.mask_rows[e];
-    if (m >= 0 && m < r.num_masks) t.mask = r.masks + (long long)m * r.mask_words;
-    else if (m != -1) bad = true;
-  }
+  if (m >= 0 && m < r.num_masks) t.mask = r.masks + (long long)m * r.mask_words;
+  else if (m != -1) bad = true;
   if (bad && report && status) atomicOr(status, B200KV_S_BAD_POSITION);
   return t;
 }
 
-constexpr uint32_t kTcSeen = 0x80000000u;  // beside how often a token stands in the output
+constexpr uint32_t kTcSeen = 0x80000000u;  // in the prompt, beside how often a token stands in the output
 
-// table[v - v0] for the columns v0 .. v0 + n of this block; cleared by the caller, with a barrier on both sides.
+// table[v - v0] for the columns v0 .. v0 + n of this block; cleared by the caller, with a barrier on both sides.  A thread takes four tokens at a time, and
+// fetches those of four times together.
 __device__ __forceinline__ void tc_count(const TcEntry& t, int V, int v0, int n, uint32_t* table, bool report, int32_t* status) {
   auto take = [&](int i, int id) {
     const int at = id - v0;
-    if (at >= 0 && at < n) {
+    if ((unsigned)at < (unsigned)n) {
       if (i >= t.prompt) atomicAdd(&table[at], 1u);
-      atomicOr(&table[at], kTcSeen);
+      else if (!(*(volatile uint32_t*)&table[at] & kTcSeen)) atomicOr(&table[at], kTcSeen);
     }
-    if (report && (id < 0 || id >= V) && status) atomicOr(status, B200KV_S_BAD_POSITION);
+    if (report && (unsigned)id >= (unsigned)V && status) atomicOr(status, B200KV_S_BAD_POSITION);
   };
-  const int head = min(t.length, (int)((16 - (reinterpret_cast<uintptr_t>(t.history) & 15)) & 15) / 4);
-  if ((int)threadIdx.x < head) take(threadIdx.x, t.history[threadIdx.x]);
-  const int quads = (t.length - head) / 4;
-  for (int i = threadIdx.x; i < quads; i += blockDim.x) {
-    const int4 q = __ldcg(reinterpret_cast<const int4*>(t.history + head) + i);
-    take(head + 4 * i, q.x);
-    take(head + 4 * i + 1, q.y);
-    take(head + 4 * i + 2, q.z);
-    take(head + 4 * i + 3, q.w);
+  const int head = min(t.length, (int)((16 - (reinterpret_cast<uintptr_t>(t.history) & 15)) & 15) / 4), quads = (t.length - head) / 4;
+  const int4* p = reinterpret_cast<const int4*>(t.history + head);
+  for (int i = threadIdx.x; i < quads; i += 4 * blockDim.x) {
+    int4 q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * (int)blockDim.x < quads) q[j] = __ldcg(p + i + j * blockDim.x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = head + 4 * (i + j * (int)blockDim.x);
+      if (i + j * (int)blockDim.x < quads) {
+        take(at, q[j].x);
+        take(at + 1, q[j].y);
+        take(at + 2, q[j].z);
+        take(at + 3, q[j].w);
+      }
+    }
   }
-  const int rest = head + 4 * quads + threadIdx.x;
-  if (rest < t.length) take(rest, t.history[rest]);
+  // in front of the first sixteen bytes, and behind the last
+  const int rest = t.length - 4 * quads;
+  if ((int)threadIdx.x < rest) {
+    const int i = (int)threadIdx.x < head ? threadIdx.x : 4 * quads + threadIdx.x;
+    take(i, __ldcg(t.history + i));
+  }
 }
 
 __device__ __forceinline__ float tc_penalised(const TcEntry& t, float l, uint32_t seen) {
@@ -128,51 +140,92 @@ __device__ __forceinline__ void tc_bias(const TcRules& r, const TcEntry& t, int 
   }
 }
 
-// kN logits from column v on (aligned to their size)
-template <typename T, int kN>
-__device__ __forceinline__ void tc_load(const T* p, float (&f)[kN]) { ld_vec(p, f); }
+// Four logits as they come from memory, so that several can be on their way.  (Four, so that a warp writes whole lines of 32-bit values.)
+template <typename T>
+struct TcRaw;
+template <>
+struct TcRaw<uint16_t> {
+  uint2 a;
+  __device__ __forceinline__ void load(const uint16_t* p) { a = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ void get(float (&f)[4]) const {
+    f[0] = __uint_as_float(a.x << 16); f[1] = __uint_as_float(a.x & 0xFFFF0000u);
+    f[2] = __uint_as_float(a.y << 16); f[3] = __uint_as_float(a.y & 0xFFFF0000u);
+  }
+};
+template <>
+struct TcRaw<float> {
+  float4 a;
+  __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; }
+};
+// Penalties and mask on four logits from column v on (a multiple of four).
+__device__ __forceinline__ void tc_settle(const TcEntry& t, int v, const uint32_t* seen, float (&f)[4]) {
+  if (t.penalties) {
+    const uint4 n = *reinterpret_cast<const uint4*>(seen);
+    if (n.x | n.y | n.z | n.w) {  // (few are)
+      f[0] = tc_penalised(t, f[0], n.x);
+      f[1] = tc_penalised(t, f[1], n.y);
+      f[2] = tc_penalised(t, f[2], n.z);
+      f[3] = tc_penalised(t, f[3], n.w);
+    }
+  }
+  if (!t.mask) return;
+  const uint32_t bits = t.mask[v >> 5] >> (v & 31);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = bits >> j & 1u ? f[j] : -INFINITY;
+}
 
 // ---------------------------------------------------------------------------------------------------------------- adjusted logits
-constexpr int kAjThreads = 256;
-constexpr int kAjCols = 4096;  // of a block
+constexpr int kAjThreads = 512;
+constexpr int kAjCols = kAjThreads * 4;  // of a block, times kAhead
 
-// grid (ceil(V / kAjCols), entries).  kVec: 8 columns of a thread at a time, rows aligned to 16 bytes on both sides.
-template <typename T, bool kVec>
+// grid (column blocks, entries).  kAhead: times that a thread takes four columns.  vec: rows aligned to four elements on both sides.  The logits are on their way
+// while the history is counted; the few that have a bias change where they lie.
+template <typename T, int kAhead>
 __global__ void __launch_bounds__(kAjThreads)
-adjust_logits_kernel(const T* logits, long long stride, const TcRules r, float* out, long long out_stride, int V, int32_t* status) {
-  __shared__ uint32_t table[kAjCols];
+adjust_logits_kernel(const T* logits, long long stride, const TcRules r, float* out, long long out_stride, int V, bool vec, int32_t* status) {
+  extern __shared__ __align__(16) uint32_t aj_table[];
+  uint32_t* table = aj_table;
   pdl_enter();
   pdl_wait();
-  const int e = blockIdx.y, v0 = blockIdx.x * kAjCols, n = min(kAjCols, V - v0), tid = threadIdx.x;
+  const int e = blockIdx.y, v0 = blockIdx.x * (kAhead * kAjCols), n = min(kAhead * kAjCols, V - v0), tid = threadIdx.x;
   const bool report = blockIdx.x == 0;
+  const T* src = logits + (long long)e * stride + v0;
+  float* dst = out + (long long)e * out_stride + v0;
+  TcRaw<T> ahead[kAhead];
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s) {
+    const int i = 4 * (tid + s * kAjThreads);
+    if (vec && i + 4 <= n) ahead[s].load(src + i);
+  }
+  for (int i = 4 * tid; i < kAhead * kAjCols; i += 4 * kAjThreads) *reinterpret_cast<uint4*>(table + i) = make_uint4(0, 0, 0, 0);
   const TcEntry t = tc_entry(r, e, report && tid == 0, status);
   if (t.idle) return;
   if (t.penalties) {
-    for (int i = tid; i < kAjCols; i += kAjThreads) table[i] = 0;
     __syncthreads();
     tc_count(t, V, v0, n, table, report, status);
     __syncthreads();
   }
-  const T* src = logits + (long long)e * stride + v0;
-  float* dst = out + (long long)e * out_stride + v0;
-  constexpr int kN = kVec ? 8 : 1;
-  for (int i = tid * kN; i < n; i += kAjThreads * kN) {
-    if (kVec && i + kN > n) {
-      for (int j = i; j < n; ++j) {
-        const float l = tc_penalised(t, ld_elem(src + j), t.penalties ? table[j] : 0u);
-        dst[j] = tc_allowed(t, v0 + j) ? l : -INFINITY;
-      }
-      break;
-    }
-    float f[kN];
-    tc_load<T, kN>(src + i, f);
-    const uint32_t bits = t.mask ? t.mask[(v0 + i) >> 5] >> ((v0 + i) & 31) : ~0u;
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      if (t.penalties) f[j] = tc_penalised(t, f[j], table[i + j]);
-      if (!(bits >> j & 1u)) f[j] = -INFINITY;
+  for (int s = 0; s < kAhead; ++s) {
+    const int i = 4 * (tid + s * kAjThreads);
+    if (i >= n) break;
+    float f[4];
+    const bool whole = vec && i + 4 <= n;
+    if (whole) {
+      ahead[s].get(f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = i + j < n ? ld_elem(src + i + j) : 0.f;
     }
-    st_vec(dst + i, f);
+    tc_settle(t, v0 + i, table + i, f);
+    if (whole) {
+      st_vec(dst + i, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < n) dst[i + j] = f[j];
+    }
   }
   if (r.num_bias) {
     __syncthreads();  // what the block's other threads wrote
@@ -532,7 +585,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
   }
 }
 
-// vec: rows aligned to 16 bytes
+// vec: rows aligned to four elements
 template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 2)
 choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const TcDraw d, int V, int cols, bool vec, bool append, long long* tokens,
@@ -576,17 +629,12 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
 
   // ---- the row; its first columns on their way while the history is counted
   const T* src = logits + (long long)e * stride + c.v0;
-  constexpr int kAhead = 2;
-  float ahead[kAhead][8];
+  constexpr int kAhead = sizeof(T) == 2 ? 10 : 5;
+  TcRaw<T> ahead[kAhead];
 #pragma unroll
   for (int s = 0; s < kAhead; ++s) {
-    const int i = 8 * (tid + s * kTcThreads);
-    if (vec && i + 8 <= n) {
-      ld_vec(src + i, ahead[s]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ahead[s][j] = i + j < n ? ld_elem(src + i + j) : -INFINITY;
-    }
+    const int i = 4 * (tid + s * kTcThreads);
+    if (vec && i + 4 <= n) ahead[s].load(src + i);
   }
   uint32_t* table = reinterpret_cast<uint32_t*>(c.row);  // each place holds a count until its logit comes
   if (t.penalties) {
@@ -596,48 +644,41 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     __syncthreads();
   }
   float best = -INFINITY;
-  const auto settle = [&](int i, float (&f)[8]) {
-    if (t.penalties) {
-      float seen[8];
-      ld_vec(c.row + i, seen);
+  const auto take = [&](int i, const TcRaw<T>& raw) {
+    float f[4];
+    if (vec && i + 4 <= n) {
+      raw.get(f);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = tc_penalised(t, f[j], __float_as_uint(seen[j]));
+      for (int j = 0; j < 4; ++j) f[j] = i + j < n ? ld_elem(src + i + j) : -INFINITY;
     }
-    const uint32_t bits = t.mask && i < n ? t.mask[(c.v0 + i) >> 5] >> ((c.v0 + i) & 31) : ~0u;
+    if (i < n) tc_settle(t, c.v0 + i, table + i, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (!(bits >> j & 1u) || f[j] != f[j]) f[j] = -INFINITY;
+    for (int j = 0; j < 4; ++j) {
+      f[j] = fmaxf(f[j], -INFINITY);  // (not a number: no token)
       best = fmaxf(best, f[j]);
     }
     st_vec(c.row + i, f);
   };
-  const auto load = [&](int i, float (&f)[8]) {
-    if (vec && i + 8 <= n) {
-      ld_vec(src + i, f);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = i + j < n ? ld_elem(src + i + j) : -INFINITY;
-    }
-  };
 #pragma unroll
   for (int s = 0; s < kAhead; ++s) {
-    const int i = 8 * (tid + s * kTcThreads);
-    if (i < padded) settle(i, ahead[s]);
+    const int i = 4 * (tid + s * kTcThreads);
+    if (i < padded) take(i, ahead[s]);
   }
-  for (int i = 8 * (tid + kAhead * kTcThreads); i < padded; i += 8 * kTcThreads) {
-    float f[8];
-    load(i, f);
-    settle(i, f);
+  for (int i = 4 * (tid + kAhead * kTcThreads); i < padded; i += 4 * kTcThreads) {
+    TcRaw<T> raw;
+    if (vec && i + 4 <= n) raw.load(src + i);
+    take(i, raw);
   }
   if (r.num_bias) {
     __syncthreads();
-    tc_bias(r, t, e, V, c.v0, n, report, status, [&](int id, float s) {
-      const float l = __fadd_rn(c.row[id - c.v0], s);
-      c.row[id - c.v0] = l == l ? l : -INFINITY;
-    });
+    tc_bias(r, t, e, V, c.v0, n, report, status, [&](int id, float s) { c.row[id - c.v0] = fmaxf(__fadd_rn(c.row[id - c.v0], s), -INFINITY); });
     __syncthreads();
     best = -INFINITY;
-    c.each([&](int, float l) { best = fmaxf(best, l); });
+    for (int i = c.lo + 4 * lane; i < c.hi; i += 128) {
+      const float4 l = *reinterpret_cast<const float4*>(c.row + i);
+      best = fmaxf(best, fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w)));
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -679,17 +720,27 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     const int i = i0 + 4 * lane;
     const float4 l4 = *reinterpret_cast<const float4*>(c.row + i);
     const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+    const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+    float far[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (l[j] == c.m) {
-        first = min(first, c.v0 + i + j);
-        ++equal;
-      } else {
-        rest += tc_exp2((l[j] - c.m) * kTcLog2e);
-        if (weighed && !same_unit) part += tc_exp2((l[j] - c.m) * c.unit);
+    for (int j = 0; j < 4; ++j) far[j] = l[j] - c.m;
+    if (top == c.m) {  // the largest are counted, and left out of the sums
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (l[j] == c.m) {
+          first = min(first, c.v0 + i + j);
+          ++equal;
+          far[j] = -INFINITY;
+        }
       }
     }
-    if (__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= likely)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) rest += tc_exp2(far[j] * kTcLog2e);
+    if (weighed && !same_unit) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part += tc_exp2(far[j] * c.unit);
+    }
+    if (__any_sync(0xffffffffu, top >= likely)) {
       const int here = (l[0] >= likely) + (l[1] >= likely) + (l[2] >= likely) + (l[3] >= likely), upto = tc_warp_scan(here);
       found_likelier += (l[0] >= likelier) + (l[1] >= likelier) + (l[2] >= likelier) + (l[3] >= likelier);
       int at = found + upto - here;
@@ -993,12 +1044,18 @@ extern "C" int b200dec_adjust_logits(const void* logits, int64_t stride, int32_t
   if ((const void*)out == logits && (elem != 4 || stride != out_stride)) return B200KV_E_SHAPE;
   TcRules r;
   if (int rc = tc_rules(rules, vocab, &r)) return rc;
-  const dim3 grid((unsigned)((vocab + kAjCols - 1) / kAjCols), (unsigned)entries);
-  const bool vec = aligned(logits, 16) && aligned(out, 16) && stride * elem % 16 == 0 && out_stride % 4 == 0;
-  cudaStream_t s = (cudaStream_t)stream;
-  auto go = [&](auto kernel, auto* src) { return launch_result(launch_chained(kernel, grid, dim3(kAjThreads), 0, s, src, (long long)stride, r, out, (long long)out_stride, (int)vocab, status)); };
-  if (elem == 4) return vec ? go(adjust_logits_kernel<float, true>, (const float*)logits) : go(adjust_logits_kernel<float, false>, (const float*)logits);
-  return vec ? go(adjust_logits_kernel<uint16_t, true>, (const uint16_t*)logits) : go(adjust_logits_kernel<uint16_t, false>, (const uint16_t*)logits);
+  const bool vec = aligned(logits, 4 * elem) && aligned(out, 16) && stride % 4 == 0 && out_stride % 4 == 0;
+  // fewer and longer blocks once there is one for every multiprocessor all the same: each reads the whole history
+  const bool wide = (long long)entries * ((vocab + 8 * kAjCols - 1) / (8 * kAjCols)) >= device_sms();
+  const int cols = wide ? 8 * kAjCols : 2 * kAjCols;
+  const dim3 grid((unsigned)((vocab + cols - 1) / cols), (unsigned)entries);
+  auto go = [&](auto kernel, auto* src) {
+    if (!allow_smem(kernel, 8 * kAjCols * 4)) return launch_result(cudaErrorInvalidValue);
+    return launch_result(launch_chained(kernel, grid, dim3(kAjThreads), (size_t)cols * 4, (cudaStream_t)stream, src, (long long)stride, r, out, (long long)out_stride,
+                                        (int)vocab, vec, status));
+  };
+  if (elem == 4) return wide ? go(adjust_logits_kernel<float, 8>, (const float*)logits) : go(adjust_logits_kernel<float, 2>, (const float*)logits);
+  return wide ? go(adjust_logits_kernel<uint16_t, 8>, (const uint16_t*)logits) : go(adjust_logits_kernel<uint16_t, 2>, (const uint16_t*)logits);
 }
 
 extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t elem, const b200dec_rules* rules, const b200dec_draw* draw,
@@ -1021,7 +1078,7 @@ extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t
   const auto share = [&](int n) { return ((vocab + n - 1) / n + 127) / 128 * 128; };
   while (blocks > 1 && share(blocks / 2) <= 20 * 1024 && (share(blocks) < 2048 || (long long)entries * blocks > device_sms() * 12 / 7)) blocks /= 2;
   const int cols = share(blocks);
-  const bool vec = aligned(logits, 16) && stride * elem % 16 == 0;
+  const bool vec = aligned(logits, 4 * elem) && stride % 4 == 0;
   auto go = [&](auto kernel, auto* src) {
     if (!allow_smem(kernel, kTcRowAt + kTcMaxLocal * 4)) return launch_result(cudaErrorInvalidValue);
     cudaLaunchConfig_t cfg = {};
