@@ -240,11 +240,12 @@ constexpr int kTcMaxCluster = 8;
 constexpr int kTcBins = 1024, kTcCoarse = 32;  // and sums of 32 bins
 constexpr int kTcMembers = 1024;               // tokens of one bin that are put in order
 constexpr int kTcMaxLocal = 48 * 1024;         // columns of a block
-constexpr int kTcShort = 512;                  // likely tokens that are drawn from without histograms: one a thread
-constexpr float kTcShortZ[2] = {16.f, 12.f};   // weights from 2^-16 on, or from 2^-12 on if those are too many
+constexpr int kTcShort = 512;                  // likely tokens that are drawn from without histograms of all: one a thread
+constexpr int kTcShare = 128;                  // of them, where a share of the weight is kept
+constexpr int kTcPlaces = 256;                 // of the threads' largest logits: 32 an octave of z + 0.5, up to a z of 127.5
 constexpr uint32_t kTcNoPlace = 1u << 20;
 constexpr int kTcShortWarp = 64;               // of a warp's columns
-static_assert(kTcShort == kTcThreads && kTcShortWarp * kTcWarps <= kTcMembers && 5 * kTcShort <= 3 * kTcBins, "places of the likely tokens");
+static_assert(kTcShort == kTcThreads && kTcShortWarp * kTcWarps <= kTcMembers && 5 * kTcShort + 2 * kTcPlaces <= 3 * kTcBins, "places of the likely tokens");
 constexpr uint32_t kTcRowAt = kTcBins * 12 + kTcMembers * 12;  // the histogram, a bin's tokens, the row
 
 struct TcDraw {
@@ -262,7 +263,7 @@ struct TcMail {
   float weight[kTcMaxCluster];   // of the tokens among which a share is kept
   uint32_t coarse[2][kTcCoarse];   // of this block: sums of 32 bins
   uint32_t listed_by[kTcMaxCluster];
-  uint32_t likely[2][kTcMaxCluster];  // number of likely tokens, and of the likelier ones; kTcNoPlace: some warp had no place for its own
+  uint32_t likely[kTcMaxCluster];  // number of likely tokens; kTcNoPlace: some warp had no place for its own
   uint32_t settled;
   uint32_t ties[kTcMaxCluster];
   // within the block
@@ -595,7 +596,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   __shared__ float tmp_f[kTcWarps];
   __shared__ int tmp_i[kTcWarps], tmp_n[kTcWarps];
   __shared__ double tmp_d[kTcWarps];
-  __shared__ int tmp_s[kTcWarps], tmp_l[kTcWarps];
+  __shared__ int tmp_s[kTcWarps];
   __shared__ unsigned long long tmp_u[kTcWarps];
   pdl_enter();
   pdl_wait();
@@ -712,15 +713,18 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   float rest = 0.f, part = 0.f;
   int first = 0x7fffffff, equal = 0;
   const bool some = k > 0 && k < V, share = p < 1.f, cuts = some || share || min_p > 0.f;
-  const bool in_reach = !greedy && cuts && k <= kTcShort && (some || share || min_p >= 0.00025f);  // (2^-12 is 0.000244)
+  const bool in_reach = !greedy && cuts && k <= kTcShort * 3 / 4, by_places = in_reach && (some || share);
   const bool weighed = !greedy && !some && (share || !cuts), same_unit = c.unit == kTcLog2e;
-  const float likely = in_reach ? c.floor(kTcShortZ[0]) : INFINITY, likelier = in_reach ? c.floor(kTcShortZ[1]) : INFINITY;
-  int found = 0, found_likelier = 0;  // by this warp, in order of the columns
+  uint32_t* places = c.hist + 5 * kTcShort;  // how many threads' largest logits are how far behind
+  uint32_t* all_places = places + kTcPlaces;
+  if (tid < kTcPlaces) places[tid] = 0;  // (nothing else has been there)
+  float most = -INFINITY;
   for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
     const int i = i0 + 4 * lane;
     const float4 l4 = *reinterpret_cast<const float4*>(c.row + i);
     const float l[4] = {l4.x, l4.y, l4.z, l4.w};
     const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+    most = fmaxf(most, top);
     float far[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) far[j] = l[j] - c.m;
@@ -740,22 +744,6 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
 #pragma unroll
       for (int j = 0; j < 4; ++j) part += tc_exp2(far[j] * c.unit);
     }
-    if (__any_sync(0xffffffffu, top >= likely)) {
-      const int here = (l[0] >= likely) + (l[1] >= likely) + (l[2] >= likely) + (l[3] >= likely), upto = tc_warp_scan(here);
-      found_likelier += (l[0] >= likelier) + (l[1] >= likelier) + (l[2] >= likelier) + (l[3] >= likelier);
-      int at = found + upto - here;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (l[j] >= likely) {
-          if (at < kTcShortWarp) {
-            c.list_far[warp * kTcShortWarp + at] = l[j];
-            c.list_at[warp * kTcShortWarp + at] = c.v0 + i + j;
-          }
-          ++at;
-        }
-      }
-      found += __shfl_sync(0xffffffffu, upto, 31);
-    }
   }
   part = (same_unit ? rest : part) + (float)equal;
   double mine = tc_warp_sum((double)part);
@@ -768,11 +756,12 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     tmp_i[warp] = first;
     tmp_n[warp] = equal;
     tmp_d[warp] = mine;
-    tmp_s[warp] = found;
   }
-  found_likelier = __reduce_add_sync(0xffffffffu, found_likelier);
-  if (lane == 0) tmp_l[warp] = found_likelier;
   __syncthreads();
+  if (by_places) {
+    const float x = c.z(most) + 0.5f;
+    if (x < 128.f) atomicAdd(&places[(__float_as_uint(x) >> 18) - (126u << 5)], 1u);
+  }
   if (warp == 0) {
     rest = tc_warp_sum(lane < kTcWarps ? tmp_f[lane] : 0.f);
     equal = tc_warp_sum(lane < kTcWarps ? tmp_n[lane] : 0);
@@ -786,40 +775,74 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     tc_tell(&mail.first[c.rank], first, c.blocks);
     tc_tell(&mail.mass[c.rank], block, c.blocks);
     tc_tell(&mail.weight[c.rank], (float)block, c.blocks);
-    const uint32_t many = lane < kTcWarps ? tmp_s[lane] : 0, fewer = lane < kTcWarps ? tmp_l[lane] : 0;
-    const bool full = __any_sync(0xffffffffu, many > (uint32_t)kTcShortWarp);
-    tc_tell(&mail.likely[0][c.rank], full ? kTcNoPlace : __reduce_add_sync(0xffffffffu, many), c.blocks);
-    tc_tell(&mail.likely[1][c.rank], full ? kTcNoPlace : __reduce_add_sync(0xffffffffu, fewer), c.blocks);
   }
 
-  // ---- few likely tokens
+  // ---- few likely tokens: those from a floor on that at least as many are above as are looked for, since as many threads' largest are
   if (in_reach) {
     tc_cluster_sync();
-    uint32_t num = 0, fewer = 0;
-    for (int q = 0; q < c.blocks; ++q) {
-      num += mail.likely[0][q];
-      fewer += mail.likely[1][q];
-    }
-    if (min(num, fewer) <= (uint32_t)kTcShort) {
-      // this block's side by side, of the likelier ones if there are too many of the others
-      const bool all_of_them = num <= (uint32_t)kTcShort;
-      const float least = all_of_them ? likely : likelier;
-      num = all_of_them ? num : fewer;
-      float* own_l = reinterpret_cast<float*>(c.hist);
-      int* own_at = reinterpret_cast<int*>(c.hist + kTcShort);
-      int at = 0;
-      for (int w = 0; w < warp; ++w) at += all_of_them ? tmp_s[w] : tmp_l[w];
-      for (int i0 = 0; i0 < found; i0 += 32) {
-        const int i = warp * kTcShortWarp + i0 + lane;
-        const bool in = i0 + lane < found && c.list_far[i] >= least;
-        const unsigned those = __ballot_sync(0xffffffffu, in);
-        if (in) {
-          own_l[at + __popc(those & ((1u << lane) - 1))] = c.list_far[i];
-          own_at[at + __popc(those & ((1u << lane) - 1))] = c.list_at[i];
-        }
-        at += __popc(those);
+    float reach = by_places ? 127.f : fmaxf(-log2f(min_p), 0.f) + 0.001f;
+    if (by_places) {
+      if (tid < kTcPlaces) {
+        uint32_t sum = 0;
+        for (int q = 0; q < c.blocks; ++q) sum += tc_get(tc_there(places + tid, q));
+        all_places[tid] = sum;
       }
-      tc_cluster_sync();
+      __syncthreads();
+      constexpr int kLane = kTcPlaces / 32;
+      uint32_t of[kLane], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kLane; ++j) sum += of[j] = all_places[kLane * lane + j];
+      uint32_t upto = tc_warp_scan(sum) - sum;
+      const uint32_t want = some ? (uint32_t)k : (uint32_t)kTcShare;
+      int behind = kTcPlaces;
+#pragma unroll
+      for (int j = 0; j < kLane; ++j) {
+        upto += of[j];
+        if (behind == kTcPlaces && upto >= want) behind = kLane * lane + j + 1;
+      }
+      behind = __reduce_min_sync(0xffffffffu, behind);
+      if (behind < kTcPlaces) reach = __uint_as_float(((126u << 5) + behind) << 18) - 0.5f;
+    }
+    const float floor = c.floor(reach);
+    int found = 0;  // by this warp, in order of the columns
+    for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
+      const int i = i0 + 4 * lane;
+      const float4 l4 = *reinterpret_cast<const float4*>(c.row + i);
+      const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+      if (!__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= floor)) continue;
+      const int here = (l[0] >= floor) + (l[1] >= floor) + (l[2] >= floor) + (l[3] >= floor), upto = tc_warp_scan(here);
+      int at = found + upto - here;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (l[j] >= floor) {
+          if (at < kTcShortWarp) {
+            c.list_far[warp * kTcShortWarp + at] = l[j];
+            c.list_at[warp * kTcShortWarp + at] = c.v0 + i + j;
+          }
+          ++at;
+        }
+      }
+      found += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) tmp_s[warp] = found;
+    __syncthreads();
+    // this block's side by side
+    float* own_l = reinterpret_cast<float*>(c.hist);
+    int* own_at = reinterpret_cast<int*>(c.hist + kTcShort);
+    const int by_warp = lane < kTcWarps ? tmp_s[lane] : 0, upto_warp = tc_warp_scan(by_warp), in_block = __shfl_sync(0xffffffffu, upto_warp, 31);
+    const bool placed = !__any_sync(0xffffffffu, by_warp > kTcShortWarp) && in_block <= kTcShort;
+    if (placed) {
+      const int at = __shfl_sync(0xffffffffu, upto_warp - by_warp, warp);
+      for (int i = lane; i < found; i += 32) {
+        own_l[at + i] = c.list_far[warp * kTcShortWarp + i];
+        own_at[at + i] = c.list_at[warp * kTcShortWarp + i];
+      }
+    }
+    if (warp == 0) tc_tell(&mail.likely[c.rank], placed ? (uint32_t)in_block : kTcNoPlace, c.blocks);
+    tc_cluster_sync();
+    uint32_t num = 0;
+    for (int q = 0; q < c.blocks; ++q) num += mail.likely[q];
+    if (num <= (uint32_t)kTcShort) {
       if (report) {
         // one a thread, in order of the columns
         float l = -INFINITY;
@@ -827,8 +850,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
         if (tid < num) {
           int q = 0;
           uint32_t i = tid;
-          const uint32_t* by = mail.likely[all_of_them ? 0 : 1];
-          while (i >= by[q]) i -= by[q++];
+          while (i >= mail.likely[q]) i -= mail.likely[q++];
           const uint32_t raw = tc_get(tc_there(own_l + i, q));
           col = (int)tc_get(tc_there(own_at + i, q));
           l = __uint_as_float(raw);
@@ -866,7 +888,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
         __syncthreads();
         const unsigned long long all_w = mail.all_mass;
         double target = INFINITY;
-        bool ok = num > 0 && (!some || num >= (uint32_t)k);
+        bool ok = num > 0 && (!some || num >= (uint32_t)k || reach >= 127.f);  // (weights below 2^-80 do not count)
         if (share) {
           double of;
           if (some) {
@@ -880,7 +902,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
           ok = ok && (double)all_w >= target;
         }
         if (ok) {
-          const bool keep = tid < num && (!some || mine_rank < (uint32_t)k) && (double)sorted[mine_rank] < target && (w >= min_p || l == c.m);
+          const bool keep = tid < num && (!some || mine_rank < (uint32_t)k) && (double)sorted[mine_rank] < target && w > 0.f && (w >= min_p || l == c.m);
           const double kept = keep ? (double)w : 0., upto_k = tc_warp_scan(kept);
           __syncthreads();
           if (lane == 31) tmp_d[warp] = upto_k;
