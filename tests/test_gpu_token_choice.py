@@ -202,6 +202,28 @@ def test_cuts_through_equal_and_crowded_logits(ops, V, values):
     check_choice(l, draw, tokens, logprobs)
 
 
+@pytest.mark.parametrize("V", [50, 2000, 32768, 151936])
+@pytest.mark.parametrize("values", ["falling", "rising", "peak", "far", "bulk"])
+def test_few_and_many_likely_tokens(ops, V, values):
+    """The likely ones side by side, all but one far behind the largest, or too many to be put in order at once; counts on both sides of where the
+    way changes."""
+    g = torch.Generator().manual_seed(7 + V)
+    E = 30
+    l = {"falling": torch.linspace(0, -2000, V).repeat(E, 1), "rising": torch.linspace(-300, 9, V).repeat(E, 1), "peak": torch.randn(E, V, generator=g) * 2,
+         "far": torch.full((E, V), -300.0) - torch.rand(E, V, generator=g), "bulk": torch.randn(E, V, generator=g)}[values]
+    if values in ("peak", "far"):
+        l[:, V // 3] = 25.0
+    l = l.to("cuda")
+    k = torch.tensor([0, 3, 128, 383, 384, 385, 511, 512, 513, 0] * 3).to(torch.int32)
+    p = torch.tensor([0.6] * 10 + [1.0] * 10 + [0.97] * 10)
+    m = torch.zeros(E)
+    m[9::10] = torch.tensor([1e-30, 1e-3, 0.3])
+    p[19] = 1.0
+    draw = ops.Draw(cuda(0.5 + torch.rand(E, generator=g)), cuda(torch.rand(E, generator=g)), cuda(k), cuda(p), cuda(m))
+    tokens, logprobs = ops.choose_tokens(l, draw)
+    check_choice(l, draw, tokens, logprobs)
+
+
 def test_top_k_of_equals_takes_the_first(ops):
     """Of equal logits the k first by index are kept, and u runs through them evenly."""
     V, E = 5000, 40
