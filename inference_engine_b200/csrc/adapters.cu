@@ -12,13 +12,16 @@
 // mantissa): rounded to one they would cost the sum as much as its own rounding does.
 #include "dec_tma.cuh"
 
+#include <algorithm>
+
 namespace b200kv {
 
 constexpr int kAdThreads = 256;
 constexpr int kAdWarps = kAdThreads / 32;
 constexpr int kAdMaxParts = 4;
 constexpr int kAdMaxSlots = 4096;
-constexpr int kAdPlanThreads = 1024;
+constexpr int kAdPlanThreads = 512;
+constexpr int kAdPlanAhead = 4;       // rows whose adapters a thread of the plan fetches together
 constexpr int kAdSimtChannels = 512;  // input channels that the CUDA cores' form stages at a time
 constexpr int kAdSimtCluster = 8;
 constexpr int kAdTcCols = 128;        // output columns of a product of the tensor core
@@ -63,21 +66,27 @@ adapter_plan_kernel(const int32_t* ids, int N, int slots, int tile_rows, int32_t
   for (int g = tid; g <= slots; g += threads) ad_plan_smem[g] = 0;
   for (int i = tid; i < max_tiles * tile_rows; i += threads) order[i] = -1;
   __syncthreads();
-  auto group = [&](int r) {
-    const int id = ids[r];
-    if (id >= 0 && id < slots) return id;
-    if (id != -1 && status) atomicOr(status, B200KV_S_BAD_POSITION);
-    return slots;
-  };
-  for (int base = warp * 32; base < N; base += threads) {
-    const int r = base + lane;
-    const unsigned on = __ballot_sync(0xffffffffu, r < N);
-    if (r < N) {
-      const int g = group(r);
-      const unsigned same = __match_any_sync(on, g);
-      if (lane == __ffs(same) - 1) atomicAdd(&ad_plan_smem[g], __popc(same));
+  // f(row, its adapter, the warp's lanes with a row) of all rows
+  auto each = [&](auto f) {
+    for (int base = tid; base - lane < N; base += kAdPlanAhead * threads) {
+      int id[kAdPlanAhead];
+#pragma unroll
+      for (int j = 0; j < kAdPlanAhead; ++j) id[j] = base + j * threads < N ? ids[base + j * threads] : -1;
+#pragma unroll
+      for (int j = 0; j < kAdPlanAhead; ++j) {
+        const int r = base + j * threads;
+        const unsigned on = __ballot_sync(0xffffffffu, r < N);
+        if (r < N) f(r, id[j], on);
+      }
     }
-  }
+  };
+  each([&](int, int id, unsigned on) {
+    const bool known = id >= 0 && id < slots;
+    if (!known && id != -1 && status) atomicOr(status, B200KV_S_BAD_POSITION);
+    const int g = known ? id : slots;
+    const unsigned same = __match_any_sync(on, g);
+    if (lane == __ffs(same) - 1) atomicAdd(&ad_plan_smem[g], __popc(same));
+  });
   __syncthreads();
   int tiles_before = 0;
   for (int base = 0; base <= slots; base += threads) {
@@ -105,18 +114,14 @@ adapter_plan_kernel(const int32_t* ids, int N, int slots, int tile_rows, int32_t
     __syncthreads();
   }
   for (int i = tiles_before + tid; i < max_tiles; i += threads) tiles[i] = make_int4(-1, 0, 0, 0);
-  for (int base = warp * 32; base < N; base += threads) {
-    const int r = base + lane;
-    const unsigned on = __ballot_sync(0xffffffffu, r < N);
-    if (r < N) {
-      const int id = ids[r], g = id >= 0 && id < slots ? id : slots;
-      const unsigned same = __match_any_sync(on, g);
-      int at = 0;
-      if (lane == __ffs(same) - 1) at = atomicAdd(&ad_plan_smem[g], __popc(same));
-      at = __shfl_sync(same, at, __ffs(same) - 1);
-      order[at + __popc(same & ((1u << lane) - 1))] = r;
-    }
-  }
+  each([&](int r, int id, unsigned on) {
+    const int g = id >= 0 && id < slots ? id : slots;
+    const unsigned same = __match_any_sync(on, g);
+    int at = 0;
+    if (lane == __ffs(same) - 1) at = atomicAdd(&ad_plan_smem[g], __popc(same));
+    at = __shfl_sync(same, at, __ffs(same) - 1);
+    order[at + __popc(same & ((1u << lane) - 1))] = r;
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------------------- shared pieces
@@ -883,10 +888,10 @@ static int ad_rows_of(AdArgs a, int clusters, int most_cols, cudaStream_t stream
 // a place.  us with 8, 4 and 2 blocks, rank 16, rows of 48 adapters: three parts of [2048 -> 4096] 14.9, 11.8 and 8.4, one of [2048 -> 2048] 6.7, 6.3 and
 // 7.3, two of [2048 -> 12288] 16.7, 12.3 and 16.4, [6144 -> 2048] 7.7, 8.2 and 10.2; one row beside [2048 -> 12288] 5.6, 7.7 and 12.0.
 template <int kNT, int kKB, int kStages>
-static int ad_rows(const AdArgs& a, int clusters, int most_cols, cudaStream_t stream) {
+static int ad_rows(const AdArgs& a, int clusters, long long used, int most_cols, cudaStream_t stream) {
   const int room = 3 * device_sms();
-  if ((long long)clusters * 8 <= room) return ad_rows_of<kNT, kKB, 8, kStages>(a, clusters, most_cols, stream);
-  if ((long long)clusters * 4 <= room) return ad_rows_of<kNT, kKB, 4, kStages>(a, clusters, most_cols, stream);
+  if (used * 8 <= room) return ad_rows_of<kNT, kKB, 8, kStages>(a, clusters, most_cols, stream);
+  if (used * 4 <= room) return ad_rows_of<kNT, kKB, 4, kStages>(a, clusters, most_cols, stream);
   return ad_rows_of<kNT, kKB, 2, kStages>(a, clusters, most_cols, stream);
 }
 
@@ -923,13 +928,33 @@ extern "C" int b200dec_adapter_plan(const int32_t* ids, const b200dec_adapter_pl
   if (!ids) return B200KV_E_NULL;
   if (int rc = ad_check_plan(plan)) return rc;
   if (!aligned(ids, 4)) return B200KV_E_ALIGN;
-  const int threads = plan->num_rows <= 256 && plan->slots < 256 ? 256 : kAdPlanThreads;
+  const int threads = plan->num_rows <= 256 && plan->slots < 256 ? kAdPlanThreads / 2 : kAdPlanThreads;
   return launch_result(launch_chained(adapter_plan_kernel, dim3(1), dim3(threads), (size_t)(plan->slots + 1) * 4, (cudaStream_t)stream, ids,
                                       (int)plan->num_rows, (int)plan->slots, (int)plan->tile_rows, plan->order, (int4*)plan->tiles, (int)plan->max_tiles, status));
 }
 
+// Clusters of sixteen rows and a part that can have any.
+static long long ad_used(const b200dec_adapters* ad, const b200dec_adapter_plan_t* plan) {
+  const long long tiles = plan->num_rows / 16 + std::min(plan->num_rows, plan->slots + 1);
+  return ad->parts * std::min(tiles, (long long)plan->max_tiles * (plan->tile_rows / 16));
+}
+
+// Whether tiles of 128 rows go to tcgen05 in whole, and not sixteen rows by sixteen to mma.sync, as a plan of small tiles does.  The latter is one launch without
+// a workspace, and a row's weights are little at a low rank; at a higher one every sixteen rows fetch them again.  us, mma.sync and tcgen05, four adapters:
+//     rank 16, three parts of [2048 -> 4096]: 1000 rows (201 clusters) 12.2 and 14.8, 1250 rows (249) 18.4 and 15.2
+//     rank 16, two parts of [2048 -> 12288]: 1500 rows (196) 24.3 and 27.1, 1750 rows (228) 32.9 and 28.8
+//     rank 32, [2048 -> 2048]: 1000 rows (67) 9.4 and 12.0, 1250 rows (83) 15.8 and 12.2; two parts of [2048 -> 12288]: 300 rows (46) 23.7 and 15.7
+//     rank 64, [2048 -> 2048]: 512 rows (37) 18.0 and 11.5
+static bool ad_whole_tiles(const b200dec_adapters* ad, const b200dec_adapter_plan_t* plan) {
+  if (plan->tile_rows != 128) return false;
+  int most = 0;
+  for (int p = 0; p < ad->parts && p < kAdMaxParts; ++p) most = std::max(most, ad->ends[p] - (p ? ad->ends[p - 1] : 0));
+  const long long used = ad_used(ad, plan);
+  return ad->rank <= 16 ? 2 * used > 3 * device_sms() : ad->rank > 32 || most > 4096 || 2 * used > device_sms();
+}
+
 extern "C" size_t b200dec_add_adapters_workspace(const b200dec_adapters* ad, const b200dec_adapter_plan_t* plan) {
-  if (!ad || !plan || plan->tile_rows != 128 || ad->elem != 2 || plan->max_tiles < 1 || ad->parts < 1 || ad->rank < 8) return 0;
+  if (!ad || !plan || !ad_whole_tiles(ad, plan) || ad->elem != 2 || plan->max_tiles < 1 || ad->parts < 1 || ad->rank < 8) return 0;
   return (size_t)plan->max_tiles * ad->parts * ad_terms_blocks(ad->rank) * 16384;
 }
 
@@ -976,7 +1001,7 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     return ad->elem == 4 ? ad_launch(adapter_simt_kernel<float>, a, fine, kAdSimtCluster, smem, s)
                          : ad_launch(adapter_simt_kernel<uint16_t>, a, fine, kAdSimtCluster, smem, s);
   }
-  if (tile_rows == 128) {
+  if (ad_whole_tiles(ad, plan)) {
     a.blocks = ad_terms_blocks(a.rank);
     a.terms = workspace;
     if (!workspace || workspace_bytes < b200dec_add_adapters_workspace(ad, plan)) return B200KV_E_WORKSPACE;
@@ -1007,8 +1032,9 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     return launch_result(launch_kernel(true, kernel, grid, dim3(kAdSecondThreads), second, s, a));
   }
   const int kb = (a.rank + 15) / 16;
-  if (kb <= 1) return ad_rows<2, 1, 3>(a, fine, most, s);
-  if (kb <= 2) return ad_rows<4, 2, 3>(a, fine, most, s);
-  if (kb <= 4) return ad_rows<8, 4, 2>(a, fine, most, s);
-  return ad_rows<8, 8, 2>(a, fine, most, s);
+  const long long used = ad_used(ad, plan);
+  if (kb <= 1) return ad_rows<2, 1, 3>(a, fine, used, most, s);
+  if (kb <= 2) return ad_rows<4, 2, 3>(a, fine, used, most, s);
+  if (kb <= 4) return ad_rows<8, 4, 2>(a, fine, used, most, s);
+  return ad_rows<8, 8, 2>(a, fine, used, most, s);
 }

@@ -81,6 +81,19 @@ def test_against_the_formula(ops, rows, width, parts, rank, slots, dtype, tile_r
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("rows,width,parts,rank", [
+    (1300, 256, (512, 520, 40), 16), (1300, 264, (24, 96, 130), 8), (2500, 72, (70,), 24), (300, 512, (4200,), 32), (999, 2048, (2048, 1024, 1024), 16),
+    (1000, 136, (2048,), 32), (257, 64, (128,), 8), (400, 512, (96, 40, 8, 200), 128)])
+def test_portions_in_either_form(ops, rows, width, parts, rank):
+    """Many rows of few adapters: at each rank enough of them, or columns, for whole tiles of 128, and fewer."""
+    g = torch.Generator().manual_seed(rows)
+    ids = torch.randint(-1, 3, (5,), generator=g).repeat_interleave(rows // 5 + 1)[:rows]
+    ids[rows // 2] = 2
+    ad, ids, x, y = make(ops, rows, width, parts, rank, 3, torch.bfloat16, seed=rows, ids=ids)
+    got = ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 3), out=torch.empty_like(y))
+    check(ad, ids, x, y, got)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_strided_rows_and_what_lies_beside_them(ops, dtype):
     ad, ids, x, y = make(ops, 50, 128, (64, 32), 16, 3, dtype, seed=4)
