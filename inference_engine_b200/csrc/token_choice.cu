@@ -713,7 +713,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   float rest = 0.f, part = 0.f;
   int first = 0x7fffffff, equal = 0;
   const bool some = k > 0 && k < V, share = p < 1.f, cuts = some || share || min_p > 0.f;
-  const bool in_reach = !greedy && cuts && k <= kTcShort * 3 / 4, by_places = in_reach && (some || share);
+  const bool in_reach = !greedy && cuts && (!some || k <= kTcShort * 3 / 4), by_places = in_reach && (some || share);
   const bool weighed = !greedy && !some && (share || !cuts), same_unit = c.unit == kTcLog2e;
   uint32_t* places = c.hist + 5 * kTcShort;  // how many threads' largest logits are how far behind
   uint32_t* all_places = places + kTcPlaces;
@@ -1067,8 +1067,10 @@ extern "C" int b200dec_adjust_logits(const void* logits, int64_t stride, int32_t
   TcRules r;
   if (int rc = tc_rules(rules, vocab, &r)) return rc;
   const bool vec = aligned(logits, 4 * elem) && aligned(out, 16) && stride % 4 == 0 && out_stride % 4 == 0;
-  // fewer and longer blocks once there is one for every multiprocessor all the same: each reads the whole history
-  const bool wide = (long long)entries * ((vocab + 8 * kAjCols - 1) / (8 * kAjCols)) >= device_sms();
+  // Fewer and longer blocks once there are nearly as many as multiprocessors all the same: each reads the whole history.  us, long and short blocks: 8 entries
+  // of 151936 (80 long blocks) with histories of 1000 tokens 6.3 and 5.0, 64 of 32768 (128) with 8000 10.4 and 12.1 and with 1000 the same, 32 of 151936
+  // (320) 10.5 and 11.4.
+  const bool wide = (long long)entries * ((vocab + 8 * kAjCols - 1) / (8 * kAjCols)) * 4 >= (long long)device_sms() * 3;
   const int cols = wide ? 8 * kAjCols : 2 * kAjCols;
   const dim3 grid((unsigned)((vocab + cols - 1) / cols), (unsigned)entries);
   auto go = [&](auto kernel, auto* src) {
@@ -1094,11 +1096,13 @@ extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t
   TcRules r;
   if (int rc = tc_rules(rules, vocab, &r)) return rc;
   const TcDraw d{draw->temperature, draw->top_k, draw->top_p, draw->min_p, draw->uniform};
-  // Halved while that leaves a block few columns, or as many blocks as are not resident at once (two a multiprocessor, but for the rest of a graphics
-  // cluster), and two blocks still share a multiprocessor.
+  // Halved while that leaves a block few columns, or more blocks than are resident at once (two a multiprocessor, but for what clusters of eight leave of a
+  // graphics cluster), and two blocks still share a multiprocessor.  us with 8, 4, 2 and 1 blocks, 50 and 0.9 kept of 32768: one entry 12.8, 13.3, 15.8 and
+  // 20.1, 32 entries 15.5, 14.0, 15.8 and 20.0, 64 entries 29, 16.2, 16.0 and 20.1, 128 entries 56, 31, 19 and 20; of 8000, 256 entries 103, 51, 29 and 17;
+  // 64 entries of 151936 with 8 and 4 (one block a multiprocessor) 37 and 41.
   int blocks = kTcMaxCluster;
   const auto share = [&](int n) { return ((vocab + n - 1) / n + 127) / 128 * 128; };
-  while (blocks > 1 && share(blocks / 2) <= 20 * 1024 && (share(blocks) < 2048 || (long long)entries * blocks > device_sms() * 12 / 7)) blocks /= 2;
+  while (blocks > 1 && share(blocks / 2) <= 20 * 1024 && (share(blocks) < 2048 || (long long)entries * blocks > device_sms() * (blocks == 8 ? 12 : 12.25) / 7)) blocks /= 2;
   const int cols = share(blocks);
   const bool vec = aligned(logits, 4 * elem) && stride % 4 == 0;
   auto go = [&](auto kernel, auto* src) {
