@@ -241,12 +241,13 @@ constexpr int kTcBins = 1024, kTcCoarse = 32;  // and sums of 32 bins
 constexpr int kTcMembers = 1024;               // tokens of one bin that are put in order
 constexpr int kTcMaxLocal = 48 * 1024;         // columns of a block
 constexpr int kTcShort = 512;                  // likely tokens that are drawn from without histograms of all: one a thread
-constexpr int kTcShare = 128;                  // of them, where a share of the weight is kept
+constexpr int kTcShare = 112;                  // of them, where a share of the weight is kept
 constexpr int kTcPlaces = 256;                 // of the threads' largest logits: 32 an octave of z + 0.5, up to a z of 127.5
 constexpr uint32_t kTcNoPlace = 1u << 20;
 constexpr int kTcShortWarp = 64;               // of a warp's columns
-static_assert(kTcShort == kTcThreads && kTcShortWarp * kTcWarps <= kTcMembers && 5 * kTcShort + 2 * kTcPlaces <= 3 * kTcBins, "places of the likely tokens");
-constexpr uint32_t kTcRowAt = kTcBins * 12 + kTcMembers * 12;  // the histogram, a bin's tokens, the row
+static_assert(kTcShort == kTcThreads && kTcShortWarp * kTcWarps <= kTcMembers && 2 * kTcMembers + 2 * kTcPlaces <= 3 * kTcBins &&
+              kTcMembers == 2 * kTcThreads, "places of the likely tokens");
+constexpr uint32_t kTcRowAt = kTcBins * 12 + kTcMembers * 8;  // the histogram, a bin's tokens, the row
 
 struct TcDraw {
   const float* temperature;
@@ -270,7 +271,7 @@ struct TcMail {
   uint32_t fetched[2][kTcMaxCluster][kTcCoarse];
   uint32_t listed;
   unsigned long long all_mass;
-  float cut_behind;
+  unsigned long long cut;  // a token's key
   int cut_at;
 };
 
@@ -341,9 +342,8 @@ struct TcRow {
   float unit;       // log2(e) / temperature: z below is in units of ln 2
   TcMail* mail;
   uint32_t* hist;   // counts, or upper and lower halves of weights
-  float* list_far;  // a bin's tokens: how far behind the largest, column, weight
+  float* list_far;  // a bin's tokens: how far behind the largest, column
   int* list_at;
-  uint32_t* list_w;
   // how far behind the largest logit
   __device__ __forceinline__ float behind(float l) const { return l == m ? 0.f : m - l; }
   __device__ __forceinline__ float z(float l) const { return __fmul_rn(behind(l), unit); }
@@ -397,6 +397,38 @@ struct TcCut {
     return s < 0 || (s == 0 && c.v0 + i <= at);
   }
 };
+
+// Tokens in order: how far behind the largest, then the column.
+__device__ __forceinline__ unsigned long long tc_key(float far, int at) { return (unsigned long long)__float_as_uint(far) << 32 | (uint32_t)at; }
+__device__ __forceinline__ float tc_key_far(unsigned long long key) { return __uint_as_float((uint32_t)(key >> 32)); }
+constexpr unsigned long long kTcNoKey = ~0ull;  // behind all
+// Puts the num keys that lie in `keys` in ascending order, which has room for a power of two from 64 to twice the block's threads.  By all threads: a bitonic
+// sort, a pair a thread; for pairs up to 32 apart a warp has its 64 keys to itself.  (Counting those in front of each instead took 140 us for 535
+// tokens and 6 for 50.)
+__device__ __forceinline__ void tc_sort(unsigned long long* keys, int num) {
+  const int tid = threadIdx.x;
+  int n = 64;
+  while (n < num) n *= 2;
+  for (int i = num + tid; i < n; i += kTcThreads) keys[i] = kTcNoKey;
+  bool wide = true;  // the step before has been one of several warps
+#pragma unroll 1
+  for (int k = 2; k <= n; k <<= 1) {
+#pragma unroll 1
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (wide || j > 32) __syncthreads();
+      else __syncwarp();
+      wide = j > 32;
+      if (tid >= n / 2) continue;
+      const int i = 2 * tid - (tid & (j - 1));
+      const unsigned long long a = keys[i], b = keys[i + j];
+      if ((a > b) == ((i & k) == 0)) {
+        keys[i] = b;
+        keys[i + j] = a;
+      }
+    }
+  }
+  __syncthreads();
+}
 
 // Where the cut lies that keeps the first `k` tokens (kMass false), or the shortest run with `p` of the weight (kMass true), of those that `had` keeps;
 // off where nothing is cut.  By all threads of the cluster.  weighed: every block has told its tokens' weight.
@@ -502,7 +534,6 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       if (at >= (uint32_t)kTcMembers) return;
       c.list_far[at] = c.behind(l);
       c.list_at[at] = c.v0 + i;
-      if (kMass) c.list_w[at] = c.steps(z);
     });
     __syncthreads();
     if (warp == 0) tc_tell(&mail.listed_by[c.rank], mail.listed, c.blocks);
@@ -510,37 +541,38 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     uint32_t members = 0;
     for (int q = 0; q < c.blocks; ++q) members += mail.listed_by[q];
     if (members <= (uint32_t)kTcMembers) {
-      const uint32_t num = members;
-      float* all_far = reinterpret_cast<float*>(c.hist);
-      int* all_at = reinterpret_cast<int*>(c.hist + kTcMembers);
-      uint32_t* all_w = c.hist + 2 * kTcMembers;
-      for (uint32_t i = tid; i < num; i += kTcThreads) {
+      unsigned long long* keys = reinterpret_cast<unsigned long long*>(c.hist);
+      const int num = (int)members;
+      for (int i = tid; i < num; i += kTcThreads) {
         int q = 0;
         uint32_t at = i;
         while (at >= mail.listed_by[q]) at -= mail.listed_by[q++];
-        const uint32_t far = tc_get(tc_there(c.list_far + at, q)), column = tc_get(tc_there(c.list_at + at, q)), w = kMass ? tc_get(tc_there(c.list_w + at, q)) : 0;
-        all_far[i] = __uint_as_float(far);
-        all_at[i] = (int)column;
-        if (kMass) all_w[i] = w;
+        const uint32_t far = tc_get(tc_there(c.list_far + at, q)), column = tc_get(tc_there(c.list_at + at, q));
+        keys[i] = tc_key(__uint_as_float(far), (int)column);
       }
       tc_cluster_sync();  // (and nobody reads another block's list behind this)
-      for (uint32_t i = tid; i < num; i += kTcThreads) {
-        const float far = all_far[i];
-        const int at = all_at[i];
-        unsigned long long front = before;
-        for (uint32_t j = 0; j < num; ++j) {
-          const float other = all_far[j];
-          if (other < far || (other == far && all_at[j] < at)) front += kMass ? all_w[j] : 1u;
+      tc_sort(keys, num);
+      if (kMass) {
+        unsigned long long w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < num ? c.steps(__fmul_rn(tc_key_far(keys[2 * tid + i]), c.unit)) : 0;
+        const unsigned long long upto_w = tc_warp_scan(w[0] + w[1]);
+        unsigned long long* by_warp = reinterpret_cast<unsigned long long*>(c.list_far);
+        if (lane == 31) by_warp[warp] = upto_w;
+        __syncthreads();
+        unsigned long long front = before + upto_w - w[0] - w[1];
+        for (int v = 0; v < warp; ++v) front += by_warp[v];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (2 * tid + i < num && (double)front < target && (double)(front + w[i]) >= target) mail.cut = keys[2 * tid + i];
+          front += w[i];
         }
-        if ((double)front < target && (double)(front + (kMass ? all_w[i] : 1u)) >= target) {
-          mail.cut_behind = far;
-          mail.cut_at = at;
-        }
+        __syncthreads();
       }
-      __syncthreads();
+      const unsigned long long key = kMass ? mail.cut : keys[k - (uint32_t)before - 1];
       cut.exact = true;
-      cut.behind = mail.cut_behind;
-      cut.at = mail.cut_at;
+      cut.behind = tc_key_far(key);
+      cut.at = (int)(uint32_t)key;
       return cut;
     }
     if (level < 2) {
@@ -619,7 +651,6 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   c.hist = reinterpret_cast<uint32_t*>(tc_smem);
   c.list_far = reinterpret_cast<float*>(c.hist + 3 * kTcBins);
   c.list_at = reinterpret_cast<int*>(c.list_far + kTcMembers);
-  c.list_w = reinterpret_cast<uint32_t*>(c.list_at + kTcMembers);
   c.row = reinterpret_cast<float*>(tc_smem + kTcRowAt);
   c.mail = &mail;
   c.v0 = c.rank * cols;
@@ -715,7 +746,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   const bool some = k > 0 && k < V, share = p < 1.f, cuts = some || share || min_p > 0.f;
   const bool in_reach = !greedy && cuts && (!some || k <= kTcShort * 3 / 4), by_places = in_reach && (some || share);
   const bool weighed = !greedy && !some && (share || !cuts), same_unit = c.unit == kTcLog2e;
-  uint32_t* places = c.hist + 5 * kTcShort;  // how many threads' largest logits are how far behind
+  uint32_t* places = c.hist + 2 * kTcMembers;  // how many threads' largest logits are how far behind
   uint32_t* all_places = places + kTcPlaces;
   if (tid < kTcPlaces) places[tid] = 0;  // (nothing else has been there)
   float most = -INFINITY;
@@ -866,7 +897,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
         sorted[tid] = 0;
         __syncthreads();
         const uint32_t each = num ? (uint32_t)kTcThreads / num : 1, group = each ? tid / num : 0;
-        if (group < each) {
+        if (by_places && group < each) {  // (a weight beside the largest's alone needs no order)
           const uint32_t i = tid - group * num;
           const float mine_l = all_l[i];
           uint32_t front = 0;
@@ -874,7 +905,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
           atomicAdd(&rank_of[i], front);
         }
         __syncthreads();
-        const uint32_t mine_rank = rank_of[tid];
+        const uint32_t mine_rank = by_places ? rank_of[tid] : tid;
         if (tid < num) sorted[mine_rank] = q;
         __syncthreads();
         // weights in front of each place
