@@ -1007,12 +1007,17 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     if (!workspace || workspace_bytes < b200dec_add_adapters_workspace(ad, plan)) return B200KV_E_WORKSPACE;
     if (!aligned(workspace, 16)) return B200KV_E_ALIGN;
     // Clusters are of eight blocks where that many fit at once (a graphics cluster's multiprocessors are rarely a multiple of eight: about a seventh is left
-    // over), else of four, and copies run further ahead where a multiprocessor has one block anyway.
+    // over), else of four, and copies run further ahead where a multiprocessor has one block anyway.  us of both products with 8 blocks and 3 or 5 stages,
+    // and 4 and 3 or 5: 1000 rows of rank 64 (9 clusters) beside [2048 -> 2048] 13.7, 12.3, 15.7, 14.3, beside [6144 -> 2048] 18.9, 17.3, 25.9, 24.1; 2000 rows
+    // of rank 16 (21) beside [2048 -> 12288] 32.8, 39.8, 35.9, 41.9; of rank 64 beside [6144 -> 2048] 23.2, 30.7, 28.6, 26.3, beside three parts of
+    // [2048 -> 4096] (one block a multiprocessor) 30.5, 28.6, 23.7, 24.3.  Where the columns are most of the work, few blocks that leave room for none of the
+    // second product's beside them are the faster: beside [2048 -> 12288], 2000 rows of rank 64 43.1, 40.5, 47.7, 37.3, 4000 of rank 32 78.6, 67.4, 80.3, 62.4.
     const size_t smem = ad_first(&a, 3), deep = ad_first(&a, 5);
     const int first = max_tiles * a.part_groups, sms = device_sms();
     const int fit = (int)(227 * 1024 / (smem + 2048)), room = sms * 6 / 7;
     int rc;
-    if (first * 8 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<8, 5>, a, first, 8, deep, s);
+    if (first * 8 > room && deep <= kAdMostSmem && a.rank > 16 && cols >= 4 * a.width) rc = ad_launch(adapter_first_kernel<4, 5>, a, first, 4, deep, s);
+    else if (first * 8 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<8, 5>, a, first, 8, deep, s);
     else if (first * 8 <= room * fit) rc = ad_launch(adapter_first_kernel<8, 3>, a, first, 8, smem, s);
     else if (first * 4 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<4, 5>, a, first, 4, deep, s);
     else rc = ad_launch(adapter_first_kernel<4, 3>, a, first, 4, smem, s);
