@@ -22,7 +22,7 @@ constexpr int kAdMaxParts = 4;
 constexpr int kAdMaxSlots = 4096;
 constexpr int kAdPlanThreads = 512;
 constexpr int kAdPlanAhead = 4;       // rows whose adapters a thread of the plan fetches together
-constexpr int kAdSimtChannels = 512;  // input channels that the CUDA cores' form stages at a time
+constexpr int kAdSimtChannels = kAdThreads;  // input channels that the CUDA cores' form stages at a time
 constexpr int kAdSimtCluster = 8;
 constexpr int kAdTcCols = 128;        // output columns of a product of the tensor core
 constexpr int kAdSecondThreads = 320;
@@ -771,6 +771,7 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
 template <typename T>
 __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ __align__(16) uint8_t ad_smem[];
+  __shared__ int rows_of[16];
   constexpr int kC = kAdSimtCluster;
   const uint32_t smem = (uint32_t)__cvta_generic_to_shared(ad_smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -784,30 +785,55 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
   const T* up = (const T*)a.up + (long long)job.slot * a.ends[a.parts - 1] * a.rank;
   float* part = reinterpret_cast<float*>(ad_smem);
   float* xs = part + 16 * a.inner_row;
+  if (tid < 16) rows_of[tid] = tid < job.count ? job.order[tid] : -1;
+  __syncthreads();
+  // y of this thread's first column on its way
+  const int cols = job.end - job.begin, c1 = job.begin + (int)((long long)cols * (rank + 1) / kC);
+  int col = job.begin + (int)((long long)cols * rank / kC) + tid;
+  float y[16];
+  const auto load_y = [&]() {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) y[r] = col < c1 && rows_of[r] >= 0 ? ld_elem((const T*)a.y + (long long)rows_of[r] * a.y_stride + col) : 0.f;
+  };
+  load_y();
   const int k0 = (int)((long long)a.width * rank / kC), k1 = (int)((long long)a.width * (rank + 1) / kC);
   for (int i = tid; i < 16 * a.inner_row; i += kAdThreads) part[i] = 0.f;
   for (int s0 = k0; s0 < k1; s0 += kAdSimtChannels) {
     const int n = min(k1 - s0, kAdSimtChannels);
-    __syncthreads();
-    for (int i = tid; i < 16 * kAdSimtChannels; i += kAdThreads) {
-      const int row = i / kAdSimtChannels, k = i % kAdSimtChannels;
-      xs[i] = row < job.count && k < n ? ld_elem((const T*)a.x + (long long)job.order[row] * a.x_stride + s0 + k) : 0.f;
-    }
+    float x[16], w[kAdSimtChannels / 32];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = tid < n && rows_of[r] >= 0 ? ld_elem((const T*)a.x + (long long)rows_of[r] * a.x_stride + s0 + tid) : 0.f;
+    const auto load_w = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < kAdSimtChannels / 32; ++i) w[i] = j < a.rank && lane + 32 * i < n ? ld_elem(down + (long long)j * a.width + s0 + lane + 32 * i) : 0.f;
+    };
+    load_w(warp);
+    __syncthreads();  // (the channels before have been read)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) xs[r * kAdSimtChannels + tid] = x[r];
     __syncthreads();
     for (int j = warp; j < a.rank; j += kAdWarps) {
       float s[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = 0.f;
-      for (int k = lane; k < n; k += 32) {
-        const float w = ld_elem(down + (long long)j * a.width + s0 + k);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] += w * xs[r * kAdSimtChannels + k];
-      }
+      for (int i = 0; i < kAdSimtChannels / 32; ++i) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float v = warp_sum(s[r]);
-        if (lane == r) part[r * a.inner_row + j] += v;
+        for (int r = 0; r < 16; ++r) s[r] += w[i] * xs[r * kAdSimtChannels + lane + 32 * i];
       }
+      load_w(j + kAdWarps);
+      // sums over the lanes: each step halves the rows that a lane has, so that in the end pairs of lanes have one
+#pragma unroll
+      for (int m = 8; m > 0; m >>= 1) {
+        const bool high = lane & (2 * m);
+#pragma unroll
+        for (int r = 0; r < m; ++r) {
+          const float other = __shfl_xor_sync(0xffffffffu, high ? s[r] : s[r + m], 2 * m);
+          s[r] = (high ? s[r + m] : s[r]) + other;
+        }
+      }
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], 1);
+      if (!(lane & 1)) part[(lane >> 1) * a.inner_row + j] += s[0];
     }
   }
   ad_cluster_arrive();
@@ -820,13 +846,12 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
   }
   ad_cluster_arrive();
   __syncthreads();
-  const int cols = job.end - job.begin;
-  const int c1 = job.begin + (int)((long long)cols * (rank + 1) / kC);
-  for (int col = job.begin + (int)((long long)cols * rank / kC) + tid; col < c1; col += kAdThreads) {
+  for (; col < c1; col += kAdThreads) {
     float d[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) d[r] = 0.f;
     const uint8_t* ts = ad_smem + a.off_t;
+#pragma unroll 2
     for (int j = 0; j < a.rank; j += 4) {
       float u[4];
       ld_elem4(up + (long long)col * a.rank + j, u);
@@ -837,11 +862,12 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
       }
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      if (r < job.count) {
-        const long long row = job.order[r];
-        st_elem((T*)a.out + row * a.out_stride + col, ld_elem((const T*)a.y + row * a.y_stride + col) + d[r]);
-      }
+    for (int r = 0; r < 16; ++r)
+      if (rows_of[r] >= 0) st_elem((T*)a.out + (long long)rows_of[r] * a.out_stride + col, y[r] + d[r]);
+    if (col + kAdThreads < c1) {
+      col += kAdThreads;
+      load_y();
+      col -= kAdThreads;
     }
   }
   ad_cluster_wait();
