@@ -182,7 +182,7 @@ constexpr int kAjCols = kAjThreads * 4;  // of a block, times kAhead
 // grid (column blocks, entries).  kAhead: times that a thread takes four columns.  vec: rows aligned to four elements on both sides.  The logits are on their way
 // while the history is counted; the few that have a bias change where they lie.
 template <typename T, int kAhead>
-__global__ void __launch_bounds__(kAjThreads)
+__global__ void __launch_bounds__(kAjThreads, kAhead > 2 || sizeof(T) == 4 ? 2 : 3)
 adjust_logits_kernel(const T* logits, long long stride, const TcRules r, float* out, long long out_stride, int V, bool vec, int32_t* status) {
   extern __shared__ __align__(16) uint32_t aj_table[];
   uint32_t* table = aj_table;
