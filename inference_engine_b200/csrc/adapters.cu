@@ -2,14 +2,19 @@
 //     out[r] = y[r] + scale[a] * (x[r] . down[a]^T) . up[a]^T,   a = the adapter of row r
 // A packed projection has a `down` of its own for each part; a column of `up` meets the inner values of its part.
 //
-// The plan (one block, once per step) sorts the rows by adapter into tiles of at most `tile_rows` rows of one adapter.  A product is then
-// one launch: a cluster of blocks takes a tile and one part.  Its blocks share the input channels, so that a tile's `down` is fetched by many
-// multiprocessors at once; their partial inner values are summed through distributed shared memory, in a fixed order; then the blocks
-// share the part's columns.  Tiles of 16 rows (decoding: weights are what is read) go through mma.sync from registers; tiles of 128 (portions: x, y
-// and the result are) through tcgen05.
+// The plan (one block, once per step) sorts the rows by adapter into tiles of at most `tile_rows` rows of one adapter.  The products have a form for
+// few rows of an adapter, where its weights are what is read (sixteen rows, mma.sync, one launch), one for portions, where x, y and the result
+// are (128 rows, tcgen05, two launches), and one for rows on the CUDA cores.  In all, a cluster of blocks takes a tile and shares its input channels, so
+// that a tile's `down` is fetched by many multiprocessors at once; the blocks' partial inner values are summed through distributed shared memory, in a fixed
+// order.
 //
 // Precision: bf16 operands, 32-bit sums.  The inner values are scaled in 32 bits and enter the second product as two bf16 terms (16 bits of
 // mantissa): rounded to one they would cost the sum as much as its own rounding does.
+//
+// Measured, the plan and [2048 -> 4096] (three parts), [2048 -> 2048], [2048 -> 12288] (two parts) and [6144 -> 2048] in turn: one row, rank 16, 2.5 and 3.9,
+// 4.2, 5.4 and 4.9 us; 64 rows of 48 adapters of rank 16 3.3 and 8.4, 6.7, 12.1 (28 MB, 2.4 TB/s) and 7.6; 992 rows of 3 adapters of rank 16 3.8 and 11, 7,
+// 19 and 9.5; 2000 rows of 4 adapters of rank 64 4.3 and 25, 17, 38 (115 MB, 3 TB/s) and 24.  What bounds the small ones is a chain of latencies: tile, rows,
+// first product, exchange, second product, result.
 #include "dec_tma.cuh"
 
 #include <algorithm>
@@ -409,11 +414,13 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kern
 // ---------------------------------------------------------------------------------------------------------------- portions: tcgen05
 // Two launches.  First product: a cluster takes a tile of 128 rows (the M of tcgen05.mma) and all parts side by side (N), its blocks share the channels, 64
 // at a time through a ring in shared memory; the sums go to a workspace as the second product's operand lies in shared memory.  Second product: a
-// block takes a tile and a run of columns of a part, 128 at a time; K = the inner values' first terms and then their second ones.  With both in one launch, clusters of whole tiles were the unit that
-// multiprocessors are filled by: 2000 rows of rank 64 beside [2048 -> 12288] took 55 us, of which the columns were 23.
+// block takes a tile and a run of columns of a part, 128 at a time; K = the inner values' first terms and then their second ones.  With both in one
+// launch, clusters of whole tiles were the unit that multiprocessors are filled by: 2000 rows of rank 64 beside [2048 -> 12288] took 55 us, of which the
+// columns were 23, and in two 38.  The first one is bound by the latency of its chain, the second by memory.  What did not
+// help there: y brought to L2 beside the first product (41 to 47 us), or no further than 2 or 4 column blocks ahead of the second (44 to 48).
 // Operands lie in the 128-byte-swizzled K-major layout; they come by 16-byte asynchronous copies, since rows lie in any order and the columns of
 // `up` are put so that the accumulator's fragments hold eight columns side by side.
-// No block of a cluster may wait for tensor memory that another cluster's holds, as clusters could then wait for one another: ad_first_smem sees to it that the
+// No block of a cluster may wait for tensor memory that another cluster's holds, as clusters could then wait for one another: ad_first sees to it that the
 // blocks that fit a multiprocessor fit three quarters of its tensor memory, and the next kernel is not brought up before they have theirs.
 __device__ __forceinline__ uint64_t ad_desc(uint32_t saddr) {
   return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -479,7 +486,8 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_word)), "r"(a.tmem_cols) : "memory");
+    const uint32_t word = (uint32_t)__cvta_generic_to_shared(&tmem_word);
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(word), "r"(a.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   ad_before_sync();
@@ -582,8 +590,8 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
   ad_cluster_wait();  // nobody reads another block's memory behind this
 }
 
-// grid (runs of a.run column blocks over all parts, tiles).  Warps 0 to 7 add to y, a product's two halves of columns in four quarters of rows; one lane of warp 8
-// issues the products, into two accumulators in turn; warp 9 brings the columns of `up`, two blocks in shared memory or on their way.  Two blocks
+// grid (runs of a.run column blocks over all parts, tiles).  Warps 0 to 7 add to y, a product's two halves of columns in four quarters of rows; one lane of
+// warp 8 issues the products, into two accumulators in turn; warp 9 brings the columns of `up`, two blocks in shared memory or on their way.  Two blocks
 // share a multiprocessor and hold half of its tensor memory each; neither waits for another one, so that a third could only wait for their end.
 __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ uint8_t ad_raw[];
@@ -682,7 +690,8 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_word)), "r"(2 * kAdTcCols) : "memory");
+    const uint32_t word = (uint32_t)__cvta_generic_to_shared(&tmem_word);
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(word), "r"(2 * kAdTcCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   ad_before_sync();
@@ -767,7 +776,9 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
 }
 
 // ---------------------------------------------------------------------------------------------------------------- CUDA cores
-// 32-bit models, and bf16 rows that cannot be read in 16 bytes: sixteen rows a cluster, 32-bit products.
+// 32-bit models, and bf16 rows that cannot be read in 16 bytes: sixteen rows a cluster, 32-bit products.  Bound by its chain of loads, so each thread has
+// what it needs of sixteen rows on its way at once, y from the start: 40 rows of rank 8 beside [2048 -> 3456] 6.6 us, 13.6
+// with a row's loads one after the other.
 template <typename T>
 __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ __align__(16) uint8_t ad_smem[];
@@ -954,9 +965,10 @@ extern "C" int b200dec_adapter_plan(const int32_t* ids, const b200dec_adapter_pl
   if (!ids) return B200KV_E_NULL;
   if (int rc = ad_check_plan(plan)) return rc;
   if (!aligned(ids, 4)) return B200KV_E_ALIGN;
+  // us with 256, 512 and 1024 threads, a row fetched at a time: 64 rows of 48 adapters 3.4, 3.7 and 4.6, 1000 rows 6.7, 6.2 and 7.3, 2000 rows 10.4, 9.1 and 9.8
   const int threads = plan->num_rows <= 256 && plan->slots < 256 ? kAdPlanThreads / 2 : kAdPlanThreads;
-  return launch_result(launch_chained(adapter_plan_kernel, dim3(1), dim3(threads), (size_t)(plan->slots + 1) * 4, (cudaStream_t)stream, ids,
-                                      (int)plan->num_rows, (int)plan->slots, (int)plan->tile_rows, plan->order, (int4*)plan->tiles, (int)plan->max_tiles, status));
+  return launch_result(launch_chained(adapter_plan_kernel, dim3(1), dim3(threads), (size_t)(plan->slots + 1) * 4, (cudaStream_t)stream, ids, (int)plan->num_rows,
+                                      (int)plan->slots, (int)plan->tile_rows, plan->order, (int4*)plan->tiles, (int)plan->max_tiles, status));
 }
 
 // Clusters of sixteen rows and a part that can have any.
@@ -965,8 +977,9 @@ static long long ad_used(const b200dec_adapters* ad, const b200dec_adapter_plan_
   return ad->parts * std::min(tiles, (long long)plan->max_tiles * (plan->tile_rows / 16));
 }
 
-// Whether tiles of 128 rows go to tcgen05 in whole, and not sixteen rows by sixteen to mma.sync, as a plan of small tiles does.  The latter is one launch without
-// a workspace, and a row's weights are little at a low rank; at a higher one every sixteen rows fetch them again.  us, mma.sync and tcgen05, four adapters:
+// Whether tiles of 128 rows go to tcgen05 in whole, and not sixteen rows by sixteen to mma.sync, as a plan of small tiles does.  The latter is one launch
+// without a workspace, and a row's weights are little at a low rank; at a higher one every sixteen rows fetch them again.  us, mma.sync and
+// tcgen05, four adapters:
 //     rank 16, three parts of [2048 -> 4096]: 1000 rows (201 clusters) 12.2 and 14.8, 1250 rows (249) 18.4 and 15.2
 //     rank 16, two parts of [2048 -> 12288]: 1500 rows (196) 24.3 and 27.1, 1750 rows (228) 32.9 and 28.8
 //     rank 32, [2048 -> 2048]: 1000 rows (67) 9.4 and 12.0, 1250 rows (83) 15.8 and 12.2; two parts of [2048 -> 12288]: 300 rows (46) 23.7 and 15.7
@@ -1051,7 +1064,8 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     const int ublocks = ((a.rank + 15) / 16 * 16 + 63) / 64;
     int col_blocks = 0, runs = 0;
     for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) col_blocks += (a.ends[p] - begin + kAdTcCols - 1) / kAdTcCols;
-    // runs for which all blocks are resident at once, two a multiprocessor
+    // Runs for which all blocks are resident at once, two a multiprocessor.  2000 rows of rank 64 beside [2048 -> 12288], all on clusters of eight: 42 us,
+    // with runs of a single block 48, one block longer 47, three longer 54.
     a.run = (int)(((long long)col_blocks * max_tiles + 2 * sms - 1) / (2 * sms));
     if (a.run < 1) a.run = 1;
     for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) runs += ((a.ends[p] - begin + kAdTcCols - 1) / kAdTcCols + a.run - 1) / a.run;

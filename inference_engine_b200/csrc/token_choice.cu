@@ -13,11 +13,20 @@
 // happens on the multiprocessors.  With m the largest, z = (m - l) / temperature and w = exp(-z), tokens are ordered by l (equal ones by
 // index).  Kept are the first top_k; of these the shortest run whose weight is at least top_p of theirs; of these the ones with w >= min_p.
 // The token is the first, by index, at which the kept weights so far exceed uniform * their sum.
-// Where no more than 512 tokens are within a weight of 2^-16, or else of 2^-12, of the largest and the cuts lie among those, one block takes them all, puts them in order and draws.
-// Otherwise a cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the likelier tokens, or over the others if
-// it does not lie there, down to the few tokens of one bin, which are put in order by comparison.  Blocks tell one another sums of bins, and read
-// from one another only the bins among which the cut lies: a barrier of the cluster each for the largest logit, the histogram, the bin's
-// tokens and the kept weights.
+//
+// Few tokens are kept, mostly.  A thread's largest logit is a token, so as many tokens are above a floor as threads' largest are: a histogram of those alone,
+// one addition a thread, gives a floor with at least k tokens above it and few more (64 of 151936: 64 to 83, 200: 202 to 400), where one of all tokens cost
+// an addition for each in reach.  One block takes the tokens above the floor from the others, puts them in order and draws.  Where they are too many, or
+// the share of weight lies further out, a cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the
+// likelier tokens, or over the others if it does not lie there, down to the few tokens of one bin, which are sorted.  Blocks tell one another sums of bins, and
+// read from one another only the bins among which the cut lies.  A token of top-k of 64 requests took 42 us that way, and 25 by a floor.
+//
+// Precision: 32-bit logits and weights; a weight's integer is in steps of 2^-32 of the largest one, sums are in 64 bits.
+//
+// Measured: rules for 64 rows of 151936 bf16 logits and histories of up to 8192 tokens 22 us (58 MB, 2.6 TB/s), for a row of 32768 4.3.  Choice for 64 such
+// rows with settings of their own 57 us, without cuts 34, for one row 17.  What bounds both is not the bytes but chains: entry, history, row,
+// largest logit, weights, floor, list, draw, each a few hundred cycles of memory or a barrier of the cluster (1 to 1.5 us each beside another block), and that
+// in two rounds of blocks for a full batch, whose rows of 32 bits (39 MB) do not fit the multiprocessors' memory (33 MB) at once.
 #include "dec_common.cuh"
 
 namespace b200kv {
@@ -74,8 +83,8 @@ __device__ __forceinline__ TcEntry tc_entry(const TcRules& r, int e, bool report
 
 constexpr uint32_t kTcSeen = 0x80000000u;  // in the prompt, beside how often a token stands in the output
 
-// table[v - v0] for the columns v0 .. v0 + n of this block; cleared by the caller, with a barrier on both sides.  A thread takes four tokens at a time, and
-// fetches those of four times together.
+// table[v - v0] for the columns v0 .. v0 + n of this block; cleared by the caller, with a barrier on both sides.  A thread takes four tokens at a
+// time, and fetches those of four times together.
 __device__ __forceinline__ void tc_count(const TcEntry& t, int V, int v0, int n, uint32_t* table, bool report, int32_t* status) {
   auto take = [&](int i, int id) {
     const int at = id - v0;
@@ -179,8 +188,10 @@ __device__ __forceinline__ void tc_settle(const TcEntry& t, int v, const uint32_
 constexpr int kAjThreads = 512;
 constexpr int kAjCols = kAjThreads * 4;  // of a block, times kAhead
 
-// grid (column blocks, entries).  kAhead: times that a thread takes four columns.  vec: rows aligned to four elements on both sides.  The logits are on their way
-// while the history is counted; the few that have a bias change where they lie.
+// grid (column blocks, entries).  kAhead: times that a thread takes four columns.  vec: rows aligned to four elements on both sides.  The logits are on
+// their way while the history is counted; the few that have a bias change where they lie.  (Reading back and changing only the columns that the history
+// names, beside a plain copy, took 26 to 30 us for 64 rows of 151936, a table for all columns 22.)  The registers of two blocks a multiprocessor: with those
+// that eight times four 32-bit logits ask for there was one, and 64 rows of 151936 took 34.8 us instead of 25.2.
 template <typename T, int kAhead>
 __global__ void __launch_bounds__(kAjThreads, kAhead > 2 || sizeof(T) == 4 ? 2 : 3)
 adjust_logits_kernel(const T* logits, long long stride, const TcRules r, float* out, long long out_stride, int V, bool vec, int32_t* status) {
@@ -241,7 +252,8 @@ constexpr int kTcBins = 1024, kTcCoarse = 32;  // and sums of 32 bins
 constexpr int kTcMembers = 1024;               // tokens of one bin that are put in order
 constexpr int kTcMaxLocal = 48 * 1024;         // columns of a block
 constexpr int kTcShort = 512;                  // likely tokens that are drawn from without histograms of all: one a thread
-constexpr int kTcShare = 112;                  // of them, where a share of the weight is kept
+constexpr int kTcShare = 112;                  // of them that are looked for where a share of the weight is kept: of 300 rows of 151936 and shares of
+                                               // 0.5 to 0.99, 282 need 44 tokens at most, the others thousands
 constexpr int kTcPlaces = 256;                 // of the threads' largest logits: 32 an octave of z + 0.5, up to a z of 127.5
 constexpr uint32_t kTcNoPlace = 1u << 20;
 constexpr int kTcShortWarp = 64;               // of a warp's columns
@@ -497,7 +509,10 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     unsigned long long sum, upto;  // of counts or of weights
     const auto add_up = [&]() {
       sum = 0;
-      for (int q = 0; q < c.blocks; ++q) sum += kMass ? ((unsigned long long)mail.fetched[0][q][lane] << 16) + mail.fetched[kWords - 1][q][lane] : mail.fetched[0][q][lane];
+      for (int q = 0; q < c.blocks; ++q) {
+        const unsigned long long upper = mail.fetched[0][q][lane];
+        sum += kMass ? (upper << 16) + mail.fetched[kWords - 1][q][lane] : upper;
+      }
       upto = before + tc_warp_scan(sum);
       return __ballot_sync(0xffffffffu, (double)upto >= target);
     };
@@ -506,7 +521,8 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     if (!hit) {
       before = __shfl_sync(0xffffffffu, upto, 31);
       tc_cluster_sync();  // (the blocks read this one's sums)
-      if (base > 0.f) return TcCut();  // fewer tokens, or less weight, than would be kept; weights below 2^-80 do not count.  (A bin's parts have the bin's sums.)
+      // fewer tokens, or less weight, than would be kept; weights below 2^-80 do not count.  (A bin's parts have the bin's sums.)
+      if (base > 0.f) return TcCut();
       base = 16.f;
       scale = kTcBins / 64.f;
       top = 80.f;
@@ -584,7 +600,8 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       continue;
     }
     // more tokens than that within 2^-24 of one another: equal ones, by index
-    const uint32_t want = kMass ? (uint32_t)fmin(fmax(ceil((target - (double)before) * members / fmax((double)in_bin, 1.)), 1.), (double)members) : k - (uint32_t)before;
+    uint32_t want = k - (uint32_t)before;
+    if (kMass) want = (uint32_t)fmin(fmax(ceil((target - (double)before) * members / fmax((double)in_bin, 1.)), 1.), (double)members);
     const auto member = [&](int i, float l) { return cut.side(c.z(l)) == 0 && had.keeps(c, i, l); };
     uint32_t mine = 0;
     c.each([&](int i, float l) { mine += member(i, l); });
@@ -1106,8 +1123,8 @@ extern "C" int b200dec_adjust_logits(const void* logits, int64_t stride, int32_t
   const dim3 grid((unsigned)((vocab + cols - 1) / cols), (unsigned)entries);
   auto go = [&](auto kernel, auto* src) {
     if (!allow_smem(kernel, 8 * kAjCols * 4)) return launch_result(cudaErrorInvalidValue);
-    return launch_result(launch_chained(kernel, grid, dim3(kAjThreads), (size_t)cols * 4, (cudaStream_t)stream, src, (long long)stride, r, out, (long long)out_stride,
-                                        (int)vocab, vec, status));
+    return launch_result(launch_chained(kernel, grid, dim3(kAjThreads), (size_t)cols * 4, (cudaStream_t)stream, src, (long long)stride, r, out,
+                                        (long long)out_stride, (int)vocab, vec, status));
   };
   if (elem == 4) return wide ? go(adjust_logits_kernel<float, 8>, (const float*)logits) : go(adjust_logits_kernel<float, 2>, (const float*)logits);
   return wide ? go(adjust_logits_kernel<uint16_t, 8>, (const uint16_t*)logits) : go(adjust_logits_kernel<uint16_t, 2>, (const uint16_t*)logits);
@@ -1122,7 +1139,8 @@ extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t
   if (entries < 0 || entries > (1 << 24) || vocab < 1 || vocab > kTcMaxCluster * kTcMaxLocal) return B200KV_E_RANGE;
   if ((elem != 2 && elem != 4) || stride < vocab) return B200KV_E_SHAPE;
   if (!aligned(logits, elem) || !aligned(tokens, 8) || !aligned(logprobs, 4)) return B200KV_E_ALIGN;
-  for (const void* p : {(const void*)draw->temperature, (const void*)draw->top_k, (const void*)draw->top_p, (const void*)draw->min_p, (const void*)draw->uniform})
+  const void* numbers[] = {draw->temperature, draw->top_k, draw->top_p, draw->min_p, draw->uniform};
+  for (const void* p : numbers)
     if (!aligned(p, 4)) return B200KV_E_ALIGN;
   TcRules r;
   if (int rc = tc_rules(rules, vocab, &r)) return rc;
@@ -1133,7 +1151,8 @@ extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t
   // 64 entries of 151936 with 8 and 4 (one block a multiprocessor) 37 and 41.
   int blocks = kTcMaxCluster;
   const auto share = [&](int n) { return ((vocab + n - 1) / n + 127) / 128 * 128; };
-  while (blocks > 1 && share(blocks / 2) <= 20 * 1024 && (share(blocks) < 2048 || (long long)entries * blocks > device_sms() * (blocks == 8 ? 12 : 12.25) / 7)) blocks /= 2;
+  const auto resident = [&](int n) { return (long long)entries * n <= device_sms() * (n == 8 ? 12 : 12.25) / 7; };
+  while (blocks > 1 && share(blocks / 2) <= 20 * 1024 && (share(blocks) < 2048 || !resident(blocks))) blocks /= 2;
   const int cols = share(blocks);
   const bool vec = aligned(logits, 4 * elem) && stride % 4 == 0;
   auto go = [&](auto kernel, auto* src) {
@@ -1151,7 +1170,8 @@ extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = take_chained_launch((cudaStream_t)stream) ? 2 : 1;
-    return launch_result(cudaLaunchKernelEx(&cfg, kernel, src, (long long)stride, r, d, (int)vocab, cols, vec, append != 0, (long long*)tokens, logprobs, status));
+    return launch_result(cudaLaunchKernelEx(&cfg, kernel, src, (long long)stride, r, d, (int)vocab, cols, vec, append != 0, (long long*)tokens,
+                                            logprobs, status));
   };
   return elem == 4 ? go(choose_tokens_kernel<float>, (const float*)logits) : go(choose_tokens_kernel<uint16_t>, (const uint16_t*)logits);
 }
