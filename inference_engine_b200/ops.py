@@ -648,7 +648,7 @@ class Adapters:
         ends = [sum(parts[: i + 1]) for i in range(len(parts))]
         st = _lib.Adapters(d.data_ptr(), u.data_ptr(), s.data_ptr(), slots, rank, d.shape[2], len(parts), _elem(d.dtype))
         st.ends[: len(ends)] = ends
-        for name, value in dict(parts=parts, struct=st, ref=ctypes.byref(st), slots=slots, out=out, rank=rank, width=d.shape[2],
+        for name, value in dict(parts=parts, struct=st, ref=ctypes.byref(st), slots=slots, out=out, rank=rank, width=d.shape[2], dtype=u.dtype,
                                 device_index=u.get_device()).items():
             object.__setattr__(self, name, value)
 
@@ -694,6 +694,7 @@ class AdapterPlan:
     def __init__(self, buf: torch.Tensor, rows: int, slots: int, tiles: int, tile_rows: int):
         self.buf, self.rows, self.slots, self.num_tiles, self.tile_rows = buf, rows, slots, tiles, tile_rows
         self.device_index = buf.get_device()
+        self.status = K.status_word(buf.device).data_ptr()
         at = buf.data_ptr()
         self.struct = _lib.AdapterPlan(at + 16 * tiles, at, tiles, tile_rows, rows, slots)
         self.ref = ctypes.byref(self.struct)
@@ -727,8 +728,10 @@ def _here(t: torch.Tensor) -> None:
 def plan_adapters(ids: torch.Tensor, slots: int, tile_rows: int | None = None) -> AdapterPlan:
     """Sort a step's rows by adapter.  ids int32 [rows]: each row's slot, -1: none; others outside [0, slots) count as that and set a status bit.  One launch per
     step, for every add_adapters of it."""
-    K._require_cuda(ids)
-    _here(ids)
+    dev = ids.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        K._require_cuda(ids)
+        _here(ids)
     if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous():
         raise ValueError("plan_adapters: contiguous int32 ids [rows] are wanted")
     if not 1 <= slots <= 4096:
@@ -738,9 +741,10 @@ def plan_adapters(ids: torch.Tensor, slots: int, tile_rows: int | None = None) -
     if rows not in (16, 128):
         raise ValueError(f"plan_adapters: tiles of 16 or 128 rows, not {rows}")
     most = N // rows + min(N, slots + 1)
-    plan = AdapterPlan(torch.empty((4 + rows) * most, dtype=torch.int32, device=ids.device), N, slots, most, rows)
-    rc = _lib_dec().b200dec_adapter_plan(ids.data_ptr(), plan.ref, K.status_word(ids.device).data_ptr(), K._stream())
-    _lib.check(rc, "plan_adapters")
+    plan = AdapterPlan(ids.new_empty((4 + rows) * most), N, slots, most, rows)
+    rc = _lib_dec().b200dec_adapter_plan(ids.data_ptr(), plan.ref, plan.status, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, "plan_adapters")
     return plan
 
 
@@ -750,15 +754,16 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Ada
     Written over y unless `out` is given, which shares no memory with y or x."""
     if out is None:
         out = y
-    N, dtype, dev = plan.rows, adapters.up.dtype, plan.device_index
+    N, dtype, dev = plan.rows, adapters.dtype, plan.device_index
     if not y.get_device() == x.get_device() == out.get_device() == adapters.device_index == dev:
         K._require_cuda(y, x, out, adapters.up)
         raise ValueError("add_adapters: rows, adapters and plan on one device are wanted")
     if dev != torch._C._cuda_getDevice():
         _here(y)
-    if y.dtype != dtype or x.dtype != dtype or out.dtype != dtype:
+    if not y.dtype is x.dtype is out.dtype is dtype:
         raise ValueError(f"add_adapters: rows of {x.dtype}, {y.dtype} and {out.dtype} beside adapters of {dtype}")
-    if x.shape != (N, adapters.width) or y.shape != (N, adapters.out) or out.shape != y.shape:
+    wide = (N, adapters.out)
+    if x.shape != (N, adapters.width) or y.shape != wide or out.shape != wide:
         raise ValueError(f"add_adapters: {tuple(x.shape)}, {tuple(y.shape)} and {tuple(out.shape)} for a plan of {N} rows")
     if plan.slots != adapters.slots:
         raise ValueError(f"add_adapters: a plan for {plan.slots} slots and {adapters.slots} adapters")
@@ -775,7 +780,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Ada
         nbytes = lib.b200dec_add_adapters_workspace(adapters.ref, plan.ref)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=y.device)
     rc = lib.b200dec_add_adapters(adapters.ref, plan.ref, x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, None if ws is None else ws.data_ptr(), nbytes,
-                                  K.status_word(y.device).data_ptr(), K._stream())
+                                  plan.status, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, "add_adapters")
     return out
@@ -906,12 +911,13 @@ def adjust_logits(logits: torch.Tensor, rules: Rules, out: torch.Tensor | None =
     over are left there as they are (uninitialised without it)."""
     E, V, stride, elem = _check_logits("adjust_logits", logits, rules)
     if out is None:
-        out = torch.empty(E, V, dtype=torch.float32, device=logits.device)
+        out = logits.new_empty(E, V, dtype=torch.float32)
     elif out.dtype != torch.float32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or out.device != logits.device:
         raise ValueError("adjust_logits: fp32 rows of the logits' shape are wanted")
     rc = _lib_dec().b200dec_adjust_logits(logits.data_ptr(), stride, elem, rules.ref, out.data_ptr(),
                                           out.stride(0) if E > 1 else _round8(V), E, V, K.status_word(logits.device).data_ptr(), K._stream())
-    _lib.check(rc, "adjust_logits")
+    if rc:
+        _lib.check(rc, "adjust_logits")
     return out
 
 
@@ -927,9 +933,9 @@ def choose_tokens(logits: torch.Tensor, draw: Draw, rules: Rules | None = None, 
         raise ValueError(f"choose_tokens: {V} tokens, at most {MAX_CHOICE_VOCAB}")
     if append and (rules is None or rules.history is None):
         raise ValueError("choose_tokens: nowhere to append to")
-    tokens = torch.empty(E, dtype=torch.int64, device=logits.device)
-    logprobs = torch.empty(E, dtype=torch.float32, device=logits.device)
-    rc = _lib_dec().b200dec_choose_tokens(logits.data_ptr(), stride, elem, None if rules is None else rules.ref, draw.ref, E, V, int(append), tokens.data_ptr(), logprobs.data_ptr(),
-                                          K.status_word(logits.device).data_ptr(), K._stream())
-    _lib.check(rc, "choose_tokens")
+    tokens, logprobs = draw.uniform.new_empty(E, dtype=torch.int64), draw.uniform.new_empty(E)
+    rc = _lib_dec().b200dec_choose_tokens(logits.data_ptr(), stride, elem, None if rules is None else rules.ref, draw.ref, E, V, int(append),
+                                          tokens.data_ptr(), logprobs.data_ptr(), K.status_word(logits.device).data_ptr(), K._stream())
+    if rc:
+        _lib.check(rc, "choose_tokens")
     return tokens, logprobs
