@@ -352,6 +352,7 @@ struct TcRow {
   int rank, blocks;
   float m;
   float unit;       // log2(e) / temperature: z below is in units of ln 2
+  float apart;      // the same, of a temperature of up to 64: places in the order keep apart what a higher one gives the same weight
   TcMail* mail;
   uint32_t* hist;   // counts, or upper and lower halves of weights
   float* list_far;  // a bin's tokens: how far behind the largest, column
@@ -361,8 +362,10 @@ struct TcRow {
   __device__ __forceinline__ float z(float l) const { return __fmul_rn(behind(l), unit); }
   // a weight in steps of 2^-32 of the largest (which is one step short)
   __device__ __forceinline__ uint32_t steps(float z) const { return __float2uint_rn(tc_exp2(-z) * 4294967296.f); }
-  // no token with a smaller logit has a z up to this
-  __device__ __forceinline__ float floor(float z) const { return __fsub_rd(m, __fmul_ru(__fdiv_ru(z, unit), 1.00001f)); }
+  __device__ __forceinline__ float place(float l) const { return __fmul_rn(behind(l), apart); }
+  // no token with a smaller logit has a place (or with `per` unit, a z) up to this
+  __device__ __forceinline__ float floor(float place, float per) const { return __fsub_rd(m, __fmul_ru(__fdiv_ru(place, per), 1.00001f)); }
+  __device__ __forceinline__ float floor(float place) const { return floor(place, apart); }
   // f(column of the block, logit) of all, and of those that are not below a floor: few, where it cuts the bulk of a vocabulary off
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
@@ -387,7 +390,7 @@ struct TcRow {
   }
 };
 
-// A bin of z, and the last token that is kept: of all (exact: how far it is behind the largest, and its column), or of the bin's (its column).
+// A bin of places, and the last token that is kept: of all (exact: how far it is behind the largest, and its column), or of the bin's (its column).
 struct TcCut {
   bool on = false, exact = false;
   float behind = 0.f;
@@ -396,8 +399,8 @@ struct TcCut {
   int bin = 0;
   float floor = -INFINITY;  // no token below it is kept
   // -1: in front of the bin, 0: in it, 1: behind it.  Differences of nearby values and products with powers of two are exact.
-  __device__ __forceinline__ int side(float z) const {
-    const float x = (z - base) * scale;
+  __device__ __forceinline__ int side(float place) const {
+    const float x = (place - base) * scale;
     if (!(x >= 0.f && x < (float)kTcBins)) return x < 0.f ? -1 : 1;
     const int b = (int)x;
     return b < bin ? -1 : b > bin;
@@ -405,7 +408,7 @@ struct TcCut {
   __device__ __forceinline__ bool keeps(const TcRow& c, int i, float l) const {
     if (!on) return true;
     const float far = c.behind(l);
-    const int s = exact ? (far < behind ? -1 : far > behind) : side(__fmul_rn(far, c.unit));
+    const int s = exact ? (far < behind ? -1 : far > behind) : side(__fmul_rn(far, c.apart));
     return s < 0 || (s == 0 && c.v0 + i <= at);
   }
 };
@@ -462,7 +465,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     __syncthreads();
     float weight = 0.f;
     c.each_above(weigh ? had.floor : fmaxf(had.floor, c.floor(top)), [&](int i, float l) {
-      const float z = c.z(l), x = (z - base) * scale;
+      const float z = c.z(l), x = (c.place(l) - base) * scale;
       if (!had.keeps(c, i, l)) return;
       if (weigh) weight += tc_exp2(-z);
       if (!(x >= 0.f && x < (float)kTcBins)) return;
@@ -544,8 +547,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     cut.floor = c.floor(base + (float)(bin + 1) / scale);
     // the bin's tokens: every block's own, then all of them where the histogram was
     c.each_above(cut.floor, [&](int i, float l) {
-      const float z = c.z(l);
-      if (cut.side(z) != 0 || !had.keeps(c, i, l)) return;
+      if (cut.side(c.place(l)) != 0 || !had.keeps(c, i, l)) return;
       const uint32_t at = atomicAdd(&mail.listed, 1u);
       if (at >= (uint32_t)kTcMembers) return;
       c.list_far[at] = c.behind(l);
@@ -602,7 +604,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     // more tokens than that within 2^-24 of one another: equal ones, by index
     uint32_t want = k - (uint32_t)before;
     if (kMass) want = (uint32_t)fmin(fmax(ceil((target - (double)before) * members / fmax((double)in_bin, 1.)), 1.), (double)members);
-    const auto member = [&](int i, float l) { return cut.side(c.z(l)) == 0 && had.keeps(c, i, l); };
+    const auto member = [&](int i, float l) { return cut.side(c.place(l)) == 0 && had.keeps(c, i, l); };
     uint32_t mine = 0;
     c.each([&](int i, float l) { mine += member(i, l); });
     mine = tc_warp_sum(mine);
@@ -755,7 +757,8 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   const int k = d.top_k ? d.top_k[e] : 0;
   const float p = d.top_p ? d.top_p[e] : 1.f, min_p = d.min_p ? d.min_p[e] : 0.f;
   const bool greedy = !(tau > 0.f) || k == 1;
-  c.unit = greedy ? kTcLog2e : fminf(__fdiv_rn(kTcLog2e, tau), 3e38f);  // (finite: the largest is 0 units behind itself)
+  c.unit = greedy ? kTcLog2e : fminf(fmaxf(__fdiv_rn(kTcLog2e, tau), 1e-30f), 3e38f);  // (neither 0 nor infinite: products with infinity and 0 are numbers)
+  c.apart = fmaxf(c.unit, kTcLog2e / 64.f);
 
   // ---- weights beside the largest ones', at temperature 1: a token's probability is exp(-behind) / (number of the largest + rest); and at the entry's
   float rest = 0.f, part = 0.f;
@@ -807,7 +810,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   }
   __syncthreads();
   if (by_places) {
-    const float x = c.z(most) + 0.5f;
+    const float x = c.place(most) + 0.5f;
     if (x < 128.f) atomicAdd(&places[(__float_as_uint(x) >> 18) - (126u << 5)], 1u);
   }
   if (warp == 0) {
@@ -851,7 +854,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
       behind = __reduce_min_sync(0xffffffffu, behind);
       if (behind < kTcPlaces) reach = __uint_as_float(((126u << 5) + behind) << 18) - 0.5f;
     }
-    const float floor = c.floor(reach);
+    const float floor = c.floor(reach, by_places ? c.apart : c.unit);
     int found = 0;  // by this warp, in order of the columns
     for (int i0 = c.lo; i0 < c.hi; i0 += 128) {
       const int i = i0 + 4 * lane;
@@ -1007,7 +1010,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     if (!report || tid != 0) return;
   } else {
     // ---- the kept weights, warp after warp in order of the columns
-    const float floor = fmaxf(fmaxf(by_count.floor, by_mass.floor), min_p > 0.f ? c.floor(fmaxf(-log2f(min_p), 0.f) + 0.001f) : -INFINITY);
+    const float floor = fmaxf(fmaxf(by_count.floor, by_mass.floor), min_p > 0.f ? c.floor(fmaxf(-log2f(min_p), 0.f) + 0.001f, c.unit) : -INFINITY);
     const auto weight = [&](int i, float l) {
       if (l < floor) return 0.f;
       const float w = tc_exp2(-c.z(l));

@@ -43,6 +43,9 @@ from collections.abc import Callable
 from dataclasses import dataclass, field
 
 
+MOST_FLOAT, LEAST_FLOAT = (2 - 2.0 ** -23) * 2.0 ** 127, 2.0 ** -126  # of 32 bits
+
+
 @dataclass(frozen=True)
 class Sampling:
     """How one request's tokens are chosen (ops.Draw, ops.Rules): by default the most likely one.  bias: token -> what is added to its logit.
@@ -62,9 +65,10 @@ class Sampling:
 
     def __post_init__(self):
         numbers = (self.temperature, self.top_p, self.min_p, self.repetition, self.presence, self.frequency, *self.bias.values())
-        if not all(math.isfinite(x) for x in numbers):
-            raise ValueError("sampling: a number is infinite or none")
-        if self.temperature < 0 or self.top_k < 0 or not 0 < self.top_p <= 1 or not 0 <= self.min_p <= 1 or self.repetition <= 0:
+        if not all(abs(x) <= MOST_FLOAT for x in numbers):
+            raise ValueError("sampling: a number is none, or infinite in 32 bits")
+        if (self.temperature < 0 or not 0 <= self.top_k < 2 ** 31 or not 0 < self.top_p <= 1 or not 0 <= self.min_p <= 1
+                or self.repetition < LEAST_FLOAT or (self.seed is not None and self.seed < 0)):
             raise ValueError(f"sampling: {self} is out of range")
 
 
@@ -336,14 +340,13 @@ class Engine:
                 raise ValueError(f"up to {self.max_bias} biased tokens of 0 .. {self.model.vocab - 1} are wanted")
         if adapter != -1 and not 0 <= adapter < self.adapter_slots:
             raise ValueError(f"adapter {adapter}: the engine has {self.adapter_slots} slots")
+        if self.own_sampling and any(not 0 <= t < self.model.vocab for t in prompt_ids):
+            raise ValueError(f"a prompt has ids outside 0 .. {self.model.vocab - 1}")
         r = self.sched.submit(prompt_ids, max_new_tokens)
         r.sampling, r.adapter = sampling, adapter
         if self.own_sampling:
-            if any(not 0 <= t < self.model.vocab for t in r.prompt_ids):
-                self.sched.waiting.pop()
-                raise ValueError(f"a prompt has ids outside 0 .. {self.model.vocab - 1}")
             s = sampling.seed if sampling is not None else None
-            r.rng = self.np.random.default_rng([self.seed, r.id] if s is None else s)
+            r.rng = self.np.random.default_rng([self.seed % 2 ** 64, r.id] if s is None else s)
         return r
 
     def set_mask(self, row: int, allowed) -> None:

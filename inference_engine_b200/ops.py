@@ -925,7 +925,7 @@ def adjust_logits(logits: torch.Tensor, rules: Rules, out: torch.Tensor | None =
 def choose_tokens(logits: torch.Tensor, draw: Draw, rules: Rules | None = None, append: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """Every entry's next token under its rules and its way of drawing: (int64 [entries], its log-probability under the softmax of the adjusted
     logits, fp32 [entries]); (-1, -inf) where nothing is allowed or the entry is passed over.  append: the token goes behind the entry's
-    history where there is room."""
+    history where there is room; the entries' rows are different ones then."""
     E, V, stride, elem = _check_logits("choose_tokens", logits, rules)
     if draw.entries != E or draw.device_index != logits.get_device():
         raise ValueError(f"choose_tokens: a draw for {draw.entries} entries on {draw.uniform.device}, logits of {E} on {logits.device}")

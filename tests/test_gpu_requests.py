@@ -237,6 +237,8 @@ def test_what_is_refused():
         with pytest.raises(ValueError):
             eng.set_mask(row, ids)
     assert eng.sched.idle()
+    eng = build(model, False, own_sampling=True, seed=-3)  # (any number is a seed of an engine)
+    assert len(eng.generate([[1, 2]], 2, Sampling(temperature=1.0))[0].output) == 2
 
 
 @pytest.mark.parametrize("graphs", [False, True])

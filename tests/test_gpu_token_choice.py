@@ -224,6 +224,23 @@ def test_few_and_many_likely_tokens(ops, V, values):
     check_choice(l, draw, tokens, logprobs)
 
 
+@pytest.mark.parametrize("V", [1000, 60000])
+@pytest.mark.parametrize("tau", [64.0, 1e3, 1e7, 3e38, math.inf])
+def test_high_temperatures_weigh_alike_and_keep_the_order(ops, V, tau):
+    g = torch.Generator().manual_seed(V)
+    E = 12
+    l = (torch.randn(E, V, generator=g) * 4).to("cuda")
+    k = torch.tensor([0, 5, 380, 390, 900, 0, 0, 0, 700, 20, 0, 0], dtype=torch.int32)
+    p = torch.tensor([1.0, 1.0, 1.0, 1.0, 1.0, 0.5, 0.001, 0.9, 0.5, 0.5, 1.0, 1.0])
+    m = torch.tensor([0.0] * 10 + [0.5, 1e-6])
+    draw = ops.Draw(torch.full((E,), tau, device="cuda"), cuda(torch.rand(E, generator=g)), cuda(k), cuda(p), cuda(m))
+    tokens, logprobs = ops.choose_tokens(l, draw)
+    check_choice(l, draw, tokens, logprobs)
+    l[:, 3:-3] = -math.inf  # what is not allowed is not drawn, however high
+    tokens, _ = ops.choose_tokens(l, draw)
+    assert ((tokens < 3) | (tokens >= V - 3)).all()
+
+
 def test_top_k_of_equals_takes_the_first(ops):
     """Of equal logits the k first by index are kept, and u runs through them evenly."""
     V, E = 5000, 40

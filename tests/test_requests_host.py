@@ -124,7 +124,8 @@ def test_adapter_entry_points_refuse():
     assert add(xs=63) == add(ys=47) == add(os=47) == add(out=FAKE) == add(out=2 * FAKE, os=56) == -2
     assert add(ad=dict(down=FAKE + 8)) == add(y=2 * FAKE + 1) == -3
     many = dict(num_rows=600, tile_rows=128, max_tiles=65)
-    assert add(pl=many) == -4 and add(pl=many, ws=FAKE, n=100) == -4 and add(pl=many, ws=FAKE + 8, n=1 << 30) == -3
+    high = dict(rank=64)  # (whole tiles)
+    assert add(high, many) == -4 and add(high, many, ws=FAKE, n=100) == -4 and add(high, many, ws=FAKE + 8, n=1 << 30) == -3
     st = _lib.Adapters(FAKE, FAKE, FAKE, 60, 24, 64, 2, 2)
     assert lib.b200dec_add_adapters_workspace(ctypes.byref(st), ctypes.byref(plan(**many))) == 65 * 2 * 16384
     assert lib.b200dec_add_adapters_workspace(ctypes.byref(st), ctypes.byref(plan())) == 0
@@ -161,7 +162,8 @@ def test_logit_entry_points_refuse():
 
 
 @pytest.mark.parametrize("bad", [dict(temperature=-0.1), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.1), dict(min_p=1.5), dict(repetition=0.0),
-                                 dict(presence=float("nan")), dict(bias={3: float("inf")})])
+                                 dict(presence=float("nan")), dict(bias={3: float("inf")}), dict(bias={3: 1e300}), dict(temperature=3.5e38),
+                                 dict(top_k=2 ** 31), dict(repetition=1e-60), dict(seed=-1)])
 def test_sampling_that_is_refused(bad):
     with pytest.raises(ValueError):
         Sampling(**bad)
