@@ -903,7 +903,7 @@ static int ad_launch(void (*kernel)(KArgs...), const AdArgs& a, int clusters, in
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = take_chained_launch(stream) ? 2 : 1;
+  cfg.numAttrs = take_early_launch(stream) ? 2 : 1;
   return launch_result(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
@@ -967,7 +967,7 @@ extern "C" int b200dec_adapter_plan(const int32_t* ids, const b200dec_adapter_pl
   if (!aligned(ids, 4)) return B200KV_E_ALIGN;
   // us with 256, 512 and 1024 threads, a row fetched at a time: 64 rows of 48 adapters 3.4, 3.7 and 4.6, 1000 rows 6.7, 6.2 and 7.3, 2000 rows 10.4, 9.1 and 9.8
   const int threads = plan->num_rows <= 256 && plan->slots < 256 ? kAdPlanThreads / 2 : kAdPlanThreads;
-  return launch_result(launch_chained(adapter_plan_kernel, dim3(1), dim3(threads), (size_t)(plan->slots + 1) * 4, (cudaStream_t)stream, ids, (int)plan->num_rows,
+  return launch_result(launch_kernel(take_early_launch((cudaStream_t)stream), adapter_plan_kernel, dim3(1), dim3(threads), (size_t)(plan->slots + 1) * 4, (cudaStream_t)stream, ids, (int)plan->num_rows,
                                       (int)plan->slots, (int)plan->tile_rows, plan->order, (int4*)plan->tiles, (int)plan->max_tiles, status));
 }
 

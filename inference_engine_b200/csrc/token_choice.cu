@@ -1126,8 +1126,8 @@ extern "C" int b200dec_adjust_logits(const void* logits, int64_t stride, int32_t
   const dim3 grid((unsigned)((vocab + cols - 1) / cols), (unsigned)entries);
   auto go = [&](auto kernel, auto* src) {
     if (!allow_smem(kernel, 8 * kAjCols * 4)) return launch_result(cudaErrorInvalidValue);
-    return launch_result(launch_chained(kernel, grid, dim3(kAjThreads), (size_t)cols * 4, (cudaStream_t)stream, src, (long long)stride, r, out,
-                                        (long long)out_stride, (int)vocab, vec, status));
+    return launch_result(launch_kernel(take_early_launch((cudaStream_t)stream), kernel, grid, dim3(kAjThreads), (size_t)cols * 4, (cudaStream_t)stream, src,
+                                       (long long)stride, r, out, (long long)out_stride, (int)vocab, vec, status));
   };
   if (elem == 4) return wide ? go(adjust_logits_kernel<float, 8>, (const float*)logits) : go(adjust_logits_kernel<float, 2>, (const float*)logits);
   return wide ? go(adjust_logits_kernel<uint16_t, 8>, (const uint16_t*)logits) : go(adjust_logits_kernel<uint16_t, 2>, (const uint16_t*)logits);
@@ -1172,7 +1172,7 @@ extern "C" int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = take_chained_launch((cudaStream_t)stream) ? 2 : 1;
+    cfg.numAttrs = take_early_launch((cudaStream_t)stream) ? 2 : 1;
     return launch_result(cudaLaunchKernelEx(&cfg, kernel, src, (long long)stride, r, d, (int)vocab, cols, vec, append != 0, (long long*)tokens,
                                             logprobs, status));
   };
