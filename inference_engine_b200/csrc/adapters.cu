@@ -570,22 +570,33 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
   const int quads = inner >> 2, rank16 = (a.rank + 15) & ~15, row0 = 128 / kC * rank;
   const int items = max(0, min(128 / kC, count - row0)) * quads;
   uint8_t* out = (uint8_t*)a.terms + ((long long)at * a.parts + p0) * a.blocks * 16384;
-  for (int i = tid; i < items; i += kAdThreads) {
-    const int r = i / quads, row = row0 + r, col = (i - r * quads) * 4, p = col / a.rank, j = col - p * a.rank;
-    uint2 hi, lo;
-    ad_split(ad_total<kC>(smem + (row * a.inner_row + col) * 4, scale), hi, lo);
-    uint8_t* to = out + (long long)p * a.blocks * 16384 + row * 128;
-    const auto place = [&](int k) { return reinterpret_cast<uint2*>(to + (k >> 6) * 16384 + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2); };
-    *place(j) = hi;
-    *place(rank16 + j) = lo;
-    if (j >= a.rank - 8 && (a.rank & 8)) {  // what lies behind a term's values is zero
-      *place(j + 8) = make_uint2(0, 0);
-      *place(rank16 + j + 8) = make_uint2(0, 0);
+  constexpr int kMany = 8 / kC;  // of a thread's values on their way together
+  for (int i0 = 0; i0 < items || i0 == 0; i0 += kMany * kAdThreads) {
+    float4 sums[kMany];
+#pragma unroll
+    for (int m = 0; m < kMany; ++m) {
+      const int i = i0 + m * kAdThreads + tid, r = i / quads;
+      if (i < items) sums[m] = ad_total<kC>(smem + ((row0 + r) * a.inner_row + (i - r * quads) * 4) * 4, scale);
+    }
+    if (i0 + kMany * kAdThreads >= items) ad_cluster_arrive();  // (all of this block's reading is done)
+#pragma unroll
+    for (int m = 0; m < kMany; ++m) {
+      const int i = i0 + m * kAdThreads + tid, r = i / quads, row = row0 + r, col = (i - r * quads) * 4, p = col / a.rank, j = col - p * a.rank;
+      if (i >= items) break;
+      uint2 hi, lo;
+      ad_split(sums[m], hi, lo);
+      uint8_t* to = out + (long long)p * a.blocks * 16384 + row * 128;
+      const auto place = [&](int k) { return reinterpret_cast<uint2*>(to + (k >> 6) * 16384 + ((((k >> 3) & 7) ^ (row & 7)) << 4) + (k & 7) * 2); };
+      *place(j) = hi;
+      *place(rank16 + j) = lo;
+      if (j >= a.rank - 8 && (a.rank & 8)) {  // what lies behind a term's values is zero
+        *place(j + 8) = make_uint2(0, 0);
+        *place(rank16 + j + 8) = make_uint2(0, 0);
+      }
     }
   }
   asm volatile("fence.proxy.async.global;\n" ::: "memory");  // (the next kernel reads them by bulk copies)
   if (dead && a.status) atomicOr(a.status, B200KV_S_TIMEOUT);
-  ad_cluster_arrive();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
   ad_cluster_wait();  // nobody reads another block's memory behind this
 }
@@ -1046,19 +1057,23 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     if (!workspace || workspace_bytes < b200dec_add_adapters_workspace(ad, plan)) return B200KV_E_WORKSPACE;
     if (!aligned(workspace, 16)) return B200KV_E_ALIGN;
     // Clusters are of eight blocks where that many fit at once (a graphics cluster's multiprocessors are rarely a multiple of eight: about a seventh is left
-    // over), else of four, and copies run further ahead where a multiprocessor has one block anyway.  us of both products with 8 blocks and 3 or 5 stages,
-    // and 4 and 3 or 5: 1000 rows of rank 64 (9 clusters) beside [2048 -> 2048] 13.7, 12.3, 15.7, 14.3, beside [6144 -> 2048] 18.9, 17.3, 25.9, 24.1; 2000 rows
-    // of rank 16 (21) beside [2048 -> 12288] 32.8, 39.8, 35.9, 41.9; of rank 64 beside [6144 -> 2048] 23.2, 30.7, 28.6, 26.3, beside three parts of
-    // [2048 -> 4096] (one block a multiprocessor) 30.5, 28.6, 23.7, 24.3.  Where the columns are most of the work, few blocks that leave room for none of the
-    // second product's beside them are the faster: beside [2048 -> 12288], 2000 rows of rank 64 43.1, 40.5, 47.7, 37.3, 4000 of rank 32 78.6, 67.4, 80.3, 62.4.
-    const size_t smem = ad_first(&a, 3), deep = ad_first(&a, 5);
-    const int first = max_tiles * a.part_groups, sms = device_sms();
-    const int fit = (int)(227 * 1024 / (smem + 2048)), room = sms * 6 / 7;
+    // over), else of four, and copies run as far ahead as leaves room for as many blocks.  us of both products with 8 blocks and 3, 4 or 5 stages, and with 4
+    // and 5: 1000 rows of rank 64 (12 clusters) beside [2048 -> 2048] 13.8, 13.5, 12.4, 14.8, beside [6144 -> 2048] 19.2, 18.4, 17.1, 24.5; 2000 rows of rank
+    // 64 (19) beside these 18.6, 17.1, 20.9, 17.0 and 24.6, 22.7, 30.6, 26.9, beside three parts of [2048 -> 4096] (one block a multiprocessor) 31.4, 29.4,
+    // 29.5, 24.3; of rank 16 beside [2048 -> 12288] 33.3, 32.8, 40.3, 42.1.  Where the columns are most of the work, few blocks that leave room for none of the
+    // second product's beside them are the faster at higher ranks: beside [2048 -> 12288], 2000 rows of rank 64 44.0, 40.1, 40.2, 37.3, 4000 of rank 32 79.0,
+    // 85.0, 67.5, 63.0.
+    const size_t smem = ad_first(&a, 3), more = ad_first(&a, 4), deep = ad_first(&a, 5);
+    const int first = max_tiles * a.part_groups, sms = device_sms(), room = sms * 6 / 7;
+    // clusters that are likely to have rows: an adapter's last tile is half full
+    const int groups = std::min(plan->num_rows, plan->slots + 1), used = a.part_groups * (int)std::min<long long>(max_tiles, (plan->num_rows + 64ll * groups + 127) / 128);
+    const auto fits = [&](size_t bytes) { return used * 8 <= room * (int)(227 * 1024 / (bytes + 2048)); };
     int rc;
-    if (first * 8 > room && deep <= kAdMostSmem && a.rank > 16 && cols >= 4 * a.width) rc = ad_launch(adapter_first_kernel<4, 5>, a, first, 4, deep, s);
-    else if (first * 8 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<8, 5>, a, first, 8, deep, s);
-    else if (first * 8 <= room * fit) rc = ad_launch(adapter_first_kernel<8, 3>, a, first, 8, smem, s);
-    else if (first * 4 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<4, 5>, a, first, 4, deep, s);
+    if (used * 8 > room && deep <= kAdMostSmem && a.rank > 16 && cols >= 4 * a.width) rc = ad_launch(adapter_first_kernel<4, 5>, a, first, 4, deep, s);
+    else if (used * 8 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<8, 5>, a, first, 8, deep, s);
+    else if (fits(more)) rc = ad_launch(adapter_first_kernel<8, 4>, a, first, 8, more, s);
+    else if (fits(smem)) rc = ad_launch(adapter_first_kernel<8, 3>, a, first, 8, smem, s);
+    else if (used * 4 <= room && deep <= kAdMostSmem) rc = ad_launch(adapter_first_kernel<4, 5>, a, first, 4, deep, s);
     else rc = ad_launch(adapter_first_kernel<4, 3>, a, first, 4, smem, s);
     if (rc) return rc;
     const int ublocks = ((a.rank + 15) / 16 * 16 + 63) / 64;
