@@ -459,9 +459,8 @@ class Engine:
         np, at = self.np, 0
         if self.adapter_slots:
             buf[:rows] = -1
-            for r, toks in step.entries:
-                buf[at : at + len(toks)] = r.adapter
-                at += len(toks)
+            of = [r.adapter for r, toks in step.entries for _ in toks]
+            buf[: len(of)] = of
             at = rows
         if not self.own_sampling:
             return
@@ -474,6 +473,7 @@ class Engine:
         bias = buf[at + ids.size : at + 2 * ids.size].view(np.float32).reshape(entries, self.max_bias)
         ints[:], floats[:], ids[:] = np.array([[-1], [0], [0], [-1], [0]]), np.array([[1], [0], [0], [0], [1], [0], [0]], np.float32), -1
         plain = Sampling()
+        places, own_ints, own_floats = [], [], []
         for e, (r, toks) in enumerate(step.entries):
             if r.history < 0 or r.cached_len + len(toks) < len(r.prompt_ids):
                 continue
@@ -484,11 +484,14 @@ class Engine:
             mask = -1 if s.grammar is None else int(s.grammar(r.output))
             if not -1 <= mask < self.masks.shape[0]:
                 raise ValueError(f"request {r.id}: its grammar asks for mask {mask} of {self.masks.shape[0]}")
-            ints[:, e] = r.history, len(r.prompt_ids) + len(r.output), len(r.prompt_ids), mask, s.top_k
-            floats[:, e] = s.repetition, s.presence, s.frequency, s.temperature, s.top_p, s.min_p, r.rng.random()
+            places.append(e)
+            own_ints.append((r.history, len(r.prompt_ids) + len(r.output), len(r.prompt_ids), mask, s.top_k))
+            own_floats.append((s.repetition, s.presence, s.frequency, s.temperature, s.top_p, s.min_p, r.rng.random()))
             if s.bias:
                 ids[e, : len(s.bias)] = list(s.bias)
                 bias[e, : len(s.bias)] = list(s.bias.values())
+        if places:
+            ints[:, places], floats[:, places] = np.array(own_ints).T, np.array(own_floats).T
 
     def asks_views(self, dev, entries: int, rows: int, first: int | None = None, first_rows: int | None = None):
         """The model's view of what was filled in, of the first entries and rows."""
