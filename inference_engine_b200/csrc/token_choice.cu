@@ -16,7 +16,7 @@
 //
 // Few tokens are kept, mostly.  A thread's largest logit is a token, so as many tokens are above a floor as threads' largest are: a histogram of those alone,
 // one addition a thread, gives a floor with at least k tokens above it and few more (64 of 151936: 64 to 83, 200: 202 to 400), where one of all tokens cost
-// an addition for each in reach.  One block takes the tokens above the floor from the others, puts them in order and draws.  Where they are too many, or
+// an addition for each in reach.  One block takes the tokens above the floor from the others, which end, puts them in order and draws.  Where they are too many, or
 // the share of weight lies further out, a cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the
 // likelier tokens, or over the others if it does not lie there, down to the few tokens of one bin, which are sorted.  Blocks tell one another sums of bins, and
 // read from one another only the bins among which the cut lies.  A token of top-k of 64 requests took 42 us that way, and 25 by a floor.
@@ -24,7 +24,7 @@
 // Precision: 32-bit logits and weights; a weight's integer is in steps of 2^-32 of the largest one, sums are in 64 bits.
 //
 // Measured: rules for 64 rows of 151936 bf16 logits and histories of up to 8192 tokens 22 us (58 MB, 2.6 TB/s), for a row of 32768 4.3.  Choice for 64 such
-// rows with settings of their own 57 us, without cuts 34, for one row 17.  What bounds both is not the bytes but chains: entry, history, row,
+// rows with settings of their own 54 us, without cuts 33, for one row 16.  What bounds both is not the bytes but chains: entry, history, row,
 // largest logit, weights, floor, list, draw, each a few hundred cycles of memory or a barrier of the cluster (1 to 1.5 us each beside another block), and that
 // in two rounds of blocks for a full batch, whose rows of 32 bits (39 MB) do not fit the multiprocessors' memory (33 MB) at once.
 #include "dec_common.cuh"
@@ -277,7 +277,7 @@ struct TcMail {
   uint32_t coarse[2][kTcCoarse];   // of this block: sums of 32 bins
   uint32_t listed_by[kTcMaxCluster];
   uint32_t likely[kTcMaxCluster];  // number of likely tokens; kTcNoPlace: some warp had no place for its own
-  uint32_t settled;
+  unsigned long long listed_mass[kTcMaxCluster];  // the likely tokens' weights
   uint32_t ties[kTcMaxCluster];
   // within the block
   uint32_t fetched[2][kTcMaxCluster][kTcCoarse];
@@ -882,119 +882,129 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     int* own_at = reinterpret_cast<int*>(c.hist + kTcShort);
     const int by_warp = lane < kTcWarps ? tmp_s[lane] : 0, upto_warp = tc_warp_scan(by_warp), in_block = __shfl_sync(0xffffffffu, upto_warp, 31);
     const bool placed = !__any_sync(0xffffffffu, by_warp > kTcShortWarp) && in_block <= kTcShort;
+    const bool by_share = share && !some;
+    unsigned long long listed_mass = 0;
     if (placed) {
       const int at = __shfl_sync(0xffffffffu, upto_warp - by_warp, warp);
       for (int i = lane; i < found; i += 32) {
-        own_l[at + i] = c.list_far[warp * kTcShortWarp + i];
+        const float l = c.list_far[warp * kTcShortWarp + i];
+        own_l[at + i] = l;
         own_at[at + i] = c.list_at[warp * kTcShortWarp + i];
+        if (by_share) listed_mass += c.steps(c.z(l));
       }
+    }
+    if (by_share) {
+      listed_mass = tc_warp_sum(listed_mass);
+      if (lane == 0) tmp_u[warp] = listed_mass;
+      __syncthreads();
+      if (warp == 0) tc_tell(&mail.listed_mass[c.rank], tc_warp_sum(lane < kTcWarps ? tmp_u[lane] : 0ull), c.blocks);
     }
     if (warp == 0) tc_tell(&mail.likely[c.rank], placed ? (uint32_t)in_block : kTcNoPlace, c.blocks);
     tc_cluster_sync();
+    // every block finds out whether the cuts lie among them (the first k's weights are, if the first k are)
     uint32_t num = 0;
     for (int q = 0; q < c.blocks; ++q) num += mail.likely[q];
-    if (num <= (uint32_t)kTcShort) {
-      if (report) {
-        // one a thread, in order of the columns
-        float l = -INFINITY;
-        int col = 0x7fffffff;
-        if (tid < num) {
-          int q = 0;
-          uint32_t i = tid;
-          while (i >= mail.likely[q]) i -= mail.likely[q++];
-          const uint32_t raw = tc_get(tc_there(own_l + i, q));
-          col = (int)tc_get(tc_there(own_at + i, q));
-          l = __uint_as_float(raw);
-        }
-        const float far = c.behind(l), w = tid < num ? tc_exp2(-__fmul_rn(far, c.unit)) : 0.f;
-        const uint32_t q = tid < num ? __float2uint_rn(w * 4294967296.f) : 0u;
-        // how many of them are in front of each, shared out over the threads
-        float* all_l = c.list_far;
-        uint32_t* rank_of = c.hist + 2 * kTcShort;
-        unsigned long long* sorted = reinterpret_cast<unsigned long long*>(c.hist + 3 * kTcShort);
-        all_l[tid] = l;
-        rank_of[tid] = 0;
-        sorted[tid] = 0;
-        __syncthreads();
-        const uint32_t each = num ? (uint32_t)kTcThreads / num : 1, group = each ? tid / num : 0;
-        if (by_places && group < each) {  // (a weight beside the largest's alone needs no order)
-          const uint32_t i = tid - group * num;
-          const float mine_l = all_l[i];
-          uint32_t front = 0;
-          for (uint32_t j = group; j < num; j += each) front += all_l[j] > mine_l || (all_l[j] == mine_l && j < i);
-          atomicAdd(&rank_of[i], front);
-        }
-        __syncthreads();
-        const uint32_t mine_rank = by_places ? rank_of[tid] : tid;
-        if (tid < num) sorted[mine_rank] = q;
-        __syncthreads();
-        // weights in front of each place
-        const unsigned long long here = sorted[tid], upto_w = tc_warp_scan(here);
-        if (lane == 31) tmp_u[warp] = upto_w;
-        __syncthreads();
-        unsigned long long front_w = upto_w - here;
-        for (int w2 = 0; w2 < warp; ++w2) front_w += tmp_u[w2];
-        sorted[tid] = front_w;
-        if (tid == kTcThreads - 1) mail.all_mass = front_w + here;  // of all
-        __syncthreads();
-        const unsigned long long all_w = mail.all_mass;
-        double target = INFINITY;
-        bool ok = num > 0 && (!some || num >= (uint32_t)k || reach >= 127.f);  // (weights below 2^-80 do not count)
-        if (share) {
-          double of;
-          if (some) {
-            of = (double)((uint32_t)k < num ? sorted[k] : all_w);
-          } else {
-            of = 0.;
-            for (int b = 0; b < c.blocks; ++b) of += mail.mass[b];
-            of *= 4294967296.;
-          }
-          target = fmax((double)(p > 0.f ? p : 0.f) * of, 0.5);
-          ok = ok && (double)all_w >= target;
-        }
-        if (ok) {
-          const bool keep = tid < num && (!some || mine_rank < (uint32_t)k) && (double)sorted[mine_rank] < target && w > 0.f && (w >= min_p || l == c.m);
-          const double kept = keep ? (double)w : 0., upto_k = tc_warp_scan(kept);
-          __syncthreads();
-          if (lane == 31) tmp_d[warp] = upto_k;
-          __syncthreads();
-          double from = 0., all = 0.;
-          for (int w2 = 0; w2 < kTcWarps; ++w2) {
-            if (w2 == warp) from = all;
-            all += tmp_d[w2];
-          }
-          const float u = d.uniform ? d.uniform[e] : 0.f;
-          const double goal = all * (double)fminf(fmaxf(u, 0.f), 1.f - 5.9604645e-8f);
-          // the first kept one that reaches beyond the goal; by a sum's last bit perhaps none, then the last one
-          const unsigned hit = __ballot_sync(0xffffffffu, keep && from + upto_k > goal), any = __ballot_sync(0xffffffffu, keep);
-          if (lane == 0) {
-            tmp_i[warp] = hit ? warp * 32 + __ffs(hit) - 1 : 0x7fffffff;
-            tmp_n[warp] = any ? warp * 32 + 31 - __clz(any) : -1;
-          }
-          __syncthreads();
-          int pick = 0x7fffffff, last = -1;
-          for (int w2 = 0; w2 < kTcWarps; ++w2) {
-            pick = min(pick, tmp_i[w2]);
-            last = max(last, tmp_n[w2]);
-          }
-          if (pick == 0x7fffffff) pick = last;
-          if (tid == pick) {
-            double others = 0.;
-            int same = 0;
-            for (int b = 0; b < c.blocks; ++b) {
-              others += mail.rest[b];
-              same += mail.equal[b];
-            }
-            tokens[e] = col;
-            logprobs[e] = -(float)((double)far + log1p(others + (same - 1)));
-            if (append && t.history && t.length < r.capacity) r.history[(long long)t.slot * r.capacity + t.length] = col;
-          }
-        }
-        __syncthreads();
-        if (warp == 0) tc_tell(&mail.settled, (uint32_t)ok, c.blocks);
+    bool ok = num > 0 && num <= (uint32_t)kTcShort && (!some || num >= (uint32_t)k || reach >= 127.f);  // (weights below 2^-80 do not count)
+    double target = INFINITY;
+    if (by_share) {
+      double of = 0.;
+      listed_mass = 0;
+      for (int q = 0; q < c.blocks; ++q) {
+        of += mail.mass[q];
+        listed_mass += mail.listed_mass[q];
       }
-      tc_cluster_sync();
-      if (mail.settled) return;
+      target = fmax((double)(p > 0.f ? p : 0.f) * (of * 4294967296.), 0.5);
+      ok = ok && (double)listed_mass >= target;
+    }
+    if (ok) {
+      if (!report) {
+        tc_cluster_sync();  // (the first block has this one's tokens)
+        return;
+      }
+      // one a thread, in order of the columns
+      float l = -INFINITY;
+      int col = 0x7fffffff;
+      if (tid < num) {
+        int q = 0;
+        uint32_t i = tid;
+        while (i >= mail.likely[q]) i -= mail.likely[q++];
+        const uint32_t raw = tc_get(tc_there(own_l + i, q));
+        col = (int)tc_get(tc_there(own_at + i, q));
+        l = __uint_as_float(raw);
+      }
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+      const float far = c.behind(l), w = tid < num ? tc_exp2(-__fmul_rn(far, c.unit)) : 0.f;
+      const uint32_t q = tid < num ? __float2uint_rn(w * 4294967296.f) : 0u;
+      // how many of them are in front of each, shared out over the threads
+      float* all_l = c.list_far;
+      uint32_t* rank_of = c.hist + 2 * kTcShort;
+      unsigned long long* sorted = reinterpret_cast<unsigned long long*>(c.hist + 3 * kTcShort);
+      all_l[tid] = l;
+      rank_of[tid] = 0;
+      sorted[tid] = 0;
+      __syncthreads();
+      const uint32_t each = num ? (uint32_t)kTcThreads / num : 1, group = each ? tid / num : 0;
+      if (by_places && group < each) {  // (a weight beside the largest's alone needs no order)
+        const uint32_t i = tid - group * num;
+        const float mine_l = all_l[i];
+        uint32_t front = 0;
+        for (uint32_t j = group; j < num; j += each) front += all_l[j] > mine_l || (all_l[j] == mine_l && j < i);
+        atomicAdd(&rank_of[i], front);
+      }
+      __syncthreads();
+      const uint32_t mine_rank = by_places ? rank_of[tid] : tid;
+      if (tid < num) sorted[mine_rank] = q;
+      __syncthreads();
+      // weights in front of each place
+      const unsigned long long here = sorted[tid], upto_w = tc_warp_scan(here);
+      if (lane == 31) tmp_u[warp] = upto_w;
+      __syncthreads();
+      unsigned long long front_w = upto_w - here;
+      for (int w2 = 0; w2 < warp; ++w2) front_w += tmp_u[w2];
+      sorted[tid] = front_w;
+      if (tid == kTcThreads - 1) mail.all_mass = front_w + here;  // of all
+      __syncthreads();
+      if (share && some) target = fmax((double)(p > 0.f ? p : 0.f) * (double)((uint32_t)k < num ? sorted[k] : mail.all_mass), 0.5);
+      const bool keep = tid < num && (!some || mine_rank < (uint32_t)k) && (double)sorted[mine_rank] < target && w > 0.f && (w >= min_p || l == c.m);
+      const double kept = keep ? (double)w : 0., upto_k = tc_warp_scan(kept);
+      __syncthreads();
+      if (lane == 31) tmp_d[warp] = upto_k;
+      __syncthreads();
+      double from = 0., all = 0.;
+      for (int w2 = 0; w2 < kTcWarps; ++w2) {
+        if (w2 == warp) from = all;
+        all += tmp_d[w2];
+      }
+      const float u = d.uniform ? d.uniform[e] : 0.f;
+      const double goal = all * (double)fminf(fmaxf(u, 0.f), 1.f - 5.9604645e-8f);
+      // the first kept one that reaches beyond the goal; by a sum's last bit perhaps none, then the last one
+      const unsigned hit = __ballot_sync(0xffffffffu, keep && from + upto_k > goal), any = __ballot_sync(0xffffffffu, keep);
+      if (lane == 0) {
+        tmp_i[warp] = hit ? warp * 32 + __ffs(hit) - 1 : 0x7fffffff;
+        tmp_n[warp] = any ? warp * 32 + 31 - __clz(any) : -1;
+      }
+      __syncthreads();
+      int pick = 0x7fffffff, last = -1;
+      for (int w2 = 0; w2 < kTcWarps; ++w2) {
+        pick = min(pick, tmp_i[w2]);
+        last = max(last, tmp_n[w2]);
+      }
+      if (pick == 0x7fffffff) pick = last;
+      if (tid == pick) {
+        double others = 0.;
+        int same = 0;
+        for (int b = 0; b < c.blocks; ++b) {
+          others += mail.rest[b];
+          same += mail.equal[b];
+        }
+        tokens[e] = col;
+        logprobs[e] = -(float)((double)far + log1p(others + (same - 1)));
+        if (append && t.history && t.length < r.capacity) r.history[(long long)t.slot * r.capacity + t.length] = col;
+      }
+      __syncwarp();
+      asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+      return;
     }
   }
 
