@@ -219,3 +219,42 @@ def test_chained_launches(ops):
     finally:
         K.set_early_start(False)
     assert torch.equal(got, want)
+
+
+def test_calls_on_two_streams_at_once(ops):
+    """Portions of both kinds of part beside one another: neither waits for what the other holds."""
+    made = [make(ops, 1400, 512, parts, rank, 3, torch.bfloat16, seed=rank, ids=torch.arange(1400) // 500)
+            for parts, rank in (((512, 256, 256), 64), ((2048,), 40), ((256, 256), 128), ((512,), 32))]
+    plans = [ops.plan_adapters(m[1], 3) for m in made]
+    want = [ops.add_adapters(y, x, ad, plan, out=torch.empty_like(y)) for (ad, _, x, y), plan in zip(made, plans)]
+    streams = [torch.cuda.Stream() for _ in made]
+    outs = [[torch.empty_like(w) for _ in range(6)] for w in want]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for s, (ad, _, x, y), plan, out in zip(streams, made, plans, outs):
+            with torch.cuda.stream(s):
+                ops.add_adapters(y, x, ad, plan, out=out[i])
+    torch.cuda.synchronize()
+    for w, out in zip(want, outs):
+        assert all(torch.equal(o, w) for o in out)
+
+
+def test_two_recorded_steps(ops):
+    """Each has a plan and a workspace of its own, and sees the ids and rows of its replay."""
+    ad, ids, x, y = make(ops, 1300, 256, (512, 64), 64, 4, torch.bfloat16, seed=9, ids=torch.arange(1300) // 400)
+    ops.add_adapters(y, x, ad, ops.plan_adapters(ids, 4), out=torch.empty_like(y))
+    steps = []
+    for n in (1300, 700):
+        graph, out = torch.cuda.CUDAGraph(), torch.empty_like(y[:n])
+        with torch.cuda.graph(graph):
+            plan = ops.plan_adapters(ids[:n], 4)
+            ops.add_adapters(y[:n], x[:n], ad, plan, out=out)
+        steps.append((graph, out, plan, n))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for _ in range(2):
+        ids.copy_(torch.randint(-1, 4, (1300,), generator=g, device="cuda").sort().values)
+        x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        for graph, out, _, n in steps:
+            graph.replay()
+        for graph, out, _, n in steps:
+            check(ad, ids[:n], x[:n], y[:n], out)
