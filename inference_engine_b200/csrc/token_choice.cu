@@ -24,7 +24,7 @@
 // Precision: 32-bit logits and weights; a weight's integer is in steps of 2^-32 of the largest one, sums are in 64 bits.
 //
 // Measured: rules for 64 rows of 151936 bf16 logits and histories of up to 8192 tokens 22 us (58 MB, 2.6 TB/s), for a row of 32768 4.3.  Choice for 64 such
-// rows with settings of their own 54 us, without cuts 33, for one row 16.  What bounds both is not the bytes but chains: entry, history, row,
+// rows with settings of their own 53 us, without cuts 33, for one row 15.  What bounds both is not the bytes but chains: entry, history, row,
 // largest logit, weights, floor, list, draw, each a few hundred cycles of memory or a barrier of the cluster (1 to 1.5 us each beside another block), and that
 // in two rounds of blocks for a full batch, whose rows of 32 bits (39 MB) do not fit the multiprocessors' memory (33 MB) at once.
 #include "dec_common.cuh"
@@ -282,7 +282,7 @@ struct TcMail {
   // within the block
   uint32_t fetched[2][kTcMaxCluster][kTcCoarse];
   uint32_t listed;
-  unsigned long long all_mass;
+  unsigned long long some_mass;  // of the first k
   unsigned long long cut;  // a token's key
   int cut_at;
 };
@@ -936,62 +936,43 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
       asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
       const float far = c.behind(l), w = tid < num ? tc_exp2(-__fmul_rn(far, c.unit)) : 0.f;
       const uint32_t q = tid < num ? __float2uint_rn(w * 4294967296.f) : 0u;
-      // how many of them are in front of each, shared out over the threads
-      float* all_l = c.list_far;
-      uint32_t* rank_of = c.hist + 2 * kTcShort;
-      unsigned long long* sorted = reinterpret_cast<unsigned long long*>(c.hist + 3 * kTcShort);
-      all_l[tid] = l;
-      rank_of[tid] = 0;
-      sorted[tid] = 0;
+      // how many of them, and what weight, are in front of each (a weight beside the largest's alone needs no order)
+      uint2* all = reinterpret_cast<uint2*>(c.list_far);
+      all[tid] = make_uint2(__float_as_uint(l), q);
       __syncthreads();
-      const uint32_t each = num ? (uint32_t)kTcThreads / num : 1, group = each ? tid / num : 0;
-      if (by_places && group < each) {  // (a weight beside the largest's alone needs no order)
-        const uint32_t i = tid - group * num;
-        const float mine_l = all_l[i];
-        uint32_t front = 0;
-        for (uint32_t j = group; j < num; j += each) front += all_l[j] > mine_l || (all_l[j] == mine_l && j < i);
-        atomicAdd(&rank_of[i], front);
+      int place = 0;
+      unsigned long long front_w = 0;
+      if (by_places && tid < (int)num) {
+#pragma unroll 4
+        for (int j = 0; j < (int)num; ++j) {
+          const uint2 other = all[j];
+          const float other_l = __uint_as_float(other.x);
+          if (other_l > l || (other_l == l && j < tid)) {
+            ++place;
+            front_w += other.y;
+          }
+        }
       }
-      __syncthreads();
-      const uint32_t mine_rank = by_places ? rank_of[tid] : tid;
-      if (tid < num) sorted[mine_rank] = q;
-      __syncthreads();
-      // weights in front of each place
-      const unsigned long long here = sorted[tid], upto_w = tc_warp_scan(here);
-      if (lane == 31) tmp_u[warp] = upto_w;
-      __syncthreads();
-      unsigned long long front_w = upto_w - here;
-      for (int w2 = 0; w2 < warp; ++w2) front_w += tmp_u[w2];
-      sorted[tid] = front_w;
-      if (tid == kTcThreads - 1) mail.all_mass = front_w + here;  // of all
-      __syncthreads();
-      if (share && some) target = fmax((double)(p > 0.f ? p : 0.f) * (double)((uint32_t)k < num ? sorted[k] : mail.all_mass), 0.5);
-      const bool keep = tid < num && (!some || mine_rank < (uint32_t)k) && (double)sorted[mine_rank] < target && w > 0.f && (w >= min_p || l == c.m);
+      if (share && some) {
+        if (tid < (int)num && place == min(k, (int)num) - 1) mail.some_mass = front_w + q;
+        __syncthreads();
+        target = fmax((double)(p > 0.f ? p : 0.f) * (double)mail.some_mass, 0.5);
+      }
+      const bool keep = tid < (int)num && (!some || place < k) && (double)front_w < target && w > 0.f && (w >= min_p || l == c.m);
       const double kept = keep ? (double)w : 0., upto_k = tc_warp_scan(kept);
-      __syncthreads();
       if (lane == 31) tmp_d[warp] = upto_k;
       __syncthreads();
-      double from = 0., all = 0.;
+      double from = 0., to = 0., sum = 0.;
       for (int w2 = 0; w2 < kTcWarps; ++w2) {
-        if (w2 == warp) from = all;
-        all += tmp_d[w2];
+        if (w2 == warp) from = sum;
+        sum += tmp_d[w2];
+        if (w2 == warp) to = sum;
       }
       const float u = d.uniform ? d.uniform[e] : 0.f;
-      const double goal = all * (double)fminf(fmaxf(u, 0.f), 1.f - 5.9604645e-8f);
-      // the first kept one that reaches beyond the goal; by a sum's last bit perhaps none, then the last one
-      const unsigned hit = __ballot_sync(0xffffffffu, keep && from + upto_k > goal), any = __ballot_sync(0xffffffffu, keep);
-      if (lane == 0) {
-        tmp_i[warp] = hit ? warp * 32 + __ffs(hit) - 1 : 0x7fffffff;
-        tmp_n[warp] = any ? warp * 32 + 31 - __clz(any) : -1;
-      }
-      __syncthreads();
-      int pick = 0x7fffffff, last = -1;
-      for (int w2 = 0; w2 < kTcWarps; ++w2) {
-        pick = min(pick, tmp_i[w2]);
-        last = max(last, tmp_n[w2]);
-      }
-      if (pick == 0x7fffffff) pick = last;
-      if (tid == pick) {
+      const double goal = sum * (double)fminf(fmaxf(u, 0.f), 1.f - 5.9604645e-8f);
+      // the first kept one that reaches beyond the goal (which is less than the sum)
+      const unsigned hit = __ballot_sync(0xffffffffu, from + upto_k > goal);
+      if (goal >= from && goal < to && lane == __ffs(hit) - 1) {
         double others = 0.;
         int same = 0;
         for (int b = 0; b < c.blocks; ++b) {
