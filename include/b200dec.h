@@ -307,7 +307,8 @@ int b200dec_adjust_logits(const void* logits, int64_t stride, int32_t elem, cons
  * first top_k (0: all), of these the shortest run with top_p of their weight (1: all), of these the ones with w >= min_p (0: all, at most 1); the
  * largest always.  The token is the first by index at which the kept weights so far exceed uniform (in [0, 1)) times their sum.  temperature 0:
  * the largest logit, the first of equals.  NaN logits count as -inf.  Cuts count weights in steps of 2^-32 of the largest, and one among
- * tokens with z >= 31.98 drops all of those.  NULL: temperature 1 (uniform 0 with it) and nothing cut; temperature needs uniform. */
+ * tokens with z >= 31.98 drops all of those.  Where a cut falls among more than 1024 tokens of the same 32-bit distance from the largest,
+ * those are in order of their index.  NULL: temperature 1 (uniform 0 with it) and nothing cut; temperature needs uniform. */
 typedef struct b200dec_draw {
   const float* temperature;
   const int32_t* top_k;

@@ -355,7 +355,7 @@ struct TcRow {
   float apart;      // the same, of a temperature of up to 64: places in the order keep apart what a higher one gives the same weight
   TcMail* mail;
   uint32_t* hist;   // counts, or upper and lower halves of weights
-  float* list_far;  // a bin's tokens: how far behind the largest, column
+  float* list_l;    // a bin's tokens: logit, column
   int* list_at;
   // how far behind the largest logit
   __device__ __forceinline__ float behind(float l) const { return l == m ? 0.f : m - l; }
@@ -390,10 +390,10 @@ struct TcRow {
   }
 };
 
-// A bin of places, and the last token that is kept: of all (exact: how far it is behind the largest, and its column), or of the bin's (its column).
+// A bin of places, and the last token that is kept: of all (exact: its logit and its column), or of the bin's (its column).
 struct TcCut {
   bool on = false, exact = false;
-  float behind = 0.f;
+  float logit = 0.f;
   int at = 0;
   float base = 0.f, scale = 1.f;
   int bin = 0;
@@ -407,15 +407,20 @@ struct TcCut {
   }
   __device__ __forceinline__ bool keeps(const TcRow& c, int i, float l) const {
     if (!on) return true;
-    const float far = c.behind(l);
-    const int s = exact ? (far < behind ? -1 : far > behind) : side(__fmul_rn(far, c.apart));
+    const int s = exact ? (l > logit ? -1 : l < logit) : side(c.place(l));
     return s < 0 || (s == 0 && c.v0 + i <= at);
   }
 };
 
-// Tokens in order: how far behind the largest, then the column.
-__device__ __forceinline__ unsigned long long tc_key(float far, int at) { return (unsigned long long)__float_as_uint(far) << 32 | (uint32_t)at; }
-__device__ __forceinline__ float tc_key_far(unsigned long long key) { return __uint_as_float((uint32_t)(key >> 32)); }
+// Tokens in order: the logit (not how far it is behind the largest, which rounding makes the same for some), then the column.
+__device__ __forceinline__ unsigned long long tc_key(float l, int at) {
+  const uint32_t u = __float_as_uint(__fadd_rn(l, 0.f));  // (one zero)
+  return (unsigned long long)(u >> 31 ? u : ~u & 0x7fffffffu) << 32 | (uint32_t)at;
+}
+__device__ __forceinline__ float tc_key_logit(unsigned long long key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u >> 31 ? u : ~u & 0x7fffffffu);
+}
 constexpr unsigned long long kTcNoKey = ~0ull;  // behind all
 // Puts the num keys that lie in `keys` in ascending order, which has room for a power of two from 64 to twice the block's threads.  By all threads: a bitonic
 // sort, a pair a thread; for pairs up to 32 apart a warp has its 64 keys to itself.  (Counting those in front of each instead took 140 us for 535
@@ -480,10 +485,10 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     });
     if (weigh) {
       weight = tc_warp_sum(weight);
-      if (lane == 0) c.list_far[warp] = weight;  // (nothing is listed yet)
+      if (lane == 0) c.list_l[warp] = weight;  // (nothing is listed yet)
     }
     __syncthreads();
-    if (weigh && warp == 0) tc_tell(&mail.weight[c.rank], tc_warp_sum(lane < kTcWarps ? c.list_far[lane] : 0.f), c.blocks);
+    if (weigh && warp == 0) tc_tell(&mail.weight[c.rank], tc_warp_sum(lane < kTcWarps ? c.list_l[lane] : 0.f), c.blocks);
     for (int i = warp; i < kTcCoarse; i += kTcWarps) {
       const int b = 32 * i + lane;  // (no sum of halves reaches 2^32: a block has fewer than 2^16 columns)
 #pragma unroll
@@ -550,7 +555,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       if (cut.side(c.place(l)) != 0 || !had.keeps(c, i, l)) return;
       const uint32_t at = atomicAdd(&mail.listed, 1u);
       if (at >= (uint32_t)kTcMembers) return;
-      c.list_far[at] = c.behind(l);
+      c.list_l[at] = l;
       c.list_at[at] = c.v0 + i;
     });
     __syncthreads();
@@ -565,17 +570,17 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
         int q = 0;
         uint32_t at = i;
         while (at >= mail.listed_by[q]) at -= mail.listed_by[q++];
-        const uint32_t far = tc_get(tc_there(c.list_far + at, q)), column = tc_get(tc_there(c.list_at + at, q));
-        keys[i] = tc_key(__uint_as_float(far), (int)column);
+        const uint32_t l = tc_get(tc_there(c.list_l + at, q)), column = tc_get(tc_there(c.list_at + at, q));
+        keys[i] = tc_key(__uint_as_float(l), (int)column);
       }
       tc_cluster_sync();  // (and nobody reads another block's list behind this)
       tc_sort(keys, num);
       if (kMass) {
         unsigned long long w[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < num ? c.steps(__fmul_rn(tc_key_far(keys[2 * tid + i]), c.unit)) : 0;
+        for (int i = 0; i < 2; ++i) w[i] = 2 * tid + i < num ? c.steps(c.z(tc_key_logit(keys[2 * tid + i]))) : 0;
         const unsigned long long upto_w = tc_warp_scan(w[0] + w[1]);
-        unsigned long long* by_warp = reinterpret_cast<unsigned long long*>(c.list_far);
+        unsigned long long* by_warp = reinterpret_cast<unsigned long long*>(c.list_l);
         if (lane == 31) by_warp[warp] = upto_w;
         __syncthreads();
         unsigned long long front = before + upto_w - w[0] - w[1];
@@ -589,7 +594,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       }
       const unsigned long long key = kMass ? mail.cut : keys[k - (uint32_t)before - 1];
       cut.exact = true;
-      cut.behind = tc_key_far(key);
+      cut.logit = tc_key_logit(key);
       cut.at = (int)(uint32_t)key;
       return cut;
     }
@@ -601,14 +606,14 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       ++level;
       continue;
     }
-    // more tokens than that within 2^-24 of one another: equal ones, by index
+    // more tokens than that at the same distance, in 32 bits, from the largest: by index
     uint32_t want = k - (uint32_t)before;
     if (kMass) want = (uint32_t)fmin(fmax(ceil((target - (double)before) * members / fmax((double)in_bin, 1.)), 1.), (double)members);
     const auto member = [&](int i, float l) { return cut.side(c.place(l)) == 0 && had.keeps(c, i, l); };
     uint32_t mine = 0;
     c.each([&](int i, float l) { mine += member(i, l); });
     mine = tc_warp_sum(mine);
-    uint32_t* tmp = reinterpret_cast<uint32_t*>(c.list_far);
+    uint32_t* tmp = reinterpret_cast<uint32_t*>(c.list_l);
     if (lane == 0) tmp[warp] = mine;
     __syncthreads();
     if (warp == 0) tc_tell(&mail.ties[c.rank], tc_warp_sum(lane < kTcWarps ? tmp[lane] : 0u), c.blocks);
@@ -668,8 +673,8 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
   // no block writes to another one before that has begun
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
   c.hist = reinterpret_cast<uint32_t*>(tc_smem);
-  c.list_far = reinterpret_cast<float*>(c.hist + 3 * kTcBins);
-  c.list_at = reinterpret_cast<int*>(c.list_far + kTcMembers);
+  c.list_l = reinterpret_cast<float*>(c.hist + 3 * kTcBins);
+  c.list_at = reinterpret_cast<int*>(c.list_l + kTcMembers);
   c.row = reinterpret_cast<float*>(tc_smem + kTcRowAt);
   c.mail = &mail;
   c.v0 = c.rank * cols;
@@ -867,7 +872,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
       for (int j = 0; j < 4; ++j) {
         if (l[j] >= floor) {
           if (at < kTcShortWarp) {
-            c.list_far[warp * kTcShortWarp + at] = l[j];
+            c.list_l[warp * kTcShortWarp + at] = l[j];
             c.list_at[warp * kTcShortWarp + at] = c.v0 + i + j;
           }
           ++at;
@@ -887,7 +892,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     if (placed) {
       const int at = __shfl_sync(0xffffffffu, upto_warp - by_warp, warp);
       for (int i = lane; i < found; i += 32) {
-        const float l = c.list_far[warp * kTcShortWarp + i];
+        const float l = c.list_l[warp * kTcShortWarp + i];
         own_l[at + i] = l;
         own_at[at + i] = c.list_at[warp * kTcShortWarp + i];
         if (by_share) listed_mass += c.steps(c.z(l));
@@ -937,7 +942,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
       const float far = c.behind(l), w = tid < num ? tc_exp2(-__fmul_rn(far, c.unit)) : 0.f;
       const uint32_t q = tid < num ? __float2uint_rn(w * 4294967296.f) : 0u;
       // how many of them, and what weight, are in front of each (a weight beside the largest's alone needs no order)
-      uint2* all = reinterpret_cast<uint2*>(c.list_far);
+      uint2* all = reinterpret_cast<uint2*>(c.list_l);
       all[tid] = make_uint2(__float_as_uint(l), q);
       __syncthreads();
       int place = 0;

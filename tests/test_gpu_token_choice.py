@@ -241,6 +241,21 @@ def test_high_temperatures_weigh_alike_and_keep_the_order(ops, V, tau):
     assert ((tokens < 3) | (tokens >= V - 3)).all()
 
 
+@pytest.mark.parametrize("V", [900, 3000])
+def test_order_is_the_logits_where_their_distances_from_the_largest_round_alike(ops, V):
+    """Logits 1e-9 apart beside one of 8: some 480 of them are the same distance from it in 32 bits, and are ordered all the same."""
+    g = torch.Generator().manual_seed(V)
+    E = 64
+    l = torch.stack([torch.randperm(V, generator=g) for _ in range(E)]).float() * 1e-9
+    l[:, V // 2] = 8.0
+    l = l.to("cuda")
+    k = torch.tensor([50, 200, 390, 555, 700, 0, 0, 0] * 8).to(torch.int32)
+    p = torch.tensor([1.0, 0.9, 1.0, 1.0, 0.95, 0.93, 0.8, 0.85] * 8)
+    draw = ops.Draw(torch.full((E,), 1.0, device="cuda"), cuda(0.9 + 0.1 * torch.rand(E, generator=g)), cuda(k), cuda(p))
+    tokens, logprobs = ops.choose_tokens(l, draw)
+    check_choice(l, draw, tokens, logprobs)
+
+
 def test_top_k_of_equals_takes_the_first(ops):
     """Of equal logits the k first by index are kept, and u runs through them evenly."""
     V, E = 5000, 40
