@@ -76,7 +76,7 @@ adapter_plan_kernel(const int32_t* ids, int N, int slots, int tile_rows, int32_t
     for (int base = tid; base - lane < N; base += kAdPlanAhead * threads) {
       int id[kAdPlanAhead];
 #pragma unroll
-      for (int j = 0; j < kAdPlanAhead; ++j) id[j] = base + j * threads < N ? ids[base + j * threads] : -1;
+      for (int j = 0; j < kAdPlanAhead; ++j) id[j] = base + j * threads < N ? ld_fresh(ids + base + j * threads) : -1;
 #pragma unroll
       for (int j = 0; j < kAdPlanAhead; ++j) {
         const int r = base + j * threads;
@@ -167,6 +167,8 @@ __device__ __forceinline__ void ad_commit() { asm volatile("cp.async.commit_grou
 template <int kLeft>
 __device__ __forceinline__ void ad_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(kLeft) : "memory"); }
 
+// Tiles, rows' places, x and y are read through L2.  A chained kernel is brought up beside the two or three in front of it: the multiprocessor's L1 may hold
+// lines of theirs that were read before others wrote them (an older plan at the same address, say).
 // The rows [first, first + n) of a cluster's tile and the columns of its part.
 struct AdJob {
   int slot, count, part, begin, end;
@@ -175,7 +177,7 @@ struct AdJob {
 template <int kRows, int kC>
 __device__ __forceinline__ AdJob ad_job(const AdArgs& a) {
   const int subs = a.tile_rows / kRows, cl = blockIdx.x / kC, at = cl / a.parts, part = cl - at * a.parts;
-  const int4 tile = a.tiles[at / subs];
+  const int4 tile = __ldcg(a.tiles + at / subs);
   return {tile.x, min(tile.y - (at % subs) * kRows, kRows), part, part ? a.ends[part - 1] : 0, a.ends[part], a.order + (long long)at * kRows};
 }
 
@@ -185,8 +187,8 @@ __device__ __forceinline__ void ad_copy_rows(const AdArgs& a, const AdJob& job, 
   if (a.out == a.y) return;
   for (int col = job.begin + rank * kAdThreads + threadIdx.x; col < job.end; col += cluster * kAdThreads) {
     for (int i = 0; i < job.count; ++i) {
-      const long long r = job.order[i];
-      ((T*)a.out)[r * a.out_stride + col] = ((const T*)a.y)[r * a.y_stride + col];
+      const long long r = ld_fresh(job.order + i);
+      ((T*)a.out)[r * a.out_stride + col] = __ldcg((const T*)a.y + r * a.y_stride + col);
     }
   }
 }
@@ -237,7 +239,7 @@ __device__ __forceinline__ void ad_store(const uint16_t* from, uint16_t* to, int
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < left) st_elem(to + e, ld_elem(from + e) + f[e]);
+      if (e < left) st_elem(to + e, ld_fresh(from + e) + f[e]);
   }
 }
 
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kern
   pdl_enter();
   pdl_wait();
   const AdJob job = ad_job<16, kC>(a);
-  const int row0 = job.order[gid], row1 = job.order[gid + 8];
+  const int row0 = ld_fresh(job.order + gid), row1 = ld_fresh(job.order + gid + 8);
   if (job.count <= 0) return;  // (with the whole cluster)
   if (job.slot < 0) return ad_copy_rows<uint16_t>(a, job, rank, kC);
   const uint16_t* down = (const uint16_t*)a.down + ((long long)job.slot * a.parts + job.part) * a.rank * a.width;
@@ -307,8 +309,8 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kern
       const int j = n0 + 8 * n + gid;
       w[n] = in && j < a.rank ? __ldg(reinterpret_cast<const uint4*>(down + (long long)j * a.width + k)) : zero4;
     }
-    const uint4 u0 = in && row0 >= 0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero4;
-    const uint4 u1 = in && row1 >= 0 ? *reinterpret_cast<const uint4*>(x1 + k) : zero4;
+    const uint4 u0 = in && row0 >= 0 ? __ldcg(reinterpret_cast<const uint4*>(x0 + k)) : zero4;
+    const uint4 u1 = in && row1 >= 0 ? __ldcg(reinterpret_cast<const uint4*>(x1 + k)) : zero4;
     if (first) {
 #pragma unroll
       for (int i = 0; i < kStages; ++i) fetch(g0 + warp + i * kAdWarps, i);
@@ -474,13 +476,13 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
   pdl_wait();
   // the parts that this cluster takes
   const int cl = blockIdx.x / kC, at = cl / a.part_groups, p0 = (cl - at * a.part_groups) * a.group_parts, np = min(a.group_parts, a.parts - p0);
-  const int4 tile = a.tiles[at];
+  const int4 tile = __ldcg(a.tiles + at);
   const int count = tile.y;
   if (count <= 0 || tile.x < 0) return;  // (with the whole cluster)
   const uint32_t smem = ((uint32_t)__cvta_generic_to_shared(ad_raw) + 1023u) & ~1023u;
   uint8_t* base = ad_raw + (smem - (uint32_t)__cvta_generic_to_shared(ad_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
-  if (tid < 128) rows_of[tid] = a.order[(long long)at * 128 + tid];
+  if (tid < 128) rows_of[tid] = ld_fresh(a.order + (long long)at * 128 + tid);
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) dt_mbar_init(bar + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -610,8 +612,9 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
   __shared__ uint32_t tmem_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
   if ((blockIdx.x | blockIdx.y) == 0) pdl_wait();
-  // What the first product's kernel waited for is there as soon as this one is brought up; the inner values are not.
-  const int4 tile = a.tiles[blockIdx.y];
+  // What the first product's kernel waited for (plan and y) is in L2 as soon as this one is brought up, since every block of that one had its wait behind it
+  // then; it is not promised to this grid before its own wait, so L1, which may hold older lines, is passed by.  The inner values are not there yet.
+  const int4 tile = __ldcg(a.tiles + blockIdx.y);
   const int count = tile.y;
   int part = 0, run = blockIdx.x, begin = 0;
   for (; part < a.parts - 1; ++part) {
@@ -628,8 +631,8 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
     pdl_wait();
     if (a.out == a.y) return;
     for (int i = warp; i < count; i += kAdSecondThreads / 32) {
-      const long long r = order[i];
-      for (int c = begin + lane; c < begin + cols; c += 32) ((uint16_t*)a.out)[r * a.out_stride + c] = ((const uint16_t*)a.y)[r * a.y_stride + c];
+      const long long r = ld_fresh(order + i);
+      for (int c = begin + lane; c < begin + cols; c += 32) ((uint16_t*)a.out)[r * a.out_stride + c] = __ldcg((const uint16_t*)a.y + r * a.y_stride + c);
     }
     return;
   }
@@ -647,20 +650,20 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
   uint4 v[2][4] = {};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    rows[i] = warp < 8 ? order[32 * q + 8 * i + gid] : -1;
+    rows[i] = warp < 8 ? ld_fresh(order + 32 * q + 8 * i + gid) : -1;
     from[i] = (const uint16_t*)a.y + (long long)max(rows[i], 0) * a.y_stride + begin + 64 * half + 8 * t;
   }
   auto load_y = [&](int c, int g) {  // 32 columns
     const bool whole = a.vec && cols - (kAdTcCols * c + 64 * half + 32 * g + 8 * t) >= 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (whole && rows[i] >= 0) v[g][i] = *reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c + 32 * g);
+      if (whole && rows[i] >= 0) v[g][i] = __ldcg(reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c + 32 * g));
   };
   load_y(0, 0);
   load_y(0, 1);
   // the rest of y on its way to L2, so that no load waits for memory
   if (tid < 128 && a.vec && cols > kAdTcCols + 8) {
-    const int row = order[tid];
+    const int row = ld_fresh(order + tid);
     if (row >= 0)
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"((const uint16_t*)a.y + (long long)row * a.y_stride + begin + kAdTcCols),
                    "r"((cols - kAdTcCols) / 8 * 16) : "memory");
@@ -807,7 +810,7 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
   const T* up = (const T*)a.up + (long long)job.slot * a.ends[a.parts - 1] * a.rank;
   float* part = reinterpret_cast<float*>(ad_smem);
   float* xs = part + 16 * a.inner_row;
-  if (tid < 16) rows_of[tid] = tid < job.count ? job.order[tid] : -1;
+  if (tid < 16) rows_of[tid] = tid < job.count ? ld_fresh(job.order + tid) : -1;
   __syncthreads();
   // y of this thread's first column on its way
   const int cols = job.end - job.begin, c1 = job.begin + (int)((long long)cols * (rank + 1) / kC);
@@ -815,7 +818,7 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
   float y[16];
   const auto load_y = [&]() {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) y[r] = col < c1 && rows_of[r] >= 0 ? ld_elem((const T*)a.y + (long long)rows_of[r] * a.y_stride + col) : 0.f;
+    for (int r = 0; r < 16; ++r) y[r] = col < c1 && rows_of[r] >= 0 ? ld_fresh((const T*)a.y + (long long)rows_of[r] * a.y_stride + col) : 0.f;
   };
   load_y();
   const int k0 = (int)((long long)a.width * rank / kC), k1 = (int)((long long)a.width * (rank + 1) / kC);
@@ -824,7 +827,7 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
     const int n = min(k1 - s0, kAdSimtChannels);
     float x[16], w[kAdSimtChannels / 32];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = tid < n && rows_of[r] >= 0 ? ld_elem((const T*)a.x + (long long)rows_of[r] * a.x_stride + s0 + tid) : 0.f;
+    for (int r = 0; r < 16; ++r) x[r] = tid < n && rows_of[r] >= 0 ? ld_fresh((const T*)a.x + (long long)rows_of[r] * a.x_stride + s0 + tid) : 0.f;
     const auto load_w = [&](int j) {
 #pragma unroll
       for (int i = 0; i < kAdSimtChannels / 32; ++i) w[i] = j < a.rank && lane + 32 * i < n ? ld_elem(down + (long long)j * a.width + s0 + lane + 32 * i) : 0.f;

@@ -33,6 +33,7 @@ __device__ __forceinline__ void ld_fresh4(const uint16_t* p, float (&f)[4]) {
   f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xFFFF0000u);
 }
 __device__ __forceinline__ float ld_fresh(const float* p) { return __ldcg(p); }
+__device__ __forceinline__ float ld_fresh(const uint16_t* p) { return bf16_bits_to_float(__ldcg(p)); }
 __device__ __forceinline__ int ld_fresh(const int32_t* p) { return __ldcg(p); }
 
 __device__ __forceinline__ void st_elem4(float* p, const float (&f)[4]) {

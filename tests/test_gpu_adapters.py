@@ -258,3 +258,37 @@ def test_two_recorded_steps(ops):
             graph.replay()
         for graph, out, _, n in steps:
             check(ad, ids[:n], x[:n], y[:n], out)
+
+
+@pytest.mark.parametrize("rows,rank,slots", [(60, 16, 20), (90, 24, 4), (700, 64, 5), (40, 8, 9)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("early", [None, True])
+def test_steps_behind_one_another_read_their_own_plan_and_rows(ops, rows, rank, slots, dtype, early):
+    """Nothing waits between the steps, whose plans lie at one address and whose rows are written over those of the step before."""
+    from inference_engine_b200 import kernels as K
+
+    ad, _, _, _ = make(ops, rows, 264, (264, 9), rank, slots, dtype, seed=rows)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    steps = [(torch.randint(-1, slots, (rows,), generator=g, device="cuda", dtype=torch.int32), torch.randn(rows, 264, generator=g, device="cuda").to(dtype),
+              torch.randn(rows, 273, generator=g, device="cuda").to(dtype)) for _ in range(12)]
+    want = []
+    for ids, x, y in steps:
+        once = ops.add_adapters(y, x, ad, ops.plan_adapters(ids, slots), out=torch.empty_like(y))
+        check(ad, ids, x, y, once)
+        h = once[:, :264].contiguous()
+        torch.cuda.synchronize()
+        want.append(ops.add_adapters(y, h, ad, ops.plan_adapters(ids, slots), out=torch.empty_like(y)))
+        torch.cuda.synchronize()
+    if early:
+        K.set_early_start(True)
+    try:
+        got, wide = [], torch.empty(rows, 280, dtype=dtype, device="cuda")[:, :273]
+        for ids, x, y in steps:
+            plan = ops.plan_adapters(ids, slots)
+            ops.add_adapters(y, x, ad, plan, out=wide)
+            got.append(ops.add_adapters(y, wide[:, :264], ad, plan, out=torch.empty_like(y)))
+            del plan
+    finally:
+        if early:
+            K.set_early_start(False)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
