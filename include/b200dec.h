@@ -306,9 +306,9 @@ int b200dec_adjust_logits(const void* logits, int64_t stride, int32_t elem, cons
 /* How the next token is drawn from adjusted logits: z = (largest - l) / temperature, w = exp(-z), tokens ordered by l, equal ones by index.  Kept are the
  * first top_k (0: all), of these the shortest run with top_p of their weight (1: all), of these the ones with w >= min_p (0: all, at most 1); the
  * largest always.  The token is the first by index at which the kept weights so far exceed uniform (in [0, 1)) times their sum.  temperature 0:
- * the largest logit, the first of equals.  NaN logits count as -inf.  Cuts count weights in steps of 2^-32 of the largest, and one among
- * tokens with z >= 31.98 drops all of those.  Where a cut falls among more than 1024 tokens of the same 32-bit distance from the largest,
- * those are in order of their index.  NULL: temperature 1 (uniform 0 with it) and nothing cut; temperature needs uniform. */
+ * the largest logit, the first of equals.  NaN logits count as -inf.  Weights are 32-bit numbers and top_p counts them in steps of 2^-32 of the largest:
+ * of tokens that have less than half a step either all are kept or none, and ones with less than 2^-80 of the largest may count as without weight.
+ * NULL: temperature 1 (uniform 0 with it) and nothing cut; temperature needs uniform. */
 typedef struct b200dec_draw {
   const float* temperature;
   const int32_t* top_k;

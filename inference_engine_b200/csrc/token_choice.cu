@@ -18,7 +18,9 @@
 // one addition a thread, gives a floor with at least k tokens above it and few more (64 of 151936: 64 to 83, 200: 202 to 400), where one of all tokens cost
 // an addition for each in reach.  One block takes the tokens above the floor from the others, which end, puts them in order and draws.  Where they are too many, or
 // the share of weight lies further out, a cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the
-// likelier tokens, or over the others if it does not lie there, down to the few tokens of one bin, which are sorted.  Blocks tell one another sums of bins, and
+// likelier tokens, or over the others if it does not lie there, down to the few tokens of one bin, which are sorted.  Bins are of z, or of what z would be at
+// a temperature of 64 where that is higher (else tokens in order would share one); where too many tokens share the
+// smallest, they are of the logits' own bits, ten at a time.  Blocks tell one another sums of bins, and
 // read from one another only the bins among which the cut lies.  A token of top-k of 64 requests took 42 us that way, and 25 by a floor.
 //
 // Precision: 32-bit logits and weights; a weight's integer is in steps of 2^-32 of the largest one, sums are in 64 bits.
@@ -390,26 +392,13 @@ struct TcRow {
   }
 };
 
-// A bin of places, and the last token that is kept: of all (exact: its logit and its column), or of the bin's (its column).
+// The last token that is kept: its logit and its column.
 struct TcCut {
-  bool on = false, exact = false;
+  bool on = false;
   float logit = 0.f;
   int at = 0;
-  float base = 0.f, scale = 1.f;
-  int bin = 0;
   float floor = -INFINITY;  // no token below it is kept
-  // -1: in front of the bin, 0: in it, 1: behind it.  Differences of nearby values and products with powers of two are exact.
-  __device__ __forceinline__ int side(float place) const {
-    const float x = (place - base) * scale;
-    if (!(x >= 0.f && x < (float)kTcBins)) return x < 0.f ? -1 : 1;
-    const int b = (int)x;
-    return b < bin ? -1 : b > bin;
-  }
-  __device__ __forceinline__ bool keeps(const TcRow& c, int i, float l) const {
-    if (!on) return true;
-    const int s = exact ? (l > logit ? -1 : l < logit) : side(c.place(l));
-    return s < 0 || (s == 0 && c.v0 + i <= at);
-  }
+  __device__ __forceinline__ bool keeps(const TcRow& c, int i, float l) const { return !on || l > logit || (l == logit && c.v0 + i <= at); }
 };
 
 // Tokens in order: the logit (not how far it is behind the largest, which rounding makes the same for some), then the column.
@@ -417,6 +406,7 @@ __device__ __forceinline__ unsigned long long tc_key(float l, int at) {
   const uint32_t u = __float_as_uint(__fadd_rn(l, 0.f));  // (one zero)
   return (unsigned long long)(u >> 31 ? u : ~u & 0x7fffffffu) << 32 | (uint32_t)at;
 }
+__device__ __forceinline__ uint32_t tc_key_of(float l) { return (uint32_t)(tc_key(l, 0) >> 32); }
 __device__ __forceinline__ float tc_key_logit(unsigned long long key) {
   const uint32_t u = (uint32_t)(key >> 32);
   return __uint_as_float(u >> 31 ? u : ~u & 0x7fffffffu);
@@ -450,6 +440,24 @@ __device__ __forceinline__ void tc_sort(unsigned long long* keys, int num) {
   __syncthreads();
 }
 
+// What a step of a selection tells apart: bins of places, or, where too many tokens are in the smallest, ten
+// bits of the logits' keys at a time, so that in the end only equal logits are in one bin.
+struct TcBins {
+  bool keys = false;
+  float base = 0.f, scale = kTcBins / 16.f;  // places
+  int shift = 22, bits = 10;                 // keys: of those that begin with `prefix`
+  uint32_t prefix = 0;
+  // the token's bin, or one outside [0, kTcBins).  Differences of nearby places and products with powers of two are exact.
+  __device__ __forceinline__ int of(const TcRow& c, float l) const {
+    if (keys) {
+      const uint32_t k = tc_key_of(l) >> shift;
+      return k >> bits == prefix ? (int)(k & ((1u << bits) - 1)) : -1;
+    }
+    const float x = (c.place(l) - base) * scale;
+    return x >= 0.f && x < (float)kTcBins ? (int)x : -1;
+  }
+};
+
 // Where the cut lies that keeps the first `k` tokens (kMass false), or the shortest run with `p` of the weight (kMass true), of those that `had` keeps;
 // off where nothing is cut.  By all threads of the cluster.  weighed: every block has told its tokens' weight.
 template <bool kMass>
@@ -457,11 +465,17 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
   constexpr int kWords = kMass ? 2 : 1;  // of a bin: its count, or its weight's halves
   TcMail& mail = *c.mail;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // z < 16, weights above 2^-16; then up to 80; then down into a bin
-  float base = 0.f, scale = kTcBins / 16.f, top = 16.f;
+  // places below 16; then up to 80; then down into a bin; then keys
+  TcBins bins;
+  float top = 16.f;
   int level = 0;
   unsigned long long before = 0;  // counts, or weights, in front of the bins
   double target = (double)k;
+  const auto by_keys = [&]() {
+    bins.keys = true;
+    before = 0;
+  };
+#pragma unroll 1
   for (bool first = true;; first = false) {
     const bool weigh = kMass && first && !weighed;
     __syncthreads();  // (what was found before has been read)
@@ -469,12 +483,12 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     if (tid == 0) mail.listed = 0;
     __syncthreads();
     float weight = 0.f;
-    c.each_above(weigh ? had.floor : fmaxf(had.floor, c.floor(top)), [&](int i, float l) {
-      const float z = c.z(l), x = (c.place(l) - base) * scale;
+    c.each_above(weigh || bins.keys ? had.floor : fmaxf(had.floor, c.floor(top)), [&](int i, float l) {
+      const float z = c.z(l);
+      const int b = bins.of(c, l);
       if (!had.keeps(c, i, l)) return;
       if (weigh) weight += tc_exp2(-z);
-      if (!(x >= 0.f && x < (float)kTcBins)) return;
-      const int b = (int)x;
+      if (b < 0) return;
       if (kMass) {
         const uint32_t q = c.steps(z);
         atomicAdd(&c.hist[b], q >> 16);
@@ -530,9 +544,9 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       before = __shfl_sync(0xffffffffu, upto, 31);
       tc_cluster_sync();  // (the blocks read this one's sums)
       // fewer tokens, or less weight, than would be kept; weights below 2^-80 do not count.  (A bin's parts have the bin's sums.)
-      if (base > 0.f) return TcCut();
-      base = 16.f;
-      scale = kTcBins / 64.f;
+      if (bins.keys || bins.base > 0.f) return TcCut();
+      bins.base = 16.f;
+      bins.scale = kTcBins / 64.f;
       top = 80.f;
       continue;
     }
@@ -546,13 +560,11 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     before = __shfl_sync(0xffffffffu, upto - sum, in_group);
     TcCut cut;
     cut.on = true;
-    cut.base = base;
-    cut.scale = scale;
-    cut.bin = bin;
-    cut.floor = c.floor(base + (float)(bin + 1) / scale);
+    const float bin_floor = bins.keys ? had.floor : c.floor(bins.base + (float)(bin + 1) / bins.scale);
+    const auto member = [&](int i, float l) { return bins.of(c, l) == bin && had.keeps(c, i, l); };
     // the bin's tokens: every block's own, then all of them where the histogram was
-    c.each_above(cut.floor, [&](int i, float l) {
-      if (cut.side(c.place(l)) != 0 || !had.keeps(c, i, l)) return;
+    c.each_above(bin_floor, [&](int i, float l) {
+      if (!member(i, l)) return;
       const uint32_t at = atomicAdd(&mail.listed, 1u);
       if (at >= (uint32_t)kTcMembers) return;
       c.list_l[at] = l;
@@ -593,23 +605,29 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
         __syncthreads();
       }
       const unsigned long long key = kMass ? mail.cut : keys[k - (uint32_t)before - 1];
-      cut.exact = true;
-      cut.logit = tc_key_logit(key);
+      cut.logit = cut.floor = tc_key_logit(key);
       cut.at = (int)(uint32_t)key;
       return cut;
     }
-    if (level < 2) {
+    if (!bins.keys || bins.shift > 0) {
       tc_cluster_sync();  // (the blocks read this one's bins)
-      top = base + (float)(bin + 1) / scale;
-      base += (float)bin / scale;
-      scale *= (float)kTcBins;
-      ++level;
+      if (bins.keys) {  // bits 31 to 22, 21 to 12, 11 to 2, 1 and 0
+        bins.prefix = bins.prefix << bins.bits | (uint32_t)bin;
+        bins.bits = bins.shift < 10 ? bins.shift : 10;
+        bins.shift -= bins.bits;
+      } else if (level < 2) {
+        top = bins.base + (float)(bin + 1) / bins.scale;
+        bins.base += (float)bin / bins.scale;
+        bins.scale *= (float)kTcBins;
+        ++level;
+      } else {
+        by_keys();
+      }
       continue;
     }
-    // more tokens than that at the same distance, in 32 bits, from the largest: by index
+    // more equal logits than that: by index
     uint32_t want = k - (uint32_t)before;
     if (kMass) want = (uint32_t)fmin(fmax(ceil((target - (double)before) * members / fmax((double)in_bin, 1.)), 1.), (double)members);
-    const auto member = [&](int i, float l) { return cut.side(c.place(l)) == 0 && had.keeps(c, i, l); };
     uint32_t mine = 0;
     c.each([&](int i, float l) { mine += member(i, l); });
     mine = tc_warp_sum(mine);
@@ -637,6 +655,7 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
       }
     }
     tc_cluster_sync();
+    cut.logit = cut.floor = tc_key_logit((unsigned long long)(bins.prefix << bins.bits | (uint32_t)bin) << 32);
     cut.at = mail.cut_at;
     return cut;
   }

@@ -423,3 +423,19 @@ def test_empty_batch(ops):
     tokens, logprobs = ops.choose_tokens(torch.zeros(0, 100, device="cuda"), draw)
     assert tokens.shape == logprobs.shape == (0,)
     assert ops.adjust_logits(torch.zeros(0, 100, device="cuda"), ops.Rules()).shape == (0, 100)
+
+
+@pytest.mark.parametrize("V", [1500, 6000, 60000])
+@pytest.mark.parametrize("tau", [0.9, 40.0, 900.0])
+@pytest.mark.parametrize("values", ["different", "few", "signs"])
+def test_more_logits_side_by_side_than_are_sorted_at_once(ops, V, tau, values):
+    """Thousands of logits within 1e-8 of the largest keep their order, and equal ones that of their index."""
+    g = torch.Generator().manual_seed(V + 2)
+    E = 24
+    l = {"different": torch.stack([torch.randperm(V, generator=g) for _ in range(E)]).float() * (1e-8 / V), "few": torch.randint(0, 3, (E, V), generator=g) * 1e-10,
+         "signs": torch.randn(E, V, generator=g) * 1e-10}[values].to("cuda")
+    k = torch.tensor([1100, 2, 37, 500, 1400, 0, 0, 0] * 3).to(torch.int32)
+    p = torch.tensor([1.0, 1.0, 1.0, 1.0, 0.5, 0.9, 0.5, 0.01] * 3)
+    draw = ops.Draw(torch.full((E,), tau, device="cuda"), cuda(torch.rand(E, generator=g)), cuda(k), cuda(p))
+    tokens, logprobs = ops.choose_tokens(l, draw)
+    check_choice(l, draw, tokens, logprobs)
