@@ -19,7 +19,7 @@
 // an addition for each in reach.  One block takes the tokens above the floor from the others, which end, puts them in order and draws.  Where they are too many, or
 // the share of weight lies further out, a cut is found by a histogram of z (counts, and weights as integers, so that no order of additions matters) over the
 // likelier tokens, or over the others if it does not lie there, down to the few tokens of one bin, which are sorted.  Bins are of z, or of what z would be at
-// a temperature of 64 where that is higher (else tokens in order would share one); where too many tokens share the
+// a temperature of 64 where that is higher (else tokens in order would share one); where they do not reach a cut, or too many tokens share the
 // smallest, they are of the logits' own bits, ten at a time.  Blocks tell one another sums of bins, and
 // read from one another only the bins among which the cut lies.  A token of top-k of 64 requests took 42 us that way, and 25 by a floor.
 //
@@ -440,7 +440,7 @@ __device__ __forceinline__ void tc_sort(unsigned long long* keys, int num) {
   __syncthreads();
 }
 
-// What a step of a selection tells apart: bins of places, or, where too many tokens are in the smallest, ten
+// What a step of a selection tells apart: bins of places, or, where those do not (tokens further behind than they reach, too many in the smallest bin), ten
 // bits of the logits' keys at a time, so that in the end only equal logits are in one bin.
 struct TcBins {
   bool keys = false;
@@ -543,11 +543,15 @@ __device__ __forceinline__ TcCut tc_select(const TcRow& c, uint32_t k, float p, 
     if (!hit) {
       before = __shfl_sync(0xffffffffu, upto, 31);
       tc_cluster_sync();  // (the blocks read this one's sums)
-      // fewer tokens, or less weight, than would be kept; weights below 2^-80 do not count.  (A bin's parts have the bin's sums.)
-      if (bins.keys || bins.base > 0.f) return TcCut();
-      bins.base = 16.f;
-      bins.scale = kTcBins / 64.f;
-      top = 80.f;
+      // Fewer tokens, or less weight, than would be kept.  (A bin's parts have the bin's sums.)  Places that are weights: those below 2^-80 do not count.
+      if (bins.keys || (bins.base > 0.f && c.apart == c.unit)) return TcCut();
+      if (bins.base > 0.f) {
+        by_keys();
+      } else {
+        bins.base = 16.f;
+        bins.scale = kTcBins / 64.f;
+        top = 80.f;
+      }
       continue;
     }
     const int group = __ffs(hit) - 1;
@@ -928,7 +932,7 @@ choose_tokens_kernel(const T* logits, long long stride, const TcRules r, const T
     // every block finds out whether the cuts lie among them (the first k's weights are, if the first k are)
     uint32_t num = 0;
     for (int q = 0; q < c.blocks; ++q) num += mail.likely[q];
-    bool ok = num > 0 && num <= (uint32_t)kTcShort && (!some || num >= (uint32_t)k || reach >= 127.f);  // (weights below 2^-80 do not count)
+    bool ok = num > 0 && num <= (uint32_t)kTcShort && (!some || num >= (uint32_t)k || (reach >= 127.f && c.apart == c.unit));  // (weights below 2^-80 do not count)
     double target = INFINITY;
     if (by_share) {
       double of = 0.;

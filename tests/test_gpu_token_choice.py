@@ -425,6 +425,26 @@ def test_empty_batch(ops):
     assert ops.adjust_logits(torch.zeros(0, 100, device="cuda"), ops.Rules()).shape == (0, 100)
 
 
+@pytest.mark.parametrize("V", [700, 5000, 60000])
+@pytest.mark.parametrize("tau", [65.0, 1e3, 5e3, 1e7, math.inf])
+@pytest.mark.parametrize("values", ["ahead", "spread", "steps", "two"])
+def test_cuts_at_high_temperatures_among_tokens_far_apart(ops, V, tau, values):
+    """At a high temperature tokens thousands behind the largest weigh nearly as much: they count in every cut."""
+    g = torch.Generator().manual_seed(V + 1)
+    E = 30
+    l = {"ahead": torch.randn(E, V, generator=g), "spread": torch.rand(E, V, generator=g) * 2e5, "steps": -4000.0 * torch.randint(0, 9, (E, V), generator=g),
+         "two": torch.randint(0, 2, (E, V), generator=g) * 6e3}[values]
+    if values == "ahead":
+        l[torch.arange(E), torch.randint(0, V, (E,), generator=g)] = 1e4
+    l = l.to("cuda")
+    k = torch.tensor([50, 7, 383, 384, 385, 600, 2, 0, 0, 0] * 3).to(torch.int32)
+    p = torch.tensor([1.0] * 7 + [0.5, 0.01, 0.97] + [0.5] * 7 + [0.999, 0.3, 0.8] + [0.9] * 10)
+    m = torch.tensor([0.0] * 20 + [0.4, 1e-3] * 5)
+    draw = ops.Draw(torch.full((E,), tau, device="cuda"), cuda(torch.rand(E, generator=g)), cuda(k), cuda(p), cuda(m))
+    tokens, logprobs = ops.choose_tokens(l, draw)
+    check_choice(l, draw, tokens, logprobs)
+
+
 @pytest.mark.parametrize("V", [1500, 6000, 60000])
 @pytest.mark.parametrize("tau", [0.9, 40.0, 900.0])
 @pytest.mark.parametrize("values", ["different", "few", "signs"])
