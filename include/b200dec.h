@@ -318,8 +318,8 @@ typedef struct b200dec_draw {
 } b200dec_draw;
 
 /* tokens[e], and logprobs[e], its logarithmic probability under the softmax of all adjusted logits (temperature 1).  -1 and -inf where every token is
- * masked or the entry is passed over.  rules may be NULL.  append: the token is put behind the entry's history if there is room (and lengths are the
- * caller's to count on); entries then have rows of their own.  vocab up to 393216. */
+ * masked or the entry is passed over.  rules may be NULL.  append: the token is put behind the entry's history if its length is none below zero and there
+ * is room (and lengths are the caller's to count on); entries then have rows of their own.  vocab up to 393216. */
 int b200dec_choose_tokens(const void* logits, int64_t stride, int32_t elem, const b200dec_rules* rules, const b200dec_draw* draw, int32_t entries,
                           int32_t vocab, int32_t append, int64_t* tokens, float* logprobs, int32_t* status, void* stream);
 

@@ -72,8 +72,8 @@ __device__ __forceinline__ TcEntry tc_entry(const TcRules& r, int e, bool report
     t.length = 0;
   } else {
     if (t.length < 0 || t.length > r.capacity || t.prompt < 0) bad = true;
+    if (t.length >= 0) t.history = r.history + (long long)t.slot * r.capacity;  // (nothing is appended behind a length that is none)
     t.length = max(0, min(t.length, r.capacity));
-    t.history = r.history + (long long)t.slot * r.capacity;
   }
   t.penalties = t.length > 0 && (t.repetition != 1.f || t.presence != 0.f || t.frequency != 0.f);
   t.mask = nullptr;

@@ -372,6 +372,23 @@ def test_tokens_are_appended(ops):
     assert torch.equal(history, before)  # the third is passed over, the fourth has no room
 
 
+@pytest.mark.parametrize("tau", [0.0, 0.7])
+def test_nothing_is_appended_behind_a_length_out_of_range(ops, tau):
+    from inference_engine_b200 import kernels as K
+
+    E, V, cap = 4, 600, 9
+    i32 = dict(dtype=torch.int32, device="cuda")
+    history = torch.arange(E * cap, **i32).view(E, cap)
+    want = history.clone()
+    rules = ops.Rules(history=history, lengths=torch.tensor([-1, cap + 1, 3, -(1 << 31)], **i32))
+    draw = ops.Draw(torch.full((E,), tau, device="cuda"), torch.full((E,), 0.4, device="cuda"), torch.full((E,), 5, **i32))
+    K.check_status()
+    tokens, _ = ops.choose_tokens(make_logits(E, V, torch.float32, torch.Generator().manual_seed(3)), draw, rules, append=True)
+    assert K.check_status() == 2
+    want[2, 3] = tokens[2]
+    assert torch.equal(history, want) and (tokens >= 0).all()
+
+
 def test_many_biases_and_a_long_history_of_one_token(ops):
     E, V = 3, 151936
     g = torch.Generator().manual_seed(5)
