@@ -49,8 +49,8 @@ MOST_FLOAT, LEAST_FLOAT = (2 - 2.0 ** -23) * 2.0 ** 127, 2.0 ** -126  # of 32 bi
 @dataclass(frozen=True)
 class Sampling:
     """How one request's tokens are chosen (ops.Draw, ops.Rules): by default the most likely one.  bias: token -> what is added to its logit.
-    grammar: called with the output so far, returns the row of the engine's masks for the next token, -1: none.  seed: of the request's random
-    numbers (default: the engine's and the request's number)."""
+    grammar: called with the output so far, returns the row of the engine's masks for the next token, -1: none; if it raises or there is no such
+    row, the request ends with that error.  seed: of the request's random numbers (default: the engine's and the request's number)."""
 
     temperature: float = 0.0
     top_k: int = 0
@@ -86,6 +86,7 @@ class Request:
     adapter: int = -1
     history: int = -1  # row of the engine's token histories, for requests with a way of sampling
     rng: object = None
+    error: Exception | None = None  # what its grammar ended it with
     admitted: bool = False
     t_submit: float = 0.0
     t_first_token: float | None = None
@@ -147,6 +148,7 @@ class SlotPool:
 class Step:
     entries: list[tuple[Request, list[int]]]  # decoding requests first (one token each), then prefill chunks
     num_decoding: int
+    masks: dict[int, int] = field(default_factory=dict)  # request id -> the mask that its grammar asks for
 
     @property
     def decode_only(self) -> bool:
@@ -239,18 +241,21 @@ class Scheduler:
                     if len(r.output) == 1:
                         r.t_first_token = now
                 if none or tok == self.stop_token_id or len(r.output) >= r.max_new_tokens or r.cached_len + 1 >= self.max_len:
-                    self.pool.release(r.pages, r.committed)
-                    r.pages, r.committed = [], 0
-                    if self.histories is not None:
-                        self.histories.release(r.history)
-                        r.history = -1
-                    if self.slots is not None:
-                        self.slots.release(r.slot)
-                        r.slot = -1
-                    self.running.remove(r)
-                    r.t_finish = now
+                    self.end(r, now)
                     finished.append(r)
         return finished
+
+    def end(self, r: Request, now: float) -> None:
+        self.pool.release(r.pages, r.committed)
+        r.pages, r.committed = [], 0
+        if self.histories is not None:
+            self.histories.release(r.history)
+            r.history = -1
+        if self.slots is not None:
+            self.slots.release(r.slot)
+            r.slot = -1
+        self.running.remove(r)
+        r.t_finish = now
 
 
 class Engine:
@@ -372,10 +377,11 @@ class Engine:
         step = self.sched.plan()
         if step is None:
             return []
+        finished = self.ask_grammars(step)
         t1 = time.perf_counter()
-        tokens = self.run(step).tokens[: len(step.entries)].tolist()  # the read-back ends the step
+        tokens = self.run(step).tokens[: len(step.entries)].tolist() if step.entries else []  # the read-back ends the step
         t2 = time.perf_counter()
-        finished = self.sched.commit(step, tokens)
+        finished += self.sched.commit(step, tokens)
         for r in finished:
             self.rows.pop(r.id, None)
         self.seconds["plan"] += t1 - t0
@@ -454,6 +460,34 @@ class Engine:
             n += (len(self.SAMPLING_INTS) + len(self.SAMPLING_FLOATS) + 2 * self.max_bias) * entries
         return n
 
+    def wants_token(self, r: Request, toks: list[int]) -> bool:
+        return r.history >= 0 and r.cached_len + len(toks) >= len(r.prompt_ids)
+
+    def mask_of(self, r: Request) -> int:
+        grammar = None if r.sampling is None else r.sampling.grammar
+        mask = -1 if grammar is None else int(grammar(r.output))
+        if not -1 <= mask < self.masks.shape[0]:
+            raise ValueError(f"request {r.id}: its grammar asks for mask {mask} of {self.masks.shape[0]}")
+        return mask
+
+    def ask_grammars(self, step: Step) -> list[Request]:
+        """The masks of the step's requests, before anything of it is done: a request whose grammar fails ends, and the others have their step."""
+        failed = []
+        for r, toks in step.entries:
+            if r.sampling is None or r.sampling.grammar is None or not self.wants_token(r, toks):
+                continue
+            try:
+                step.masks[r.id] = self.mask_of(r)
+            except Exception as e:
+                r.error = e
+                failed.append(r)
+        for r in failed:
+            at = next(i for i, (q, _) in enumerate(step.entries) if q is r)
+            step.num_decoding -= at < step.num_decoding
+            del step.entries[at]
+            self.sched.end(r, time.perf_counter())
+        return failed
+
     def fill_asks(self, buf, step: Step, entries: int, rows: int) -> None:
         """What the step's requests ask, into its part of the host buffer."""
         np, at = self.np, 0
@@ -475,15 +509,13 @@ class Engine:
         plain = Sampling()
         places, own_ints, own_floats = [], [], []
         for e, (r, toks) in enumerate(step.entries):
-            if r.history < 0 or r.cached_len + len(toks) < len(r.prompt_ids):
+            if not self.wants_token(r, toks):
                 continue
             if not r.output:  # the first token comes next: its history is the prompt
                 host = self.torch.tensor(r.prompt_ids, dtype=self.torch.int32).pin_memory()
                 self.history[r.history, : len(host)].copy_(host, non_blocking=True)
             s = r.sampling or plain
-            mask = -1 if s.grammar is None else int(s.grammar(r.output))
-            if not -1 <= mask < self.masks.shape[0]:
-                raise ValueError(f"request {r.id}: its grammar asks for mask {mask} of {self.masks.shape[0]}")
+            mask = step.masks[r.id] if r.id in step.masks else self.mask_of(r)
             places.append(e)
             own_ints.append((r.history, len(r.prompt_ids) + len(r.output), len(r.prompt_ids), mask, s.top_k))
             own_floats.append((s.repetition, s.presence, s.frequency, s.temperature, s.top_p, s.min_p, r.rng.random()))

@@ -274,3 +274,24 @@ def test_command_line(tmp_path):
     greedy = run()
     assert run("--top-k", "1", "--tau", "1.0") == greedy
     assert len(run("--tau", "0.9", "--top-p", "0.9", "--repetition-penalty", "1.3", "--frequency-penalty", "0.1", "--presence-penalty", "0.1", "--min-p", "0.01")) == 4
+
+
+@pytest.mark.parametrize("use_graphs", [False, True])
+def test_a_grammar_that_fails_ends_its_request_and_no_other(use_graphs):
+    from inference_engine_b200.engine import Sampling
+
+    def outputs(grammar):
+        eng = build(scaffold(), use_graphs, own_sampling=True, seed=4)
+        reqs = [eng.submit_request(p, 6, Sampling(temperature=1.0, top_k=9, grammar=grammar if i == 1 else None)) for i, p in enumerate(prompts()[:4])]
+        while not eng.sched.idle():
+            eng.step()
+        assert eng.pool.uncommitted() == eng.pool.capacity and eng.sched.histories.free == [3, 2, 1, 0]
+        return reqs
+
+    def failing(out):
+        return -1 if len(out) < 2 else 1 // 0
+
+    whole, cut = outputs(lambda out: -1), outputs(failing)
+    assert isinstance(cut[1].error, ZeroDivisionError) and cut[1].output == whole[1].output[:2]
+    assert [r.output for i, r in enumerate(cut) if i != 1] == [r.output for i, r in enumerate(whole) if i != 1]
+    status_clear()

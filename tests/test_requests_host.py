@@ -225,3 +225,73 @@ def test_a_step_s_fields():
     eng.own_sampling = True
     with pytest.raises(ValueError):
         eng.fill_asks(np.zeros(eng.asks_size(6, 8), np.int32), Step([(first, [9])], 1), 6, 8)
+
+
+def host_engine(max_batch=3):
+    """An engine whose steps run on the host: a request's next token is its random number in thousandths."""
+    from types import SimpleNamespace
+
+    from inference_engine_b200.engine import Engine
+
+    class OnHost(Engine):
+        def __init__(self):
+            self.np, self.torch, self.model, self.tau = np, torch, SimpleNamespace(vocab=1000), 0.0
+            self.own_sampling, self.max_bias, self.adapter_slots, self.seed = True, 2, 0, 9
+            self.history, self.masks = torch.zeros(max_batch, 64, dtype=torch.int32), torch.full((2, 32), -1, dtype=torch.int32)
+            self.pool = PagePool(64)
+            self.sched = Scheduler(max_batch, 64, 16, self.pool, 24, 8, -1, None, SlotPool(max_batch))
+            self.rows, self.steps, self.seconds = {}, [], {"plan": 0.0, "run (inputs, launch, read-back)": 0.0, "commit": 0.0}
+
+        def run(self, step):
+            assert step.entries and [r.decoding for r, _ in step.entries] == [i < step.num_decoding for i in range(len(step.entries))]
+            self.steps.append([r.id for r, _ in step.entries])
+            n = len(step.entries)
+            buf = np.zeros(self.asks_size(n, 8), np.int32)
+            self.fill_asks(buf, step, n, 8)
+            return SimpleNamespace(tokens=(self.asks_views(torch.from_numpy(buf), n, 8)["asks"].draw.uniform * 1000).long())
+
+    return OnHost()
+
+
+@pytest.mark.parametrize("when,how", [(0, "raise"), (2, "raise"), (0, "row"), (3, "row")])
+def test_a_grammar_that_fails_ends_its_own_request(monkeypatch, when, how):
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
+
+    def grammar(out):
+        if len(out) == when:
+            if how == "raise":
+                raise KeyError("no such state")
+            return 2
+        return len(out) % 2
+
+    prompts, sampling = [[1, 2], [3] * 20, [4], [5, 6, 7]], Sampling(temperature=1.0)
+    alone = []
+    for i, p in enumerate(prompts):
+        eng = host_engine()
+        eng.sched.next_id = i
+        alone.append(eng.generate([p], 6, sampling)[0].output)
+    eng = host_engine()
+    for p in prompts:
+        eng.submit_request(p, 6, sampling)
+    bad = eng.sched.waiting[2]
+    bad.sampling = Sampling(temperature=1.0, grammar=grammar)
+    reqs, ended = list(eng.sched.waiting), []
+    for _ in range(40):
+        ended += eng.step()
+    assert eng.sched.idle() and sorted(r.id for r in ended) == [0, 1, 2, 3]
+    assert isinstance(bad.error, KeyError if how == "raise" else ValueError) and bad.t_finish is not None
+    assert [r.output for r in reqs] == [a[:when] if i == 2 else a for i, a in enumerate(alone)]
+    assert all(r.error is None for r in reqs if r is not bad)
+    assert eng.pool.uncommitted() == eng.pool.capacity and eng.sched.histories.free == [2, 1, 0] and not eng.rows
+
+
+def test_a_step_of_requests_that_all_fail(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
+    eng = host_engine()
+    reqs = [eng.submit_request([1], 3, Sampling(grammar=lambda out: 7)) for _ in range(4)]
+    assert {r.id for r in eng.step()} == {0, 1, 2} and eng.steps == [] and eng.step() == [reqs[3]] and eng.step() == [] and eng.sched.idle()
+    calls = []
+    r = eng.submit_request([1, 2, 3], 4, Sampling(grammar=lambda out: calls.append(list(out)) or 0))
+    while not eng.sched.idle():
+        eng.step()
+    assert len(r.output) == 4 and calls == [r.output[:n] for n in range(4)]  # once for each token
