@@ -261,7 +261,7 @@ class Scheduler:
 class Engine:
     """Scheduler + device execution.  `model`: an instance of a registered model class on a CUDA device.  `num_slots`: state
     slots of a stateful model, one per live request (default: one per request of the largest batch).  `own_sampling`: requests may have a
-    Sampling of their own (the others take the most likely token; tau is for engines without), of up to `max_bias` biased tokens, under grammars of
+    Sampling of their own (the others are drawn at the temperature tau, as in engines without), of up to `max_bias` biased tokens, under grammars of
     up to `num_masks` masks (set_mask).  `adapters`: requests may name a slot of the model's adapters (model.make_adapters before)."""
 
     slots: SlotPool | None = None
@@ -300,7 +300,7 @@ class Engine:
         self.pool = PagePool(num_pages, first=self.scratch_pages)
         if getattr(model, "stateful", False):
             self.slots = SlotPool(max_batch_size if num_slots is None else num_slots)
-        self.own_sampling, self.max_bias, self.seed = own_sampling, max_bias, seed
+        self.own_sampling, self.max_bias, self.seed, self.tau = own_sampling, max_bias, seed, float(tau)
         self.adapter_slots = 0
         if adapters:
             if getattr(model, "adapters", None) is None:
@@ -348,6 +348,8 @@ class Engine:
         if self.own_sampling and any(not 0 <= t < self.model.vocab for t in prompt_ids):
             raise ValueError(f"a prompt has ids outside 0 .. {self.model.vocab - 1}")
         r = self.sched.submit(prompt_ids, max_new_tokens)
+        if sampling is None and self.own_sampling and self.tau > 0:
+            sampling = Sampling(self.tau)
         r.sampling, r.adapter = sampling, adapter
         if self.own_sampling:
             s = sampling.seed if sampling is not None else None

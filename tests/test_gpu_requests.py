@@ -295,3 +295,13 @@ def test_a_grammar_that_fails_ends_its_request_and_no_other(use_graphs):
     assert isinstance(cut[1].error, ZeroDivisionError) and cut[1].output == whole[1].output[:2]
     assert [r.output for i, r in enumerate(cut) if i != 1] == [r.output for i, r in enumerate(whole) if i != 1]
     status_clear()
+
+
+@pytest.mark.parametrize("use_graphs", [False, True])
+def test_the_engine_s_temperature_is_that_of_requests_without_their_own(use_graphs):
+    from inference_engine_b200.engine import Sampling
+
+    def outputs(sampling, **kw):
+        return [r.output for r in build(scaffold(), use_graphs, own_sampling=True, seed=2, **kw).generate(prompts()[:3], 6, sampling)]
+
+    assert outputs(None, tau=1.5) == outputs(Sampling(1.5)) != outputs(None) == outputs(Sampling(), tau=1.5)

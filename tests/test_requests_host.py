@@ -295,3 +295,13 @@ def test_a_step_of_requests_that_all_fail(monkeypatch):
     while not eng.sched.idle():
         eng.step()
     assert len(r.output) == 4 and calls == [r.output[:n] for n in range(4)]  # once for each token
+
+
+def test_requests_without_a_way_of_sampling_have_the_engine_s_temperature():
+    eng = host_engine()
+    assert eng.submit_request([1], 2).sampling is None
+    eng.tau = 0.75
+    r, own = eng.submit_request([1], 2), eng.submit_request([1], 2, Sampling())
+    assert r.sampling == Sampling(0.75) and own.sampling.temperature == 0
+    eng.own_sampling = False  # the sampler that all requests share
+    assert eng.submit_request([1], 2).sampling is None
