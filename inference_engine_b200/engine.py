@@ -38,6 +38,7 @@ from __future__ import annotations
 
 import math
 import time
+import traceback
 from collections import deque
 from collections.abc import Callable
 from dataclasses import dataclass, field
@@ -95,6 +96,16 @@ class Request:
     @property
     def decoding(self) -> bool:
         return self.cached_len >= len(self.prompt_ids)
+
+
+def without_frames(e: Exception) -> Exception:
+    """The exception with its traceback as text: the frames would keep the engine, its cache and its graphs alive as long as the request."""
+    e.add_note("".join(traceback.format_exception(e)))
+    at = e
+    while at is not None:
+        at.__traceback__ = None
+        at = at.__cause__ or at.__context__
+    return e
 
 
 class PagePool:
@@ -481,7 +492,7 @@ class Engine:
             try:
                 step.masks[r.id] = self.mask_of(r)
             except Exception as e:
-                r.error = e
+                r.error = without_frames(e)
                 failed.append(r)
         for r in failed:
             at = next(i for i, (q, _) in enumerate(step.entries) if q is r)

@@ -285,6 +285,29 @@ def test_a_grammar_that_fails_ends_its_own_request(monkeypatch, when, how):
     assert eng.pool.uncommitted() == eng.pool.capacity and eng.sched.histories.free == [2, 1, 0] and not eng.rows
 
 
+def test_a_failed_request_keeps_no_engine_alive():
+    import gc
+    import weakref
+
+    def grammar(out):
+        try:
+            raise KeyError("first")
+        except KeyError:
+            raise LookupError("then")
+
+    eng = host_engine()
+    r = eng.submit_request([1], 3, Sampling(grammar=grammar))
+    alive = weakref.ref(eng)
+    gc.disable()
+    try:
+        assert eng.step() == [r]
+        del eng
+        assert alive() is None
+    finally:
+        gc.enable()
+    assert isinstance(r.error, LookupError) and "in grammar" in r.error.__notes__[0] and "first" in r.error.__notes__[0]
+
+
 def test_a_step_of_requests_that_all_fail(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
     eng = host_engine()
