@@ -273,7 +273,7 @@ class Engine:
     """Scheduler + device execution.  `model`: an instance of a registered model class on a CUDA device.  `num_slots`: state
     slots of a stateful model, one per live request (default: one per request of the largest batch).  `own_sampling`: requests may have a
     Sampling of their own (the others are drawn at the temperature tau, as in engines without), of up to `max_bias` biased tokens, under grammars of
-    up to `num_masks` masks (set_mask).  `adapters`: requests may name a slot of the model's adapters (model.make_adapters before)."""
+    up to `num_masks` masks (set_mask).  `adapters`: requests may name a slot of the model's adapters (model.make_adapters before, and not again)."""
 
     slots: SlotPool | None = None
     # what an entry's sampling comes to on the device, an array each, int32 and then fp32
@@ -312,10 +312,11 @@ class Engine:
         if getattr(model, "stateful", False):
             self.slots = SlotPool(max_batch_size if num_slots is None else num_slots)
         self.own_sampling, self.max_bias, self.seed, self.tau = own_sampling, max_bias, seed, float(tau)
-        self.adapter_slots = 0
+        self.adapter_slots, self.adapters = 0, None
         if adapters:
             if getattr(model, "adapters", None) is None:
                 raise ValueError("the model has no slots for adapters: make_adapters comes first")
+            self.adapters = model.adapters  # (the recorded steps read these)
             self.adapter_slots = next(iter(model.adapters[0].values())).slots
         if own_sampling:
             if max_bias < 0 or num_masks < 1:
@@ -674,6 +675,8 @@ class Engine:
 
     def run(self, step: Step):
         """Execute a planned step; the outputs' first entries / rows are the step's own."""
+        if self.adapters is not None and self.model.adapters is not self.adapters:
+            raise RuntimeError("the model was given other slots for adapters than the engine was made with")
         return self.run_decode(step) if step.decode_only else self.run_mixed(step)
 
     def run_decode(self, step: Step):

@@ -305,3 +305,24 @@ def test_the_engine_s_temperature_is_that_of_requests_without_their_own(use_grap
         return [r.output for r in build(scaffold(), use_graphs, own_sampling=True, seed=2, **kw).generate(prompts()[:3], 6, sampling)]
 
     assert outputs(None, tau=1.5) == outputs(Sampling(1.5)) != outputs(None) == outputs(Sampling(), tau=1.5)
+
+
+@pytest.mark.parametrize("use_graphs", [False, True])
+def test_slots_made_anew_behind_the_engine_s_back_are_refused(use_graphs):
+    """Recorded steps would read memory that the old slots had."""
+    model = scaffold()
+    model.make_adapters(3, 8)
+    eng = build(model, use_graphs, adapters=True)
+    fill(model, 1, 5)
+    want = eng.generate([[1, 2, 3]], 3, adapter=1)[0].output
+    old = model.adapters
+    model.make_adapters(1, 8)
+    eng.submit_request([1, 2, 3], 3, adapter=1)
+    with pytest.raises(RuntimeError, match="slots"):
+        eng.step()
+    model.adapters = old
+    r, = eng.sched.running
+    while not eng.sched.idle():
+        eng.step()
+    assert r.output == want
+    status_clear()
