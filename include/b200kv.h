@@ -242,6 +242,9 @@ int b200kv_skinny_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
  * in the reference. */
 void b200kv_set_chained_launch(int enabled);
 int b200kv_get_chained_launch(void);
+/* Whether kernels that read nothing at all before their wait (adapters, rules on logits, the choice of tokens) are chained where nothing is
+ * recorded, and the adapters' second product behind its first anywhere: until b200kv_set_chained_launch(0) says no. */
+int b200kv_get_early_launch(void);
 
 /* Calls that do not need one another, side by side in a graph that `stream` records: what is enqueued between _begin and
  * _next, between one _next and another, and between the last of them and _end forms a branch each.  All start behind what the stream held

@@ -142,6 +142,7 @@ SIGNATURES = {
                                        c_int32, c_void_p, c_void_p]),
     "b200kv_set_chained_launch": (None, [c_int32]),
     "b200kv_get_chained_launch": (c_int32, []),
+    "b200kv_get_early_launch": (c_int32, []),
     "b200kv_plain_next": (None, [c_void_p]),
     "b200kv_branches_begin": (c_void_p, [c_void_p]),
     "b200kv_branches_next": (c_int32, [c_void_p]),
@@ -214,11 +215,12 @@ DECODER_SIGNATURES = {
     "b200dec_choose_tokens": (c_int32, [c_void_p, c_int64, c_int32, P_RULES, P_DRAW, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                         c_void_p]),
 }
-SHARED_SIGNATURES = ("b200kv_version", "b200kv_error_string", "b200kv_set_chained_launch", "b200kv_get_chained_launch",
+SHARED_SIGNATURES = ("b200kv_version", "b200kv_error_string", "b200kv_set_chained_launch", "b200kv_get_chained_launch", "b200kv_get_early_launch",
                      "b200kv_plain_next", "b200kv_branches_begin", "b200kv_branches_next", "b200kv_branches_end", "b200kv_sample_workspace_bytes", "b200kv_sample")
 
 _lib = None
 _decoder_lib = None
+chained: bool | None = None  # what kernels.set_early_start said, for a library that is loaded later
 
 
 class B200KVError(RuntimeError):
@@ -271,6 +273,8 @@ def load_decoder() -> C.CDLL:
         getattr(lib, name).restype, getattr(lib, name).argtypes = SIGNATURES[name]
     for name, (res, args) in DECODER_SIGNATURES.items():
         getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
+    if chained is not None:
+        lib.b200kv_set_chained_launch(int(chained))
     _decoder_lib = lib
     return lib
 

@@ -7,8 +7,8 @@
 #include <new>
 
 namespace b200kv {
-static std::atomic<int> g_chained{0};
-static bool chained() { return g_chained.load(std::memory_order_relaxed) != 0; }
+static std::atomic<int> g_chained{-1};  // 1: on, 0: off, -1: nobody has said
+static bool chained() { return g_chained.load(std::memory_order_relaxed) > 0; }
 
 // A recording stream's place in its graph is the set of nodes that the next one will wait for: up to `room` of them to `to`;
 // -1: not recording, or more than that.
@@ -120,6 +120,7 @@ extern "C" int b200kv_branches_end(void* branches) {
 
 extern "C" void b200kv_set_chained_launch(int enabled) { b200kv::g_chained.store(enabled ? 1 : 0, std::memory_order_relaxed); }
 extern "C" int b200kv_get_chained_launch(void) { return b200kv::chained() ? 1 : 0; }
+extern "C" int b200kv_get_early_launch(void) { return b200kv::g_chained.load(std::memory_order_relaxed) != 0 ? 1 : 0; }
 
 extern "C" void b200kv_plain_next(void* stream) { b200kv::mark_place((cudaStream_t)stream); }
 

@@ -1091,8 +1091,8 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     const size_t second = 1024 + (size_t)a.blocks * 16384 + (size_t)2 * ublocks * kAdTcCols * 128;
     auto kernel = adapter_second_kernel;
     if (!allow_smem(kernel, kAdMostSmem)) return launch_result(cudaErrorInvalidValue);
-    // brought up while the first one runs, whatever launches of the library are: it waits for it, and nothing else stands between them
-    return launch_result(launch_kernel(true, kernel, grid, dim3(kAdSecondThreads), second, s, a));
+    // brought up while the first one runs, also in recorded steps: it waits for it, and nothing else stands between them
+    return launch_result(launch_kernel(b200kv_get_early_launch() != 0, kernel, grid, dim3(kAdSecondThreads), second, s, a));
   }
   const int kb = (a.rank + 15) / 16;
   const long long used = ad_used(ad, plan);

@@ -46,7 +46,8 @@ inline CacheView make_view(const b200kv_cache* c, const b200kv_table* t) {
 // before it on the stream (pdl_wait) before it reads anything that kernel may have written or writes global
 // memory itself, having read at most caller-provided metadata by then (and weights where b200kv_set_chained_launch says so), and (b) tells the stream when the next
 // kernel may be brought up (pdl_trigger).  Both are no-ops for a kernel launched the ordinary way; the launch
-// attribute is only set while b200kv_set_chained_launch(1) is in force.
+// attribute is only set while b200kv_set_chained_launch(1) is in force, or, by kernels that read nothing before their wait, until it is forbidden
+// (b200kv_get_early_launch).
 bool take_chained_launch(cudaStream_t stream);  // whether the launch at hand is chained: asked once for each, as the first one behind a fork or join of branches is not
 bool take_plain_launch(cudaStream_t stream);    // whether it is such a first one
 // What a kernel may not read before the wait is not declared `const ... __restrict__`: the compiler takes such memory to be constant while

@@ -167,12 +167,12 @@ inline int dec_attn_opt(const b200dec_attn_options* o, int heads, int v_dim, Dec
   return B200KV_OK;
 }
 
-// Whether the launch at hand of a kernel that reads nothing before its wait is chained: where nothing is recorded always (64 rows of 48 adapters beside four
+// Whether the launch at hand of a kernel that reads nothing before its wait is chained: where nothing is recorded unless that is forbidden (64 rows of 48 adapters beside four
 // projections 50.6 us without and 42.3 with it, 992 rows 63.2 and 59.1, 37 choices of 32768 tokens 22.0 and 19.7), in recorded steps as the library's
 // launches are (the first two 44.8 and 41.5, 54.7 and 57.6, 2000 rows 107.6 and 113.8).
 inline bool take_early_launch(cudaStream_t stream) {
   cudaStreamCaptureStatus status;
-  if (cudaStreamIsCapturing(stream, &status) == cudaSuccess && status == cudaStreamCaptureStatusNone) return true;
+  if (cudaStreamIsCapturing(stream, &status) == cudaSuccess && status == cudaStreamCaptureStatusNone) return b200kv_get_early_launch() != 0;
   return take_chained_launch(stream);
 }
 

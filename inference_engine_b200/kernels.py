@@ -91,9 +91,11 @@ def set_early_start(enabled: bool) -> None:
     too) afterwards.  Safe when no kernel that precedes one of these ops on its stream, with ops of
     this module alone in between, writes those arrays, which holds for the engine:
     it uploads them once per step, before the first layer (engine.py:347-356), and the ops are
-    preceded by GEMMs or by one another (architecture.py:99-198).  Off by default."""
+    preceded by GEMMs or by one another (architecture.py:99-198).  Off by default, but for the adapters, rules and
+    choices of ops.py: those read nothing before their wait, and are brought up early outside recorded steps until this is
+    called with False."""
     global _early_start
-    _early_start = bool(enabled)
+    _early_start = _lib.chained = bool(enabled)
     _lib.load().b200kv_set_chained_launch(1 if enabled else 0)
     if _lib._decoder_lib is not None:
         _lib._decoder_lib.b200kv_set_chained_launch(1 if enabled else 0)

@@ -20,10 +20,7 @@ MAX_TENSOR_CORE_DIM = 128  # head sizes up to this run on the tensor-core attent
 
 
 def _lib_dec():
-    lib = _lib.load_decoder()
-    if K._early_start and not lib.b200kv_get_chained_launch():
-        lib.b200kv_set_chained_launch(1)
-    return lib
+    return _lib.load_decoder()
 
 
 def _ptr(t: torch.Tensor | None):

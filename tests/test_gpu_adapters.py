@@ -292,3 +292,21 @@ def test_steps_behind_one_another_read_their_own_plan_and_rows(ops, rows, rank, 
         if early:
             K.set_early_start(False)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_without_early_starts(ops):
+    from inference_engine_b200 import kernels as K
+
+    made = [(slots, make(ops, rows, 512, (512,), rank, slots, torch.bfloat16, seed=8)) for rows, rank, slots in ((64, 16, 20), (900, 64, 3))]
+
+    def results():
+        return [ops.add_adapters(y, x, ad, ops.plan_adapters(ids, slots), out=torch.empty_like(y)) for slots, (ad, ids, x, y) in made]
+
+    K.set_early_start(True)
+    want = results()
+    K.set_early_start(False)
+    got, graph = results(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = results()
+    graph.replay()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, recorded))

@@ -328,3 +328,23 @@ def test_requests_without_a_way_of_sampling_have_the_engine_s_temperature():
     assert r.sampling == Sampling(0.75) and own.sampling.temperature == 0
     eng.own_sampling = False  # the sampler that all requests share
     assert eng.submit_request([1], 2).sampling is None
+
+
+def test_early_starts_can_be_switched_off():
+    """In a process of its own: what is said before a library is loaded holds for it too."""
+    import subprocess
+    import sys
+
+    code = """
+from inference_engine_b200 import _lib, kernels as K
+lib = _lib.load()
+both = lambda: (lib.b200kv_get_chained_launch(), lib.b200kv_get_early_launch())
+assert both() == (0, 1)
+K.set_early_start(False)
+dec = _lib.load_decoder()
+assert both() == (0, 0) and (dec.b200kv_get_chained_launch(), dec.b200kv_get_early_launch()) == (0, 0)
+K.set_early_start(True)
+assert both() == (1, 1) and (dec.b200kv_get_chained_launch(), dec.b200kv_get_early_launch()) == (1, 1)
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
