@@ -612,8 +612,8 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
   __shared__ uint32_t tmem_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
   if ((blockIdx.x | blockIdx.y) == 0) pdl_wait();
-  // What the first product's kernel waited for (plan and y) is in L2 as soon as this one is brought up, since every block of that one had its wait behind it
-  // then; it is not promised to this grid before its own wait, so L1, which may hold older lines, is passed by.  The inner values are not there yet.
+  // What the first product's kernel waited for is in L2 as soon as this one is brought up, since every block of that one had its wait behind it then; but it is
+  // not promised to this grid before its own wait, so L1, which may hold older lines, is passed by: the plan is read and y brought to L2.
   const int4 tile = __ldcg(a.tiles + blockIdx.y);
   const int count = tile.y;
   int part = 0, run = blockIdx.x, begin = 0;
@@ -645,29 +645,24 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
   const uint32_t bar_terms = bar + 64;
   const int q = warp & 3, half = (warp >> 2) & 1;  // this warp's lanes of tensor memory, its half of 128 columns
   // this lane's first column of its four rows
+  const int lane_row = warp < 8 ? ld_fresh(order + 32 * q + lane) : -1;
   int rows[4];
   const uint16_t* from[4];
   uint4 v[2][4] = {};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    rows[i] = warp < 8 ? ld_fresh(order + 32 * q + 8 * i + gid) : -1;
+    rows[i] = __shfl_sync(0xffffffffu, lane_row, 8 * i + gid);
     from[i] = (const uint16_t*)a.y + (long long)max(rows[i], 0) * a.y_stride + begin + 64 * half + 8 * t;
   }
   auto load_y = [&](int c, int g) {  // 32 columns
     const bool whole = a.vec && cols - (kAdTcCols * c + 64 * half + 32 * g + 8 * t) >= 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (whole && rows[i] >= 0) v[g][i] = __ldcg(reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c + 32 * g));
+      if (whole && rows[i] >= 0) v[g][i] = *reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c + 32 * g);
   };
-  load_y(0, 0);
-  load_y(0, 1);
-  // the rest of y on its way to L2, so that no load waits for memory
-  if (tid < 128 && a.vec && cols > kAdTcCols + 8) {
-    const int row = ld_fresh(order + tid);
-    if (row >= 0)
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"((const uint16_t*)a.y + (long long)row * a.y_stride + begin + kAdTcCols),
-                   "r"((cols - kAdTcCols) / 8 * 16) : "memory");
-  }
+  // y on its way to L2, so that no load waits for memory
+  if (warp < 4 && a.vec && cols >= 8 && lane_row >= 0)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"((const uint16_t*)a.y + (long long)lane_row * a.y_stride + begin), "r"(cols / 8 * 16) : "memory");
   const int rank16 = (a.rank + 15) & ~15, vecs = rank16 >> 3;
   const uint32_t us = smem + a.blocks * 16384, u_stage = ((rank16 + 63) >> 6) * kAdTcCols * 128;  // `up` lies behind the inner values
   auto fetch_up = [&](int c) {
@@ -753,6 +748,8 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
     }
     __syncwarp();
   } else {
+    load_y(0, 0);
+    load_y(0, 1);
     for (int c = 0; c < products; ++c) {
       if (!dt_mbar_wait(acc_full(c), (c >> 1) & 1)) dead = true;
       dead = __any_sync(0xffffffffu, dead);
