@@ -255,7 +255,8 @@ typedef struct b200dec_adapters {
 } b200dec_adapters;
 
 /* A step's rows sorted by adapter, for every projection of the step: the caller's buffers and the numbers that they are for.  order int32
- * [max_tiles, tile_rows]: a tile's rows, -1 behind them; tiles int32 [max_tiles, 4] (16-byte aligned): its adapter (or -1) and number of rows.
+ * [max_tiles, tile_rows]: a tile's rows, -1 behind them; tiles int32 [max_tiles, 4] (16-byte aligned): its adapter (or -1) and number of rows; the first
+ * one's third number: how many tiles have rows.
  * tile_rows: 16 or 128; max_tiles >= num_rows / tile_rows + min(num_rows, slots + 1). */
 typedef struct b200dec_adapter_plan {
   int32_t* order;

@@ -40,7 +40,7 @@ struct AdArgs {
   long long x_stride, y_stride, out_stride;
   const int32_t* order;
   const int4* tiles;
-  int tile_rows;  // of the plan
+  int tile_rows, max_tiles;  // of the plan
   int rank, width, parts;
   int ends[kAdMaxParts];
   int inner_row;          // floats between rows of partial inner values
@@ -55,7 +55,7 @@ struct AdArgs {
   int blocks;
   int group_parts, part_groups;  // parts of a cluster of the first product
   uint32_t tmem_cols;
-  int run;                // column blocks of a block of the second product
+  int col_blocks, room;   // of the second product: all parts' blocks of columns, blocks that are resident at once
 };
 
 // ---------------------------------------------------------------------------------------------------------------- the plan
@@ -119,6 +119,7 @@ adapter_plan_kernel(const int32_t* ids, int N, int slots, int tile_rows, int32_t
     __syncthreads();
   }
   for (int i = tiles_before + tid; i < max_tiles; i += threads) tiles[i] = make_int4(-1, 0, 0, 0);
+  if (tid == 0) tiles[0].z = tiles_before;  // (there is a row; its tile was written before the last barrier)
   each([&](int r, int id, unsigned on) {
     const int g = id >= 0 && id < slots ? id : slots;
     const unsigned same = __match_any_sync(on, g);
@@ -603,7 +604,9 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
   ad_cluster_wait();  // nobody reads another block's memory behind this
 }
 
-// grid (runs of a.run column blocks over all parts, tiles).  Warps 0 to 7 add to y, a product's two halves of columns in four quarters of rows; one lane of
+// A block has a tile and a run of column blocks of one part; the runs of all tiles that have rows are as short as leaves them resident at once, or as long as
+// a part.  How many tiles have rows only the plan knows, and most of its slots may be unused: 2000 rows of 4 adapters of rank 64 beside [2048 -> 12288] took
+// 37.7, 62.7 and 102.3 us of 4, 64 and 256 slots with runs for as many tiles as there could be, and 37.0, 35.6 and 42.0 so.  Blocks behind the last run end at once.  Warps 0 to 7 add to y, a product's two halves of columns in four quarters of rows; one lane of
 // warp 8 issues the products, into two accumulators in turn; warp 9 brings the columns of `up`, two blocks in shared memory or on their way.  Two blocks
 // share a multiprocessor and hold half of its tensor memory each; neither waits for another one, so that a third could only wait for their end.
 __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(const __grid_constant__ AdArgs a) {
@@ -611,22 +614,31 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
   __shared__ __align__(8) uint64_t bars[9];
   __shared__ uint32_t tmem_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
-  if ((blockIdx.x | blockIdx.y) == 0) pdl_wait();
+  if (blockIdx.x == 0) pdl_wait();
   // What the first product's kernel waited for is in L2 as soon as this one is brought up, since every block of that one had its wait behind it then; but it is
   // not promised to this grid before its own wait, so L1, which may hold older lines, is passed by: the plan is read and y brought to L2.
-  const int4 tile = __ldcg(a.tiles + blockIdx.y);
-  const int count = tile.y;
-  int part = 0, run = blockIdx.x, begin = 0;
+  const int tiles = min(__ldcg(&a.tiles[0].z), a.max_tiles);
+  const auto runs_of = [&](int part, int run) { return ((a.ends[part] - (part ? a.ends[part - 1] : 0) + kAdTcCols - 1) / kAdTcCols + run - 1) / run; };
+  int blocks = 0, length = max(1, (a.col_blocks * tiles + a.room - 1) / a.room) - 1;  // (a tile's runs; of so many column blocks)
+  do {
+    ++length;
+    blocks = 0;
+    for (int p = 0; p < a.parts; ++p) blocks += runs_of(p, length);
+  } while (blocks * tiles > a.room && blocks > a.parts);
+  const int at_tile = blockIdx.x / blocks;
+  if (at_tile >= tiles) return;  // (the first block has waited for the grid in front)
+  int part = 0, run = blockIdx.x - at_tile * blocks;
   for (; part < a.parts - 1; ++part) {
-    const int n = ((a.ends[part] - begin + kAdTcCols - 1) / kAdTcCols + a.run - 1) / a.run;
+    const int n = runs_of(part, length);
     if (run < n) break;
     run -= n;
-    begin = a.ends[part];
   }
-  begin += run * a.run * kAdTcCols;
-  const int cols = min(a.ends[part] - begin, a.run * kAdTcCols), products = (cols + kAdTcCols - 1) / kAdTcCols;
-  const int32_t* order = a.order + (long long)blockIdx.y * 128;
-  if (count <= 0) return pdl_wait();
+  const int begin = (part ? a.ends[part - 1] : 0) + run * length * kAdTcCols;
+  const int cols = min(a.ends[part] - begin, length * kAdTcCols), products = (cols + kAdTcCols - 1) / kAdTcCols;
+  const int4 tile = __ldcg(a.tiles + at_tile);
+  const int count = tile.y;
+  const int32_t* order = a.order + (long long)at_tile * 128;
+  if (count <= 0) return;
   if (tile.x < 0) {
     pdl_wait();
     if (a.out == a.y) return;
@@ -729,7 +741,7 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
       asm volatile("fence.proxy.async.global;\n" ::: "memory");
       dt_expect_tx(bar_terms, bytes);
       asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                   ::"r"(smem), "l"((const uint8_t*)a.terms + ((long long)blockIdx.y * a.parts + part) * bytes), "r"(bytes), "r"(bar_terms) : "memory");
+                   ::"r"(smem), "l"((const uint8_t*)a.terms + ((long long)at_tile * a.parts + part) * bytes), "r"(bytes), "r"(bar_terms) : "memory");
       if (!dt_mbar_wait(bar_terms, 0)) dead = true;
       const uint32_t idesc = ad_idesc(kAdTcCols);
       const uint64_t da = ad_desc(smem), db = ad_desc(us);  // (in steps of 16 bytes)
@@ -1024,7 +1036,7 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
   AdArgs a = {};
   a.down = ad->down; a.up = ad->up; a.scale = ad->scale; a.x = x; a.y = y; a.out = out;
   a.x_stride = x_stride; a.y_stride = y_stride; a.out_stride = out_stride;
-  a.order = order; a.tiles = (const int4*)tiles; a.tile_rows = tile_rows;
+  a.order = order; a.tiles = (const int4*)tiles; a.tile_rows = tile_rows; a.max_tiles = max_tiles;
   a.rank = ad->rank; a.width = ad->width; a.parts = ad->parts; a.status = status;
   bool even = true;
   int most = 0;
@@ -1077,14 +1089,11 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     else rc = ad_launch(adapter_first_kernel<4, 3>, a, first, 4, smem, s);
     if (rc) return rc;
     const int ublocks = ((a.rank + 15) / 16 * 16 + 63) / 64;
-    int col_blocks = 0, runs = 0;
-    for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) col_blocks += (a.ends[p] - begin + kAdTcCols - 1) / kAdTcCols;
-    // Runs for which all blocks are resident at once, two a multiprocessor.  2000 rows of rank 64 beside [2048 -> 12288], all on clusters of eight: 42 us,
-    // with runs of a single block 48, one block longer 47, three longer 54.
-    a.run = (int)(((long long)col_blocks * max_tiles + 2 * sms - 1) / (2 * sms));
-    if (a.run < 1) a.run = 1;
-    for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) runs += ((a.ends[p] - begin + kAdTcCols - 1) / kAdTcCols + a.run - 1) / a.run;
-    const dim3 grid((unsigned)runs, (unsigned)max_tiles);
+    a.room = 2 * sms;
+    for (int p = 0, begin = 0; p < a.parts; begin = a.ends[p++]) a.col_blocks += (a.ends[p] - begin + kAdTcCols - 1) / kAdTcCols;
+    // as many blocks as any number of tiles can have runs.  2000 rows of rank 64 beside [2048 -> 12288], all on clusters of eight: 42 us with runs for one
+    // round of blocks, 48 with runs of a single column block, 47 with runs one longer, 54 with three longer
+    const dim3 grid((unsigned)std::min((long long)max_tiles * a.col_blocks, std::max<long long>(a.room, (long long)max_tiles * a.parts)));
     const size_t second = 1024 + (size_t)a.blocks * 16384 + (size_t)2 * ublocks * kAdTcCols * 128;
     auto kernel = adapter_second_kernel;
     if (!allow_smem(kernel, kAdMostSmem)) return launch_result(cudaErrorInvalidValue);

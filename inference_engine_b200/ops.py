@@ -698,7 +698,7 @@ class AdapterPlan:
 
     @property
     def tiles(self) -> torch.Tensor:
-        """int32 [tiles, 4]: adapter (-1: none) and number of rows."""
+        """int32 [tiles, 4]: adapter (-1: none) and number of rows; the first one's third number: tiles that have rows."""
         return self.buf[: 4 * self.num_tiles].view(self.num_tiles, 4)
 
     @property

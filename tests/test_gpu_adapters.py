@@ -310,3 +310,21 @@ def test_without_early_starts(ops):
         recorded = results()
     graph.replay()
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, recorded))
+
+
+@pytest.mark.parametrize("rows,width,parts,rank,slots,used", [
+    (1300, 256, (512, 520, 40), 64, 700, 3), (300, 72, (4200, 130), 40, 300, 300), (520, 128, (256,), 64, 4096, 1), (2000, 64, (96, 4000), 128, 48, 5),
+    (700, 128, (40000,), 64, 2, 2)])
+def test_portions_beside_slots_that_nobody_uses(ops, rows, width, parts, rank, slots, used):
+    """Tiles that could have rows and do not, up to many times those that do; and runs of many columns."""
+    g = torch.Generator().manual_seed(rows)
+    of = torch.randperm(slots, generator=g)[:used]
+    ids = of[torch.arange(rows) * used // rows]
+    ids[rows // 3] = -1
+    ad, ids, x, y = make(ops, rows, width, parts, rank, slots, torch.bfloat16, seed=rows, ids=ids)
+    plan = ops.plan_adapters(ids, slots)
+    assert plan.tile_rows == 128
+    live = plan.tiles[:, 1].gt(0)
+    assert plan.tiles[0, 2] == live.sum() and live[: live.sum()].all()
+    got = ops.add_adapters(y, x, ad, plan, out=torch.empty_like(y))
+    check(ad, ids, x, y, got)
