@@ -249,8 +249,12 @@ __device__ __forceinline__ void ad_store(const uint16_t* from, uint16_t* to, int
 // registers.  The order of a product's channels is free, so that a lane loads whole 16 bytes: lane t of a row's four has channels 8t ..
 // 8t + 7 of 32.  Second product: a warp takes groups of 32 columns, whose `up` and y come through a ring of its own.
 // kNT: blocks of eight inner values of a warp.  kKB: blocks of sixteen inner values.  kC: blocks of a cluster.  kStages: groups on their way.
+// Blocks that a multiprocessor's registers are shared among.  Three (80 registers) spilled above rank 32, where shared memory has room for one or two for the
+// most part: one row of rank 64 beside [2048 -> 12288] 9.4 us, and 8.6 so.
+constexpr int ad_rows_blocks(int inner_blocks) { return inner_blocks > 4 ? 1 : inner_blocks > 2 ? 2 : 3; }
+
 template <int kNT, int kKB, int kC, int kStages>
-__global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kernel(const __grid_constant__ AdArgs a) {
+__global__ void __launch_bounds__(kAdThreads, ad_rows_blocks(kKB)) adapter_rows_kernel(const __grid_constant__ AdArgs a) {
   extern __shared__ __align__(16) uint8_t ad_smem[];
   const uint32_t smem = (uint32_t)__cvta_generic_to_shared(ad_smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t = lane & 3;
@@ -258,7 +262,8 @@ __global__ void __launch_bounds__(kAdThreads, kKB > 4 ? 1 : 3) adapter_rows_kern
   pdl_enter();
   pdl_wait();
   const AdJob job = ad_job<16, kC>(a);
-  const int row0 = ld_fresh(job.order + gid), row1 = ld_fresh(job.order + gid + 8);
+  const int lane_row = ld_fresh(job.order + (lane & 15));
+  const int row0 = __shfl_sync(0xffffffffu, lane_row, gid), row1 = __shfl_sync(0xffffffffu, lane_row, gid + 8);
   if (job.count <= 0) return;  // (with the whole cluster)
   if (job.slot < 0) return ad_copy_rows<uint16_t>(a, job, rank, kC);
   const uint16_t* down = (const uint16_t*)a.down + ((long long)job.slot * a.parts + job.part) * a.rank * a.width;
@@ -930,29 +935,49 @@ static int ad_launch(void (*kernel)(KArgs...), const AdArgs& a, int clusters, in
   return launch_result(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
-template <int kNT, int kKB, int kC, int kStages>
-static int ad_rows_of(AdArgs a, int clusters, int most_cols, cudaStream_t stream) {
-  a.inner_row = a.rank + 4;                    // (rows apart by other banks)
-  a.t_row = (a.rank * 4 + 63) / 64 * 64 + 32;  // both terms; four rows at different banks
-  a.u_row = a.rank * 2;
-  while (a.u_row % 64 != 32) a.u_row += 16;    // four columns at different banks
-  const int deep = a.rank <= 8 * kNT ? kAdWarps : kAdWarps / 2;
-  a.off_t = (uint32_t)(deep * 16 * a.inner_row * 4);
-  a.off_u = a.off_t + 16 * a.t_row;
-  a.ring = ((most_cols + 31) / 32 + kC * kAdWarps - 1) / (kC * kAdWarps);  // (a warp has no more groups than that)
-  if (a.ring > kStages) a.ring = kStages;
-  return ad_launch(adapter_rows_kernel<kNT, kKB, kC, kStages>, a, clusters, kC, a.off_u + (size_t)kAdWarps * a.ring * (32 * a.u_row + 1024), stream);
+// Shared memory of a block of few rows, and how it is laid out.
+static size_t ad_rows_layout(AdArgs* a, int inner_blocks, int cluster, int stages, int most_cols) {
+  a->inner_row = a->rank + 4;                    // (rows apart by other banks)
+  a->t_row = (a->rank * 4 + 63) / 64 * 64 + 32;  // both terms; four rows at different banks
+  a->u_row = a->rank * 2;
+  while (a->u_row % 64 != 32) a->u_row += 16;    // four columns at different banks
+  const int deep = a->rank <= 8 * inner_blocks ? kAdWarps : kAdWarps / 2;
+  a->off_t = (uint32_t)(deep * 16 * a->inner_row * 4);
+  a->off_u = a->off_t + 16 * a->t_row;
+  a->ring = std::min(stages, ((most_cols + 31) / 32 + cluster * kAdWarps - 1) / (cluster * kAdWarps));  // (a warp has no more groups than that)
+  return a->off_u + (size_t)kAdWarps * a->ring * (32 * a->u_row + 1024);
 }
 
-// A cluster has as many blocks as leave all of them resident at once, three a multiprocessor: fewer fetch a tile's weights one after the other, more wait for
-// a place.  us with 8, 4 and 2 blocks, rank 16, rows of 48 adapters: three parts of [2048 -> 4096] 14.9, 11.8 and 8.4, one of [2048 -> 2048] 6.7, 6.3 and
-// 7.3, two of [2048 -> 12288] 16.7, 12.3 and 16.4, [6144 -> 2048] 7.7, 8.2 and 10.2; one row beside [2048 -> 12288] 5.6, 7.7 and 12.0.
+// The cluster for which rounds of clusters times a cluster's time are least.  By itself a cluster of C blocks takes about 3.6 us + (columns (21 + rank) + channels
+// (13 + 0.3 rank)) 0.07 ns / C (rank 64 beside [2048 -> 12288] with 8, 4 and 2 blocks: 8.7, 13.5 and 22.2 us; rank 16 beside [2048 -> 2048] 4.3, 5.3 and 7.3).
+// Blocks are resident by their shared memory (fewer at higher ranks beside wide parts) and registers; of the places for clusters of eight a seventh is left
+// over, as a graphics cluster's multiprocessors are rarely a multiple of eight, but where three blocks share one.  us with 8, 4 and 2 blocks, 64 rows of 48
+// adapters and then 16 of 16, the first taken up to rank 16 whatever the rank before (the last two of these 18.4 and 25.1 us):
+//     rank 16: three parts of [2048 -> 4096] 15.1, 11.9, 8.6 and 6.5, 6.4, 7.4; two of [2048 -> 12288] 15.1, 12.5, 16.4 and 7.4, 8.1, 12.0; [6144 -> 2048] 7.6, 8.2, 10.2
+//     rank 32: 18.2, 18.7, 20.9 and 7.4, 8.0, 9.5; 42.0, 30.1, 35.3 and 18.4, 10.5, 16.7; 10.1, 12.5, 19.4
+//     rank 64: 31.2, 34.0, 27.5 and 12.5, 13.6, 12.3; 55.3, 41.4, 47.6 and 23.3, 13.8, 22.7; 19.2, 26.3, 24.3
 template <int kNT, int kKB, int kStages>
-static int ad_rows(const AdArgs& a, int clusters, long long used, int most_cols, cudaStream_t stream) {
-  const int room = 3 * device_sms();
-  if (used * 8 <= room) return ad_rows_of<kNT, kKB, 8, kStages>(a, clusters, most_cols, stream);
-  if (used * 4 <= room) return ad_rows_of<kNT, kKB, 4, kStages>(a, clusters, most_cols, stream);
-  return ad_rows_of<kNT, kKB, 2, kStages>(a, clusters, most_cols, stream);
+static int ad_rows(const AdArgs& args, int clusters, int tiles, int most_cols, cudaStream_t stream) {
+  constexpr int kShared = 228 * 1024;  // of a multiprocessor; a block has one of these KB to itself
+  const int sms = device_sms(), used = tiles * args.parts;
+  const long long work = (long long)most_cols * (21 + args.rank) + (long long)args.width * (13 + 3 * args.rank / 10);
+  AdArgs a = args, best = args;
+  long long least = 0;
+  int cluster = 0;
+  size_t smem = 0;
+  for (int c = 8; c >= 2; c /= 2) {
+    const size_t bytes = ad_rows_layout(&a, kNT, c, kStages, most_cols);
+    const int fit = std::min(ad_rows_blocks(kKB), (int)(kShared / (bytes + 1024))), room = c == 8 && fit < 3 ? sms * fit * 6 / 7 : sms * fit;
+    const long long cost = ((long long)used * c + room - 1) / std::max(room, 1) * (50000 + work / c);
+    if (cluster && cost >= least) continue;
+    least = cost;
+    cluster = c;
+    smem = bytes;
+    best = a;
+  }
+  if (cluster == 8) return ad_launch(adapter_rows_kernel<kNT, kKB, 8, kStages>, best, clusters, 8, smem, stream);
+  if (cluster == 4) return ad_launch(adapter_rows_kernel<kNT, kKB, 4, kStages>, best, clusters, 4, smem, stream);
+  return ad_launch(adapter_rows_kernel<kNT, kKB, 2, kStages>, best, clusters, 2, smem, stream);
 }
 
 // Tiles of 128 rows: the parts of a cluster, tensor memory and shared memory of the first product.
@@ -1101,7 +1126,8 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     return launch_result(launch_kernel(b200kv_get_early_launch() != 0, kernel, grid, dim3(kAdSecondThreads), second, s, a));
   }
   const int kb = (a.rank + 15) / 16;
-  const long long used = ad_used(ad, plan);
+  // sixteen rows of one adapter that can be expected: as many rows of each
+  const int groups = std::min(plan->num_rows, plan->slots + 1), used = std::min(fine / a.parts, groups * ((plan->num_rows + 16 * groups - 1) / (16 * groups)));
   if (kb <= 1) return ad_rows<2, 1, 3>(a, fine, used, most, s);
   if (kb <= 2) return ad_rows<4, 2, 3>(a, fine, used, most, s);
   if (kb <= 4) return ad_rows<8, 4, 2>(a, fine, used, most, s);

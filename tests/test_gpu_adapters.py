@@ -328,3 +328,13 @@ def test_portions_beside_slots_that_nobody_uses(ops, rows, width, parts, rank, s
     assert plan.tiles[0, 2] == live.sum() and live[: live.sum()].all()
     got = ops.add_adapters(y, x, ad, plan, out=torch.empty_like(y))
     check(ad, ids, x, y, got)
+
+
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 56, 64, 72, 128])
+@pytest.mark.parametrize("rows,used,slots", [(1, 1, 40), (16, 16, 16), (64, 48, 48), (40, 3, 9)])
+def test_clusters_of_every_size_at_every_rank(ops, rank, rows, used, slots):
+    g = torch.Generator().manual_seed(rank)
+    ids = torch.randperm(slots, generator=g)[:used][torch.arange(rows) % used]
+    for width, parts in ((264, (512, 33)), (1024, (2600,)), (72, (1032, 1032, 8, 64))):
+        ad, at, x, y = make(ops, rows, width, parts, rank, slots, torch.bfloat16, seed=rank, ids=ids)
+        check(ad, at, x, y, ops.add_adapters(y, x, ad, ops.plan_adapters(at, slots, 16), out=torch.empty_like(y)))
