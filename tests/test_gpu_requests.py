@@ -326,3 +326,55 @@ def test_slots_made_anew_behind_the_engine_s_back_are_refused(use_graphs):
         eng.step()
     assert r.output == want
     status_clear()
+
+
+def test_adapters_and_ways_of_sampling_in_the_same_steps():
+    """Every request with an adapter, a grammar or a way of sampling, or several of them: tokens follow from the step's logits, which follow from the adapters."""
+    from inference_engine_b200 import ops
+    from inference_engine_b200.engine import Sampling
+
+    even = list(range(0, 1000, 2))
+    asks = [(0, Sampling(temperature=0.9, top_k=12, seed=1)), (2, Sampling(temperature=1.1, top_p=0.9, frequency=0.4, grammar=lambda out: len(out) % 2 - 1)),
+            (-1, Sampling(repetition=1.3, bias={7: 3.0})), (2, None), (1, Sampling(temperature=0.7, min_p=0.05, grammar=lambda out: 0)), (-1, None)]
+
+    def run(use_graphs, adapters=True, watch=None):
+        model = scaffold()
+        model.make_adapters(3, 8)
+        for slot in range(3):
+            fill(model, slot, 20 + slot)
+        eng = build(model, use_graphs, adapters=True, own_sampling=True, seed=13)
+        eng.set_mask(0, even)
+        reqs = [eng.submit_request(p, 6, s, adapter=a if adapters else -1) for p, (a, s) in zip(prompts(), asks)]
+        if watch is not None:
+            choose = ops.choose_tokens
+            watch.append((choose, []))
+
+            def keep(logits, draw, rules, append):
+                l, same = logits.clone(), lambda t: None if t is None else t.clone()  # noqa: E731
+                own = ops.Draw(*(same(getattr(draw, n)) for n in ("temperature", "uniform", "top_k", "top_p", "min_p")))
+                r = ops.Rules(**{k: same(v) for k, v in vars(rules).items() if k in ops.Rules.__dataclass_fields__})
+                got = choose(logits, draw, rules, append)
+                watch[0][1].append((l, own, r, got))
+                return got
+
+            ops.choose_tokens = keep
+        try:
+            while not eng.sched.idle():
+                eng.step()
+        finally:
+            if watch is not None:
+                ops.choose_tokens = watch[0][0]
+        status_clear()
+        return [r.output for r in reqs]
+
+    seen = []
+    eager = run(False, watch=seen)
+    assert eager == run(True) and all(len(o) == 6 for o in eager)
+    assert all(t % 2 == 0 for t in eager[4]) and all(t % 2 == 0 for t in eager[1][1::2])
+    without = run(False, adapters=False)
+    assert all((a == b) == (ask[0] < 0) for a, b, ask in zip(eager, without, asks))
+    for l, draw, rules, (tokens, logprobs) in seen[0][1]:
+        live = rules.slots >= 0
+        assert ((tokens >= 0) == live).all()
+        adj = ops.adjust_logits(l, rules, out=torch.full(l.shape, -float("inf"), device="cuda"))  # (rows that are passed over: nothing)
+        check_choice(adj, draw, tokens, logprobs)
