@@ -169,7 +169,7 @@ template <int kLeft>
 __device__ __forceinline__ void ad_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(kLeft) : "memory"); }
 
 // Tiles, rows' places, x and y are read through L2.  A chained kernel is brought up beside the two or three in front of it: the multiprocessor's L1 may hold
-// lines of theirs that were read before others wrote them (an older plan at the same address, say).
+// lines of theirs that were read before others wrote them (an older plan at the same address, say), and keeps none of what this one reads for the next.
 // The rows [first, first + n) of a cluster's tile and the columns of its part.
 struct AdJob {
   int slot, count, part, begin, end;
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
     const bool whole = a.vec && cols - (kAdTcCols * c + 64 * half + 32 * g + 8 * t) >= 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (whole && rows[i] >= 0) v[g][i] = *reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c + 32 * g);
+      if (whole && rows[i] >= 0) v[g][i] = __ldcg(reinterpret_cast<const uint4*>(from[i] + kAdTcCols * c + 32 * g));
   };
   // y on its way to L2, so that no load waits for memory
   if (warp < 4 && a.vec && cols >= 8 && lane_row >= 0)

@@ -476,3 +476,31 @@ def test_more_logits_side_by_side_than_are_sorted_at_once(ops, V, tau, values):
     draw = ops.Draw(torch.full((E,), tau, device="cuda"), cuda(torch.rand(E, generator=g)), cuda(k), cuda(p))
     tokens, logprobs = ops.choose_tokens(l, draw)
     check_choice(l, draw, tokens, logprobs)
+
+
+@pytest.mark.parametrize("early", [False, True])
+def test_rules_and_choices_behind_one_another_see_what_was_written(ops, early):
+    """Rows whose ends share lines, written over one another's, with nothing waiting in between."""
+    from inference_engine_b200 import kernels as K
+
+    E, V = 40, 20001
+    g = torch.Generator().manual_seed(12)
+    rules, draw = make_rules(ops, E, V, 300, g, bias=200), make_draw(ops, E, g)
+    logits = [make_logits(E, V, torch.float32, g, pad=3) for _ in range(8)]
+    want = []
+    for l in logits:
+        adj = ops.adjust_logits(l, rules)
+        torch.cuda.synchronize()
+        want.append((adj, *ops.choose_tokens(adj, draw)))
+        torch.cuda.synchronize()
+    K.set_early_start(early)
+    try:
+        got, over = [], torch.empty(E, V, device="cuda")
+        for l in logits:
+            ops.adjust_logits(l, rules, out=over)
+            got.append(ops.choose_tokens(over, draw))
+    finally:
+        K.set_early_start(False)
+    for (adj, tokens, logprobs), (t, p) in zip(want, got):
+        assert torch.equal(t, tokens) and torch.equal(p, logprobs)
+        check_choice(adj, draw, tokens, logprobs)
