@@ -487,7 +487,7 @@ class Engine:
     def ask_grammars(self, step: Step) -> list[Request]:
         """The masks of the step's requests, before anything of it is done: a request whose grammar fails ends, and the others have their step."""
         failed = []
-        for r, toks in step.entries:
+        for r, toks in step.entries if self.own_sampling else ():
             if r.sampling is None or r.sampling.grammar is None or not self.wants_token(r, toks):
                 continue
             try:
