@@ -182,14 +182,20 @@ __device__ __forceinline__ AdJob ad_job(const AdArgs& a) {
   return {tile.x, min(tile.y - (at % subs) * kRows, kRows), part, part ? a.ends[part - 1] : 0, a.ends[part], a.order + (long long)at * kRows};
 }
 
-// Rows without an adapter: copied where the result has a place of its own.
+// Rows without an adapter: copied where the result has a place of its own, sixteen at a time (lane i % 16 has row i) so that their loads are on their way together.
 template <typename T>
-__device__ __forceinline__ void ad_copy_rows(const AdArgs& a, const AdJob& job, int rank, int cluster) {
-  if (a.out == a.y) return;
-  for (int col = job.begin + rank * kAdThreads + threadIdx.x; col < job.end; col += cluster * kAdThreads) {
-    for (int i = 0; i < job.count; ++i) {
-      const long long r = ld_fresh(job.order + i);
-      ((T*)a.out)[r * a.out_stride + col] = __ldcg((const T*)a.y + r * a.y_stride + col);
+__device__ __forceinline__ void ad_copy_rows(const AdArgs& a, int lane_row, int count, int col, int end, int step) {
+  for (; __any_sync(0xffffffffu, col < end); col += step) {
+    T v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = __shfl_sync(0xffffffffu, lane_row, i);
+      if (i < count && col < end) v[i] = __ldcg((const T*)a.y + r * a.y_stride + col);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = __shfl_sync(0xffffffffu, lane_row, i);
+      if (i < count && col < end) ((T*)a.out)[r * a.out_stride + col] = v[i];
     }
   }
 }
@@ -265,7 +271,10 @@ __global__ void __launch_bounds__(kAdThreads, ad_rows_blocks(kKB)) adapter_rows_
   const int lane_row = ld_fresh(job.order + (lane & 15));
   const int row0 = __shfl_sync(0xffffffffu, lane_row, gid), row1 = __shfl_sync(0xffffffffu, lane_row, gid + 8);
   if (job.count <= 0) return;  // (with the whole cluster)
-  if (job.slot < 0) return ad_copy_rows<uint16_t>(a, job, rank, kC);
+  if (job.slot < 0) {
+    if (a.out != a.y) ad_copy_rows<uint16_t>(a, lane_row, job.count, job.begin + rank * kAdThreads + tid, job.end, kC * kAdThreads);
+    return;
+  }
   const uint16_t* down = (const uint16_t*)a.down + ((long long)job.slot * a.parts + job.part) * a.rank * a.width;
   const uint16_t* up = (const uint16_t*)a.up + (long long)job.slot * a.ends[a.parts - 1] * a.rank;
   const uint16_t* y = (const uint16_t*)a.y;
@@ -483,12 +492,13 @@ __global__ void __launch_bounds__(kAdThreads) adapter_first_kernel(const __grid_
   // the parts that this cluster takes
   const int cl = blockIdx.x / kC, at = cl / a.part_groups, p0 = (cl - at * a.part_groups) * a.group_parts, np = min(a.group_parts, a.parts - p0);
   const int4 tile = __ldcg(a.tiles + at);
+  const int row_of = tid < 128 ? ld_fresh(a.order + (long long)at * 128 + tid) : -1;  // (on its way beside the tile)
   const int count = tile.y;
   if (count <= 0 || tile.x < 0) return;  // (with the whole cluster)
   const uint32_t smem = ((uint32_t)__cvta_generic_to_shared(ad_raw) + 1023u) & ~1023u;
   uint8_t* base = ad_raw + (smem - (uint32_t)__cvta_generic_to_shared(ad_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
-  if (tid < 128) rows_of[tid] = ld_fresh(a.order + (long long)at * 128 + tid);
+  if (tid < 128) rows_of[tid] = row_of;
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) dt_mbar_init(bar + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -641,16 +651,15 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
   const int begin = (part ? a.ends[part - 1] : 0) + run * length * kAdTcCols;
   const int cols = min(a.ends[part] - begin, length * kAdTcCols), products = (cols + kAdTcCols - 1) / kAdTcCols;
   const int4 tile = __ldcg(a.tiles + at_tile);
-  const int count = tile.y;
   const int32_t* order = a.order + (long long)at_tile * 128;
+  const int q = warp & 3, half = (warp >> 2) & 1;  // this warp's lanes of tensor memory, its half of 128 columns
+  const int lane_row = ld_fresh(order + 32 * q + lane);
+  const int count = tile.y;
   if (count <= 0) return;
   if (tile.x < 0) {
     pdl_wait();
     if (a.out == a.y) return;
-    for (int i = warp; i < count; i += kAdSecondThreads / 32) {
-      const long long r = ld_fresh(order + i);
-      for (int c = begin + lane; c < begin + cols; c += 32) ((uint16_t*)a.out)[r * a.out_stride + c] = __ldcg((const uint16_t*)a.y + r * a.y_stride + c);
-    }
+    if (warp < 8) ad_copy_rows<uint16_t>(a, ld_fresh(order + 16 * warp + (lane & 15)), count - 16 * warp, begin + lane, begin + cols, 32);
     return;
   }
   const uint32_t smem = ((uint32_t)__cvta_generic_to_shared(ad_raw) + 1023u) & ~1023u;
@@ -660,9 +669,7 @@ __global__ void __launch_bounds__(kAdSecondThreads, 2) adapter_second_kernel(con
   const auto up_full = [&](int i) { return bar + 32 + 8 * (i & 1); };
   const auto up_free = [&](int i) { return bar + 48 + 8 * (i & 1); };
   const uint32_t bar_terms = bar + 64;
-  const int q = warp & 3, half = (warp >> 2) & 1;  // this warp's lanes of tensor memory, its half of 128 columns
   // this lane's first column of its four rows
-  const int lane_row = warp < 8 ? ld_fresh(order + 32 * q + lane) : -1;
   int rows[4];
   const uint16_t* from[4];
   uint4 v[2][4] = {};
@@ -819,7 +826,10 @@ __global__ void __launch_bounds__(kAdThreads) adapter_simt_kernel(const __grid_c
   pdl_wait();
   const AdJob job = ad_job<16, kC>(a);
   if (job.count <= 0) return;
-  if (job.slot < 0) return ad_copy_rows<T>(a, job, rank, kC);
+  if (job.slot < 0) {
+    if (a.out != a.y) ad_copy_rows<T>(a, ld_fresh(job.order + (lane & 15)), job.count, job.begin + rank * kAdThreads + tid, job.end, kC * kAdThreads);
+    return;
+  }
   const T* down = (const T*)a.down + ((long long)job.slot * a.parts + job.part) * a.rank * a.width;
   const T* up = (const T*)a.up + (long long)job.slot * a.ends[a.parts - 1] * a.rank;
   float* part = reinterpret_cast<float*>(ad_smem);

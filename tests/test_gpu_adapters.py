@@ -338,3 +338,20 @@ def test_clusters_of_every_size_at_every_rank(ops, rank, rows, used, slots):
     for width, parts in ((264, (512, 33)), (1024, (2600,)), (72, (1032, 1032, 8, 64))):
         ad, at, x, y = make(ops, rows, width, parts, rank, slots, torch.bfloat16, seed=rank, ids=ids)
         check(ad, at, x, y, ops.add_adapters(y, x, ad, ops.plan_adapters(at, slots, 16), out=torch.empty_like(y)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,rank,slots,tile_rows", [(70, 16, 3, 16), (300, 64, 2, 128), (300, 8, 2, 128), (5, 128, 1, 16)])
+def test_rows_without_an_adapter_are_copied_or_left(ops, dtype, rows, rank, slots, tile_rows):
+    g = torch.Generator().manual_seed(rows)
+    ids = torch.where(torch.rand(rows, generator=g) < 0.7, torch.full((rows,), -1), torch.randint(0, slots, (rows,), generator=g))
+    for width, parts in ((128, (700, 70)), (72, (33,)), (2048, (1024,))):
+        ad, at, x, y = make(ops, rows, width, parts, rank, slots, dtype, seed=rank, ids=ids)
+        y[ids == -1] = float("nan")
+        plan = ops.plan_adapters(at, slots, tile_rows)
+        wide = torch.full((rows, y.shape[1] + 5), 7.0, dtype=dtype, device="cuda")
+        got = ops.add_adapters(y, x, ad, plan, out=wide[:, : y.shape[1]])
+        none = (ids == -1).cuda()
+        assert got[none].isnan().all() and got[~none].isfinite().all() and (wide[:, y.shape[1] :] == 7).all()
+        check(ad, at[~none], x[~none], y[~none], got[~none])
+        assert torch.equal(ops.add_adapters(y.clone(), x, ad, plan)[~none], got[~none])
