@@ -270,8 +270,8 @@ int b200dec_adapter_plan(const int32_t* ids, const b200dec_adapter_plan_t* plan,
 
 /* out[r] = y[r] + scale[a] * (x[r] . down[a]_p^T) . up[a]^T for the rows of a plan with as many slots; out[r] = y[r] for rows without an adapter.
  * x [num_rows, width], y and out [num_rows, out] of element size elem, strides in elements.  out may be y itself, with the same stride; otherwise it
- * overlaps neither y nor x.  32-bit sums, rounded once.  workspace: 16-byte aligned, of the size that b200dec_add_adapters_workspace says (0 where
- * none is needed); nothing in it outlasts the call. */
+ * overlaps neither y nor x.  32-bit sums, rounded once; in bf16 the inner values are two bf16 terms, 2^-16 of each left out at most.  workspace:
+ * 16-byte aligned, of the size that b200dec_add_adapters_workspace says (0 where none is needed); nothing in it outlasts the call. */
 size_t b200dec_add_adapters_workspace(const b200dec_adapters* adapters, const b200dec_adapter_plan_t* plan);
 int b200dec_add_adapters(const b200dec_adapters* adapters, const b200dec_adapter_plan_t* plan, const void* x, int64_t x_stride, const void* y,
                          int64_t y_stride, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, int32_t* status,

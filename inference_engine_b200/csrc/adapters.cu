@@ -8,12 +8,13 @@
 // that a tile's `down` is fetched by many multiprocessors at once; the blocks' partial inner values are summed through distributed shared memory, in a fixed
 // order.
 //
-// Precision: bf16 operands, 32-bit sums.  The inner values are scaled in 32 bits and enter the second product as two bf16 terms (16 bits of
-// mantissa): rounded to one they would cost the sum as much as its own rounding does.
+// Precision: bf16 operands, 32-bit sums.  The inner values are scaled in 32 bits and enter the second product as two bf16 terms, which leave out 2^-16 of each
+// at most: rounded to one they would cost the sum as much as its own rounding does, and with all of their bits a result comes out
+// otherwise for one element in a thousand, by a last bit of its own (as near to the formula in 64 bits).  On the CUDA cores they keep their 32 bits.
 //
-// Measured, the plan and [2048 -> 4096] (three parts), [2048 -> 2048], [2048 -> 12288] (two parts) and [6144 -> 2048] in turn: one row, rank 16, 2.5 and 3.9,
-// 4.2, 5.4 and 4.9 us; 64 rows of 48 adapters of rank 16 3.3 and 8.4, 6.7, 12.1 (28 MB, 2.4 TB/s) and 7.6; 992 rows of 3 adapters of rank 16 3.8 and 11, 7,
-// 19 and 9.5; 2000 rows of 4 adapters of rank 64 4.3 and 25, 17, 38 (115 MB, 3 TB/s) and 24.  What bounds the small ones is a chain of latencies: tile, rows,
+// Measured, the plan and [2048 -> 4096] (three parts), [2048 -> 2048], [2048 -> 12288] (two parts) and [6144 -> 2048] in turn: one row, rank 16, 3.0 and 4.0,
+// 4.0, 5.4 and 4.9 us; 64 rows of 48 adapters of rank 16 3.6 and 8.3, 6.6, 12.4 (28 MB, 2.3 TB/s) and 7.8; 992 rows of 3 adapters of rank 16 3.9 and 11, 7,
+// 19 and 9; 2000 rows of 4 adapters of rank 64 4.7 and 26, 17, 38 (115 MB, 3 TB/s) and 25.  What bounds the small ones is a chain of latencies: tile, rows,
 // first product, exchange, second product, result.
 #include "dec_tma.cuh"
 
@@ -1136,7 +1137,7 @@ extern "C" int b200dec_add_adapters(const b200dec_adapters* ad, const b200dec_ad
     return launch_result(launch_kernel(b200kv_get_early_launch() != 0, kernel, grid, dim3(kAdSecondThreads), second, s, a));
   }
   const int kb = (a.rank + 15) / 16;
-  // sixteen rows of one adapter that can be expected: as many rows of each
+  // tiles of sixteen rows that can be expected: every slot in use, and by as many rows (what is in use only the device knows)
   const int groups = std::min(plan->num_rows, plan->slots + 1), used = std::min(fine / a.parts, groups * ((plan->num_rows + 16 * groups - 1) / (16 * groups)));
   if (kb <= 1) return ad_rows<2, 1, 3>(a, fine, used, most, s);
   if (kb <= 2) return ad_rows<4, 2, 3>(a, fine, used, most, s);
